@@ -49,8 +49,9 @@ extern "C" {
 /* 2: ec_stage_stripes_to_host added; the batched kernels read every
  * descriptor entry of a stripe, also the length of an absent unit.
  * 3: ec_stage_stripes_to_host and ec_stage_to_host copy on an SDMA engine
- * (see there); ec_stage_stats.copy_engine added. */
-#define EC_ABI_VERSION 3
+ * (see there); ec_stage_stats.copy_engine added.
+ * 4: the operators of a training step added. */
+#define EC_ABI_VERSION 4
 
 /* Status codes. */
 #define EC_OK 0
@@ -64,6 +65,18 @@ extern "C" {
  * device kernels take up to EC_MAX_K data and EC_MAX_M parity shards. */
 #define EC_MAX_K 32
 #define EC_MAX_M 16
+
+/* Element types of the training-step operators. */
+#define EC_F32 0
+#define EC_BF16 1
+#define EC_F16 2
+
+/* Norms of ec_grad_norm and ec_grad_clip. */
+#define EC_NORM_INF 0 /* the largest magnitude                */
+#define EC_NORM_2 2   /* the square root of the sum of squares */
+
+/* Alternatives ec_token_logprobs returns at most. */
+#define EC_MAX_TOP 16
 
 /* A hipStream_t, passed as an opaque pointer so that callers (ctypes, cgo,
  * JNI) need no HIP header. */
@@ -334,6 +347,117 @@ typedef struct {
  * staging of coded checkpoints (tensor_aware_state_dict.py:245-274 is the
  * reference's unmeasured D2H). */
 int ec_stage_last_stats(ec_stage_stats* out);
+
+/* ---- operators of a training step around the saves -------------------- */
+
+/* What a training loop computes between two saves on the tensors the engine
+ * protects: the rows of the embedding table and their gradient, the loss over
+ * the vocabulary and its gradient, and the norm of the gradient list, whose
+ * finiteness says whether the step, and a snapshot of it, is sound.
+ *
+ * Common rules.  `type` is EC_F32, EC_BF16 or EC_F16.  Arithmetic is in fp32
+ * (sums of squares in fp64) and a result is rounded once, where it is stored.
+ * Addresses need only the alignment of their elements; rows whose starts are
+ * 16-byte aligned run fastest.  Row strides are in elements; the elements of
+ * a row are adjacent.  Results do not depend on the launch or the order of
+ * workgroups: the same inputs give the same bits.  EC_EINVAL for an unknown
+ * type, a null pointer to memory that would be touched, a stride below the row
+ * or a factor that is not finite. */
+
+/* out[i] = scale * table[tokens[i] - vocab_start] for n tokens of
+ * token_bytes 4 or 8 (signed); a token outside [vocab_start, vocab_start +
+ * vocab) gives a row of zeros, as a rank that holds a slice of the vocabulary
+ * adds nothing for the tokens of others.  out is [n, hidden], contiguous.
+ * EC_ERANGE for n >= 2^31 or hidden > 2^20. */
+int ec_embed(const void* d_tokens, int token_bytes, uint64_t n, const void* d_table, int type,
+             uint64_t vocab, uint32_t hidden, uint64_t table_stride, int64_t vocab_start,
+             float scale, void* d_out, ec_stream_t stream);
+
+/* Device memory ec_embed_grad needs at d_work, in bytes. */
+uint64_t ec_embed_grad_workspace(uint64_t n, uint64_t vocab, uint32_t hidden);
+
+/* grad[v] = scale * SUM over i with tokens[i] - vocab_start = v of dout[i], the
+ * positions added in ascending order of a fixed grouping; tokens outside the slice add nothing.
+ * dout is [n, hidden] of `type`, rows dout_stride apart; grad is [vocab,
+ * hidden] of `grad_type` (EC_F32 or `type`), rows grad_stride apart.
+ * accumulate 0: every row is written, zeros for a token that does not occur;
+ * 1: the sums are added to grad, and rows of tokens that do not occur are not
+ * touched.  The tokens are sorted in d_work (work_bytes of at least
+ * ec_embed_grad_workspace, EC_EINVAL otherwise; 16-byte aligned, EC_EALIGN),
+ * equal tokens in the order of their positions; no atomics.  EC_ERANGE for
+ * n >= 2^31, vocab >= 2^31 or hidden > 2^20. */
+int ec_embed_grad(const void* d_tokens, int token_bytes, uint64_t n, const void* d_dout, int type,
+                  uint64_t dout_stride, uint64_t vocab, uint32_t hidden, int64_t vocab_start,
+                  float scale, void* d_grad, int grad_type, uint64_t grad_stride, int accumulate,
+                  void* d_work, uint64_t work_bytes, ec_stream_t stream);
+
+/* For each row x of the [rows, vocab] logits, with z = scale * x (scale > 0)
+ * and lse = log SUM exp z:
+ *   d_logprobs[i]      z[target] - lse; 0 where the target lies outside
+ *                      [0, vocab) (a position without a loss)
+ *   d_lse[i]           lse
+ *   d_entropy[i]       -SUM p log p, p = exp(z - lse); null: not computed
+ *   d_top_logprobs[i * top + r], d_top_tokens[...]   the r-th largest z - lse
+ *                      and its index, equal ones by ascending index; top 0:
+ *                      none, at most EC_MAX_TOP (EC_ERANGE) and vocab
+ *                      (EC_EINVAL)
+ * fp32 outputs, 64-bit signed targets and indices.  -infinity is a masked
+ * logit: probability 0.  A row of nothing else has lse and log-probabilities of
+ * -infinity and entropy 0.  A row with a NaN or +infinity has NaN in lse,
+ * log-probabilities and entropy; its indices order NaN last.  One pass over
+ * the logits.  EC_ERANGE for rows or vocab >= 2^31. */
+int ec_token_logprobs(const void* d_logits, int type, uint64_t rows, uint64_t vocab,
+                      uint64_t row_stride, const int64_t* d_targets, float scale,
+                      float* d_logprobs, float* d_lse, float* d_entropy, int top,
+                      float* d_top_logprobs, int64_t* d_top_tokens, ec_stream_t stream);
+
+/* The gradient of ec_token_logprobs' log-probabilities and entropies:
+ *   dlogits[j] = scale * (g * (j == target) - p[j] * (g + h * (log p[j] + H)))
+ * with g = d_dlogprobs[i] (taken as 0 where the target lies outside [0, vocab)),
+ * h = d_dentropy[i] and H = d_entropy[i] (both null: h = 0) and p from d_lse.
+ * dlogits is of the logits' type, rows out_stride apart, and may be the logits
+ * themselves.  A masked logit's gradient is 0, and so is the whole row's where
+ * lse is -infinity or below -2^127 / log2 e (a row of nothing but masked logits, the
+ * type's lowest value as a mask included). */
+int ec_token_logprobs_grad(const void* d_logits, int type, uint64_t rows, uint64_t vocab,
+                           uint64_t row_stride, const int64_t* d_targets, const float* d_lse,
+                           const float* d_dlogprobs, const float* d_entropy,
+                           const float* d_dentropy, float scale, void* d_dlogits,
+                           uint64_t out_stride, ec_stream_t stream);
+
+/* A piece of a gradient tensor: n consecutive elements of src_type at src, and
+ * where ec_grad_clip writes them, as dst_type (dst may be src; ec_grad_norm
+ * reads neither dst nor dst_type).  At most EC_GRAD_PIECE elements: a tensor of
+ * more is several pieces. */
+typedef struct {
+  uint64_t src;
+  uint64_t dst;
+  uint32_t n;
+  uint16_t src_type;
+  uint16_t dst_type;
+} ec_grad_item;
+#define EC_GRAD_PIECE 16384
+
+/* Device memory that ec_grad_norm and ec_grad_clip need at d_work, 8-byte
+ * aligned, in bytes; a call uses it until its work has run. */
+#define EC_GRAD_WORK 8192
+
+/* *d_norm = the norm of grad_scale * g over all elements g of n_items pieces
+ * (d_items is a device array), in fp32: the square root of the sum of squares,
+ * taken in fp64, or the largest magnitude.  A NaN or infinity among the
+ * elements makes the norm NaN or infinity.  n_items 0: 0. */
+int ec_grad_norm(const ec_grad_item* d_items, uint32_t n_items, float grad_scale, int norm,
+                 void* d_work, float* d_norm, ec_stream_t stream);
+
+/* dst = src * grad_scale * min(1, max_norm / (norm + 1e-6)) for every element,
+ * and *d_norm = norm: that of ec_grad_norm, or *d_given where d_given is not
+ * null (a norm already reduced over ranks).  Where the norm is not finite the
+ * elements are scaled by grad_scale alone: the caller sees the norm and skips
+ * the step.  Where the factor is 1 and a piece's dst is its src it is left as
+ * it is.  max_norm > 0. */
+int ec_grad_clip(const ec_grad_item* d_items, uint32_t n_items, float grad_scale, int norm,
+                 float max_norm, const float* d_given, void* d_work, float* d_norm,
+                 ec_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -13,18 +13,24 @@ Modules:
            and the drop-in entry points encode / decode / update
   checkpoint  ECLocalCheckpointManager + ErasureCodedStrategy (the repl_strategy slot)
   args     --non-persistent-ckpt-type in_memory: flags, validation, checkpointing context
+  step     operators of the training step around the saves: embedding lookup and its gradient,
+           log probabilities over the vocabulary and their gradient, gradient norm and clipping
 """
 from . import _lib
 from ._lib import ECError, ECLibraryMissing, SingularError
 from .codec import (ShardPlan, cauchy_matrix, decode_matrix, gf_inv, gf_invert, gf_mul, matvec,
                     reconstruct, rs_encode, side_stream, xor_encode)
 from .layout import ParitySet, StripeLayout, decode, encode, update
+from .step import (GradList, TokenLogprobs, clip_grads, embed, embed_grad, grad_norm, token_logprobs,
+                   token_logprobs_grad)
 
 __all__ = [
     "ECError", "ECLibraryMissing", "SingularError", "ShardPlan", "cauchy_matrix", "decode_matrix",
     "gf_inv", "gf_invert", "gf_mul", "matvec", "reconstruct", "rs_encode", "side_stream",
     "xor_encode",
     "StripeLayout", "ParitySet", "encode", "decode", "update",
+    "GradList", "TokenLogprobs", "clip_grads", "embed", "embed_grad", "grad_norm", "token_logprobs",
+    "token_logprobs_grad",
 ]
 
 

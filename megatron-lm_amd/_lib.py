@@ -13,7 +13,7 @@ import threading
 
 LIB_NAME = "libec_mi355.so"
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
-ABI_VERSION = 3
+ABI_VERSION = 4
 
 EC_OK = 0
 EC_EINVAL = -1
@@ -46,6 +46,13 @@ EXPORTS = (
     "ec_stage_stripes_to_host",
     "ec_stage_to_device",
     "ec_stage_last_stats",
+    "ec_embed",
+    "ec_embed_grad_workspace",
+    "ec_embed_grad",
+    "ec_token_logprobs",
+    "ec_token_logprobs_grad",
+    "ec_grad_norm",
+    "ec_grad_clip",
 )
 
 
@@ -89,6 +96,8 @@ _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _u32 = ctypes.c_uint32
 _u64 = ctypes.c_uint64
+_i64 = ctypes.c_int64
+_f = ctypes.c_float
 
 
 def lib() -> ctypes.CDLL:
@@ -144,6 +153,23 @@ def lib() -> ctypes.CDLL:
     L.ec_stage_to_device.argtypes = [_vp, _u32, _u64, _vp, _u64, _vp, _u64, _i, _vp]
     L.ec_stage_last_stats.restype = _i
     L.ec_stage_last_stats.argtypes = [ctypes.POINTER(StageStats)]
+    L.ec_embed.restype = _i
+    L.ec_embed.argtypes = [_vp, _i, _u64, _vp, _i, _u64, _u32, _u64, _i64, _f, _vp, _vp]
+    L.ec_embed_grad_workspace.restype = _u64
+    L.ec_embed_grad_workspace.argtypes = [_u64, _u64, _u32]
+    L.ec_embed_grad.restype = _i
+    L.ec_embed_grad.argtypes = [_vp, _i, _u64, _vp, _i, _u64, _u64, _u32, _i64, _f, _vp, _i, _u64,
+                                _i, _vp, _u64, _vp]
+    L.ec_token_logprobs.restype = _i
+    L.ec_token_logprobs.argtypes = [_vp, _i, _u64, _u64, _u64, _vp, _f, _vp, _vp, _vp, _i, _vp, _vp,
+                                    _vp]
+    L.ec_token_logprobs_grad.restype = _i
+    L.ec_token_logprobs_grad.argtypes = [_vp, _i, _u64, _u64, _u64, _vp, _vp, _vp, _vp, _vp, _f, _vp,
+                                         _u64, _vp]
+    L.ec_grad_norm.restype = _i
+    L.ec_grad_norm.argtypes = [_vp, _u32, _f, _i, _vp, _vp, _vp]
+    L.ec_grad_clip.restype = _i
+    L.ec_grad_clip.argtypes = [_vp, _u32, _f, _i, _f, _vp, _vp, _vp, _vp]
     _lib = L
     return L
 

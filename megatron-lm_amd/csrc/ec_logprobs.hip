@@ -1,0 +1,453 @@
+// ec_logprobs.hip — ec_token_logprobs and ec_token_logprobs_grad: log
+// probabilities of given tokens over rows of logits, with the entropy and the
+// likeliest tokens, and their gradient.
+//
+// Everything is in base 2: with c = scale * log2 e, logit x has exponent x * c and
+// a row's reference is mc = (its largest logit) * c, rounded once.  Every term is
+// 2^fma(x, c, -mc) and the results are taken relative to the same mc,
+//   s = SUM 2^d,  d = x c - mc,    lse = (mc + log2 s) ln 2,
+//   log p = (d - log2 s) ln 2,     H = (log2 s - (SUM 2^d d) / s) ln 2,
+// so the rounding of mc cancels in log p and H.  x c leaves fp32's range where x
+// does not (a mask of the type's lowest value): rows that this touches, and rows
+// with a NaN or infinity, are gone over once more with d = (x - m) c.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "ec_types.h"
+
+namespace ec {
+namespace {
+
+constexpr int kLanes = 64;
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.693147180559945309417f;
+constexpr float kInf = __builtin_inff();
+constexpr float kMax = 3.402823466e38f;
+
+__device__ __forceinline__ float exp2_hw(float v) { return __builtin_amdgcn_exp2f(v); }
+__device__ __forceinline__ float log2_hw(float v) { return __builtin_amdgcn_logf(v); }
+
+// Group g of a row of `vocab` logits, -infinity past its end.
+template <typename T, bool STREAM>
+__device__ __forceinline__ typename Group<T>::vec load_logits(const T* row, uint32_t g,
+                                                              uint32_t vocab) {
+  typedef Group<T> G;
+  const uint32_t j = g * G::kN;
+  if (j + G::kN <= vocab) return load_group<T, STREAM>(row + j);
+  typename G::vec v;
+#pragma unroll
+  for (int e = 0; e < G::kN; ++e) v[e] = j + e < vocab ? (T)gp(row)[j + e] : (T)-kInf;
+  return v;
+}
+
+// Logits in an order: larger values first, equal ones by index, NaN last, as
+// one 64-bit key (larger key first).  -0 counts as +0.
+__device__ __forceinline__ uint32_t order_bits(float v) {
+  if (v != v) return 0u;
+  const uint32_t b = __float_as_uint(v + 0.0f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t order_key(float v, uint32_t index) {
+  return (uint64_t)order_bits(v) << 32 | (uint32_t)~index;
+}
+
+struct LogprobArgs {
+  const void* logits;
+  const int64_t* targets;
+  float* logprobs;
+  float* lse;
+  float* entropy;
+  float* top_logprobs;
+  int64_t* top_tokens;
+  uint64_t stride;
+  uint32_t vocab, groups;   // groups of a row, the last one short
+  float scale, c;           // c = scale * log2 e
+  int top;
+};
+
+// A lane's running state over the groups it has seen: the largest logit and the
+// group where it first stood, the reference, the sum and the weighted sum.  The
+// reference moves only when a group holds a larger logit, a few times per lane,
+// so a term costs one fma, one exp2 and one add (and a max and an fma for the entropy).
+template <bool ENTROPY>
+struct Running {
+  float m = -kInf, mc = 0.0f, s = 0.0f, t = 0.0f;
+  uint32_t group;
+
+  template <int N, typename W>
+  __device__ __forceinline__ void add(const W& x, uint32_t g, float c) {
+    float top = x[0];
+#pragma unroll
+    for (int e = 1; e < N; ++e) top = fmaxf(top, x[e]);
+    if (top > m) {
+      const float to = fmaxf(top * c, -kMax);   // finite: a term below it is 0
+      if (s != 0.0f) {
+        const float by = exp2_hw(mc - to);
+        if (ENTROPY) t = by * (t - (to - mc) * s);
+        s *= by;
+      }
+      m = top;
+      mc = to;
+      group = g;
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float d = __builtin_fmaf(x[e], c, -mc);
+      const float p = exp2_hw(d);
+      s += p;
+      // -200: a masked logit's -infinity would make 0 * infinity
+      if (ENTROPY) t = __builtin_fmaf(p, fmaxf(d, -200.0f), t);
+    }
+  }
+};
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+  return v;
+}
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+
+// The sums of the workgroup's s (and t), the same in every lane.
+template <int WAVES, bool BOTH>
+__device__ __forceinline__ void block_sums(float& s, float& t, float (&red)[3][WAVES]) {
+  s = wave_sum(s);
+  if (BOTH) t = wave_sum(t);
+  if (threadIdx.x % kLanes == 0) {
+    red[1][threadIdx.x / kLanes] = s;
+    if (BOTH) red[2][threadIdx.x / kLanes] = t;
+  }
+  __syncthreads();
+  s = red[1][0];
+  if (BOTH) t = red[2][0];
+  for (int w = 1; w < WAVES; ++w) {
+    s += red[1][w];
+    if (BOTH) t += red[2][w];
+  }
+}
+
+constexpr uint32_t kCandidates = 512;
+constexpr int kAhead = 4;   // groups of a lane in flight
+
+// One workgroup of B lanes per row; lane l takes groups l, l + B, ...
+//
+// The `top` largest: any lane's largest logit that is among the `top` largest of
+// the lanes' own bounds the answer from below, so the logits that are not behind
+// the top-th largest of 64 groups of lanes (lane l of every wave) hold it.  They
+// lie in the lanes whose own largest is not behind it; those lanes' groups are
+// read again (about `top` lanes: a few percent of the row, from the caches), and
+// the few logits that pass are ranked by counting.  Where more pass than
+// kCandidates (logits that repeat with the workgroup's period) the row is
+// searched `top` times instead.
+template <typename T, int B, bool ENTROPY, bool TOP>
+__global__ void __launch_bounds__(B) logprob_kernel(const LogprobArgs a) {
+  typedef Group<T> G;
+  constexpr int kWaves = B / kLanes;
+  __shared__ float red[3][kWaves];
+  const uint32_t tid = threadIdx.x, lane = tid % kLanes, wave = tid / kLanes;
+  const uint64_t r = blockIdx.x;
+  const T* row = (const T*)a.logits + r * a.stride;
+
+  float given = 0.0f;
+  int64_t target = -1;
+  if (tid == 0) {
+    target = gp(a.targets)[r];
+    if (target >= 0 && target < (int64_t)a.vocab) given = (float)gp(row)[target];
+  }
+
+  Running<ENTROPY> run;
+  run.group = tid;
+  for (uint32_t g = tid; g < a.groups; g += B * kAhead) {
+    typename G::vec v[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (g + u * B < a.groups) v[u] = load_logits<T, false>(row, g + u * B, a.vocab);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (g + u * B < a.groups) run.template add<G::kN>(widen<T>(v[u]), g + u * B, a.c);
+  }
+
+  // the workgroup's reference, then the sums relative to it
+  const float wm = wave_max(run.m);
+  if (lane == 0) red[0][wave] = wm;
+  __syncthreads();
+  float m = red[0][0];
+  for (int w = 1; w < kWaves; ++w) m = fmaxf(m, red[0][w]);
+  const float mc = fmaxf(m * a.c, -kMax);
+  float s = 0.0f, t = 0.0f;
+  if (run.s != 0.0f) {
+    const float by = exp2_hw(run.mc - mc);
+    s = run.s * by;
+    // a lane that is far behind adds nothing; its distance may be infinite
+    if (ENTROPY) t = by == 0.0f ? 0.0f : by * (run.t - (mc - run.mc) * run.s);
+  }
+  block_sums<kWaves, ENTROPY>(s, t, red);
+  // every logit -infinity, or one of the rows that need d = (x - m) c
+  const bool empty = m == -kInf && s == 0.0f;
+  const bool again = !empty && !(s > 0.0f && s < kInf);
+  if (again) {
+    s = t = 0.0f;
+    for (uint32_t g = tid; g < a.groups; g += B) {
+      const typename G::wide x = widen<T>(load_logits<T, false>(row, g, a.vocab));
+#pragma unroll
+      for (int e = 0; e < G::kN; ++e) {
+        const float d = (x[e] - m) * a.c;
+        const float p = exp2_hw(d);
+        s += p;
+        if (ENTROPY) t = __builtin_fmaf(p, fmaxf(d, -200.0f), t);
+      }
+    }
+    __syncthreads();
+    block_sums<kWaves, ENTROPY>(s, t, red);
+  }
+  const float log2s = log2_hw(s);
+  const auto logprob = [&](float x) {
+    if (empty) return -kInf;
+    return ((again ? (x - m) * a.c : __builtin_fmaf(x, a.c, -mc)) - log2s) * kLn2;
+  };
+  if (tid == 0) {
+    gp(a.lse)[r] = empty ? -kInf : again ? m * a.scale + log2s * kLn2 : (mc + log2s) * kLn2;
+    gp(a.logprobs)[r] = target >= 0 && target < (int64_t)a.vocab ? logprob(given) : 0.0f;
+    if (ENTROPY) gp(a.entropy)[r] = empty ? 0.0f : (log2s - t / s) * kLn2;
+  }
+  if constexpr (TOP) {
+    __shared__ uint64_t keys[kCandidates > B ? kCandidates : B];
+    __shared__ uint64_t bound_shared;
+    __shared__ uint32_t lanes_list[B];
+    __shared__ uint32_t n_lanes, n_keys;
+    const uint64_t mine = tid < a.groups ? order_key(run.m, run.group) : 0;
+    keys[tid] = mine;
+    if (tid == 0) n_lanes = n_keys = 0;
+    __syncthreads();
+    if (wave == 0) {
+      uint64_t best = keys[lane];
+      for (int w = 1; w < kWaves; ++w) best = max(best, keys[w * kLanes + lane]);
+      const uint32_t hi = (uint32_t)(best >> 32), lo = (uint32_t)best;
+      int above = 0;
+      for (int o = 0; o < kLanes; ++o) {
+        const uint64_t other = (uint64_t)__builtin_amdgcn_readlane(hi, o) << 32 |
+                               (uint32_t)__builtin_amdgcn_readlane(lo, o);
+        above += other > best;
+      }
+      // the key with top - 1 above it; none where fewer than `top` lanes have a
+      // group (those without one have key 0): the bound is 0, all logits pass
+      const uint64_t last = __ballot(above == a.top - 1);
+      const int src = last ? __builtin_ctzll(last) : -1;
+      uint64_t bound = 0;
+      if (src >= 0)
+        bound = (uint64_t)__builtin_amdgcn_readlane(hi, src) << 32 |
+                (uint32_t)__builtin_amdgcn_readlane(lo, src);
+      if (lane == 0) bound_shared = bound;
+    }
+    __syncthreads();
+    const uint64_t bound = bound_shared;
+    if (mine && mine >= bound) lanes_list[atomicAdd(&n_lanes, 1u)] = tid;
+    __syncthreads();
+    const uint32_t lanes = n_lanes;
+    const uint32_t bound_value = (uint32_t)(bound >> 32), bound_group = ~(uint32_t)bound;
+    for (uint32_t l = wave; l < lanes; l += kWaves) {
+      const uint32_t first = lanes_list[l];
+      for (uint32_t g = first + lane * B; g < a.groups; g += kLanes * B) {
+        const typename G::vec v = load_logits<T, false>(row, g, a.vocab);
+#pragma unroll
+        for (int e = 0; e < G::kN; ++e) {
+          const uint32_t j = g * G::kN + e, value = order_bits((float)v[e]);
+          if (j < a.vocab && (value > bound_value || (value == bound_value && g <= bound_group))) {
+            const uint32_t at = atomicAdd(&n_keys, 1u);
+            if (at < kCandidates) keys[at] = (uint64_t)value << 32 | (uint32_t)~j;
+          }
+        }
+      }
+    }
+    __syncthreads();
+    const uint32_t n = n_keys;
+    const auto put = [&](int rank, uint32_t j) {
+      gp(a.top_tokens)[r * a.top + rank] = j;
+      gp(a.top_logprobs)[r * a.top + rank] = logprob((float)gp(row)[j]);
+    };
+    if (n <= kCandidates && n >= (uint32_t)a.top) {
+      for (uint32_t i = tid; i < n; i += B) {
+        const uint64_t key = keys[i];
+        int above = 0;
+        for (uint32_t o = 0; o < n; ++o) above += keys[o] > key;
+        if (above < a.top) put(above, ~(uint32_t)key);
+      }
+    } else {
+      uint64_t before = ~0ull;
+      for (int k = 0; k < a.top; ++k) {
+        uint64_t best = 0;
+        for (uint32_t g = tid; g < a.groups; g += B) {
+          const typename G::vec v = load_logits<T, false>(row, g, a.vocab);
+#pragma unroll
+          for (int e = 0; e < G::kN; ++e) {
+            const uint32_t j = g * G::kN + e;
+            const uint64_t key = j < a.vocab ? order_key((float)v[e], j) : 0;
+            if (key < before) best = max(best, key);
+          }
+        }
+        __syncthreads();
+        keys[tid] = best;
+        __syncthreads();
+        for (int o = B / 2; o; o >>= 1) {
+          if (tid < (uint32_t)o) keys[tid] = max(keys[tid], keys[tid + o]);
+          __syncthreads();
+        }
+        before = keys[0];
+        if (tid == 0) put(k, ~(uint32_t)before);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- gradient --
+// dlogits = -p (A + B d) + scale g at the target, with d the base-2 exponent
+// relative to lse, A = scale (g + h H), B = scale h ln 2.
+struct GradArgs {
+  const void* logits;
+  void* out;
+  const int64_t* targets;
+  const float* lse;
+  const float* dlogprobs;
+  const float* entropy;
+  const float* dentropy;
+  uint64_t stride, out_stride;
+  uint32_t vocab, groups;
+  float c, scale;
+};
+
+constexpr int kGradLanes = 256;
+constexpr int kGradGroups = 4;   // per lane
+
+template <typename T, bool ENTROPY>
+__global__ void __launch_bounds__(kGradLanes) logprob_grad_kernel(const GradArgs a) {
+  typedef Group<T> G;
+  constexpr int N = G::kN;
+  const uint64_t r = blockIdx.x;
+  const T* row = (const T*)a.logits + r * a.stride;
+  T* out = (T*)a.out + r * a.out_stride;
+  const uint32_t g0 = blockIdx.y * (kGradLanes * kGradGroups) + threadIdx.x;
+  typename G::vec v[kGradGroups];
+#pragma unroll
+  for (int u = 0; u < kGradGroups; ++u)
+    if (g0 + u * kGradLanes < a.groups)
+      v[u] = load_logits<T, true>(row, g0 + u * kGradLanes, a.vocab);
+  const int64_t target = gp(a.targets)[r];
+  const float lse = gp(a.lse)[r];
+  // a row of masked logits only, also one masked with the type's lowest value
+  const float lse2 = lse * kLog2e;
+  const bool has = target >= 0 && target < (int64_t)a.vocab, empty = lse2 == -kInf;
+  const float g = has ? (float)gp(a.dlogprobs)[r] : 0.0f;
+  float A = a.scale * g, slope = 0.0f;
+  if (ENTROPY) {
+    const float h = gp(a.dentropy)[r];
+    A += a.scale * h * gp(a.entropy)[r];
+    slope = a.scale * h * kLn2;
+  }
+#pragma unroll
+  for (int u = 0; u < kGradGroups; ++u) {
+    const uint32_t gi = g0 + u * kGradLanes;
+    if (gi >= a.groups) continue;
+    const typename G::wide x = widen<T>(v[u]);
+    typename G::wide w;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float d = __builtin_fmaf(x[e], a.c, -lse2);
+      const float p = exp2_hw(d);
+      const float by = ENTROPY ? __builtin_fmaf(fmaxf(d, -200.0f), slope, A) : A;
+      w[e] = empty ? 0.0f : -p * by;
+    }
+    const uint32_t j = gi * N;
+    if (has && !empty && (uint32_t)target - j < (uint32_t)N) {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if ((uint32_t)target == j + e) w[e] += a.scale * g;
+    }
+    if (j + N <= a.vocab)
+      store_wide<T, true>(out + j, w);
+    else
+      for (int e = 0; e < N; ++e)
+        if (j + e < a.vocab) gp(out)[j + e] = (T)w[e];
+  }
+}
+
+int check_logits(const void* logits, int type, uint64_t rows, uint64_t vocab, uint64_t stride,
+                 const int64_t* targets, float scale) {
+  if (!known_type(type) || !(scale > 0.0f) || !std::isfinite(scale * kLog2e)) return EC_EINVAL;
+  if (rows >= (1ull << 31) || vocab >= (1ull << 31)) return EC_ERANGE;
+  if (rows && (!targets || (vocab && (!logits || stride < vocab)))) return EC_EINVAL;
+  return EC_OK;
+}
+
+}  // namespace
+}  // namespace ec
+
+using namespace ec;
+
+extern "C" {
+
+int ec_token_logprobs(const void* d_logits, int type, uint64_t rows, uint64_t vocab,
+                      uint64_t row_stride, const int64_t* d_targets, float scale,
+                      float* d_logprobs, float* d_lse, float* d_entropy, int top,
+                      float* d_top_logprobs, int64_t* d_top_tokens, ec_stream_t stream) {
+  if (const int st = check_logits(d_logits, type, rows, vocab, row_stride, d_targets, scale))
+    return st;
+  if (top < 0 || (uint64_t)top > vocab) return EC_EINVAL;
+  if (top > EC_MAX_TOP) return EC_ERANGE;
+  if (!rows) return EC_OK;
+  if (!d_logprobs || !d_lse || (top && (!d_top_logprobs || !d_top_tokens))) return EC_EINVAL;
+  LogprobArgs a = {d_logits, d_targets, d_logprobs, d_lse, d_entropy, d_top_logprobs,
+                   d_top_tokens, row_stride, (uint32_t)vocab, 0, scale, scale * kLog2e, top};
+  const uint32_t per_group = 16 / type_bytes(type);
+  a.groups = (uint32_t)((vocab + per_group - 1) / per_group);
+  const hipStream_t st = (hipStream_t)stream;
+  return with_type(type, [&](auto t) {
+    typedef decltype(t) T;
+    const dim3 grid((uint32_t)rows);
+    if (d_entropy) {
+      if (top) logprob_kernel<T, 256, true, true><<<grid, 256, 0, st>>>(a);
+      else logprob_kernel<T, 256, true, false><<<grid, 256, 0, st>>>(a);
+    } else {
+      if (top) logprob_kernel<T, 256, false, true><<<grid, 256, 0, st>>>(a);
+      else logprob_kernel<T, 256, false, false><<<grid, 256, 0, st>>>(a);
+    }
+    return launched();
+  });
+}
+
+int ec_token_logprobs_grad(const void* d_logits, int type, uint64_t rows, uint64_t vocab,
+                           uint64_t row_stride, const int64_t* d_targets, const float* d_lse,
+                           const float* d_dlogprobs, const float* d_entropy,
+                           const float* d_dentropy, float scale, void* d_dlogits,
+                           uint64_t out_stride, ec_stream_t stream) {
+  if (const int st = check_logits(d_logits, type, rows, vocab, row_stride, d_targets, scale))
+    return st;
+  if (!rows || !vocab) return EC_OK;
+  if (!d_lse || !d_dlogprobs || !d_dlogits || out_stride < vocab) return EC_EINVAL;
+  if (!d_entropy != !d_dentropy) return EC_EINVAL;
+  GradArgs a = {d_logits, d_dlogits, d_targets, d_lse, d_dlogprobs, d_entropy, d_dentropy,
+                row_stride, out_stride, (uint32_t)vocab, 0, scale * kLog2e, scale};
+  const uint32_t per_group = 16 / type_bytes(type);
+  a.groups = (uint32_t)((vocab + per_group - 1) / per_group);
+  const uint32_t per_block = kGradLanes * kGradGroups;
+  const uint32_t slabs = (a.groups + per_block - 1) / per_block;
+  if (slabs > 65535) return EC_ERANGE;
+  const dim3 grid((uint32_t)rows, slabs);
+  const hipStream_t st = (hipStream_t)stream;
+  return with_type(type, [&](auto t) {
+    typedef decltype(t) T;
+    if (d_dentropy)
+      logprob_grad_kernel<T, true><<<grid, kGradLanes, 0, st>>>(a);
+    else
+      logprob_grad_kernel<T, false><<<grid, kGradLanes, 0, st>>>(a);
+    return launched();
+  });
+}
+
+}  // extern "C"

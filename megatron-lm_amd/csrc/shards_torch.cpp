@@ -146,8 +146,11 @@ int64_t current_stream(int64_t device) {
 
 }  // namespace
 
+void bind_step(py::module_& mod);   // step_torch.cpp
+
 PYBIND11_MODULE(_ec_shards, mod) {
-  mod.doc() = "torch-tensor binding of the flat-shard calls of libec_mi355.so";
+  mod.doc() = "torch-tensor binding of the flat-shard and training-step calls of libec_mi355.so";
+  bind_step(mod);
   mod.attr("XOR") = static_cast<int64_t>(kXor);
   mod.attr("ENCODE") = static_cast<int64_t>(kEncode);
   mod.attr("DECODE") = static_cast<int64_t>(kDecode);
