@@ -78,155 +78,346 @@ __global__ void __launch_bounds__(kEmbedWaves * kLanes) embed_kernel(const Embed
   }
 }
 
+// ------------------------------------------------------------------- zeros --
+// The rows of tokens that do not occur, which the gradient has most of, need no
+// sorted tokens: workgroups that write zeros ride along in the sort's launches, which
+// leave the memory idle, and in the sums' launch.  Each takes 64 rows and learns which of
+// them occur from bits that the sort's first launch collected (one bit per row and tile of
+// tokens), or, for few tokens, from the tokens themselves.
+enum ZeroMode : int { kZeroSeen, kZeroScan, kZeroAll };
+
+struct Tokens {
+  const void* tokens;
+  int64_t start;
+  uint64_t vocab;
+  uint32_t n;
+  int bytes;
+
+  __device__ __forceinline__ int64_t row(uint32_t i) const {
+    return row_of(tokens, bytes, i, start, vocab);
+  }
+};
+
+struct ZeroArgs {
+  uint8_t* grad;
+  const uint32_t* seen;      // [tiles][words]
+  uint64_t stride;           // of the rows, in bytes
+  uint32_t row_bytes, words, tiles;
+  uint32_t first, blocks;    // 64-row blocks of this launch
+  int mode;
+};
+
+constexpr uint32_t kZeroRows = 64;
+
+// One row of zeros: 16 bytes at a time at aligned addresses, elements at the ends.
+__device__ __forceinline__ void zero_row(uint8_t* row, uint32_t bytes) {
+  const uint32_t lane = threadIdx.x % kLanes;
+  const uint32_t lead = min(bytes, (uint32_t)(-(uintptr_t)row % 16));
+  const uint32_t chunks = (bytes - lead) / 16, behind = lead + chunks * 16;
+  typedef uint32_t __attribute__((ext_vector_type(4))) u32x4;
+  const u32x4 zero = {};
+  if (lane * 2 < lead) *gp((uint16_t*)(row + lane * 2)) = 0;
+  if (behind + lane * 2 < bytes) *gp((uint16_t*)(row + behind + lane * 2)) = 0;
+  for (uint32_t g = lane; g < chunks; g += kLanes)
+    __builtin_nontemporal_store(zero, (global<u32x4>*)(uintptr_t)(row + lead + g * 16));
+}
+
+// By a whole workgroup of WAVES waves.
+template <int WAVES>
+__device__ __forceinline__ void zero_block(const ZeroArgs& z, const Tokens& tok, uint32_t block) {
+  const uint32_t lane = threadIdx.x % kLanes;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
+  const uint64_t first = (uint64_t)(z.first + block) * kZeroRows;
+  uint64_t occur = 0;
+  if (z.mode == kZeroSeen) {
+    uint32_t lo = 0, hi = 0;
+    const uint32_t w = (uint32_t)(first / 32);
+    for (uint32_t t = lane; t < z.tiles; t += kLanes) {
+      const uint32_t* at = z.seen + (uint64_t)t * z.words + w;
+      lo |= gp(at)[0];
+      if (w + 1 < z.words) hi |= gp(at)[1];
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) {
+      lo |= __shfl_xor(lo, o);
+      hi |= __shfl_xor(hi, o);
+    }
+    occur = (uint64_t)__builtin_amdgcn_readfirstlane(hi) << 32 |
+            (uint32_t)__builtin_amdgcn_readfirstlane(lo);
+  } else if (z.mode == kZeroScan) {
+    __shared__ uint64_t found[WAVES];
+    uint64_t mine = 0;
+    for (uint32_t i = threadIdx.x; i < tok.n; i += WAVES * kLanes * 8) {
+      int64_t row[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const uint32_t j = i + u * WAVES * kLanes;
+        row[u] = j < tok.n ? tok.row(j) : -1;
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const uint64_t r = (uint64_t)row[u] - first;
+        mine |= row[u] >= 0 && r < kZeroRows ? 1ull << r : 0ull;
+      }
+    }
+    uint32_t lo = (uint32_t)mine, hi = (uint32_t)(mine >> 32);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) {
+      lo |= __shfl_xor(lo, o);
+      hi |= __shfl_xor(hi, o);
+    }
+    if (lane == 0) found[wave] = (uint64_t)hi << 32 | lo;
+    __syncthreads();
+    for (int w = 0; w < WAVES; ++w) occur |= found[w];
+  }
+  for (uint32_t r = wave; r < kZeroRows && first + r < tok.vocab; r += WAVES)
+    if (!((occur >> r) & 1u)) zero_row(z.grad + (first + r) * z.stride, z.row_bytes);
+}
+
 // -------------------------------------------------------------------- sort --
 // The tokens' rows in ascending order, equal ones by position, as (row,
-// position) pairs: a least-significant-digit radix sort in digits of at most 10
-// bits (two of 8 for a vocabulary of 50304).  Tokens outside the slice sort as row
-// `vocab`, behind all others.  A pass is two launches: each workgroup counts
-// the digits of its tile; then each sums the counts of the tiles before its own
-// (and of the smaller digits) and scatters its tile.  The place of an item
-// within its tile is its rank among the wave's items of the same digit (ballots
-// find the equal lanes) plus the counts of the waves before it, so the order is
-// the input's and no atomic decides it.
-constexpr int kSortLanes = 256;
-constexpr int kSortWaves = kSortLanes / kLanes;
-constexpr int kSortSteps = 16;                       // items per lane
-constexpr uint32_t kSortTile = kSortLanes * kSortSteps;
-constexpr int kMaxDigit = 10;
-
+// position) pairs: a least-significant-digit radix sort.  Tokens outside the
+// slice sort as row `vocab`, behind all others.  The place of an item among those of its
+// digit is its rank among the wave's items of the same digit (ballots find the
+// equal lanes) plus the counts of the waves before it, so the order is the
+// input's and no atomic decides it.
 struct SortArgs {
-  const void* tokens;      // the first pass's input (null: the pairs)
-  const uint32_t* keys;
+  Tokens tok;
+  const uint32_t* keys;    // the pairs (null: the first pass, over the tokens)
   const uint32_t* pos;
   uint32_t* keys_out;
   uint32_t* pos_out;
   uint32_t* counts;        // [tiles][2^bits]
-  int64_t start;
-  uint64_t vocab;
-  uint32_t n, tiles;
-  int token_bytes, shift, bits;
+  uint32_t* seen;          // the first pass: [tiles][words], a bit for each row that occurs
+  ZeroArgs zero;
+  uint32_t n, tiles, words;
+  int shift, bits, passes;
 };
 
 __device__ __forceinline__ uint32_t sort_key(const SortArgs& a, uint32_t i) {
-  if (!a.tokens) return gp(a.keys)[i];
-  const int64_t row = row_of(a.tokens, a.token_bytes, i, a.start, a.vocab);
-  return row < 0 ? (uint32_t)a.vocab : (uint32_t)row;
+  if (a.keys) return gp(a.keys)[i];
+  const int64_t row = a.tok.row(i);
+  return row < 0 ? (uint32_t)a.tok.vocab : (uint32_t)row;
 }
+
+// The rank of this lane's item among those of its digit that the wave has seen;
+// `count` holds the wave's counts and takes this step's.  !in: no item.
+__device__ __forceinline__ uint32_t rank_in_wave(uint32_t* count, uint32_t digit, int bits, bool in) {
+  uint64_t same = __ballot(in);
+  for (int b = 0; b < bits; ++b) {
+    const bool one = (digit >> b) & 1u;
+    const uint64_t ones = __ballot(one);
+    same &= one ? ones : ~ones;
+  }
+  const uint32_t before = __popcll(same & ((1ull << (threadIdx.x % kLanes)) - 1));
+  uint32_t seen = 0;
+  if (in) seen = count[digit];
+  // the wave's lanes have read the count before the first of them writes it,
+  // and it is written before the next step reads it: LDS operations of one wave
+  // complete in order, and the fences keep the compiler to it
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  if (in && before == 0) count[digit] = seen + (uint32_t)__popcll(same);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  return seen + before;
+}
+
+// The exclusive sum of v over the workgroup's lanes (WAVES waves).
+template <int WAVES>
+__device__ __forceinline__ uint32_t scan_block(uint32_t v, uint32_t* shared) {
+  const uint32_t lane = threadIdx.x % kLanes, wave = threadIdx.x / kLanes;
+  uint32_t sum = v;
+#pragma unroll
+  for (int o = 1; o < kLanes; o <<= 1) {
+    const uint32_t from = __shfl_up(sum, o);
+    sum += lane >= (uint32_t)o ? from : 0;
+  }
+  if (lane == kLanes - 1) shared[wave] = sum;
+  __syncthreads();
+  uint32_t before = 0;
+  for (int w = 0; w < WAVES; ++w) before += (uint32_t)w < wave ? shared[w] : 0;
+  return before + sum - v;
+}
+
+// Up to kSmallSort tokens: one workgroup holds them in LDS and runs all passes, in
+// digits of 8 bits.  One launch of 4 to 9 us instead of two for each pass.
+constexpr int kSmallLanes = 1024;
+constexpr int kSmallWaves = kSmallLanes / kLanes;
+constexpr int kSmallSteps = 8;
+constexpr uint32_t kSmallSort = kSmallLanes * kSmallSteps;
+constexpr int kSmallBits = 8;
+
+__global__ void __launch_bounds__(kSmallLanes) sort_small_kernel(const SortArgs a) {
+  __shared__ uint32_t keys[kSmallSort], pos[kSmallSort];
+  __shared__ uint32_t count[kSmallWaves][1 << kSmallBits];
+  __shared__ uint32_t sums[kSmallWaves];
+  if (blockIdx.x) return zero_block<kSmallWaves>(a.zero, a.tok, blockIdx.x - 1);
+  const uint32_t t = threadIdx.x, lane = t % kLanes, wave = t / kLanes;
+  // a wave's items are consecutive, and all waves have some
+  const uint32_t steps = (a.n + kSmallLanes - 1) / kSmallLanes;
+  const uint32_t base = wave * steps * kLanes + lane;
+  uint32_t key[kSmallSteps], at[kSmallSteps], rank[kSmallSteps];
+#pragma unroll
+  for (int s = 0; s < kSmallSteps; ++s) {
+    const uint32_t i = base + s * kLanes;
+    at[s] = i;
+    key[s] = (uint32_t)s < steps && i < a.n ? sort_key(a, i) : 0;
+  }
+  for (int p = 0; p < a.passes; ++p) {
+    const int shift = p * kSmallBits;
+    for (uint32_t b = t; b < kSmallWaves << kSmallBits; b += kSmallLanes) (&count[0][0])[b] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < kSmallSteps; ++s)
+      if ((uint32_t)s < steps)
+        rank[s] = rank_in_wave(count[wave], (key[s] >> shift) & ((1u << kSmallBits) - 1), kSmallBits,
+                               base + s * kLanes < a.n);
+    __syncthreads();
+    uint32_t all = 0;
+    if (t < 1u << kSmallBits)
+      for (int w = 0; w < kSmallWaves; ++w) all += count[w][t];
+    uint32_t begin = scan_block<kSmallWaves>(all, sums);
+    if (t < 1u << kSmallBits)
+      for (int w = 0; w < kSmallWaves; ++w) {
+        const uint32_t c = count[w][t];
+        count[w][t] = begin;
+        begin += c;
+      }
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < kSmallSteps; ++s)
+      if ((uint32_t)s < steps && base + s * kLanes < a.n) {
+        const uint32_t to = count[wave][(key[s] >> shift) & ((1u << kSmallBits) - 1)] + rank[s];
+        keys[to] = key[s];
+        pos[to] = at[s];
+      }
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < kSmallSteps; ++s)
+      if ((uint32_t)s < steps && base + s * kLanes < a.n) {
+        key[s] = keys[base + s * kLanes];
+        at[s] = pos[base + s * kLanes];
+      }
+  }
+#pragma unroll
+  for (int s = 0; s < kSmallSteps; ++s)
+    if ((uint32_t)s < steps && base + s * kLanes < a.n) {
+      gp(a.keys_out)[base + s * kLanes] = key[s];
+      gp(a.pos_out)[base + s * kLanes] = at[s];
+    }
+}
+
+// More tokens: digits of at most 9 bits (two of 8 for a vocabulary of 50304, two of 9
+// up to 2^18), a pass of two launches.  Each workgroup counts the digits of its
+// tile; then each sums the counts of the tiles before its own (and of the smaller
+// digits) and scatters its tile.
+constexpr int kSortLanes = 512;
+constexpr int kSortWaves = kSortLanes / kLanes;
+constexpr int kSortSteps = 4;                        // items per lane
+constexpr uint32_t kSortTile = kSortLanes * kSortSteps;
+constexpr int kMaxDigit = 9;                         // a lane for each value
+constexpr uint32_t kCountsAhead = 32;
 
 __global__ void __launch_bounds__(kSortLanes) sort_count_kernel(const SortArgs a) {
   __shared__ uint32_t count[1 << kMaxDigit];
-  const uint32_t bins = 1u << a.bits;
-  for (uint32_t b = threadIdx.x; b < bins; b += kSortLanes) count[b] = 0;
+  extern __shared__ uint32_t seen[];   // the first pass: `words` of them
+  if (blockIdx.x >= a.tiles)
+    return zero_block<kSortWaves>(a.zero, a.tok, blockIdx.x - a.tiles);
+  const uint32_t bins = 1u << a.bits, t = threadIdx.x;
+  const uint32_t words = a.seen ? a.words : 0;
+  count[t] = 0;
+  for (uint32_t w = t; w < words; w += kSortLanes) seen[w] = 0;
   __syncthreads();
   const uint32_t base = blockIdx.x * kSortTile;
+  uint32_t key[kSortSteps];
 #pragma unroll
   for (int s = 0; s < kSortSteps; ++s) {
-    const uint32_t i = base + s * kSortLanes + threadIdx.x;
-    if (i < a.n) atomicAdd(&count[(sort_key(a, i) >> a.shift) & (bins - 1)], 1u);
+    const uint32_t i = base + s * kSortLanes + t;
+    key[s] = i < a.n ? sort_key(a, i) : 0;
   }
+#pragma unroll
+  for (int s = 0; s < kSortSteps; ++s)
+    if (base + s * kSortLanes + t < a.n) {
+      atomicAdd(&count[(key[s] >> a.shift) & (bins - 1)], 1u);
+      if (words && key[s] < (uint32_t)a.tok.vocab) atomicOr(&seen[key[s] / 32], 1u << (key[s] % 32));
+    }
   __syncthreads();
-  for (uint32_t b = threadIdx.x; b < bins; b += kSortLanes)
-    gp(a.counts)[(uint64_t)blockIdx.x * bins + b] = count[b];
+  if (t < bins) gp(a.counts)[(uint64_t)blockIdx.x * bins + t] = count[t];
+  for (uint32_t w = t; w < words; w += kSortLanes)
+    gp(a.seen)[(uint64_t)blockIdx.x * words + w] = seen[w];
 }
 
 __global__ void __launch_bounds__(kSortLanes) sort_scatter_kernel(const SortArgs a) {
   __shared__ uint32_t count[kSortWaves][1 << kMaxDigit];
-  __shared__ uint32_t total[kSortLanes];
+  __shared__ uint32_t sums[kSortWaves];
+  if (blockIdx.x >= a.tiles)
+    return zero_block<kSortWaves>(a.zero, a.tok, blockIdx.x - a.tiles);
   const uint32_t bins = 1u << a.bits, t = threadIdx.x, lane = t % kLanes, wave = t / kLanes;
-  for (uint32_t b = t; b < kSortWaves * bins; b += kSortLanes) count[b >> a.bits][b & (bins - 1)] = 0;
-  __syncthreads();
-
-  // ranks within the wave; the wave's items are 64 consecutive ones per step
+  // the wave's items: 64 consecutive ones per step; all loads are issued up front
   const uint32_t base = blockIdx.x * kSortTile + wave * (kLanes * kSortSteps) + lane;
-  uint32_t key[kSortSteps], rank[kSortSteps];
+  uint32_t key[kSortSteps], at[kSortSteps], rank[kSortSteps];
 #pragma unroll
   for (int s = 0; s < kSortSteps; ++s) {
     const uint32_t i = base + s * kLanes;
-    key[s] = i < a.n ? sort_key(a, i) : 0xffffffffu;
+    key[s] = i < a.n ? sort_key(a, i) : 0;
+    at[s] = !a.keys || i >= a.n ? i : gp(a.pos)[i];
   }
+  // lane t owns digit t: how many of it lie in the tiles before this one, and in all
+  uint32_t here = 0, all = 0;
+  if (t < bins) {
+    const global<uint32_t>* c = gp((const uint32_t*)a.counts) + t;
+    for (uint32_t b = 0; b < a.tiles; b += kCountsAhead) {
+      uint32_t v[kCountsAhead];
 #pragma unroll
-  for (int s = 0; s < kSortSteps; ++s) {
-    const bool in = base + s * kLanes < a.n;
-    const uint32_t digit = (key[s] >> a.shift) & (bins - 1);
-    uint64_t same = __ballot(in);
-    for (int b = 0; b < a.bits; ++b) {
-      const uint64_t ones = __ballot((digit >> b) & 1u);
-      same &= (digit >> b) & 1u ? ones : ~ones;
+      for (uint32_t u = 0; u < kCountsAhead; ++u)
+        v[u] = b + u < a.tiles ? c[(uint64_t)(b + u) * bins] : 0;
+#pragma unroll
+      for (uint32_t u = 0; u < kCountsAhead; ++u) {
+        here += b + u < blockIdx.x ? v[u] : 0;
+        all += v[u];
+      }
     }
-    const uint32_t before = __popcll(same & ((1ull << lane) - 1));
-    uint32_t seen = 0;
-    if (in) seen = count[wave][digit];
-    rank[s] = seen + before;
-    // the wave's lanes have read the count before the first of them writes it,
-    // and it is written before the next step reads it: LDS operations of one wave
-    // complete in order, and the fences keep the compiler to it
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    if (in && before == 0) count[wave][digit] = seen + (uint32_t)__popcll(same);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
   }
+  for (int w = 0; w < kSortWaves; ++w) count[w][t] = 0;
   __syncthreads();
-
-  // where each digit of this tile begins: lane t owns the digits [t * per, ...)
-  const uint32_t per = (bins + kSortLanes - 1) / kSortLanes, d0 = t * per;
-  uint32_t mine = 0, here[(1 << kMaxDigit) / kSortLanes], all[(1 << kMaxDigit) / kSortLanes];
 #pragma unroll
-  for (uint32_t j = 0; j < (1 << kMaxDigit) / kSortLanes; ++j) {
-    here[j] = all[j] = 0;
-    if (j >= per || d0 + j >= bins) continue;
-    uint32_t before = 0, sum = 0;
-    for (uint32_t b = 0; b < a.tiles; ++b) {
-      const uint32_t c = gp((const uint32_t*)a.counts)[(uint64_t)b * bins + d0 + j];
-      before += b < blockIdx.x ? c : 0;
-      sum += c;
-    }
-    here[j] = before;
-    all[j] = sum;
-    mine += sum;
-  }
-  total[t] = mine;
-  __syncthreads();
-  for (uint32_t o = 1; o < kSortLanes; o <<= 1) {   // inclusive scan
-    const uint32_t v = t >= o ? total[t - o] : 0;
-    __syncthreads();
-    total[t] += v;
-    __syncthreads();
-  }
-  uint32_t begin = total[t] - mine;
-#pragma unroll
-  for (uint32_t j = 0; j < (1 << kMaxDigit) / kSortLanes; ++j) {
-    if (j >= per || d0 + j >= bins) continue;
-    uint32_t at = begin + here[j];
-    for (int w = 0; w < kSortWaves; ++w) {
-      const uint32_t c = count[w][d0 + j];
-      count[w][d0 + j] = at;
-      at += c;
-    }
-    begin += all[j];
+  for (int s = 0; s < kSortSteps; ++s)
+    rank[s] = rank_in_wave(count[wave], (key[s] >> a.shift) & (bins - 1), a.bits,
+                           base + s * kLanes < a.n);
+  uint32_t next = scan_block<kSortWaves>(all, sums) + here;   // its barrier: all counts are there
+  for (int w = 0; w < kSortWaves; ++w) {
+    const uint32_t c = count[w][t];
+    count[w][t] = next;
+    next += c;
   }
   __syncthreads();
 #pragma unroll
   for (int s = 0; s < kSortSteps; ++s) {
-    const uint32_t i = base + s * kLanes;
-    if (i >= a.n) continue;
+    if (base + s * kLanes >= a.n) continue;
     const uint32_t to = count[wave][(key[s] >> a.shift) & (bins - 1)] + rank[s];
     gp(a.keys_out)[to] = key[s];
-    gp(a.pos_out)[to] = a.tokens ? i : gp(a.pos)[i];
+    gp(a.pos_out)[to] = at[s];
   }
 }
 
 // ------------------------------------------------------------ segment sums --
-// The sorted pairs in tiles of kTile, each summed by one wave for each 64
+// The sorted pairs in tiles of 16 or 32, each summed by one wave for each 64
 // groups of columns: the rows' loads in batches of kBatch, the running sum in
-// fp32 registers, put out where the row changes.  A run of equal rows that lies
-// within its tile goes to the gradient; one that begins before the tile, or
-// goes on behind it, leaves its part in `parts` (slot 0: a run from before; slot
-// 1: one that begins here), and join_kernel adds the parts of a run in order.
-// The split does not look at the run's length, so a token on a tenth of all
-// positions costs what others do.
-constexpr uint32_t kTile = 32;
-constexpr int kBatch = 8;
+// fp32 registers, put out where the row changes.  A run of equal rows belongs to
+// the tile it begins in, whose wave follows it into the next tile; only a run that
+// covers the whole next tile is split: every tile it touches leaves its part
+// in `parts`, and join_kernel adds them in order.  So a token on a tenth of all
+// positions costs what others do, and the common short runs cost no second pass.
+//
+// Tiles of 16 where there are few: more waves share the gathers' latency (tiles of 8 /
+// 16 / 32, us for the whole call: 2048 tokens of 1999 fp32 28.2 26.7 29.4; 16384 tokens, a
+// gradient of 131072 x 1024, 124.6 125.3 129.9; 32768 tokens, 50304 x 2048, 130.1 126.7 126.1;
+// 65536 of the same 155 152 147).
+constexpr uint32_t kFewTokens = 16384;
+constexpr uint32_t kMaxTile = 32;   // two tiles' pairs in the lanes of a wave
+constexpr uint32_t tile_for(uint64_t n) { return n <= kFewTokens ? kMaxTile / 2 : kMaxTile; }
+constexpr int kBatch = 16;
 constexpr int kSumWaves = 4;
 
 struct SumArgs {
@@ -234,136 +425,148 @@ struct SumArgs {
   const uint32_t* pos;
   const void* dout;
   void* grad;
-  float* parts;            // [tiles][2][hidden]
+  float* parts;            // [tiles][2][hidden]: a run from before, a run that begins here
+  Tokens tok;
+  ZeroArgs zero;
   uint64_t dout_stride, grad_stride, vocab;
-  uint32_t n, tiles, hidden, slabs, sum_blocks;
+  uint32_t n, tile, tiles, hidden, slabs, sum_blocks;
   int accumulate;
   float scale;
 };
 
-// Elements [c, c + N) of a row of `hidden`, N of them or what is left.
-template <typename T, int N>
+// Elements [c, c + N) of a row of `hidden`: N of them, or (TAIL) what is left.
+template <typename T, int N, bool TAIL>
 __device__ __forceinline__ void put_row(T* row, uint32_t c, uint32_t hidden, const float* sum,
                                         float scale, bool add) {
   typedef Group<T> G;
+  if constexpr (!TAIL) {
+    constexpr int kPut = N < G::kN ? N : G::kN;
+    typedef T __attribute__((ext_vector_type(kPut), aligned(sizeof(T)))) some;
+    typedef float __attribute__((ext_vector_type(kPut))) wide;
 #pragma unroll
-  for (int h = 0; h < N; h += G::kN) {
-    if (c + h + G::kN <= hidden) {
-      typename G::wide w;
+    for (int h = 0; h < N; h += kPut) {
+      auto* at = (global<some>*)(uintptr_t)(row + c + h);
+      wide w;
 #pragma unroll
-      for (int e = 0; e < G::kN; ++e) w[e] = sum[h + e] * scale;
-      if (add) w += widen<T>(load_group<T, false>(row + c + h));
-      store_wide<T, true>(row + c + h, w);
-    } else {
-#pragma unroll
-      for (int e = 0; e < G::kN; ++e)
-        if (c + h + e < hidden) {
-          float v = sum[h + e] * scale;
-          if (add) v += (float)gp(row)[c + h + e];
-          gp(row)[c + h + e] = (T)v;
-        }
+      for (int e = 0; e < kPut; ++e) w[e] = sum[h + e] * scale;
+      if (add) w += __builtin_convertvector(*at, wide);
+      *at = __builtin_convertvector(w, some);
     }
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (c + e < hidden) {
+        float v = sum[e] * scale;
+        if (add) v += (float)gp(row)[c + e];
+        gp(row)[c + e] = (T)v;
+      }
   }
 }
 
-// The rows of tokens that do not occur: a wave looks kZeroRows rows up among the
-// sorted keys, one per lane, and writes the zeros of those that are missing.
-constexpr uint32_t kZeroRows = 16;
-
-template <typename O>
-__device__ __forceinline__ void zero_rows(const SumArgs& a, uint64_t first) {
-  typedef Group<O> G;
-  const uint32_t lane = threadIdx.x % kLanes;
-  const uint64_t row = first + lane;
-  bool missing = false;
-  if (lane < kZeroRows && row < a.vocab) {
-    uint32_t lo = 0, hi = a.n;   // the first key >= row
-    while (lo < hi) {
-      const uint32_t mid = lo + (hi - lo) / 2;
-      if (gp(a.keys)[mid] < (uint32_t)row)
-        lo = mid + 1;
-      else
-        hi = mid;
-    }
-    missing = lo == a.n || gp(a.keys)[lo] != (uint32_t)row;
-  }
-  const uint64_t todo = __ballot(missing);
-  const typename G::wide zero = {};
-  for (uint32_t r = 0; r < kZeroRows; ++r) {
-    if (!((todo >> r) & 1u)) continue;
-    O* out = (O*)a.grad + (first + r) * a.grad_stride;
-    for (uint32_t c = lane * G::kN; c < a.hidden; c += kLanes * G::kN) {
-      if (c + G::kN <= a.hidden)
-        store_wide<O, true>(out + c, zero);
-      else
-        for (uint32_t e = c; e < a.hidden; ++e) gp(out)[e] = (O)0.0f;
-    }
-  }
-}
-
-template <typename T, typename O>
+// TAIL: the last group of a row is stored element by element.  Otherwise it starts
+// early, so that it ends with the row; its lane then writes some elements that its
+// neighbour writes too, the same values, which only a gradient that is written and not
+// added to allows.
+template <typename T, typename O, bool ADD, bool TAIL>
 __global__ void __launch_bounds__(kSumWaves * kLanes) sum_kernel(const SumArgs a) {
   typedef Group<T> G;
   constexpr int N = G::kN;
   const uint32_t lane = threadIdx.x % kLanes;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
-  if (blockIdx.x >= a.sum_blocks) {
-    zero_rows<O>(a, ((uint64_t)(blockIdx.x - a.sum_blocks) * kSumWaves + wave) * kZeroRows);
-    return;
-  }
-  const uint64_t job = (uint64_t)blockIdx.x * kSumWaves + wave;
+  // the workgroups that write zeros lie evenly between the others: the ones wait for
+  // gathered reads, the others fill the time with stores
+  const uint64_t blocks = (uint64_t)a.sum_blocks + a.zero.blocks;
+  const uint32_t zeros = (uint32_t)(blockIdx.x * (uint64_t)a.zero.blocks / blocks);
+  if ((uint32_t)((blockIdx.x + 1ull) * a.zero.blocks / blocks) != zeros)
+    return zero_block<kSumWaves>(a.zero, a.tok, zeros);
+  const uint64_t job = (uint64_t)(blockIdx.x - zeros) * kSumWaves + wave;
   const uint32_t tile = (uint32_t)(job / a.slabs), slab = (uint32_t)(job % a.slabs);
   if (tile >= a.tiles) return;
-  const uint32_t c = (slab * kLanes + lane) * N;   // this lane's columns
-  const uint32_t first = tile * kTile, len = min(kTile, a.n - first);
+  // this lane's columns; lanes behind the row read what the last one reads
+  uint32_t c = (slab * kLanes + lane) * N;
+  const bool on = c < a.hidden;
+  if (!TAIL) c = min(c, a.hidden - N);
+  const uint32_t first = tile * a.tile, len = min(a.tile, a.n - first);
 
-  // lane l holds pair l of the tile, and its neighbours' keys the tile's ends
-  uint32_t key = 0, pos = 0;
-  if (lane < len) {
+  // lane l holds pair l of this tile and the next; `prev` and `before` are the
+  // keys in front of this tile and of the one before it
+  uint32_t key = 0xffffffffu, pos = 0;
+  if (first + lane < a.n) {
     key = gp(a.keys)[first + lane];
     pos = gp(a.pos)[first + lane];
   }
   const uint32_t none = 0xffffffffu;
   const uint32_t prev = first ? gp(a.keys)[first - 1] : none;
-  const uint32_t next = first + len < a.n ? gp(a.keys)[first + len] : none;
+  const uint32_t before = first > a.tile ? gp(a.keys)[first - a.tile - 1] : none;
   const uint32_t vocab = (uint32_t)a.vocab;
+  const uint32_t head = __builtin_amdgcn_readlane(key, 0);
+  const uint32_t tail = __builtin_amdgcn_readlane(key, len - 1);
+  const uint32_t next_len = first + a.tile < a.n ? min(a.tile, a.n - first - a.tile) : 0;
+
+  // the run from before: whose is it?  The tile it begins in takes it to its end,
+  // unless it covers a whole tile behind that one (this one, or the one before)
+  uint32_t b = 0;
+  bool head_part = head == prev;
+  if (head_part && tail != head && before != head) {
+    b = __popcll(__ballot(lane < len && key == head));
+    head_part = false;
+  }
+  // the run at the end: split if it covers the next tile, else followed into it
+  bool tail_part = false;
+  uint32_t end = len;
+  if (next_len && tail < vocab) {
+    const uint32_t first_next = __builtin_amdgcn_readlane(key, a.tile);
+    const uint32_t last_next = __builtin_amdgcn_readlane(key, a.tile + next_len - 1);
+    const bool mine = !(head_part && tail == head);
+    if (mine && first_next == tail) {
+      if (last_next == tail)
+        tail_part = true;
+      else
+        end += __popcll(__ballot(lane >= a.tile && key == tail));
+    }
+  }
+  if (b >= end) return;
 
   float sum[N] = {};
-  uint32_t run = __builtin_amdgcn_readlane(key, 0);
-  bool from_before = run == prev;
-  for (uint32_t b = 0; b < len; b += kBatch) {
+  uint32_t run = __builtin_amdgcn_readlane(key, b);
+  bool part = head_part;
+  const auto put = [&](uint32_t slot) {
+    float* const at = a.parts + ((uint64_t)tile * 2 + slot) * a.hidden;
+    O* const row = (O*)a.grad + (uint64_t)run * a.grad_stride;
+    if constexpr (sizeof(O) == 4 && !ADD) {   // one place in the code for both
+      if (on) put_row<float, N, TAIL>(part ? at : row, c, a.hidden, sum, part ? 1.0f : a.scale, false);
+    } else if (part) {
+      if (on) put_row<float, N, TAIL>(at, c, a.hidden, sum, 1.0f, false);
+    } else {
+      if (on) put_row<O, N, TAIL>(row, c, a.hidden, sum, a.scale, ADD);
+    }
+  };
+  for (; b < end; b += kBatch) {
     typename G::vec v[kBatch];
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
       v[u] = {};
       const uint32_t k = __builtin_amdgcn_readlane(key, (b + u) & 63);
       const uint32_t p = __builtin_amdgcn_readlane(pos, (b + u) & 63);
-      if (b + u < len && k < vocab) {
-        const T* src = (const T*)a.dout + (uint64_t)p * a.dout_stride + c;
-        if (c + N <= a.hidden)
-          v[u] = load_group<T, true>(src);
+      if (b + u < end && k < vocab) {
+        const T* src = (const T*)a.dout + (uint64_t)p * a.dout_stride;
+        if (!TAIL || c + N <= a.hidden)
+          v[u] = load_group<T, true>(src + c);
         else
 #pragma unroll
           for (int e = 0; e < N; ++e)
-            if (c + e < a.hidden) v[u][e] = gp(src)[e];
+            if (c + e < a.hidden) v[u][e] = gp(src + c)[e];
       }
     }
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      if (b + u >= len) break;
+      if (b + u >= end) break;
       const uint32_t k = __builtin_amdgcn_readlane(key, (b + u) & 63);
-      if (k != run) {   // the run ended within the tile
-        if (run < vocab) {
-          if (from_before) {
-            float* part = a.parts + (uint64_t)tile * 2 * a.hidden;
-            put_row<float, N>(part, c, a.hidden, sum, 1.0f, false);
-          } else {
-            put_row<O, N>((O*)a.grad + (uint64_t)run * a.grad_stride, c, a.hidden, sum, a.scale,
-                          a.accumulate);
-          }
-        }
+      if (k != run) {   // the run ended
+        put(0);
+        if (k >= vocab) return;   // the tokens outside the slice are the last
         run = k;
-        from_before = false;
+        part = false;
 #pragma unroll
         for (int e = 0; e < N; ++e) sum[e] = 0.0f;
       }
@@ -373,81 +576,90 @@ __global__ void __launch_bounds__(kSumWaves * kLanes) sum_kernel(const SumArgs a
     }
   }
   if (run >= vocab) return;
-  if (from_before || run == next) {
-    float* part = a.parts + ((uint64_t)tile * 2 + (from_before ? 0 : 1)) * a.hidden;
-    put_row<float, N>(part, c, a.hidden, sum, 1.0f, false);
-  } else {
-    put_row<O, N>((O*)a.grad + (uint64_t)run * a.grad_stride, c, a.hidden, sum, a.scale,
-                  a.accumulate);
-  }
+  const uint32_t slot = part ? 0 : 1;
+  part = part || tail_part;
+  put(slot);
 }
 
-// A workgroup for each tile's last run and 256 columns, if the run begins in the
-// tile and goes on behind it: its waves share the tiles of the run, in order,
+// A workgroup for 256 columns of the runs that begin in one of kJoinTiles tiles (as its
+// last run) and cover the next one: its waves share the tiles of a run, in order,
 // and their sums are added in order.
+constexpr int kJoinTiles = 16;
 constexpr int kJoinWaves = 8;
 constexpr int kJoinBatch = 8;
 
 template <typename O>
 __global__ void __launch_bounds__(kJoinWaves * kLanes) join_kernel(const SumArgs a) {
   typedef Group<float> G;
-  const uint32_t tile = blockIdx.x, last = tile * kTile + kTile - 1;
-  if (last + 1 >= a.n) return;
-  const uint32_t run = gp(a.keys)[last];
-  if (run >= a.vocab || gp(a.keys)[last + 1] != run) return;
-  const uint32_t first = tile * kTile;
-  if (gp(a.keys)[first] == run && first && gp(a.keys)[first - 1] == run) return;
-  uint32_t lo = last + 1, hi = a.n;   // the first key > run
-  while (lo < hi) {
-    const uint32_t mid = lo + (hi - lo) / 2;
-    if (gp(a.keys)[mid] <= run)
-      lo = mid + 1;
-    else
-      hi = mid;
-  }
-  // the run's parts: slot 1 of `tile`, slot 0 of the tiles up to that of its end
-  const uint32_t parts = (lo - 1) / kTile - tile + 1;
-  const uint32_t lane = threadIdx.x % kLanes, wave = threadIdx.x / kLanes;
-  const uint32_t c = (blockIdx.y * kLanes + lane) * G::kN;
-  const uint32_t per = (parts + kJoinWaves - 1) / kJoinWaves;
-  const uint32_t from = min(parts, wave * per), to = min(parts, from + per);
-  float sum[G::kN] = {};
-  for (uint32_t p = from; p < to; p += kJoinBatch) {
-    G::vec v[kJoinBatch];
-#pragma unroll
-    for (int u = 0; u < kJoinBatch; ++u) {
-      v[u] = {};
-      if (p + u >= to) continue;
-      const uint64_t slot = (uint64_t)(tile + p + u) * 2 + (p + u == 0 ? 1 : 0);
-      const float* src = a.parts + slot * a.hidden + c;
-      if (c + G::kN <= a.hidden)
-        v[u] = load_group<float, true>(src);
-      else
-#pragma unroll
-        for (int e = 0; e < G::kN; ++e)
-          if (c + e < a.hidden) v[u][e] = gp(src)[e];
-    }
-#pragma unroll
-    for (int u = 0; u < kJoinBatch; ++u)
-#pragma unroll
-      for (int e = 0; e < G::kN; ++e) sum[e] += v[u][e];
-  }
   __shared__ float shared[kJoinWaves][kLanes][G::kN];
-#pragma unroll
-  for (int e = 0; e < G::kN; ++e) shared[wave][lane][e] = sum[e];
-  __syncthreads();
-  if (wave) return;
-  for (int w = 1; w < kJoinWaves; ++w)
-#pragma unroll
-    for (int e = 0; e < G::kN; ++e) sum[e] += shared[w][lane][e];
-  O* row = (O*)a.grad + (uint64_t)run * a.grad_stride;
-#pragma unroll
-  for (int e = 0; e < G::kN; ++e)
-    if (c + e < a.hidden) {
-      float v = sum[e] * a.scale;
-      if (a.accumulate) v += (float)gp(row)[c + e];
-      gp(row)[c + e] = (O)v;
+  const uint32_t lane = threadIdx.x % kLanes;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
+  const uint32_t c = (blockIdx.y * kLanes + lane) * G::kN;
+  const uint32_t first = blockIdx.x * kJoinTiles, mine = first + lane;
+  uint32_t key = 0;
+  bool head = false;
+  if (lane < kJoinTiles && mine + 1 < a.tiles) {
+    const uint32_t last = mine * a.tile + a.tile - 1;
+    key = gp(a.keys)[last];
+    const uint32_t next_last = gp(a.keys)[min(last + a.tile, a.n - 1)];
+    // where the key in front of the tile is the run's, it began before
+    const uint32_t prev = mine ? gp(a.keys)[mine * a.tile - 1] : 0xffffffffu;
+    head = key < a.vocab && next_last == key && prev != key;
+  }
+  uint64_t heads = __ballot(head);
+  while (heads) {
+    const uint32_t h = __builtin_ctzll(heads), tile = first + h;
+    heads &= heads - 1;
+    const uint32_t run = __builtin_amdgcn_readlane(key, h);
+    // the run's parts: slot 1 of `tile`, slot 0 of the tiles behind it that begin with it
+    uint32_t parts = 2;
+    for (;;) {
+      const uint64_t at = (uint64_t)(tile + parts + lane) * a.tile;
+      const uint64_t in = __ballot(at < a.n && gp(a.keys)[at < a.n ? at : 0] == run);
+      if (in != ~0ull) {
+        parts += __builtin_ctzll(~in);
+        break;
+      }
+      parts += kLanes;
     }
+    const uint32_t per = (parts + kJoinWaves - 1) / kJoinWaves;
+    const uint32_t from = min(parts, wave * per), to = min(parts, from + per);
+    float sum[G::kN] = {};
+    for (uint32_t p = from; p < to; p += kJoinBatch) {
+      G::vec v[kJoinBatch];
+#pragma unroll
+      for (int u = 0; u < kJoinBatch; ++u) {
+        v[u] = {};
+        if (p + u >= to) continue;
+        const uint64_t slot = (uint64_t)(tile + p + u) * 2 + (p + u == 0 ? 1 : 0);
+        const float* src = a.parts + slot * a.hidden + c;
+        if (c + G::kN <= a.hidden)
+          v[u] = load_group<float, true>(src);
+        else
+#pragma unroll
+          for (int e = 0; e < G::kN; ++e)
+            if (c + e < a.hidden) v[u][e] = gp(src)[e];
+      }
+#pragma unroll
+      for (int u = 0; u < kJoinBatch; ++u)
+#pragma unroll
+        for (int e = 0; e < G::kN; ++e) sum[e] += v[u][e];
+    }
+#pragma unroll
+    for (int e = 0; e < G::kN; ++e) shared[wave][lane][e] = sum[e];
+    __syncthreads();
+    if (wave == 0) {
+      for (int w = 1; w < kJoinWaves; ++w)
+#pragma unroll
+        for (int e = 0; e < G::kN; ++e) sum[e] += shared[w][lane][e];
+      O* const row = (O*)a.grad + (uint64_t)run * a.grad_stride;
+      if (c + G::kN <= a.hidden)
+        put_row<O, G::kN, false>(row, c, a.hidden, sum, a.scale, a.accumulate);
+      else
+        put_row<O, G::kN, true>(row, c, a.hidden, sum, a.scale, a.accumulate);
+    }
+    __syncthreads();
+  }
 }
 
 // ---------------------------------------------------------- host launchers --
@@ -460,32 +672,50 @@ int bits_of(uint64_t v) {   // of the largest key
 
 constexpr uint64_t up16(uint64_t v) { return (v + 15) / 16 * 16; }
 
+// Rows up to which the sort's first launch collects which rows occur: a bit each
+// in LDS.
+constexpr uint64_t kMaxSeen = 1u << 18;
+
 struct Work {
-  uint64_t keys[2], pos[2], counts, parts, bytes;
-  uint32_t sort_tiles, sum_tiles;
+  uint64_t keys[2], pos[2], counts, seen, parts, bytes;
+  uint32_t sort_tiles, sum_tiles, words;
   int passes, bits;
+  bool small;
 };
 
 Work work_of(uint64_t n, uint64_t vocab, uint32_t hidden) {
-  Work w;
-  const int all = bits_of(vocab);
-  w.passes = (all + kMaxDigit - 1) / kMaxDigit;
+  Work w = {};
+  w.small = n <= kSmallSort;
+  const int all = bits_of(vocab), digit = w.small ? kSmallBits : kMaxDigit;
+  w.passes = (all + digit - 1) / digit;
   w.bits = (all + w.passes - 1) / w.passes;
   w.sort_tiles = (uint32_t)((n + kSortTile - 1) / kSortTile);
-  w.sum_tiles = (uint32_t)((n + kTile - 1) / kTile);
+  w.sum_tiles = (uint32_t)((n + tile_for(n) - 1) / tile_for(n));
+  w.words = w.small || vocab > kMaxSeen ? 0 : (uint32_t)((vocab + 31) / 32);
   uint64_t at = 0;
   const auto take = [&at](uint64_t bytes) {
     const uint64_t here = at;
     at += up16(bytes);
     return here;
   };
-  for (int i = 0; i < 2; ++i) w.keys[i] = take(4 * n);
-  for (int i = 0; i < 2; ++i) w.pos[i] = take(4 * n);
-  w.counts = take(4ull * w.sort_tiles << w.bits);
+  for (int i = 0; i < (w.small ? 1 : 2); ++i) {
+    w.keys[i] = take(4 * n);
+    w.pos[i] = take(4 * n);
+  }
+  if (!w.small) w.counts = take(4ull * w.sort_tiles << w.bits);
+  w.seen = take(4ull * w.sort_tiles * w.words);
   w.parts = take(8ull * w.sum_tiles * hidden);
   w.bytes = at;
   return w;
 }
+
+// Bytes of zeros that a launch of the sort takes along at least: about what is written
+// while it waits for its own loads.  It takes more where the sums' launch would be
+// left with more zeros than it reads of dout, which is what hides behind its gathers.
+// 0 / 20 / 40 / 60 / 100 / 200 MiB a launch, us for the whole call: 65536 tokens, 50304 x
+// 2048 bf16 to fp32 165 159 153 150 153 160; 8192 tokens of the same 126 113 111 107 108 102;
+// 16384 tokens, 131072 x 1024 166 149 158 139 138 128.
+constexpr uint64_t kZeroBytes = 40u << 20;
 
 int check_tokens(const void* tokens, int token_bytes, uint64_t n, uint32_t hidden) {
   if (token_bytes != 4 && token_bytes != 8) return EC_EINVAL;
@@ -543,35 +773,73 @@ int ec_embed_grad(const void* d_tokens, int token_bytes, uint64_t n, const void*
   uint8_t* work = (uint8_t*)d_work;
   const hipStream_t st = (hipStream_t)stream;
 
+  const Tokens tok = {d_tokens, vocab_start, vocab, (uint32_t)n, token_bytes};
+  ZeroArgs z = {};
+  z.grad = (uint8_t*)d_grad;
+  z.seen = (const uint32_t*)(work + w.seen);
+  z.stride = grad_stride * type_bytes(grad_type);
+  z.row_bytes = hidden * type_bytes(grad_type);
+  z.words = w.words;
+  z.tiles = w.sort_tiles;
+  z.mode = w.small ? kZeroScan : w.words ? kZeroSeen : kZeroAll;
+  const uint32_t all_zero = accumulate ? 0 : (uint32_t)((vocab + kZeroRows - 1) / kZeroRows);
+  const uint64_t zero_bytes = vocab * z.row_bytes, read = n * hidden * type_bytes(type);
+  const uint64_t launches = w.small ? 1 : 2 * w.passes - (z.mode == kZeroSeen);
+  const uint64_t bytes = std::max(kZeroBytes, zero_bytes > read ? (zero_bytes - read) / launches : 0);
+  const uint64_t share = bytes / ((uint64_t)z.row_bytes * kZeroRows) + 1;
+  // the zero blocks of a launch: its share, or all that are left
+  const auto zeros = [&](bool all) {
+    z.first += z.blocks;
+    const uint32_t left = all_zero - z.first;
+    z.blocks = all ? left : (uint32_t)std::min<uint64_t>(left, share);
+    return z.blocks;
+  };
+
   SortArgs s = {};
-  s.start = vocab_start;
-  s.vocab = vocab;
+  s.tok = tok;
   s.n = (uint32_t)n;
   s.tiles = w.sort_tiles;
-  s.token_bytes = token_bytes;
+  s.words = w.words;
   s.bits = w.bits;
+  s.passes = w.passes;
   s.counts = (uint32_t*)(work + w.counts);
-  for (int p = 0; n && p < w.passes; ++p) {
-    s.tokens = p ? nullptr : d_tokens;
-    s.keys = (const uint32_t*)(work + w.keys[(p + 1) & 1]);
+  const int last = w.small ? 0 : (w.passes + 1) & 1;   // where the sorted pairs are
+  if (w.small && n) {
+    s.keys_out = (uint32_t*)(work + w.keys[0]);
+    s.pos_out = (uint32_t*)(work + w.pos[0]);
+    const uint32_t extra = zeros(false);
+    s.zero = z;
+    sort_small_kernel<<<1 + extra, kSmallLanes, 0, st>>>(s);
+  }
+  for (int p = 0; !w.small && p < w.passes; ++p) {
+    s.keys = p ? (const uint32_t*)(work + w.keys[(p + 1) & 1]) : nullptr;
     s.pos = (const uint32_t*)(work + w.pos[(p + 1) & 1]);
     s.keys_out = (uint32_t*)(work + w.keys[p & 1]);
     s.pos_out = (uint32_t*)(work + w.pos[p & 1]);
+    s.seen = p == 0 && w.words ? (uint32_t*)(work + w.seen) : nullptr;
     s.shift = p * w.bits;
-    sort_count_kernel<<<s.tiles, kSortLanes, 0, st>>>(s);
-    sort_scatter_kernel<<<s.tiles, kSortLanes, 0, st>>>(s);
+    // the first launch collects the rows that occur, so it has none to write yet; where
+    // none are collected all rows are zeroed, and before the sums write theirs
+    uint32_t extra = p || z.mode == kZeroAll ? zeros(false) : 0;
+    s.zero = z;
+    sort_count_kernel<<<s.tiles + extra, kSortLanes, s.seen ? 4 * w.words : 0, st>>>(s);
+    extra = zeros(z.mode == kZeroAll && p + 1 == w.passes);
+    s.zero = z;
+    sort_scatter_kernel<<<s.tiles + extra, kSortLanes, 0, st>>>(s);
   }
 
   SumArgs a = {};
-  a.keys = (const uint32_t*)(work + w.keys[(w.passes + 1) & 1]);
-  a.pos = (const uint32_t*)(work + w.pos[(w.passes + 1) & 1]);
+  a.keys = (const uint32_t*)(work + w.keys[last]);
+  a.pos = (const uint32_t*)(work + w.pos[last]);
   a.dout = d_dout;
   a.grad = d_grad;
   a.parts = (float*)(work + w.parts);
+  a.tok = tok;
   a.dout_stride = dout_stride;
   a.grad_stride = grad_stride;
   a.vocab = vocab;
   a.n = (uint32_t)n;
+  a.tile = tile_for(n);
   a.tiles = w.sum_tiles;
   a.hidden = hidden;
   a.accumulate = accumulate != 0;
@@ -579,15 +847,19 @@ int ec_embed_grad(const void* d_tokens, int token_bytes, uint64_t n, const void*
   const uint32_t per_group = 16 / type_bytes(type);
   a.slabs = (hidden + per_group * kLanes - 1) / (per_group * kLanes);
   const uint64_t sum_blocks = ((uint64_t)a.tiles * a.slabs + kSumWaves - 1) / kSumWaves;
-  const uint64_t per_block = kZeroRows * kSumWaves;
-  const uint64_t blocks = sum_blocks + (accumulate ? 0 : (vocab + per_block - 1) / per_block);
+  const uint64_t blocks = sum_blocks + zeros(true);
+  a.zero = z;
   if (blocks > 0x7fffffffull) return EC_ERANGE;
   a.sum_blocks = (uint32_t)sum_blocks;
-  const dim3 join(a.tiles, (hidden + kLanes * 4 - 1) / (kLanes * 4));
+  const dim3 join((a.tiles + kJoinTiles - 2) / kJoinTiles, (hidden + kLanes * 4 - 1) / (kLanes * 4));
   const auto go = [&](auto t, auto o) {
     typedef decltype(t) T;
     typedef decltype(o) O;
-    if (blocks) sum_kernel<T, O><<<(uint32_t)blocks, kSumWaves * kLanes, 0, st>>>(a);
+    // a last group that starts early needs a whole one, and rows that are written
+    const bool tail = hidden < per_group || (accumulate && hidden % per_group);
+    const auto sum = accumulate ? tail ? sum_kernel<T, O, true, true> : sum_kernel<T, O, true, false>
+                                : tail ? sum_kernel<T, O, false, true> : sum_kernel<T, O, false, false>;
+    if (blocks) sum<<<(uint32_t)blocks, kSumWaves * kLanes, 0, st>>>(a);
     if (a.tiles > 1) join_kernel<O><<<join, kJoinWaves * kLanes, 0, st>>>(a);
     return launched();
   };
