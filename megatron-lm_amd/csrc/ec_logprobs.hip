@@ -15,6 +15,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "ec_types.h"
 
@@ -65,7 +66,7 @@ struct LogprobArgs {
   uint64_t stride;
   uint32_t vocab, groups;   // groups of a row, the last one short
   float scale, c;           // c = scale * log2 e
-  int top;
+  int top, stream;
 };
 
 // A lane's running state over the groups it has seen: the largest logit and the
@@ -136,6 +137,21 @@ __device__ __forceinline__ void block_sums(float& s, float& t, float (&red)[3][W
 constexpr uint32_t kCandidates = 512;
 constexpr int kAhead = 4;   // groups of a lane in flight
 
+// Lanes per row: 512 for long rows and for few rows, 128 for many short ones.
+// Lanes 128 / 256 / 512 / 1024, bf16, us with the likeliest five (with the entropy
+// instead): 1 x 50304 17.8 11.7 8.8 9.0 (14.4 8.5 6.2 6.5); 256 x 16384 11.6 9.0 7.5 7.9;
+// 1024 x 1024 8.8 8.0 7.9 13.7; 4096 x 1024 16.1 17.0 24.0 45.5 (4.8 6.7 11.0 23.2);
+// 4096 x 16384 35.7 35.6 39.0 61.0 (29.0 27.2 26.1 36.8); 4096 x 50304 89.6 82.1
+// 79.5 99.1 (78.5 78.0 75.0 81.8).
+constexpr int kWideLanes = 512, kShortLanes = 128;
+constexpr uint64_t kFewRows = 1024;
+constexpr uint32_t kWideGroups = 2048;
+
+// Logits of more bytes than this are streamed: half the Infinity Cache, past which
+// little of what a matrix product has just written is left there.  8192 x 50304 bf16:
+// 143 us cached, 127 streamed; 64 x 131072: 25 and 29.
+constexpr uint64_t kStreamBytes = 128u << 20;
+
 // One workgroup of B lanes per row; lane l takes groups l, l + B, ...
 //
 // The `top` largest: any lane's largest logit that is among the `top` largest of
@@ -166,9 +182,15 @@ __global__ void __launch_bounds__(B) logprob_kernel(const LogprobArgs a) {
   run.group = tid;
   for (uint32_t g = tid; g < a.groups; g += B * kAhead) {
     typename G::vec v[kAhead];
+    if (a.stream) {
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u)
-      if (g + u * B < a.groups) v[u] = load_logits<T, false>(row, g + u * B, a.vocab);
+      for (int u = 0; u < kAhead; ++u)
+        if (g + u * B < a.groups) v[u] = load_logits<T, true>(row, g + u * B, a.vocab);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (g + u * B < a.groups) v[u] = load_logits<T, false>(row, g + u * B, a.vocab);
+    }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
       if (g + u * B < a.groups) run.template add<G::kN>(widen<T>(v[u]), g + u * B, a.c);
@@ -403,21 +425,27 @@ int ec_token_logprobs(const void* d_logits, int type, uint64_t rows, uint64_t vo
   if (!rows) return EC_OK;
   if (!d_logprobs || !d_lse || (top && (!d_top_logprobs || !d_top_tokens))) return EC_EINVAL;
   LogprobArgs a = {d_logits, d_targets, d_logprobs, d_lse, d_entropy, d_top_logprobs,
-                   d_top_tokens, row_stride, (uint32_t)vocab, 0, scale, scale * kLog2e, top};
+                   d_top_tokens, row_stride, (uint32_t)vocab, 0, scale, scale * kLog2e, top, 0};
   const uint32_t per_group = 16 / type_bytes(type);
   a.groups = (uint32_t)((vocab + per_group - 1) / per_group);
+  a.stream = rows * vocab * type_bytes(type) > kStreamBytes;
+  const bool wide = rows <= kFewRows || a.groups >= kWideGroups;
+  const dim3 grid((uint32_t)rows);
   const hipStream_t st = (hipStream_t)stream;
   return with_type(type, [&](auto t) {
     typedef decltype(t) T;
-    const dim3 grid((uint32_t)rows);
-    if (d_entropy) {
-      if (top) logprob_kernel<T, 256, true, true><<<grid, 256, 0, st>>>(a);
-      else logprob_kernel<T, 256, true, false><<<grid, 256, 0, st>>>(a);
-    } else {
-      if (top) logprob_kernel<T, 256, false, true><<<grid, 256, 0, st>>>(a);
-      else logprob_kernel<T, 256, false, false><<<grid, 256, 0, st>>>(a);
-    }
-    return launched();
+    const auto go = [&](auto entropy, auto tops) {
+      constexpr bool E = decltype(entropy)::value, K = decltype(tops)::value;
+      if (wide)
+        logprob_kernel<T, kWideLanes, E, K><<<grid, kWideLanes, 0, st>>>(a);
+      else
+        logprob_kernel<T, kShortLanes, E, K><<<grid, kShortLanes, 0, st>>>(a);
+      return launched();
+    };
+    const std::true_type yes;
+    const std::false_type no;
+    if (d_entropy) return top ? go(yes, yes) : go(yes, no);
+    return top ? go(no, yes) : go(no, no);
   });
 }
 
