@@ -18,6 +18,7 @@
 #include <type_traits>
 
 #include "ec_types.h"
+#include "fastdiv.h"
 
 namespace ec {
 namespace {
@@ -149,7 +150,8 @@ constexpr uint32_t kWideGroups = 2048;
 
 // Logits of more bytes than this are streamed: half the Infinity Cache, past which
 // little of what a matrix product has just written is left there.  8192 x 50304 bf16:
-// 143 us cached, 127 streamed; 64 x 131072: 25 and 29.
+// 143 us cached, 127 streamed (the gradient 253 and 247); 64 x 131072: 25 and 29, the
+// gradient of 2048 x 32001: 43 and 48.
 constexpr uint64_t kStreamBytes = 128u << 20;
 
 // One workgroup of B lanes per row; lane l takes groups l, l + B, ...
@@ -340,26 +342,32 @@ struct GradArgs {
   const float* entropy;
   const float* dentropy;
   uint64_t stride, out_stride;
-  uint32_t vocab, groups;
+  FastDiv by_slabs;
+  uint32_t vocab, groups, slabs;   // slabs: workgroups of a row
   float c, scale;
+  int stream;
 };
 
+// A lane takes one group, and the workgroups follow the memory's order: 8192 x 50304
+// bf16 in 247 us (6.7 TB/s; a copy kernel of the same form takes 244, the library's
+// copy 324), against 316 with four groups a lane and consecutive workgroups on
+// different rows, 273 with four groups a lane in memory order.
 constexpr int kGradLanes = 256;
-constexpr int kGradGroups = 4;   // per lane
 
 template <typename T, bool ENTROPY>
 __global__ void __launch_bounds__(kGradLanes) logprob_grad_kernel(const GradArgs a) {
   typedef Group<T> G;
   constexpr int N = G::kN;
-  const uint64_t r = blockIdx.x;
-  const T* row = (const T*)a.logits + r * a.stride;
-  T* out = (T*)a.out + r * a.out_stride;
-  const uint32_t g0 = blockIdx.y * (kGradLanes * kGradGroups) + threadIdx.x;
-  typename G::vec v[kGradGroups];
-#pragma unroll
-  for (int u = 0; u < kGradGroups; ++u)
-    if (g0 + u * kGradLanes < a.groups)
-      v[u] = load_logits<T, true>(row, g0 + u * kGradLanes, a.vocab);
+  const uint32_t r = fast_div(blockIdx.x, a.by_slabs);
+  const uint32_t gi = (blockIdx.x - r * a.slabs) * kGradLanes + threadIdx.x;
+  if (gi >= a.groups) return;
+  const T* row = (const T*)a.logits + (uint64_t)r * a.stride;
+  T* out = (T*)a.out + (uint64_t)r * a.out_stride;
+  typename G::vec v;
+  if (a.stream)
+    v = load_logits<T, true>(row, gi, a.vocab);
+  else
+    v = load_logits<T, false>(row, gi, a.vocab);
   const int64_t target = gp(a.targets)[r];
   const float lse = gp(a.lse)[r];
   // a row of masked logits only, also one masked with the type's lowest value
@@ -372,31 +380,26 @@ __global__ void __launch_bounds__(kGradLanes) logprob_grad_kernel(const GradArgs
     A += a.scale * h * gp(a.entropy)[r];
     slope = a.scale * h * kLn2;
   }
+  const typename G::wide x = widen<T>(v);
+  typename G::wide w;
 #pragma unroll
-  for (int u = 0; u < kGradGroups; ++u) {
-    const uint32_t gi = g0 + u * kGradLanes;
-    if (gi >= a.groups) continue;
-    const typename G::wide x = widen<T>(v[u]);
-    typename G::wide w;
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const float d = __builtin_fmaf(x[e], a.c, -lse2);
-      const float p = exp2_hw(d);
-      const float by = ENTROPY ? __builtin_fmaf(fmaxf(d, -200.0f), slope, A) : A;
-      w[e] = empty ? 0.0f : -p * by;
-    }
-    const uint32_t j = gi * N;
-    if (has && !empty && (uint32_t)target - j < (uint32_t)N) {
-#pragma unroll
-      for (int e = 0; e < N; ++e)
-        if ((uint32_t)target == j + e) w[e] += a.scale * g;
-    }
-    if (j + N <= a.vocab)
-      store_wide<T, true>(out + j, w);
-    else
-      for (int e = 0; e < N; ++e)
-        if (j + e < a.vocab) gp(out)[j + e] = (T)w[e];
+  for (int e = 0; e < N; ++e) {
+    const float d = __builtin_fmaf(x[e], a.c, -lse2);
+    const float p = exp2_hw(d);
+    const float by = ENTROPY ? __builtin_fmaf(fmaxf(d, -200.0f), slope, A) : A;
+    w[e] = empty ? 0.0f : -p * by;
   }
+  const uint32_t j = gi * N;
+  if (has && !empty && (uint32_t)target - j < (uint32_t)N) {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if ((uint32_t)target == j + e) w[e] += a.scale * g;
+  }
+  if (j + N <= a.vocab)
+    store_wide<T, true>(out + j, w);
+  else
+    for (int e = 0; e < N; ++e)
+      if (j + e < a.vocab) gp(out)[j + e] = (T)w[e];
 }
 
 int check_logits(const void* logits, int type, uint64_t rows, uint64_t vocab, uint64_t stride,
@@ -460,13 +463,14 @@ int ec_token_logprobs_grad(const void* d_logits, int type, uint64_t rows, uint64
   if (!d_lse || !d_dlogprobs || !d_dlogits || out_stride < vocab) return EC_EINVAL;
   if (!d_entropy != !d_dentropy) return EC_EINVAL;
   GradArgs a = {d_logits, d_dlogits, d_targets, d_lse, d_dlogprobs, d_entropy, d_dentropy,
-                row_stride, out_stride, (uint32_t)vocab, 0, scale * kLog2e, scale};
+                row_stride, out_stride, {}, (uint32_t)vocab, 0, 0, scale * kLog2e, scale, 0};
   const uint32_t per_group = 16 / type_bytes(type);
   a.groups = (uint32_t)((vocab + per_group - 1) / per_group);
-  const uint32_t per_block = kGradLanes * kGradGroups;
-  const uint32_t slabs = (a.groups + per_block - 1) / per_block;
-  if (slabs > 65535) return EC_ERANGE;
-  const dim3 grid((uint32_t)rows, slabs);
+  a.stream = rows * vocab * type_bytes(type) > kStreamBytes;
+  a.slabs = (a.groups + kGradLanes - 1) / kGradLanes;
+  a.by_slabs = make_fastdiv(a.slabs);
+  if (rows * a.slabs > 0x7fffffffull) return EC_ERANGE;
+  const uint32_t grid = (uint32_t)rows * a.slabs;
   const hipStream_t st = (hipStream_t)stream;
   return with_type(type, [&](auto t) {
     typedef decltype(t) T;
