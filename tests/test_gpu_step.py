@@ -120,6 +120,25 @@ def test_embed_grad(pkg, dev, dtype, n, hidden, vocab):
         check(got, want, rounded(want, out, more), f"egrad {out}")
 
 
+@pytest.mark.parametrize("n,vocab,hidden", [(8192, 3000, 24), (8193, 3000, 24), (10_000, 70_001, 40), (16_385, 262_144, 8),
+                                            (33_000, 262_145, 8), (40_000, 1000, 1)])
+def test_embed_grad_over_its_rules(pkg, dev, n, vocab, hidden):
+    """Both sides of the sizes where the sort, its digits, the tiles and the zeros' bits change."""
+    g = gen("rules", n)
+    dout = torch.randn(n, hidden, generator=g).bfloat16()
+    tok = (torch.rand(n, generator=g) ** 4 * (vocab + 9)).long()
+    tok[::97] = vocab - 1
+    want, more, count = egrad_want(tok, dout, vocab, 0, 1.0)
+    buf = torch.full((vocab * hidden + 16,), 7.0, device=dev)
+    out = buf[8:-8].view(vocab, hidden)
+    got = pkg.embed_grad(tok.to(dev), dout.to(dev), vocab, out=out)
+    check(got, want, rounded(want, torch.float32, more), "rules")
+    assert not bool(got.cpu()[count[:, 0] == 0].any())
+    assert bool((buf[:8] == 7).all()) and bool((buf[-8:] == 7).all())
+    pkg.embed_grad(tok.to(dev), dout.to(dev), vocab, out=out, accumulate=True)
+    check(out, want * 2, rounded(want * 2, torch.float32, more * 2 + want.abs() * 2 * E), "twice")
+
+
 @pytest.mark.parametrize("how", ["one token", "two tokens", "none inside", "a tenth"])
 def test_embed_grad_of_repeated_tokens(pkg, dev, how):
     """Runs over many tiles, their ends anywhere, and slices that nobody asks for."""
@@ -501,6 +520,37 @@ def test_norm_and_clip(pkg, dev, sizes, kinds):
         for t, o in zip(grads, same):
             want = t.double().cpu() * by
             check(o, want, rounded(want, t.dtype, want.abs() * 8 * E), "clip in place")
+
+
+@types
+def test_norm_and_clip_of_many_pieces(pkg, dev, dtype):
+    """More pieces than the launches of a short list take: 34 M elements, the last tensors odd."""
+    sizes = [33_600_001, 17, 400_003]
+    buf = torch.randn(sum(sizes) + 1, generator=gen("many"), dtype=torch.float32).to(dtype).to(dev)[1:]
+    grads = list(buf.split(sizes))
+    norm = float((buf.double() * 0.25).norm())
+    lst = pkg.GradList(grads)
+    assert abs(float(lst.norm(grad_scale=0.25)) - norm) <= 2 * E * norm
+    assert float(lst.norm(math.inf, grad_scale=0.25)) == float((buf.double() * 0.25).abs().max())
+    by = 0.25 * 3.0 / (norm + 1e-6)
+    for out in TYPES:
+        into = torch.full((sum(sizes) + 6,), 5.0, dtype=out, device=dev)
+        got = pkg.GradList(grads, list(into[3:-3].split(sizes))).clip(3.0, grad_scale=0.25)
+        assert abs(float(got) - norm) <= 2 * E * norm
+        want = buf.double() * by
+        off = (into[3:-3].double() - want).abs() - (want.abs() * (UNIT[out] + 8 * E) * 1.01 + TINY[out])
+        assert float(off.max()) <= 0, out
+        assert bool((into[:3] == 5).all()) and bool((into[-3:] == 5).all())
+    kept = buf.clone()
+    lst.clip(1e6)
+    assert torch.equal(buf, kept)
+    given = torch.tensor(100.0, device=dev)
+    assert float(lst.clip(1.0, norm=given)) == 100.0
+    want = kept.double() * 0.01
+    assert float(((buf.double() - want).abs() - (want.abs() * (UNIT[dtype] + 8 * E) * 1.01 + TINY[dtype])).max()) <= 0
+    buf[-1] = math.inf
+    kept = buf.clone()
+    assert float(lst.clip(1.0)) == math.inf and torch.equal(buf, kept)
 
 
 def test_norm_at_the_ends_of_the_range(pkg, dev):
