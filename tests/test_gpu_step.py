@@ -5,11 +5,15 @@ out-of-slice tokens.
 Bounds.  u is half the spacing of the result's type relative to it (eps / 2) and `tiny` half its
 smallest step; e = 2^-24 is that of the fp32 arithmetic.  A sum of n terms in fp32 is off by at most n e times
 the sum of magnitudes, whatever its order.  exp2 and log2 of the hardware are taken as 2 e off."""
+import importlib.util
 import math
+import os
 import zlib
 
 import pytest
 import torch
+
+from conftest import ROOT
 
 pytestmark = pytest.mark.gpu
 
@@ -722,3 +726,13 @@ def test_offsets_past_32_bits(pkg, dev):
     tok = torch.arange(rows, device=dev).flip(0)
     grad = pkg.embed_grad(tok, x, 3, vocab_start=0, dtype=torch.bfloat16)
     assert bool((grad[0] == 2).all()) and not bool(grad[1:].any())
+
+
+def test_example_trains_saves_and_loads():
+    """The example's loop: the loss falls, and the state rebuilt from the slices answers with the same
+    bits (the example raises otherwise)."""
+    path = os.path.join(ROOT, "megatron-lm_amd", "examples", "train_step.py")
+    spec = importlib.util.spec_from_file_location("train_step_example", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    assert example.main(60) < 3.0   # ln 512 = 6.2 at the start
