@@ -55,6 +55,10 @@ __device__ __forceinline__ uint32_t order_bits(float v) {
 __device__ __forceinline__ uint64_t order_key(float v, uint32_t index) {
   return (uint64_t)order_bits(v) << 32 | (uint32_t)~index;
 }
+__device__ __forceinline__ float order_value(uint64_t key) {   // -0 comes back as +0
+  const uint32_t b = (uint32_t)(key >> 32);
+  return b == 0 ? __builtin_nanf("") : __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
+}
 
 struct LogprobArgs {
   const void* logits;
@@ -67,7 +71,7 @@ struct LogprobArgs {
   uint64_t stride;
   uint32_t vocab, groups;   // groups of a row, the last one short
   float scale, c;           // c = scale * log2 e
-  int top, stream;
+  int top;
 };
 
 // A lane's running state over the groups it has seen: the largest logit and the
@@ -154,6 +158,26 @@ constexpr uint32_t kWideGroups = 2048;
 // gradient of 2048 x 32001: 43 and 48.
 constexpr uint64_t kStreamBytes = 128u << 20;
 
+// By one wave: the top-th largest of 64 keys, each the largest of the same lane of
+// every wave; 0 where fewer than `top` lanes have a group (those without one have key 0),
+// so that all logits pass.
+template <int WAVES>
+__device__ __forceinline__ void top_bound(const uint64_t* keys, int top, uint64_t& bound) {
+  const uint32_t lane = threadIdx.x % kLanes;
+  uint64_t best = keys[lane];
+  for (int w = 1; w < WAVES; ++w) best = max(best, keys[w * kLanes + lane]);
+  const uint32_t hi = (uint32_t)(best >> 32), lo = (uint32_t)best;
+  int above = 0;
+#pragma unroll 8
+  for (int o = 0; o < kLanes; ++o) {
+    const uint64_t other = (uint64_t)__builtin_amdgcn_readlane(hi, o) << 32 |
+                           (uint32_t)__builtin_amdgcn_readlane(lo, o);
+    above += other > best;
+  }
+  const uint64_t last = __ballot(above == top - 1 && best != 0);
+  if (last ? lane == (uint32_t)__builtin_ctzll(last) : lane == 0) bound = last ? best : 0;
+}
+
 // One workgroup of B lanes per row; lane l takes groups l, l + B, ...
 //
 // The `top` largest: any lane's largest logit that is among the `top` largest of
@@ -164,7 +188,7 @@ constexpr uint64_t kStreamBytes = 128u << 20;
 // the few logits that pass are ranked by counting.  Where more pass than
 // kCandidates (logits that repeat with the workgroup's period) the row is
 // searched `top` times instead.
-template <typename T, int B, bool ENTROPY, bool TOP>
+template <typename T, int B, bool ENTROPY, bool TOP, bool STREAM>
 __global__ void __launch_bounds__(B) logprob_kernel(const LogprobArgs a) {
   typedef Group<T> G;
   constexpr int kWaves = B / kLanes;
@@ -173,35 +197,44 @@ __global__ void __launch_bounds__(B) logprob_kernel(const LogprobArgs a) {
   const uint64_t r = blockIdx.x;
   const T* row = (const T*)a.logits + r * a.stride;
 
-  float given = 0.0f;
-  int64_t target = -1;
-  if (tid == 0) {
-    target = gp(a.targets)[r];
-    if (target >= 0 && target < (int64_t)a.vocab) given = (float)gp(row)[target];
-  }
-
+  const int64_t target = gp(a.targets)[r];   // not waited for before the loop's end
   Running<ENTROPY> run;
   run.group = tid;
-  for (uint32_t g = tid; g < a.groups; g += B * kAhead) {
+  // whole groups: loads without conditions (lanes behind the row's end load its last group
+  // again), so that a batch is in flight together
+  const uint32_t full = a.vocab / G::kN;
+  for (uint32_t g = tid; g < full; g += B * kAhead) {
     typename G::vec v[kAhead];
-    if (a.stream) {
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u)
-        if (g + u * B < a.groups) v[u] = load_logits<T, true>(row, g + u * B, a.vocab);
-    } else {
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u)
-        if (g + u * B < a.groups) v[u] = load_logits<T, false>(row, g + u * B, a.vocab);
-    }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
-      if (g + u * B < a.groups) run.template add<G::kN>(widen<T>(v[u]), g + u * B, a.c);
+      v[u] = load_group<T, STREAM>(row + (uint64_t)min(g + u * B, full - 1) * G::kN);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (g + u * B < full) run.template add<G::kN>(widen<T>(v[u]), g + u * B, a.c);
   }
+  if (full < a.groups && tid == full % B)
+    run.template add<G::kN>(widen<T>(load_logits<T, false>(row, full, a.vocab)), full, a.c);
+
+  float given = 0.0f;
+  if (tid == 0 && target >= 0 && target < (int64_t)a.vocab) given = (float)gp(row)[target];
 
   // the workgroup's reference, then the sums relative to it
+  __shared__ uint64_t keys[TOP ? (kCandidates > B ? kCandidates : B) : 1];
+  __shared__ uint64_t bound_shared;
+  __shared__ uint32_t lanes_list[TOP ? B : 1];
+  __shared__ uint32_t n_lanes, n_keys;
+  uint64_t mine = 0;
+  if constexpr (TOP) {
+    mine = tid < a.groups ? order_key(run.m, run.group) : 0;
+    keys[tid] = mine;
+    if (tid == 0) n_lanes = n_keys = 0;
+  }
   const float wm = wave_max(run.m);
   if (lane == 0) red[0][wave] = wm;
   __syncthreads();
+  if constexpr (TOP) {
+    if (wave == 0) top_bound<kWaves>(keys, a.top, bound_shared);
+  }
   float m = red[0][0];
   for (int w = 1; w < kWaves; ++w) m = fmaxf(m, red[0][w]);
   const float mc = fmaxf(m * a.c, -kMax);
@@ -242,35 +275,6 @@ __global__ void __launch_bounds__(B) logprob_kernel(const LogprobArgs a) {
     if (ENTROPY) gp(a.entropy)[r] = empty ? 0.0f : (log2s - t / s) * kLn2;
   }
   if constexpr (TOP) {
-    __shared__ uint64_t keys[kCandidates > B ? kCandidates : B];
-    __shared__ uint64_t bound_shared;
-    __shared__ uint32_t lanes_list[B];
-    __shared__ uint32_t n_lanes, n_keys;
-    const uint64_t mine = tid < a.groups ? order_key(run.m, run.group) : 0;
-    keys[tid] = mine;
-    if (tid == 0) n_lanes = n_keys = 0;
-    __syncthreads();
-    if (wave == 0) {
-      uint64_t best = keys[lane];
-      for (int w = 1; w < kWaves; ++w) best = max(best, keys[w * kLanes + lane]);
-      const uint32_t hi = (uint32_t)(best >> 32), lo = (uint32_t)best;
-      int above = 0;
-      for (int o = 0; o < kLanes; ++o) {
-        const uint64_t other = (uint64_t)__builtin_amdgcn_readlane(hi, o) << 32 |
-                               (uint32_t)__builtin_amdgcn_readlane(lo, o);
-        above += other > best;
-      }
-      // the key with top - 1 above it; none where fewer than `top` lanes have a
-      // group (those without one have key 0): the bound is 0, all logits pass
-      const uint64_t last = __ballot(above == a.top - 1);
-      const int src = last ? __builtin_ctzll(last) : -1;
-      uint64_t bound = 0;
-      if (src >= 0)
-        bound = (uint64_t)__builtin_amdgcn_readlane(hi, src) << 32 |
-                (uint32_t)__builtin_amdgcn_readlane(lo, src);
-      if (lane == 0) bound_shared = bound;
-    }
-    __syncthreads();
     const uint64_t bound = bound_shared;
     if (mine && mine >= bound) lanes_list[atomicAdd(&n_lanes, 1u)] = tid;
     __syncthreads();
@@ -292,16 +296,16 @@ __global__ void __launch_bounds__(B) logprob_kernel(const LogprobArgs a) {
     }
     __syncthreads();
     const uint32_t n = n_keys;
-    const auto put = [&](int rank, uint32_t j) {
-      gp(a.top_tokens)[r * a.top + rank] = j;
-      gp(a.top_logprobs)[r * a.top + rank] = logprob((float)gp(row)[j]);
+    const auto put = [&](int rank, uint64_t key) {
+      gp(a.top_tokens)[r * a.top + rank] = (uint32_t)~key;
+      gp(a.top_logprobs)[r * a.top + rank] = logprob(order_value(key));
     };
     if (n <= kCandidates && n >= (uint32_t)a.top) {
       for (uint32_t i = tid; i < n; i += B) {
         const uint64_t key = keys[i];
         int above = 0;
         for (uint32_t o = 0; o < n; ++o) above += keys[o] > key;
-        if (above < a.top) put(above, ~(uint32_t)key);
+        if (above < a.top) put(above, key);
       }
     } else {
       uint64_t before = ~0ull;
@@ -324,7 +328,7 @@ __global__ void __launch_bounds__(B) logprob_kernel(const LogprobArgs a) {
           __syncthreads();
         }
         before = keys[0];
-        if (tid == 0) put(k, ~(uint32_t)before);
+        if (tid == 0) put(k, before);
       }
     }
   }
@@ -345,7 +349,6 @@ struct GradArgs {
   FastDiv by_slabs;
   uint32_t vocab, groups, slabs;   // slabs: workgroups of a row
   float c, scale;
-  int stream;
 };
 
 // A lane takes one group, and the workgroups follow the memory's order: 8192 x 50304
@@ -354,7 +357,7 @@ struct GradArgs {
 // different rows, 273 with four groups a lane in memory order.
 constexpr int kGradLanes = 256;
 
-template <typename T, bool ENTROPY>
+template <typename T, bool ENTROPY, bool STREAM>
 __global__ void __launch_bounds__(kGradLanes) logprob_grad_kernel(const GradArgs a) {
   typedef Group<T> G;
   constexpr int N = G::kN;
@@ -363,11 +366,7 @@ __global__ void __launch_bounds__(kGradLanes) logprob_grad_kernel(const GradArgs
   if (gi >= a.groups) return;
   const T* row = (const T*)a.logits + (uint64_t)r * a.stride;
   T* out = (T*)a.out + (uint64_t)r * a.out_stride;
-  typename G::vec v;
-  if (a.stream)
-    v = load_logits<T, true>(row, gi, a.vocab);
-  else
-    v = load_logits<T, false>(row, gi, a.vocab);
+  const typename G::vec v = load_logits<T, STREAM>(row, gi, a.vocab);
   const int64_t target = gp(a.targets)[r];
   const float lse = gp(a.lse)[r];
   // a row of masked logits only, also one masked with the type's lowest value
@@ -428,27 +427,31 @@ int ec_token_logprobs(const void* d_logits, int type, uint64_t rows, uint64_t vo
   if (!rows) return EC_OK;
   if (!d_logprobs || !d_lse || (top && (!d_top_logprobs || !d_top_tokens))) return EC_EINVAL;
   LogprobArgs a = {d_logits, d_targets, d_logprobs, d_lse, d_entropy, d_top_logprobs,
-                   d_top_tokens, row_stride, (uint32_t)vocab, 0, scale, scale * kLog2e, top, 0};
+                   d_top_tokens, row_stride, (uint32_t)vocab, 0, scale, scale * kLog2e, top};
   const uint32_t per_group = 16 / type_bytes(type);
   a.groups = (uint32_t)((vocab + per_group - 1) / per_group);
-  a.stream = rows * vocab * type_bytes(type) > kStreamBytes;
+  const bool streamed = rows * vocab * type_bytes(type) > kStreamBytes;
   const bool wide = rows <= kFewRows || a.groups >= kWideGroups;
   const dim3 grid((uint32_t)rows);
   const hipStream_t st = (hipStream_t)stream;
   return with_type(type, [&](auto t) {
     typedef decltype(t) T;
-    const auto go = [&](auto entropy, auto tops) {
+    const auto go = [&](auto entropy, auto tops, auto stream_) {
       constexpr bool E = decltype(entropy)::value, K = decltype(tops)::value;
+      constexpr bool S = decltype(stream_)::value;
       if (wide)
-        logprob_kernel<T, kWideLanes, E, K><<<grid, kWideLanes, 0, st>>>(a);
+        logprob_kernel<T, kWideLanes, E, K, S><<<grid, kWideLanes, 0, st>>>(a);
       else
-        logprob_kernel<T, kShortLanes, E, K><<<grid, kShortLanes, 0, st>>>(a);
+        logprob_kernel<T, kShortLanes, E, K, S><<<grid, kShortLanes, 0, st>>>(a);
       return launched();
     };
     const std::true_type yes;
     const std::false_type no;
-    if (d_entropy) return top ? go(yes, yes) : go(yes, no);
-    return top ? go(no, yes) : go(no, no);
+    const auto with = [&](auto entropy, auto tops) {
+      return streamed ? go(entropy, tops, yes) : go(entropy, tops, no);
+    };
+    if (d_entropy) return top ? with(yes, yes) : with(yes, no);
+    return top ? with(no, yes) : with(no, no);
   });
 }
 
@@ -463,10 +466,10 @@ int ec_token_logprobs_grad(const void* d_logits, int type, uint64_t rows, uint64
   if (!d_lse || !d_dlogprobs || !d_dlogits || out_stride < vocab) return EC_EINVAL;
   if (!d_entropy != !d_dentropy) return EC_EINVAL;
   GradArgs a = {d_logits, d_dlogits, d_targets, d_lse, d_dlogprobs, d_entropy, d_dentropy,
-                row_stride, out_stride, {}, (uint32_t)vocab, 0, 0, scale * kLog2e, scale, 0};
+                row_stride, out_stride, {}, (uint32_t)vocab, 0, 0, scale * kLog2e, scale};
   const uint32_t per_group = 16 / type_bytes(type);
   a.groups = (uint32_t)((vocab + per_group - 1) / per_group);
-  a.stream = rows * vocab * type_bytes(type) > kStreamBytes;
+  const bool streamed = rows * vocab * type_bytes(type) > kStreamBytes;
   a.slabs = (a.groups + kGradLanes - 1) / kGradLanes;
   a.by_slabs = make_fastdiv(a.slabs);
   if (rows * a.slabs > 0x7fffffffull) return EC_ERANGE;
@@ -474,10 +477,11 @@ int ec_token_logprobs_grad(const void* d_logits, int type, uint64_t rows, uint64
   const hipStream_t st = (hipStream_t)stream;
   return with_type(type, [&](auto t) {
     typedef decltype(t) T;
-    if (d_dentropy)
-      logprob_grad_kernel<T, true><<<grid, kGradLanes, 0, st>>>(a);
-    else
-      logprob_grad_kernel<T, false><<<grid, kGradLanes, 0, st>>>(a);
+    const auto kernel = d_dentropy ? streamed ? logprob_grad_kernel<T, true, true>
+                                              : logprob_grad_kernel<T, true, false>
+                                   : streamed ? logprob_grad_kernel<T, false, true>
+                                              : logprob_grad_kernel<T, false, false>;
+    kernel<<<grid, kGradLanes, 0, st>>>(a);
     return launched();
   });
 }
