@@ -37,19 +37,20 @@ struct EmbedArgs {
   uint64_t vocab, table_stride;
   int64_t start;
   uint32_t n, hidden, groups;
-  int token_bytes, shift, stream;
+  int token_bytes, shift;
   float scale;
 };
 
 constexpr int kEmbedGroups = 4;
 constexpr int kEmbedWaves = 4;
 // Results of at least this many bytes, in rows of at least a KiB, are streamed past the
-// caches: 32768 rows of 2048 bf16 40.5 -> 33.1 us, 65536 of 512 21.2 -> 17.6; but 131072 of
-// 33 fp16, whose rows share lines, 6.2 -> 11.4.
+// caches: 32768 rows of 2048 bf16 39.3 -> 36.3 us, of 2047 47.2 -> 40.9, 65536 of 512 21.6 ->
+// 19.2, 16384 of 4096 fp32 78.6 -> 70.4; but 131072 of 33 fp16, whose rows share lines, 6.2
+// -> 11.4.
 constexpr uint64_t kEmbedStream = 64u << 20;
 constexpr uint32_t kEmbedStreamGroups = 64;
 
-template <typename T>
+template <typename T, bool STREAM>
 __global__ void __launch_bounds__(kEmbedWaves * kLanes) embed_kernel(const EmbedArgs a) {
   typedef Group<T> G;
   const uint32_t lane = threadIdx.x % kLanes, wave = threadIdx.x / kLanes;
@@ -66,24 +67,22 @@ __global__ void __launch_bounds__(kEmbedWaves * kLanes) embed_kernel(const Embed
         gp(out)[j] = row < 0 ? (T)0.0f : (T)((float)gp(src)[j] * a.scale);
     return;
   }
+  // (groups behind the row's end read and write its last one)
   typename G::vec v[kEmbedGroups];
   uint32_t at[kEmbedGroups];
 #pragma unroll
   for (int u = 0; u < kEmbedGroups; ++u) {
-    const uint32_t g = first + u * per_row;
-    at[u] = min(g * G::kN, a.hidden - G::kN);
-    if (g < a.groups && row >= 0) v[u] = load_group<T, false>(src + at[u]);
+    at[u] = min((first + u * per_row) * G::kN, a.hidden - G::kN);
+    v[u] = {};
+  }
+  if (row >= 0) {
+#pragma unroll
+    for (int u = 0; u < kEmbedGroups; ++u) v[u] = load_group<T, false>(src + at[u]);
   }
 #pragma unroll
-  for (int u = 0; u < kEmbedGroups; ++u) {
-    if (first + u * per_row >= a.groups) continue;
-    typename G::wide w = {};
-    if (row >= 0) w = widen<T>(v[u]) * a.scale;
-    if (a.stream)
-      store_wide<T, true>(out + at[u], w);
-    else
-      store_wide<T, false>(out + at[u], w);
-  }
+  for (int u = 0; u < kEmbedGroups; ++u)
+    if (first + u * per_row < a.groups)
+      store_wide<T, STREAM>(out + at[u], widen<T>(v[u]) * a.scale);
 }
 
 // ------------------------------------------------------------------- zeros --
@@ -425,7 +424,7 @@ constexpr uint32_t kFewTokens = 16384;
 constexpr uint32_t kMaxTile = 32;   // two tiles' pairs in the lanes of a wave
 constexpr uint32_t tile_for(uint64_t n) { return n <= kFewTokens ? kMaxTile / 2 : kMaxTile; }
 constexpr int kBatch = 16;
-constexpr int kSumWaves = 4;
+constexpr int kSumWaves = 2;
 
 struct SumArgs {
   const uint32_t* keys;
@@ -532,6 +531,8 @@ __global__ void __launch_bounds__(kSumWaves * kLanes) sum_kernel(const SumArgs a
         end += __popcll(__ballot(lane >= a.tile && key == tail));
     }
   }
+  // the tokens outside the slice are the last
+  end = min(end, (uint32_t)__popcll(__ballot(key < vocab)));
   if (b >= end) return;
 
   float sum[N] = {};
@@ -551,27 +552,24 @@ __global__ void __launch_bounds__(kSumWaves * kLanes) sum_kernel(const SumArgs a
   for (; b < end; b += kBatch) {
     typename G::vec v[kBatch];
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      v[u] = {};
-      const uint32_t k = __builtin_amdgcn_readlane(key, (b + u) & 63);
-      const uint32_t p = __builtin_amdgcn_readlane(pos, (b + u) & 63);
-      if (b + u < end && k < vocab) {
-        const T* src = (const T*)a.dout + (uint64_t)p * a.dout_stride;
-        if (!TAIL || c + N <= a.hidden)
-          v[u] = load_group<T, true>(src + c);
-        else
+    for (int u = 0; u < kBatch; ++u) {   // behind the end, the last row again
+      const uint32_t p = __builtin_amdgcn_readlane(pos, min(b + u, end - 1));
+      const T* src = (const T*)a.dout + (uint64_t)p * a.dout_stride;
+      if (!TAIL || c + N <= a.hidden) {
+        v[u] = load_group<T, true>(src + c);
+      } else {
+        v[u] = {};
 #pragma unroll
-          for (int e = 0; e < N; ++e)
-            if (c + e < a.hidden) v[u][e] = gp(src + c)[e];
+        for (int e = 0; e < N; ++e)
+          if (c + e < a.hidden) v[u][e] = gp(src + c)[e];
       }
     }
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
       if (b + u >= end) break;
-      const uint32_t k = __builtin_amdgcn_readlane(key, (b + u) & 63);
+      const uint32_t k = __builtin_amdgcn_readlane(key, b + u);
       if (k != run) {   // the run ended
         put(0);
-        if (k >= vocab) return;   // the tokens outside the slice are the last
         run = k;
         part = false;
 #pragma unroll
@@ -582,7 +580,6 @@ __global__ void __launch_bounds__(kSumWaves * kLanes) sum_kernel(const SumArgs a
       for (int e = 0; e < N; ++e) sum[e] += w[e];
     }
   }
-  if (run >= vocab) return;
   const uint32_t slot = part ? 0 : 1;
   part = part || tail_part;
   put(slot);
@@ -748,15 +745,16 @@ int ec_embed(const void* d_tokens, int token_bytes, uint64_t n, const void* d_ta
   if (!n || !hidden) return EC_OK;
   if (!d_out || (vocab && (!d_table || table_stride < hidden))) return EC_EINVAL;
   EmbedArgs a = {d_tokens, d_table, d_out, vocab, table_stride, vocab_start,
-                 (uint32_t)n, hidden, 0, token_bytes, 0, 0, scale};
+                 (uint32_t)n, hidden, 0, token_bytes, 0, scale};
   const uint32_t per_group = 16 / type_bytes(type);
   a.groups = (hidden + per_group - 1) / per_group;
-  a.stream = a.groups >= kEmbedStreamGroups && n * hidden * type_bytes(type) >= kEmbedStream;
+  const bool streamed = a.groups >= kEmbedStreamGroups && n * hidden * type_bytes(type) >= kEmbedStream;
   while (a.shift < 6 && (1u << a.shift) * kEmbedGroups < a.groups) ++a.shift;
   const uint32_t rows = kEmbedWaves * (kLanes >> a.shift), wide = kEmbedGroups << a.shift;
   const dim3 grid((a.n + rows - 1) / rows, (a.groups + wide - 1) / wide);
   return with_type(type, [&](auto t) {
-    embed_kernel<decltype(t)><<<grid, kEmbedWaves * kLanes, 0, (hipStream_t)stream>>>(a);
+    const auto kernel = streamed ? embed_kernel<decltype(t), true> : embed_kernel<decltype(t), false>;
+    kernel<<<grid, kEmbedWaves * kLanes, 0, (hipStream_t)stream>>>(a);
     return launched();
   });
 }

@@ -76,9 +76,8 @@ __device__ __forceinline__ void add_piece(Acc& acc, const T* p, uint32_t n) {
   for (uint32_t g = threadIdx.x; g < groups; g += kBlockLanes * kAhead) {
     typename G::vec v[kAhead];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u)
-      if (g + u * kBlockLanes < groups)
-        v[u] = load_group<T, STREAM>(p + (uint64_t)(g + u * kBlockLanes) * G::kN);
+    for (int u = 0; u < kAhead; ++u)   // without conditions, so that all are in flight together
+      v[u] = load_group<T, STREAM>(p + (uint64_t)min(g + u * kBlockLanes, groups - 1) * G::kN);
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
       if (g + u * kBlockLanes < groups) {
@@ -133,30 +132,43 @@ __device__ __forceinline__ float clip_factor(float norm, float scale, float max_
   return __builtin_isfinite(norm) ? scale * fminf(1.0f, max_norm / (norm + kEps)) : scale;
 }
 
-// Groups j, j + step, ... of a piece.  Where a lane's result is two groups (16-bit to
+// Group g of 16 bytes of a piece, as its raw bits; nothing where it is not whole.
+typedef uint32_t __attribute__((ext_vector_type(4))) raw_t;
+template <bool STREAM>
+__device__ __forceinline__ raw_t load_raw(const ec_grad_item& it, uint32_t g) {
+  typedef uint32_t __attribute__((ext_vector_type(4), aligned(2))) any_t;
+  const uint32_t groups = it.n / (it.src_type == EC_F32 ? 4 : 8);
+  raw_t v = {};
+  if (g < groups) {
+    const auto* p = (const global<any_t>*)(uintptr_t)(it.src + (uint64_t)g * 16);
+    v = STREAM ? __builtin_nontemporal_load(p) : *p;
+  }
+  return v;
+}
+
+// The elements of group g, scaled.  Where a lane's result is two groups (16-bit to
 // fp32) the stores go through the caches, which join the halves of a line: 534 M
 // elements, norm and clip, 730 us against 814 streamed.
-template <typename T, typename O, bool STREAM>
-__device__ __forceinline__ void scale_groups(const ec_grad_item& it, uint32_t j, uint32_t step,
-                                             float by) {
+template <typename T, typename O>
+__device__ __forceinline__ void scale_group(const ec_grad_item& it, uint32_t g, const raw_t& raw,
+                                            float by) {
   typedef Group<T> G;
   constexpr int N = G::kN;
   const T* src = (const T*)it.src;
   O* dst = (O*)it.dst;
-  for (; j < it.n; j += step) {
-    if (j + N <= it.n) {
-      const typename G::wide w = widen<T>(load_group<T, STREAM>(src + j)) * by;
-      if constexpr (N > Group<O>::kN) {
-        store_wide<O, false>(dst + j, __builtin_shufflevector(w, w, 0, 1, 2, 3));
-        store_wide<O, false>(dst + j + 4, __builtin_shufflevector(w, w, 4, 5, 6, 7));
-      } else {
-        typedef O __attribute__((ext_vector_type(N), aligned(sizeof(O)))) some;
-        __builtin_nontemporal_store((some)__builtin_convertvector(w, some),
-                                    (global<some>*)(uintptr_t)(dst + j));
-      }
+  const uint32_t j = g * N;
+  if (j + N <= it.n) {
+    const typename G::wide w = widen<T>(__builtin_bit_cast(typename G::vec, raw)) * by;
+    if constexpr (N > Group<O>::kN) {
+      store_wide<O, false>(dst + j, __builtin_shufflevector(w, w, 0, 1, 2, 3));
+      store_wide<O, false>(dst + j + 4, __builtin_shufflevector(w, w, 4, 5, 6, 7));
     } else {
-      for (uint32_t e = j; e < it.n; ++e) gp(dst)[e] = (O)((float)gp(src)[e] * by);
+      typedef O __attribute__((ext_vector_type(N), aligned(sizeof(O)))) some;
+      __builtin_nontemporal_store((some)__builtin_convertvector(w, some),
+                                  (global<some>*)(uintptr_t)(dst + j));
     }
+  } else {
+    for (uint32_t e = j; e < it.n; ++e) gp(dst)[e] = (O)((float)gp(src)[e] * by);
   }
 }
 
@@ -170,61 +182,57 @@ __device__ __forceinline__ bool unchanged(const ec_grad_item& it, float by) {
   return by == 1.0f && it.src == it.dst && it.src_type == it.dst_type;
 }
 
-// A few pieces: each workgroup joins the partials by itself.
-template <int NORM>
-__global__ void __launch_bounds__(kBlockLanes) grad_clip_few_kernel(
-    const ec_grad_item* items, uint32_t n_items, const double* parts, uint32_t n_parts,
-    float scale, float max_norm, const float* given, float* norm) {
-  const float v = given ? *gp(given) : join_parts<NORM>(parts, n_parts, scale);
-  if (blockIdx.x == 0 && threadIdx.x == 0) *gp(norm) = v;
-  const float by = clip_factor(v, scale, max_norm);
-  if (blockIdx.x >= n_items) return;   // an empty list and a given norm
-  const ec_grad_item it = items[blockIdx.x];
-  if (unchanged(it, by)) return;
-  with_types(it, [&](auto t, auto o) {
-    typedef decltype(t) T;
-    typedef decltype(o) O;
-    constexpr uint32_t kN = Group<T>::kN;
-    scale_groups<T, O, false>(it, threadIdx.x * kN, kBlockLanes * kN, by);
-  });
-}
-
-// Many: kSplit workgroups for a piece, which take neighbouring 4 KiB of it, one or two
+// kSplit workgroups for a piece, which take neighbouring 4 KiB of it, one or two
 // groups a lane, from the list's end (what the norm read last may still be in the
-// Infinity Cache).  1.3 G fp32 elements: norm 752 us (7.0 TB/s; 850 with cached reads),
+// Infinity Cache).  1.3 G fp32 elements: norm 740 us (7.1 TB/s; 850 with cached reads),
 // clip 1630 us (6.4 TB/s) against 2050 with 2048 workgroups that walk whole pieces.
+// JOIN: each workgroup joins the norm's partials by itself, a launch less.
 constexpr uint32_t kSplit = 8;
 
-__global__ void __launch_bounds__(kBlockLanes) grad_clip_kernel(const ec_grad_item* items,
-                                                                uint32_t n_items, float scale,
-                                                                float max_norm, const float* given,
-                                                                float* norm) {
-  const float v = *gp(given);
+template <int NORM, bool JOIN, bool STREAM>
+__global__ void __launch_bounds__(kBlockLanes) grad_clip_kernel(
+    const ec_grad_item* items, uint32_t n_items, const double* parts, uint32_t n_parts, float scale,
+    float max_norm, const float* given, float* norm) {
+  const uint32_t back = gridDim.x - 1 - blockIdx.x;
+  ec_grad_item it = {};
+  if (back / kSplit < n_items) it = items[back / kSplit];
+  // a lane's groups are under way while the norm is found; of long lists the second (of
+  // fp32) only behind the first one's store, which keeps to the memory's order (1.3 G
+  // elements, norm and clip, 2385 us against 2415)
+  constexpr uint32_t kStep = kSplit * kBlockLanes;
+  const uint32_t g = back % kSplit * kBlockLanes + threadIdx.x;
+  const raw_t first = load_raw<STREAM>(it, g);
+  raw_t second = {};
+  if (!STREAM) second = load_raw<STREAM>(it, g + kStep);
+  const float v = JOIN ? join_parts<NORM>(parts, n_parts, scale) : *gp(given);
   if (norm != given && blockIdx.x == 0 && threadIdx.x == 0) *gp(norm) = v;
   const float by = clip_factor(v, scale, max_norm);
-  const uint32_t back = gridDim.x - 1 - blockIdx.x;
-  const ec_grad_item it = items[back / kSplit];
   if (unchanged(it, by)) return;
   with_types(it, [&](auto t, auto o) {
     typedef decltype(t) T;
     typedef decltype(o) O;
-    constexpr uint32_t kStep = kBlockLanes * Group<T>::kN;
-    scale_groups<T, O, true>(it, back % kSplit * kStep + threadIdx.x * Group<T>::kN,
-                             kSplit * kStep, by);
+    static_assert(EC_GRAD_PIECE <= 2 * kStep * 4, "two groups a lane");
+    scale_group<T, O>(it, g, first, by);
+    if (STREAM) second = load_raw<STREAM>(it, g + kStep);
+    scale_group<T, O>(it, g + kStep, second, by);
   });
 }
+
+constexpr uint32_t kMaxPieces = 1u << 28;   // the clip's grid
 
 int check_list(const ec_grad_item* items, uint32_t n, float scale, int norm, const void* work,
                const float* out) {
   if (!std::isfinite(scale) || (norm != EC_NORM_2 && norm != EC_NORM_INF)) return EC_EINVAL;
   if (!work || !out || (n && !items)) return EC_EINVAL;
+  if (n > kMaxPieces) return EC_ERANGE;
   if ((uintptr_t)work & 7u) return EC_EALIGN;
   return EC_OK;
 }
 
-// Pieces from which the norm's reads are streamed (about 128 MiB of fp32, half the Infinity Cache)
-// and the clip takes its own launch form.
+// Pieces above which reads are streamed (about 128 MiB of fp32, half the Infinity Cache),
+// and up to which the clip joins the partials itself.
 constexpr uint32_t kManyPieces = 2048;
+constexpr uint32_t kFewPieces = 256;
 
 template <int NORM>
 uint32_t run_parts(const ec_grad_item* items, uint32_t n, double* parts, hipStream_t st) {
@@ -247,19 +255,21 @@ int run_norm(const ec_grad_item* items, uint32_t n, float scale, double* parts, 
 template <int NORM>
 int run_clip(const ec_grad_item* items, uint32_t n, float scale, float max_norm, const float* given,
              double* parts, float* norm, hipStream_t st) {
-  if (n > kManyPieces) {
-    if (!given) {
-      const int status = run_norm<NORM>(items, n, scale, parts, norm, st);
-      if (status != EC_OK) return status;
-    }
-    grad_clip_kernel<<<n * kSplit, kBlockLanes, 0, st>>>(items, n, scale, max_norm,
-                                                         given ? given : norm, norm);
+  const uint32_t blocks = std::max(1u, n) * kSplit;
+  if (n && n <= kFewPieces && !given) {
+    const uint32_t n_parts = run_parts<NORM>(items, n, parts, st);
+    grad_clip_kernel<NORM, true, false><<<blocks, kBlockLanes, 0, st>>>(
+        items, n, parts, n_parts, scale, max_norm, given, norm);
     return launched();
   }
-  if (!n && !given) return run_norm<NORM>(items, n, scale, parts, norm, st);
-  const uint32_t blocks = given ? 0 : run_parts<NORM>(items, n, parts, st);
-  grad_clip_few_kernel<NORM><<<std::max(1u, n), kBlockLanes, 0, st>>>(
-      items, n, parts, blocks, scale, max_norm, given, norm);
+  if (!given) {
+    const int status = run_norm<NORM>(items, n, scale, parts, norm, st);
+    if (status != EC_OK || !n) return status;
+    given = norm;
+  }
+  const auto kernel = n > kManyPieces ? grad_clip_kernel<NORM, false, true>
+                                      : grad_clip_kernel<NORM, false, false>;
+  kernel<<<blocks, kBlockLanes, 0, st>>>(items, n, parts, 0, scale, max_norm, given, norm);
   return launched();
 }
 
