@@ -1,9 +1,8 @@
 // Torch-tensor binding of the training-step operators (ec_embed ... ec_grad_clip),
 // part of the _ec_shards extension: the checks on the tensors, the outputs'
 // allocation, torch's current stream and the C call in one crossing from Python.
-// Each function returns the status of the C call first, then what it allocated,
-// for the caller to turn the status into its error type and to record a stream of its
-// own on the allocations.
+// Each function returns the status of the C call first, for the caller to turn into
+// its error type, then what it allocated.
 #include <torch/extension.h>
 #include <c10/hip/HIPStream.h>
 
@@ -87,11 +86,26 @@ Rows rows_of(const Tensor& t, const char* what, const c10::Device* device) {
                         "rows that do not overlap");
 }
 
-ec_stream_t stream_of(const c10::Device& device, const std::optional<int64_t>& stream) {
-  return reinterpret_cast<ec_stream_t>(
-      stream.has_value()
-          ? static_cast<intptr_t>(*stream)
-          : reinterpret_cast<intptr_t>(c10::hip::getCurrentHIPStream(device.index()).stream()));
+ec_stream_t stream_of(const c10::Device& device) {
+  return reinterpret_cast<ec_stream_t>(c10::hip::getCurrentHIPStream(device.index()).stream());
+}
+
+// Whether rows of a and rows of b, written and read by one call, share memory.
+// Rows of one pitch that lie beside each other (columns of one buffer) do not.
+bool share(const void* a, const Rows& ra, uint64_t wa, const void* b, const Rows& rb, uint64_t wb) {
+  if (!ra.n || !ra.width || !rb.n || !rb.width) return false;
+  const uint64_t a0 = reinterpret_cast<uint64_t>(a), b0 = reinterpret_cast<uint64_t>(b);
+  const uint64_t a1 = a0 + ((ra.n - 1) * ra.stride + ra.width) * wa;
+  const uint64_t b1 = b0 + ((rb.n - 1) * rb.stride + rb.width) * wb;
+  if (a1 <= b0 || b1 <= a0) return false;
+  const uint64_t pitch = ra.stride * wa;
+  if (pitch != rb.stride * wb) return true;
+  const uint64_t d = a0 <= b0 ? (b0 - a0) % pitch : (pitch - (a0 - b0) % pitch) % pitch;
+  return !(d >= ra.width * wa && d + rb.width * wb <= pitch);
+}
+
+void check_apart(bool together, const char* a, const char* b) {
+  if (together) throw py::value_error(std::string(a) + " shares memory with " + b);
 }
 
 int token_bytes(const Tensor& t) {
@@ -108,7 +122,7 @@ std::vector<int64_t> with_last(at::IntArrayRef lead, int64_t last) {
 }
 
 py::tuple embed(const Tensor& tokens, const Tensor& table, double scale, int64_t start,
-                std::optional<Tensor> out, std::optional<int64_t> stream) {
+                std::optional<Tensor> out) {
   const int type = type_code(table, "table");
   if (table.dim() != 2)
     throw py::value_error("table must be [vocabulary, hidden], has shape " +
@@ -124,11 +138,14 @@ py::tuple embed(const Tensor& tokens, const Tensor& table, double scale, int64_t
     check_dense(result, "out", &device);
     check_type(result, "out", table.scalar_type());
     check_shape(result, "out", shape);
+    const Rows o = {1, (uint64_t)result.numel(), (uint64_t)std::max<int64_t>(result.numel(), 1)};
+    const uint64_t w = result.element_size();
+    check_apart(share(result.data_ptr(), o, w, table.data_ptr(), rows, w), "out", "table");
   } else {
     result = at::empty(shape, table.options().requires_grad(false));
   }
   const uint64_t n = (uint64_t)tokens.numel();
-  const ec_stream_t st = stream_of(device, stream);
+  const ec_stream_t st = stream_of(device);
   const int status =
       rows.width > 0xffffffffull
           ? EC_ERANGE
@@ -138,8 +155,7 @@ py::tuple embed(const Tensor& tokens, const Tensor& table, double scale, int64_t
 }
 
 py::tuple embed_grad(const Tensor& tokens, const Tensor& dout, int64_t vocab, double scale,
-                     int64_t start, int64_t grad_type, std::optional<Tensor> out, bool accumulate,
-                     std::optional<int64_t> stream) {
+                     int64_t start, int64_t grad_type, std::optional<Tensor> out, bool accumulate) {
   const int type = type_code(dout, "dout");
   const Rows rows = rows_of(dout, "dout", nullptr);
   const c10::Device device = dout.device();
@@ -156,6 +172,8 @@ py::tuple embed_grad(const Tensor& tokens, const Tensor& dout, int64_t vocab, do
     check_shape(grad, "out", {vocab, (int64_t)rows.width});
     g = rows_of(grad, "out", &device);
     grad_type = type_code(grad, "out");
+    check_apart(share(grad.data_ptr(), g, grad.element_size(), dout.data_ptr(), rows,
+                      dout.element_size()), "out", "dout");
   } else {
     if (accumulate) throw py::value_error("accumulate needs out");
     grad = at::empty({vocab, (int64_t)rows.width},
@@ -170,12 +188,12 @@ py::tuple embed_grad(const Tensor& tokens, const Tensor& dout, int64_t vocab, do
   const int status = ec_embed_grad(tokens.data_ptr(), bytes, rows.n, dout.data_ptr(), type,
                                    rows.stride, (uint64_t)vocab, hidden, start, (float)scale,
                                    grad.data_ptr(), (int)grad_type, g.stride, accumulate,
-                                   work.data_ptr(), need, stream_of(device, stream));
+                                   work.data_ptr(), need, stream_of(device));
   return py::make_tuple(status, grad, work);
 }
 
 py::tuple token_logprobs(const Tensor& logits, const Tensor& targets, double scale, bool entropy,
-                         int64_t top, std::optional<int64_t> stream) {
+                         int64_t top) {
   const int type = type_code(logits, "logits");
   const Rows rows = rows_of(logits, "logits", nullptr);
   const c10::Device device = logits.device();
@@ -201,14 +219,14 @@ py::tuple token_logprobs(const Tensor& logits, const Tensor& targets, double sca
       (float)scale, logprobs.data_ptr<float>(), lse.data_ptr<float>(),
       ent ? ent->data_ptr<float>() : nullptr, (int)top,
       top ? top_logprobs->data_ptr<float>() : nullptr,
-      top ? top_tokens->data_ptr<int64_t>() : nullptr, stream_of(device, stream));
+      top ? top_tokens->data_ptr<int64_t>() : nullptr, stream_of(device));
   return py::make_tuple(status, logprobs, lse, ent, top_logprobs, top_tokens);
 }
 
 py::tuple token_logprobs_grad(const Tensor& logits, const Tensor& targets, const Tensor& lse,
                               const Tensor& dlogprobs, std::optional<Tensor> entropy,
                               std::optional<Tensor> dentropy, double scale,
-                              std::optional<Tensor> out, std::optional<int64_t> stream) {
+                              std::optional<Tensor> out) {
   const int type = type_code(logits, "logits");
   const Rows rows = rows_of(logits, "logits", nullptr);
   const c10::Device device = logits.device();
@@ -235,12 +253,16 @@ py::tuple token_logprobs_grad(const Tensor& logits, const Tensor& targets, const
     check_type(result, "out", logits.scalar_type());
     check_shape(result, "out", logits.sizes());
     o = rows_of(result, "out", &device);
+    const uint64_t w = result.element_size();
+    const bool same = result.data_ptr() == logits.data_ptr() && (o.stride == rows.stride || o.n < 2);
+    check_apart(!same && share(result.data_ptr(), o, w, logits.data_ptr(), rows, w), "out",
+                "logits");
   } else {
     result = at::empty(logits.sizes(), logits.options().requires_grad(false));
   }
   const int status = ec_token_logprobs_grad(
       logits.data_ptr(), type, rows.n, rows.width, rows.stride, targets.data_ptr<int64_t>(), l, g,
-      h, dh, (float)scale, result.data_ptr(), o.stride, stream_of(device, stream));
+      h, dh, (float)scale, result.data_ptr(), o.stride, stream_of(device));
   return py::make_tuple(status, result);
 }
 
@@ -251,6 +273,12 @@ Tensor grad_items(const std::vector<Tensor>& grads, const std::optional<std::vec
     throw py::value_error("out: expected " + std::to_string(grads.size()) + " tensors, got " +
                           std::to_string(out->size()));
   std::vector<ec_grad_item> items;
+  struct Span {
+    uint64_t from, to;
+    size_t i;
+    bool operator<(const Span& o) const { return from < o.from; }
+  };
+  std::vector<Span> read, written;
   for (size_t i = 0; i < grads.size(); ++i) {
     const std::string name = "grads[" + std::to_string(i) + "]";
     const Tensor& src = grads[i];
@@ -270,6 +298,10 @@ Tensor grad_items(const std::vector<Tensor>& grads, const std::optional<std::vec
     const uint64_t n = (uint64_t)src.numel();
     const uint64_t from = reinterpret_cast<uint64_t>(src.data_ptr());
     const uint64_t to = reinterpret_cast<uint64_t>(dst.data_ptr());
+    if (n) {
+      read.push_back({from, from + n * src.element_size(), i});
+      written.push_back({to, to + n * dst.element_size(), i});
+    }
     for (uint64_t at = 0; at < n; at += EC_GRAD_PIECE)
       items.push_back({from + at * (uint64_t)src.element_size(),
                        to + at * (uint64_t)dst.element_size(),
@@ -277,6 +309,27 @@ Tensor grad_items(const std::vector<Tensor>& grads, const std::optional<std::vec
                        (uint16_t)dt});
   }
   if (items.size() > 0xffffffffull) throw py::value_error("too many gradients");
+  // no element is written twice, and none that another tensor is read from
+  const std::string side = out ? "out" : "grads";
+  const auto name = [](const std::string& list, size_t i) { return list + "[" + std::to_string(i) + "]"; };
+  std::sort(written.begin(), written.end());
+  for (size_t j = 1; j < written.size(); ++j)
+    check_apart(written[j].from < written[j - 1].to, name(side, written[j].i).c_str(),
+                name(side, written[j - 1].i).c_str());
+  if (out) {
+    std::sort(read.begin(), read.end());
+    std::vector<uint64_t> reach(read.size());   // the furthest end of the reads up to here
+    for (size_t j = 0; j < read.size(); ++j)
+      reach[j] = std::max(read[j].to, j ? reach[j - 1] : 0);
+    for (const Span& w : written) {
+      size_t j = std::lower_bound(read.begin(), read.end(), Span{w.to, 0, 0}) - read.begin();
+      for (; j > 0 && reach[j - 1] > w.from; --j) {
+        const Span& r = read[j - 1];
+        if (r.to > w.from && !(r.i == w.i && r.from == w.from && r.to == w.to))
+          check_apart(true, name("out", w.i).c_str(), name("grads", r.i).c_str());
+      }
+    }
+  }
   const Tensor bytes = at::empty({(int64_t)(items.size() * sizeof(ec_grad_item))}, at::kByte);
   if (!items.empty()) std::memcpy(bytes.data_ptr(), items.data(), items.size() * sizeof(ec_grad_item));
   return bytes;
@@ -284,15 +337,14 @@ Tensor grad_items(const std::vector<Tensor>& grads, const std::optional<std::vec
 
 // ec_grad_norm (max_norm empty) or ec_grad_clip over an uploaded list.
 py::tuple grad_call(const Tensor& items, double grad_scale, int64_t norm,
-                    std::optional<double> max_norm, std::optional<Tensor> given,
-                    std::optional<int64_t> stream) {
+                    std::optional<double> max_norm, std::optional<Tensor> given) {
   const c10::Device device = items.device();
   const auto opts = at::TensorOptions().device(device);
   const Tensor work = at::empty({EC_GRAD_WORK}, opts.dtype(at::kByte));
   const Tensor result = at::empty({}, opts.dtype(at::kFloat));
   const auto* d = reinterpret_cast<const ec_grad_item*>(items.data_ptr());
   const uint32_t n = (uint32_t)(items.numel() / (int64_t)sizeof(ec_grad_item));
-  const ec_stream_t st = stream_of(device, stream);
+  const ec_stream_t st = stream_of(device);
   int status;
   if (max_norm.has_value()) {
     const float* g = nullptr;
@@ -316,16 +368,16 @@ py::tuple grad_call(const Tensor& items, double grad_scale, int64_t norm,
 void bind_step(py::module_& mod) {
   const auto none = py::none();
   mod.def("embed", &embed, py::arg("tokens"), py::arg("table"), py::arg("scale"), py::arg("start"),
-          py::arg("out") = none, py::arg("stream") = none);
+          py::arg("out") = none);
   mod.def("embed_grad", &embed_grad, py::arg("tokens"), py::arg("dout"), py::arg("vocab"),
           py::arg("scale"), py::arg("start"), py::arg("grad_type"), py::arg("out") = none,
-          py::arg("accumulate") = false, py::arg("stream") = none);
+          py::arg("accumulate") = false);
   mod.def("token_logprobs", &token_logprobs, py::arg("logits"), py::arg("targets"),
-          py::arg("scale"), py::arg("entropy"), py::arg("top"), py::arg("stream") = none);
+          py::arg("scale"), py::arg("entropy"), py::arg("top"));
   mod.def("token_logprobs_grad", &token_logprobs_grad, py::arg("logits"), py::arg("targets"),
           py::arg("lse"), py::arg("dlogprobs"), py::arg("entropy"), py::arg("dentropy"),
-          py::arg("scale"), py::arg("out") = none, py::arg("stream") = none);
+          py::arg("scale"), py::arg("out") = none);
   mod.def("grad_items", &grad_items, py::arg("grads"), py::arg("out") = none);
   mod.def("grad_call", &grad_call, py::arg("items"), py::arg("grad_scale"), py::arg("norm"),
-          py::arg("max_norm") = none, py::arg("given") = none, py::arg("stream") = none);
+          py::arg("max_norm") = none, py::arg("given") = none);
 }

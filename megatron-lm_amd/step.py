@@ -22,6 +22,7 @@ import math
 from typing import NamedTuple, Optional, Sequence
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .codec import _raw_stream
@@ -40,13 +41,19 @@ def _finite(v: float, what: str) -> float:
 
 
 def _call(name: str, fn, tensor, stream, *args):
-    """The binding's ``fn(*args, stream)``: what it returned after the status,
-    with a caller's own stream recorded on it."""
+    """The binding's ``fn(*args)`` on ``stream`` or torch's current one: what it returned after the
+    status.  Memory for a caller's own stream comes from that stream's share of the caching
+    allocator (a block of the current stream's may still be in use there), and is not handed
+    out again before work enqueued on the current stream, which reads the results, is done."""
     if stream is None:
-        status, *made = fn(*args, None)
+        status, *made = fn(*args)
     else:
-        status, *made = fn(*args, _raw_stream(stream, getattr(tensor, "device", None)))
-        _hold(stream, *[t for t in made if t is not None])
+        device = getattr(tensor, "device", None)
+        _raw_stream(stream, device)   # the devices agree
+        current = torch.cuda.current_stream(device)
+        with torch.cuda.stream(stream):
+            status, *made = fn(*args)
+        _hold(current, *[t for t in made if t is not None])
     if status != _lib.EC_OK:
         _lib.check(status, name)
     return made
@@ -62,6 +69,7 @@ class _Embed(torch.autograd.Function):
         return embed(tokens, table.detach(), scale=scale, vocab_start=vocab_start)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         (tokens,) = ctx.saved_tensors
         vocab, dtype, scale, start = ctx.like
@@ -126,6 +134,7 @@ class _TokenLogprobs(torch.autograd.Function):
         return tuple(r)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dlogprobs, _lse, dentropy, _top, _tokens):
         logits, targets, lse, entropy = ctx.saved_tensors
         if dlogprobs is None and dentropy is None:
@@ -189,8 +198,8 @@ class GradList:
     """A list of gradient tensors (contiguous, on one device, any mix of types and sizes) prepared
     once for ``norm`` and ``clip``: a training loop keeps its gradient buffers, and the list of
     their pieces stays on the device.  ``clip`` writes to the tensors of ``out`` (same element
-    counts, any of the types: bf16 gradients into fp32 ones), or in place.  The list keeps the tensors
-    alive; gradients that are replaced by other tensors need a new list."""
+    counts, any of the types: bf16 gradients into fp32 ones), or in place; no two of the tensors
+    written may overlap.  The list keeps the tensors alive; gradients that are replaced by other tensors need a new list."""
 
     def __init__(self, grads: Sequence[torch.Tensor], out: Optional[Sequence[torch.Tensor]] = None):
         self.grads = list(grads)

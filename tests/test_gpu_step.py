@@ -611,6 +611,43 @@ def test_grad_list_refusals(pkg, dev):
             call()
 
 
+def test_memory_that_is_written_and_read(pkg, dev):
+    """Results over their own operands are refused where a value could be read after it was written;
+    the gradient over its logits, and columns beside each other, are not."""
+    buf = torch.randn(40, 64, device=dev)
+    tok = torch.arange(20, device=dev)
+    for call in (lambda: pkg.embed(tok, buf[:20], out=buf[:20]),
+                 lambda: pkg.embed(tok, buf[:20, :32], out=buf.view(-1)[16:656].view(20, 32)),
+                 lambda: pkg.embed_grad(tok, buf[:20], 20, out=buf[10:30]),
+                 lambda: pkg.embed_grad(tok, buf[:20, :32], 20, out=buf[:20, 16:48]),
+                 lambda: pkg.token_logprobs_grad(buf[:20], tok, buf[0, :20], buf[0, :20], out=buf[1:21]),
+                 lambda: pkg.GradList([buf[:20], buf[10:30]]), lambda: pkg.GradList([buf, buf]),
+                 lambda: pkg.GradList([buf[:20]], out=[buf[1:21]]),
+                 lambda: pkg.GradList([buf[:20], buf[20:]], out=[buf[20:], buf[:20]]),
+                 lambda: pkg.GradList([buf[:10].bfloat16(), buf[20:]], out=[buf[25:35], buf.new_zeros(20, 64)])):
+        with pytest.raises(ValueError, match="shares memory"):
+            call()
+    # neighbours, the same place, and reads that overlap
+    left, right = buf[:20, :32], buf[:20, 32:]
+    want = pkg.embed_grad(tok, left, 20)
+    assert torch.equal(pkg.embed_grad(tok, left, 20, out=right), want)
+    outs = [torch.empty(20, 64, device=dev) for _ in range(2)]
+    assert float(pkg.GradList([buf[:20], buf[10:30]], out=outs).clip(1e9)) > 0
+    assert torch.equal(outs[1], buf[10:30])
+    pkg.GradList([buf[:20], buf[20:]], out=[buf[:20], buf[20:]]).clip(1e9)
+    pkg.GradList([buf[:20], buf[20:], buf[:0]]).clip(1e9)
+
+
+def test_a_second_derivative_is_refused(pkg, dev):
+    table = torch.randn(5, 8, device=dev, requires_grad=True)
+    x = torch.randn(3, 20, device=dev, requires_grad=True)
+    tok = torch.tensor([0, 1, 2], device=dev)
+    for out, leaf in ((pkg.embed(tok, table), table), (pkg.token_logprobs(x, tok).logprobs, x)):
+        (g,) = torch.autograd.grad(out.square().sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            g.sum().backward()
+
+
 def test_refusals_on_device(pkg, dev):
     table, tok = torch.zeros(10, 8, device=dev), torch.zeros(3, dtype=torch.int64, device=dev)
     x, lse = torch.zeros(3, 50, device=dev), torch.zeros(3, device=dev)
@@ -663,10 +700,15 @@ def test_on_a_caller_stream(pkg, dev):
                *pkg.token_logprobs(x, target, entropy=True, top=4, stream=side), lst.norm(stream=side)]
         got.append(pkg.token_logprobs_grad(x, target, r.lse, r.lse, stream=side))
         junk = [torch.full((4000, 256), 3.0, device=dev) for _ in range(4)]
+        # the result's block goes back while the current stream has yet to read it
+        torch.cuda.current_stream().wait_stream(side)
+        kept = got[0] + 0
+        got[0] = kept
+        again = pkg.embed(tok, table, scale=2.0, stream=side)
         side.synchronize()
         torch.cuda.current_stream().synchronize()
         assert all(torch.equal(u, v) for u, v in zip(got, want))
-        del junk, got
+        del junk, got, kept, again
     with torch.cuda.stream(side):   # torch's current stream is another than the list was made on
         n = lst.norm()
     side.synchronize()
