@@ -7,6 +7,7 @@
 #include <cmath>
 
 #include "ec_types.h"
+#include "fastdiv.h"
 
 namespace ec {
 namespace {
@@ -88,9 +89,9 @@ __global__ void __launch_bounds__(kEmbedWaves * kLanes) embed_kernel(const Embed
 // ------------------------------------------------------------------- zeros --
 // The rows of tokens that do not occur, which the gradient has most of, need no
 // sorted tokens: workgroups that write zeros ride along in the sort's launches, which
-// leave the memory idle, and in the sums' launch.  Each takes up to 64 rows and learns which of
-// them occur from bits that the sort's first launch collected (one bit per row and tile of
-// tokens), or, for few tokens, from the tokens themselves.
+// leave the memory idle, and in the sums' launch.  Each takes the rows of 32 to 256 KiB and learns
+// which of them occur from bits that the sort's first launch collected (one bit per row
+// and tile of tokens), or, for few tokens, from the tokens themselves.
 enum ZeroMode : int { kZeroSeen, kZeroScan, kZeroAll };
 
 struct Tokens {
@@ -109,75 +110,103 @@ struct ZeroArgs {
   uint8_t* grad;
   const uint32_t* seen;      // [tiles][words]
   uint64_t stride;           // of the rows, in bytes
+  FastDiv by_row;            // by row_bytes
   uint32_t row_bytes, words, tiles;
-  uint32_t rows;             // of a workgroup: 32 or 64
+  int shift;                 // a workgroup's rows: 32 << shift
   uint32_t first, blocks;    // workgroups before this launch's, and in it
   int mode;
 };
 
-// One row of zeros: 16 bytes at a time at aligned addresses, elements at the ends.
+// Bytes of a workgroup's rows, about: a 256th of the gradient's within these bounds, and at
+// most 2048 rows.
+constexpr uint64_t kLeastSpan = 32u << 10, kMostSpan = 256u << 10, kZeroSpans = 256;
+constexpr int kZeroShift = 6;
+// Rows of this many bytes and more are written one by a wave.  Narrower ones would leave most
+// of a wave idle, and share lines: 67 tokens, 116317 x 64 fp32, 38 us by rows, 16 flat;
+// 65536 tokens, 50304 x 2048, 147 and 172 (the flat form looks each 16 bytes' row up).
+constexpr uint32_t kWideRow = 1024;
+
+typedef uint32_t __attribute__((ext_vector_type(4))) zero16_t;
+__device__ __forceinline__ void put_zeros(uint8_t* at) {
+  const zero16_t zero = {};
+  __builtin_nontemporal_store(zero, (global<zero16_t>*)(uintptr_t)at);
+}
+__device__ __forceinline__ void put_zero(uint8_t* at) { *gp((uint16_t*)at) = 0; }
+
+// The rows of a span that lie back to back, as one range of memory: 16 bytes at a time at
+// aligned addresses, where no row in them occurs, else (and at the range's ends) two.
+__device__ __forceinline__ void zero_flat(const ZeroArgs& z, const uint32_t* bits, uint8_t* span,
+                                          uint32_t rows) {
+  const uint32_t bytes = rows * z.row_bytes;
+  const auto occurs = [&](uint32_t r) { return (bits[r / 32] >> (r % 32)) & 1u; };
+  const auto single = [&](uint32_t off) {
+    if (!occurs(fast_div(off, z.by_row))) put_zero(span + off);
+  };
+  const uint32_t lead = min(bytes, (uint32_t)(-(uintptr_t)span % 16));
+  const uint32_t chunks = (bytes - lead) / 16, behind = lead + chunks * 16;
+  if (threadIdx.x < 8) {
+    if (threadIdx.x * 2 < lead) single(threadIdx.x * 2);
+    if (behind + threadIdx.x * 2 < bytes) single(behind + threadIdx.x * 2);
+  }
+  for (uint32_t i = threadIdx.x; i < chunks; i += blockDim.x) {
+    const uint32_t off = lead + i * 16;
+    const uint32_t r0 = fast_div(off, z.by_row), r1 = fast_div(off + 15, z.by_row);
+    if (r1 - r0 <= 1 && !occurs(r0) && !occurs(r1))
+      put_zeros(span + off);
+    else if (r1 != r0 || !occurs(r0))
+      for (uint32_t e = 0; e < 16; e += 2) single(off + e);
+  }
+}
+
+// One row by a wave.
 __device__ __forceinline__ void zero_row(uint8_t* row, uint32_t bytes) {
   const uint32_t lane = threadIdx.x % kLanes;
   const uint32_t lead = min(bytes, (uint32_t)(-(uintptr_t)row % 16));
   const uint32_t chunks = (bytes - lead) / 16, behind = lead + chunks * 16;
-  typedef uint32_t __attribute__((ext_vector_type(4))) u32x4;
-  const u32x4 zero = {};
-  if (lane * 2 < lead) *gp((uint16_t*)(row + lane * 2)) = 0;
-  if (behind + lane * 2 < bytes) *gp((uint16_t*)(row + behind + lane * 2)) = 0;
-  for (uint32_t g = lane; g < chunks; g += kLanes)
-    __builtin_nontemporal_store(zero, (global<u32x4>*)(uintptr_t)(row + lead + g * 16));
+  if (lane * 2 < lead) put_zero(row + lane * 2);
+  if (behind + lane * 2 < bytes) put_zero(row + behind + lane * 2);
+  for (uint32_t g = lane; g < chunks; g += kLanes) put_zeros(row + lead + g * 16);
 }
 
 // By a whole workgroup of WAVES waves.
 template <int WAVES>
 __device__ __forceinline__ void zero_block(const ZeroArgs& z, const Tokens& tok, uint32_t block) {
-  const uint32_t lane = threadIdx.x % kLanes;
-  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
-  const uint64_t first = (uint64_t)(z.first + block) * z.rows;
-  uint64_t occur = 0;   // bit r: row first + r
+  __shared__ uint32_t bits[1 << kZeroShift];   // the span's rows that occur
+  constexpr uint32_t kAll = WAVES * kLanes;
+  const uint32_t t = threadIdx.x, words = 1u << z.shift;
+  const uint32_t w0 = (z.first + block) << z.shift;   // vocab < 2^31: fits
+  const uint64_t first = (uint64_t)w0 * 32;
+  if (t < words) bits[t] = 0;
+  __syncthreads();
   if (z.mode == kZeroSeen) {
-    uint32_t lo = 0, hi = 0;
-    const uint32_t w = (uint32_t)(first / 32);
-    for (uint32_t t = lane; t < z.tiles; t += kLanes) {
-      const uint32_t* at = z.seen + (uint64_t)t * z.words + w;
-      lo |= gp(at)[0];
-      if (w + 1 < z.words) hi |= gp(at)[1];
-    }
-#pragma unroll
-    for (int o = 32; o; o >>= 1) {
-      lo |= __shfl_xor(lo, o);
-      hi |= __shfl_xor(hi, o);
-    }
-    occur = ((uint64_t)__builtin_amdgcn_readfirstlane(hi) << 32 |
-             (uint32_t)__builtin_amdgcn_readfirstlane(lo)) >> (first % 32);
+    const uint32_t w = t & (words - 1);
+    uint32_t found = 0;
+    if (w0 + w < z.words)
+      for (uint32_t tile = t >> z.shift; tile < z.tiles; tile += kAll >> z.shift)
+        found |= gp(z.seen)[(uint64_t)tile * z.words + w0 + w];
+    if (found) atomicOr(&bits[w], found);
   } else if (z.mode == kZeroScan) {
-    __shared__ uint64_t found[WAVES];
-    uint64_t mine = 0;
-    for (uint32_t i = threadIdx.x; i < tok.n; i += WAVES * kLanes * 8) {
+    for (uint32_t i = t; i < tok.n; i += kAll * 8) {
       int64_t row[8];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const uint32_t j = i + u * WAVES * kLanes;
-        row[u] = j < tok.n ? tok.row(j) : -1;
-      }
+      for (int u = 0; u < 8; ++u) row[u] = tok.row(min(i + u * kAll, tok.n - 1));
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        const uint64_t r = (uint64_t)row[u] - first;
-        mine |= row[u] >= 0 && r < 64 ? 1ull << r : 0ull;
+        const uint64_t r = (uint64_t)row[u] - first;   // far off for a token outside (-1)
+        if (r < (uint64_t)words * 32) atomicOr(&bits[r / 32], 1u << (r % 32));
       }
     }
-    uint32_t lo = (uint32_t)mine, hi = (uint32_t)(mine >> 32);
-#pragma unroll
-    for (int o = 32; o; o >>= 1) {
-      lo |= __shfl_xor(lo, o);
-      hi |= __shfl_xor(hi, o);
-    }
-    if (lane == 0) found[wave] = (uint64_t)hi << 32 | lo;
-    __syncthreads();
-    for (int w = 0; w < WAVES; ++w) occur |= found[w];
   }
-  for (uint32_t r = wave; r < z.rows && first + r < tok.vocab; r += WAVES)
-    if (!((occur >> r) & 1u)) zero_row(z.grad + (first + r) * z.stride, z.row_bytes);
+  __syncthreads();
+  if (first >= tok.vocab) return;
+  const uint32_t rows = (uint32_t)min((uint64_t)words * 32, tok.vocab - first);
+  uint8_t* span = z.grad + first * z.stride;
+  if (z.stride == z.row_bytes && z.row_bytes < kWideRow) {
+    zero_flat(z, bits, span, rows);
+  } else {
+    for (uint32_t r = __builtin_amdgcn_readfirstlane(t / kLanes); r < rows; r += WAVES)
+      if (!((bits[r / 32] >> (r % 32)) & 1u)) zero_row(span + r * z.stride, z.row_bytes);
+  }
 }
 
 // -------------------------------------------------------------------- sort --
@@ -790,14 +819,16 @@ int ec_embed_grad(const void* d_tokens, int token_bytes, uint64_t n, const void*
   z.words = w.words;
   z.tiles = w.sort_tiles;
   z.mode = w.small ? kZeroScan : w.words ? kZeroSeen : kZeroAll;
-  // 16 / 32 / 64: 4096 tokens, 50304 x 2048, 89 90 96 us; 65536 of the same 152 148 147
-  z.rows = w.small ? 32 : 64;
-  const uint32_t all_zero = accumulate ? 0 : (uint32_t)((vocab + z.rows - 1) / z.rows);
+  z.by_row = make_fastdiv(z.row_bytes);
+  const uint64_t span = std::min(kMostSpan, std::max(kLeastSpan, vocab * z.row_bytes / kZeroSpans));
+  while (z.shift < kZeroShift && (64ull << z.shift) * z.row_bytes <= span) ++z.shift;
+  const uint64_t zero_rows = 32ull << z.shift;
+  const uint32_t all_zero = accumulate ? 0 : (uint32_t)((vocab + zero_rows - 1) / zero_rows);
   const uint64_t zero_bytes = vocab * z.row_bytes, read = n * hidden * type_bytes(type);
   const uint64_t launches = 2 * w.passes - (z.mode == kZeroSeen);
   const uint64_t bytes = std::max(kZeroBytes, zero_bytes > read ? (zero_bytes - read) / launches : 0);
-  const uint64_t share = bytes / ((uint64_t)z.row_bytes * z.rows) + 1;
-  const auto with_join = (uint32_t)std::min<uint64_t>(all_zero, kZeroBytes / ((uint64_t)z.row_bytes * z.rows));
+  const uint64_t share = bytes / (z.row_bytes * zero_rows) + 1;
+  const auto with_join = (uint32_t)std::min<uint64_t>(all_zero, kZeroBytes / (z.row_bytes * zero_rows));
   // the next launch's zero blocks: all that are left but `leave`
   const auto zeros = [&](uint64_t leave) {
     z.first += z.blocks;

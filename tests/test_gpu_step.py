@@ -143,6 +143,30 @@ def test_embed_grad_over_its_rules(pkg, dev, n, vocab, hidden):
     check(out, want * 2, rounded(want * 2, torch.float32, more * 2 + want.abs() * 2 * E), "twice")
 
 
+@pytest.mark.parametrize("n", [5, 9000])
+@pytest.mark.parametrize("hidden,pad", [(1, 0), (3, 0), (7, 0), (8, 0), (9, 0), (33, 0), (250, 0), (511, 0), (513, 0), (33, 4),
+                                        (300, 1), (700, 5)])
+@types
+def test_embed_grad_zeros_between_rows(pkg, dev, dtype, hidden, pad, n):
+    """Rows of zeros next to rows that occur, narrow ones that share 16 bytes and lines, dense and strided, into
+    a gradient that held something else, at an odd element."""
+    g = gen("zeros", hidden, pad, n)
+    vocab = 2600
+    dout = torch.randn(n, hidden, generator=g).to(dtype)
+    tok = torch.randint(0, 900, (n,), generator=g) * 3 % vocab
+    tok[0], tok[1] = 0, vocab - 1
+    buf = torch.full((vocab * (hidden + pad) + 9,), 7.0, dtype=dtype, device=dev)
+    out = buf[3:3 + vocab * (hidden + pad)].view(vocab, hidden + pad)[:, :hidden]
+    got = pkg.embed_grad(tok.to(dev), dout.to(dev), vocab, out=out)
+    want, more, count = egrad_want(tok, dout, vocab, 0, 1.0)
+    check(got, want, rounded(want, dtype, more), "zeros between")
+    assert not bool(got.cpu()[count[:, 0] == 0].any())
+    rest = buf.cpu()
+    inside = torch.zeros(rest.numel(), dtype=torch.bool)
+    inside[3:3 + vocab * (hidden + pad)].view(vocab, hidden + pad)[:, :hidden] = True
+    assert bool((rest[~inside] == 7).all())
+
+
 @pytest.mark.parametrize("how", ["one token", "two tokens", "none inside", "a tenth"])
 def test_embed_grad_of_repeated_tokens(pkg, dev, how):
     """Runs over many tiles, their ends anywhere, and slices that nobody asks for."""
