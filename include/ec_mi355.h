@@ -3,7 +3,8 @@
  *
  * The engine computes XOR parity and systematic Reed-Solomon codes over
  * GF(2^8) (reduction polynomial x^8+x^4+x^3+x^2+1 = 0x11D, generator 0x02)
- * on device-resident checkpoint shards, and reconstructs lost shards.
+ * on device-resident checkpoint shards, and reconstructs lost shards.  The last
+ * section holds operators of the training step around the saves.
  *
  * Code conventions (fixed; every entry point follows them):
  *   - generator matrix G = [ I_k ; C ] with the m x k Cauchy block

@@ -4,7 +4,8 @@ Serialized checkpoint shards held in HIP tensors pass through the C ABI of
 ``include/ec_mi355.h`` (libec_mi355.so, built in-tree) to hand-written gfx950
 kernels: XOR parity, GF(2^8) Reed-Solomon encode (polynomial 0x11D, Cauchy
 generator), erasure reconstruction and a batched ragged-stripe launcher with
-incremental parity update.
+incremental parity update.  Beside it, the operators of the training step that runs
+between the saves.
 
 Modules:
   codec    equal-size shards: xor_encode, rs_encode, reconstruct, ShardPlan (a

@@ -3,7 +3,7 @@
 The shared library is built in-tree by ``__graft_entry__.build()``.  There is
 no fallback: if the library is missing, every call raises
 ``ECLibraryMissing``.  ``shards()`` loads the torch-tensor binding of the
-flat-shard calls, built beside it.
+flat-shard calls and the training-step operators, built beside it.
 """
 from __future__ import annotations
 
@@ -181,8 +181,9 @@ _shards_lock = threading.Lock()
 
 
 def shards():
-    """The torch-tensor binding of the flat-shard calls (``_ec_shards.so``,
-    csrc/shards_torch.cpp), which links libec_mi355.so.  Raises
+    """The torch-tensor binding of the flat-shard calls and the training-step
+    operators (``_ec_shards.so``, csrc/shards_torch.cpp and step_torch.cpp), which links
+    libec_mi355.so.  Raises
     ``ECLibraryMissing`` when it is not built; there is no fallback."""
     global _shards_mod
     if _shards_mod is not None:
