@@ -481,24 +481,19 @@ struct SumArgs {
   float scale;
 };
 
-// Elements [c, c + N) of a row of `hidden`: N of them, or (TAIL) what is left.
+// Elements [c, c + N) of a row of `hidden`: N of them, 16 bytes or 8, or (TAIL) what is left.
 template <typename T, int N, bool TAIL>
 __device__ __forceinline__ void put_row(T* row, uint32_t c, uint32_t hidden, const float* sum,
                                         float scale, bool add) {
-  typedef Group<T> G;
   if constexpr (!TAIL) {
-    constexpr int kPut = N < G::kN ? N : G::kN;
-    typedef T __attribute__((ext_vector_type(kPut), aligned(sizeof(T)))) some;
-    typedef float __attribute__((ext_vector_type(kPut))) wide;
+    typedef T __attribute__((ext_vector_type(N), aligned(sizeof(T)))) some;
+    typedef float __attribute__((ext_vector_type(N))) wide;
+    auto* at = (global<some>*)(uintptr_t)(row + c);
+    wide w;
 #pragma unroll
-    for (int h = 0; h < N; h += kPut) {
-      auto* at = (global<some>*)(uintptr_t)(row + c + h);
-      wide w;
-#pragma unroll
-      for (int e = 0; e < kPut; ++e) w[e] = sum[h + e] * scale;
-      if (add) w += __builtin_convertvector(*at, wide);
-      *at = __builtin_convertvector(w, some);
-    }
+    for (int e = 0; e < N; ++e) w[e] = sum[e] * scale;
+    if (add) w += __builtin_convertvector(*at, wide);
+    *at = __builtin_convertvector(w, some);
   } else {
 #pragma unroll
     for (int e = 0; e < N; ++e)
@@ -510,14 +505,26 @@ __device__ __forceinline__ void put_row(T* row, uint32_t c, uint32_t hidden, con
   }
 }
 
+// A lane's columns of a slab of 64 groups: a group, or, of 16-bit rows summed into fp32 ones,
+// two halves of one that lie 64 halves apart, so that each store of the wave's is whole
+// lines of the gradient.
+template <typename T, typename O>
+struct Columns {
+  static constexpr int kPieces = sizeof(O) > sizeof(T) ? 2 : 1;
+  static constexpr int kN = Group<T>::kN / kPieces;   // columns of a piece
+  typedef T __attribute__((ext_vector_type(kN), aligned(sizeof(T)))) any;
+  typedef T __attribute__((ext_vector_type(kN))) vec;
+  typedef float __attribute__((ext_vector_type(kN))) wide;
+};
+
 // TAIL: the last group of a row is stored element by element.  Otherwise it starts
 // early, so that it ends with the row; its lane then writes some elements that its
 // neighbour writes too, the same values, which only a gradient that is written and not
 // added to allows.
 template <typename T, typename O, bool ADD, bool TAIL>
 __global__ void __launch_bounds__(kSumWaves * kLanes) sum_kernel(const SumArgs a) {
-  typedef Group<T> G;
-  constexpr int N = G::kN;
+  typedef Columns<T, O> C;
+  constexpr int N = C::kN, P = C::kPieces;
   const uint32_t lane = threadIdx.x % kLanes;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
   // the workgroups that write zeros lie evenly between the others: the ones wait for
@@ -530,9 +537,14 @@ __global__ void __launch_bounds__(kSumWaves * kLanes) sum_kernel(const SumArgs a
   const uint32_t tile = (uint32_t)(job / a.slabs), slab = (uint32_t)(job % a.slabs);
   if (tile >= a.tiles) return;
   // this lane's columns; lanes behind the row read what the last one reads
-  uint32_t c = (slab * kLanes + lane) * N;
-  const bool on = c < a.hidden;
-  if (!TAIL) c = min(c, a.hidden - N);
+  uint32_t c[P];
+  bool on[P];
+#pragma unroll
+  for (int q = 0; q < P; ++q) {
+    c[q] = ((slab * P + q) * kLanes + lane) * N;
+    on[q] = c[q] < a.hidden;
+    if (!TAIL) c[q] = min(c[q], a.hidden - N);
+  }
   const uint32_t first = tile * a.tile, len = min(a.tile, a.n - first);
 
   // lane l holds pair l of this tile and the next; `prev` and `before` are the
@@ -576,33 +588,39 @@ __global__ void __launch_bounds__(kSumWaves * kLanes) sum_kernel(const SumArgs a
   end = min(end, (uint32_t)__popcll(__ballot(key < vocab)));
   if (b >= end) return;
 
-  float sum[N] = {};
+  float sum[P][N] = {};
   uint32_t run = __builtin_amdgcn_readlane(key, b);
   bool part = head_part;
   const auto put = [&](uint32_t slot) {
     float* const at = a.parts + ((uint64_t)tile * 2 + slot) * a.hidden;
     O* const row = (O*)a.grad + (uint64_t)run * a.grad_stride;
-    if constexpr (sizeof(O) == 4 && !ADD) {   // one place in the code for both
-      if (on) put_row<float, N, TAIL>(part ? at : row, c, a.hidden, sum, part ? 1.0f : a.scale, false);
-    } else if (part) {
-      if (on) put_row<float, N, TAIL>(at, c, a.hidden, sum, 1.0f, false);
-    } else {
-      if (on) put_row<O, N, TAIL>(row, c, a.hidden, sum, a.scale, ADD);
+#pragma unroll
+    for (int q = 0; q < P; ++q) {
+      if (!on[q]) continue;
+      if constexpr (sizeof(O) == 4 && !ADD)   // one place in the code for both
+        put_row<float, N, TAIL>(part ? at : row, c[q], a.hidden, sum[q], part ? 1.0f : a.scale, false);
+      else if (part)
+        put_row<float, N, TAIL>(at, c[q], a.hidden, sum[q], 1.0f, false);
+      else
+        put_row<O, N, TAIL>(row, c[q], a.hidden, sum[q], a.scale, ADD);
     }
   };
   for (; b < end; b += kBatch) {
-    typename G::vec v[kBatch];
+    typename C::vec v[kBatch][P];
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {   // behind the end, the last row again
       const uint32_t p = __builtin_amdgcn_readlane(pos, min(b + u, end - 1));
       const T* src = (const T*)a.dout + (uint64_t)p * a.dout_stride;
-      if (!TAIL || c + N <= a.hidden) {
-        v[u] = load_group<T, true>(src + c);
-      } else {
-        v[u] = {};
 #pragma unroll
-        for (int e = 0; e < N; ++e)
-          if (c + e < a.hidden) v[u][e] = gp(src + c)[e];
+      for (int q = 0; q < P; ++q) {
+        if (!TAIL || c[q] + N <= a.hidden) {
+          v[u][q] = __builtin_nontemporal_load((const global<typename C::any>*)(uintptr_t)(src + c[q]));
+        } else {
+          v[u][q] = {};
+#pragma unroll
+          for (int e = 0; e < N; ++e)
+            if (c[q] + e < a.hidden) v[u][q][e] = gp(src + c[q])[e];
+        }
       }
     }
 #pragma unroll
@@ -614,11 +632,16 @@ __global__ void __launch_bounds__(kSumWaves * kLanes) sum_kernel(const SumArgs a
         run = k;
         part = false;
 #pragma unroll
-        for (int e = 0; e < N; ++e) sum[e] = 0.0f;
-      }
-      const typename G::wide w = widen<T>(v[u]);
+        for (int q = 0; q < P; ++q)
 #pragma unroll
-      for (int e = 0; e < N; ++e) sum[e] += w[e];
+          for (int e = 0; e < N; ++e) sum[q][e] = 0.0f;
+      }
+#pragma unroll
+      for (int q = 0; q < P; ++q) {
+        const typename C::wide w = __builtin_convertvector(v[u][q], typename C::wide);
+#pragma unroll
+        for (int e = 0; e < N; ++e) sum[q][e] += w[e];
+      }
     }
   }
   const uint32_t slot = part ? 0 : 1;
@@ -918,8 +941,9 @@ int ec_embed_grad(const void* d_tokens, int token_bytes, uint64_t n, const void*
   const auto go = [&](auto t, auto o) {
     typedef decltype(t) T;
     typedef decltype(o) O;
-    // a last group that starts early needs a whole one, and rows that are written
-    const bool tail = hidden < per_group || (accumulate && hidden % per_group);
+    // a last piece that starts early needs a whole one, and rows that are written
+    constexpr uint32_t kPiece = Columns<T, O>::kN;
+    const bool tail = hidden < kPiece || (accumulate && hidden % kPiece);
     const auto sum = accumulate ? tail ? sum_kernel<T, O, true, true> : sum_kernel<T, O, true, false>
                                 : tail ? sum_kernel<T, O, false, true> : sum_kernel<T, O, false, false>;
     uint32_t extra = zeros(behind);
