@@ -454,6 +454,28 @@ def test_token_logprobs_strided_rows(pkg, dev, dtype):
     assert none.logprobs.shape == (0, 3) and none.top_logprobs.shape == (0, 3, 2)
 
 
+def test_token_logprobs_of_one_row_and_of_no_vocabulary(pkg, dev):
+    x = torch.randn(40, generator=gen("one row")).to(dev)
+    target = torch.tensor(7, device=dev)
+    r = pkg.token_logprobs(x, target, entropy=True, top=4)
+    rows = pkg.token_logprobs(x[None], target[None], entropy=True, top=4)
+    assert r.logprobs.shape == () and r.top_tokens.shape == (4,)
+    assert all(torch.equal(a, b[0]) for a, b in zip(r, rows))
+    d = pkg.token_logprobs_grad(x, target, r.lse, r.entropy)
+    assert d.shape == (40,) and torch.equal(d, pkg.token_logprobs_grad(x[None], target[None], rows.lse, rows.entropy)[0])
+    none = torch.zeros(3, 0, device=dev)
+    t = torch.tensor([0, -100, 5], device=dev)
+    r = pkg.token_logprobs(none, t, entropy=True)
+    assert r.logprobs.tolist() == [0, 0, 0] and r.entropy.tolist() == [0, 0, 0]
+    assert r.lse.tolist() == [-math.inf] * 3
+    assert pkg.token_logprobs_grad(none, t, r.lse, r.lse).shape == (3, 0)
+    # one token, and rows that are one element apart from being broadcast
+    table = torch.randn(5, 12, device=dev)
+    assert torch.equal(pkg.embed(torch.tensor(3, device=dev), table), table[3])
+    g = pkg.embed_grad(torch.tensor(3, device=dev), table[0], 5)
+    assert torch.equal(g[3], table[0]) and int(g.count_nonzero(dim=1).ne(0).sum()) == 1
+
+
 @types
 def test_token_logprobs_grad_of_masked_rows(pkg, dev, dtype):
     vocab, low = 1000, torch.finfo(dtype).min
