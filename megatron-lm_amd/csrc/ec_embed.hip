@@ -126,8 +126,8 @@ struct ZeroArgs {
 constexpr uint64_t kLeastSpan = 32u << 10, kMostSpan = 256u << 10, kZeroSpans = 256;
 constexpr int kZeroShift = 6;
 // Rows of this many bytes and more are written one by a wave.  Narrower ones would leave most
-// of a wave idle, and share lines: 67 tokens, 116317 x 64 fp32, 38 us by rows, 16 flat;
-// 65536 tokens, 50304 x 2048, 147 and 172 (the flat form looks each 16 bytes' row up).
+// of a wave idle, and share lines: 67 tokens, 116317 x 64 fp32, 24 us by rows, 17 flat;
+// 65536 tokens, 50304 x 2048, 134 and 162 (the flat form looks each 16 bytes' row up).
 constexpr uint32_t kWideRow = 1024;
 
 typedef uint32_t __attribute__((ext_vector_type(4))) zero16_t;
@@ -453,14 +453,14 @@ __global__ void __launch_bounds__(kSortLanes) sort_scatter_kernel(const SortArgs
 // (With every run that crosses a tile's end split, the join took 35 us, now 9.)
 //
 // Bound by memory, gathered rows of 4 KiB at that: 65536 tokens of 2048 bf16, with the zeros
-// that ride along, in 104 us, 274 MB read and 294 MB written (5.5 TB/s).  The sums go
-// through the caches: a lane's 8 fp32 are two half-filled stores of a line (streamed
-// 170 us, cached 130).
+// that ride along, in 95 us, 274 MB read and 294 MB written (6.0 TB/s).  The sums go through
+// the caches, in whole lines (Columns): the whole call takes 134 us; whole lines streamed
+// 156, a lane's 8 fp32 as two stores of half lines 143.
 //
 // Tiles of 16 where there are few: more waves share the gathers' latency (tiles of 8 /
-// 16 / 32, us for the whole call: 2048 tokens of 1999 fp32 28.2 26.7 29.4; 16384 tokens, a
-// gradient of 131072 x 1024, 124.6 125.3 129.9; 32768 tokens, 50304 x 2048, 130.1 126.7 126.1;
-// 65536 of the same 155 152 147).
+// 16 / 32, us for the whole call: 67 tokens of 64 bf16 15.7 16.7 19.4; 2048 of 1999 fp32
+// 25.1 24.9 25.6; 16384 tokens, a gradient of 131072 x 1024, 120 120 121; 32768 tokens,
+// 50304 x 2048, 128 116 114; 65536 of the same 163 139 134).
 constexpr uint32_t kFewTokens = 16384;
 constexpr uint32_t kMaxTile = 32;   // two tiles' pairs in the lanes of a wave
 constexpr uint32_t tile_for(uint64_t n) { return n <= kFewTokens ? kMaxTile / 2 : kMaxTile; }
@@ -782,9 +782,10 @@ Work work_of(uint64_t n, uint64_t vocab, uint32_t hidden) {
 // Bytes of zeros that a launch of the sort takes along at least: about what is written
 // while it waits for its own loads.  It takes more where the sums' launch would be
 // left with more zeros than it reads of dout, which is what hides behind its gathers.
-// 0 / 20 / 40 / 60 / 100 / 200 MiB a launch, us for the whole call: 65536 tokens, 50304 x
-// 2048 bf16 to fp32 165 159 153 150 153 160; 8192 tokens of the same 126 113 111 107 108 102;
-// 16384 tokens, 131072 x 1024 166 149 158 139 138 128.
+// At least 0 / 20 / 40 / 60 / 100 / 200 MiB a launch, us for the whole call: 65536 tokens, 50304
+// x 2048 bf16 to fp32 137 136 134 134 142 151; 32768 tokens of the same 115 115 114 112 115
+// 125; 16384 tokens, 131072 x 1024 124 124 120 120 120 122.  (With all zeros in the sums'
+// launch 65536 tokens took 165 us where 40 MiB a launch took 153.)
 constexpr uint64_t kZeroBytes = 40u << 20;
 
 int check_tokens(const void* tokens, int token_bytes, uint64_t n, uint32_t hidden) {
