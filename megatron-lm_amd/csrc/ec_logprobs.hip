@@ -92,7 +92,9 @@ struct Running {
       const float to = fmaxf(top * c, -kMax);   // finite: a term below it is 0
       if (s != 0.0f) {
         const float by = exp2_hw(mc - to);
-        if (ENTROPY) t = by * (t - (to - mc) * s);
+        // (far behind, 0 times a distance that may be infinite with this lane's s: a mask's
+        // terms are 2^(the rounding of its x c), up to 2^128)
+        if (ENTROPY) t = by == 0.0f ? 0.0f : by * (t - (to - mc) * s);
         s *= by;
       }
       m = top;
@@ -250,7 +252,7 @@ __global__ void __launch_bounds__(B) logprob_kernel(const LogprobArgs a) {
   block_sums<kWaves, ENTROPY>(s, t, red);
   // every logit -infinity, or one of the rows that need d = (x - m) c
   const bool empty = m == -kInf && s == 0.0f;
-  const bool again = !empty && !(s > 0.0f && s < kInf);
+  const bool again = !empty && !(s > 0.0f && s < kInf && (!ENTROPY || __builtin_isfinite(t)));
   if (again) {
     s = t = 0.0f;
     for (uint32_t g = tid; g < a.groups; g += B) {
