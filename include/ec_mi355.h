@@ -415,11 +415,14 @@ int ec_token_logprobs(const void* d_logits, int type, uint64_t rows, uint64_t vo
 /* The gradient of ec_token_logprobs' log-probabilities and entropies:
  *   dlogits[j] = scale * (g * (j == target) - p[j] * (g + h * (log p[j] + H)))
  * with g = d_dlogprobs[i] (taken as 0 where the target lies outside [0, vocab)),
- * h = d_dentropy[i] and H = d_entropy[i] (both null: h = 0) and p from d_lse.
+ * h = d_dentropy[i] and H = d_entropy[i] (both null: h = 0) and p = exp(z - d_lse[i]),
+ * at most 1, z = scale * x rounded to fp32.
  * dlogits is of the logits' type, rows out_stride apart, and may be the logits
  * themselves.  A masked logit's gradient is 0, and so is the whole row's where
- * lse is -infinity or below -2^127 / log2 e (a row of nothing but masked logits, the
- * type's lowest value as a mask included). */
+ * lse is -infinity or below -2^127 / log2 e * min(1, scale) (a row of nothing but masked
+ * logits, the lowest value of fp32 or bf16 as a mask included; that of fp16 is a logit
+ * like others).  A row with a NaN or +infinity has NaN gradients, and a logit whose z
+ * overflows to +infinity has one. */
 int ec_token_logprobs_grad(const void* d_logits, int type, uint64_t rows, uint64_t vocab,
                            uint64_t row_stride, const int64_t* d_targets, const float* d_lse,
                            const float* d_dlogprobs, const float* d_entropy,

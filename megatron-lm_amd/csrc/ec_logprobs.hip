@@ -7,7 +7,9 @@
 // 2^fma(x, c, -mc) and the results are taken relative to the same mc,
 //   s = SUM 2^d,  d = x c - mc,    lse = (mc + log2 s) ln 2,
 //   log p = (d - log2 s) ln 2,     H = (log2 s - (SUM 2^d d) / s) ln 2,
-// so the rounding of mc cancels in log p and H.  x c leaves fp32's range where x
+// so the rounding of mc cancels in log p and H.  lse is given relative to z = scale * m as fp32
+// rounds it, m the largest logit: lse = z + (log2 s - fma(m, c, -mc)) ln 2, so that the
+// gradient, which takes z - lse, gives a logit that dominates probability 1.  x c leaves fp32's range where x
 // does not (a mask of the type's lowest value): rows that this touches, and rows
 // with a NaN or infinity, are gone over once more with d = (x - m) c.
 #include <hip/hip_runtime.h>
@@ -31,6 +33,13 @@ constexpr float kMax = 3.402823466e38f;
 
 __device__ __forceinline__ float exp2_hw(float v) { return __builtin_amdgcn_exp2f(v); }
 __device__ __forceinline__ float log2_hw(float v) { return __builtin_amdgcn_logf(v); }
+
+// scale * x and the sum with `more`, each rounded (not as one fma): the same product must be
+// rounded alike in the log of the sum and in what is compared with it.
+__device__ __forceinline__ float scaled_plus(float x, float scale, float more) {
+#pragma clang fp contract(off)
+  return x * scale + more;
+}
 
 // Group g of a row of `vocab` logits, -infinity past its end.
 template <typename T, bool STREAM>
@@ -274,7 +283,9 @@ __global__ void __launch_bounds__(B) logprob_kernel(const LogprobArgs a) {
     return ((again ? (x - m) * a.c : __builtin_fmaf(x, a.c, -mc)) - log2s) * kLn2;
   };
   if (tid == 0) {
-    gp(a.lse)[r] = empty ? -kInf : again ? m * a.scale + log2s * kLn2 : (mc + log2s) * kLn2;
+    // (an exponent of m is 0 but for the rounding of mc)
+    const float rest = again ? log2s : log2s - __builtin_fmaf(m, a.c, -mc);
+    gp(a.lse)[r] = empty ? -kInf : scaled_plus(m, a.scale, rest * kLn2);
     gp(a.logprobs)[r] = target >= 0 && target < (int64_t)a.vocab ? logprob(given) : 0.0f;
     if (ENTROPY) gp(a.entropy)[r] = empty ? 0.0f : (log2s - t / s) * kLn2;
   }
@@ -339,8 +350,11 @@ __global__ void __launch_bounds__(B) logprob_kernel(const LogprobArgs a) {
 }
 
 // ---------------------------------------------------------------- gradient --
-// dlogits = -p (A + B d) + scale g at the target, with d the base-2 exponent
-// relative to lse, A = scale (g + h H), B = scale h ln 2.
+// dlogits = -p (A + B d) + scale g at the target, with d = z - lse, p = e^d, A = scale (g + h H),
+// B = scale h.  z and the difference are rounded as in the forward pass, and only then taken to
+// base 2: fma(x, c, -lse log2 e) is one instruction less, but off by the rounding of the two
+// factors times log2 e, 2^-24 |lse|, and made probabilities above 1 of logits from 1e6 on.
+// p is at most 1, also from an lse that was found elsewhere and rounded otherwise.
 struct GradArgs {
   const void* logits;
   void* out;
@@ -352,8 +366,12 @@ struct GradArgs {
   uint64_t stride, out_stride;
   FastDiv by_slabs;
   uint32_t vocab, groups, slabs;   // slabs: workgroups of a row
-  float c, scale;
+  float scale, masked;             // an lse below `masked`: a row of nothing but masked logits
 };
+
+// (fp32 has lost what tells such a row's logits apart; 2^127 / log2 e, a third of the range, and
+// as much less as a scale below 1 brings the type's lowest value nearer)
+constexpr float kMaskedLse = -0x1p127f / kLog2e;
 
 // A lane takes one group, and the workgroups follow the memory's order: 8192 x 50304
 // bf16 in 247 us (6.7 TB/s; a copy kernel of the same form takes 244, the library's
@@ -373,22 +391,20 @@ __global__ void __launch_bounds__(kGradLanes) logprob_grad_kernel(const GradArgs
   const typename G::vec v = load_logits<T, STREAM>(row, gi, a.vocab);
   const int64_t target = gp(a.targets)[r];
   const float lse = gp(a.lse)[r];
-  // a row of masked logits only, also one masked with the type's lowest value
-  const float lse2 = lse * kLog2e;
-  const bool has = target >= 0 && target < (int64_t)a.vocab, empty = lse2 == -kInf;
+  const bool has = target >= 0 && target < (int64_t)a.vocab, empty = lse < a.masked;
   const float g = has ? (float)gp(a.dlogprobs)[r] : 0.0f;
   float A = a.scale * g, slope = 0.0f;
   if (ENTROPY) {
     const float h = gp(a.dentropy)[r];
     A += a.scale * h * gp(a.entropy)[r];
-    slope = a.scale * h * kLn2;
+    slope = a.scale * h;
   }
   const typename G::wide x = widen<T>(v);
   typename G::wide w;
 #pragma unroll
   for (int e = 0; e < N; ++e) {
-    const float d = __builtin_fmaf(x[e], a.c, -lse2);
-    const float p = exp2_hw(d);
+    const float d = __builtin_elementwise_minimum(scaled_plus(x[e], a.scale, -lse), 0.0f);   // NaN stays
+    const float p = exp2_hw(d * kLog2e);
     const float by = ENTROPY ? __builtin_fmaf(fmaxf(d, -200.0f), slope, A) : A;
     w[e] = empty ? 0.0f : -p * by;
   }
@@ -470,7 +486,7 @@ int ec_token_logprobs_grad(const void* d_logits, int type, uint64_t rows, uint64
   if (!d_lse || !d_dlogprobs || !d_dlogits || out_stride < vocab) return EC_EINVAL;
   if (!d_entropy != !d_dentropy) return EC_EINVAL;
   GradArgs a = {d_logits, d_dlogits, d_targets, d_lse, d_dlogprobs, d_entropy, d_dentropy,
-                row_stride, out_stride, {}, (uint32_t)vocab, 0, 0, scale * kLog2e, scale};
+                row_stride, out_stride, {}, (uint32_t)vocab, 0, 0, scale, kMaskedLse * std::min(scale, 1.0f)};
   const uint32_t per_group = 16 / type_bytes(type);
   a.groups = (uint32_t)((vocab + per_group - 1) / per_group);
   const bool streamed = rows * vocab * type_bytes(type) > kStreamBytes;
