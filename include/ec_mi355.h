@@ -386,7 +386,8 @@ uint64_t ec_embed_grad_workspace(uint64_t n, uint64_t vocab, uint32_t hidden);
  * touched.  The tokens are sorted in d_work (work_bytes of at least
  * ec_embed_grad_workspace, EC_EINVAL otherwise; 16-byte aligned, EC_EALIGN),
  * equal tokens in the order of their positions; no atomics.  EC_ERANGE for
- * n >= 2^31, vocab >= 2^31 or hidden > 2^20. */
+ * n >= 2^31, vocab >= 2^31, hidden > 2^20, or a launch of 2^32 lanes (n within a few
+ * thousand of 2^31; 500 GB and more of dout or of the gradient). */
 int ec_embed_grad(const void* d_tokens, int token_bytes, uint64_t n, const void* d_dout, int type,
                   uint64_t dout_stride, uint64_t vocab, uint32_t hidden, int64_t vocab_start,
                   float scale, void* d_grad, int grad_type, uint64_t grad_stride, int accumulate,

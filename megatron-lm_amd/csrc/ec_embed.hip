@@ -8,6 +8,7 @@
 
 #include "ec_types.h"
 #include "fastdiv.h"
+#include "routes.h"
 
 namespace ec {
 namespace {
@@ -816,10 +817,16 @@ int ec_embed(const void* d_tokens, int token_bytes, uint64_t n, const void* d_ta
   const bool streamed = a.groups >= kEmbedStreamGroups && n * hidden * type_bytes(type) >= kEmbedStream;
   while (a.shift < 6 && (1u << a.shift) * kEmbedGroups < a.groups) ++a.shift;
   const uint32_t rows = kEmbedWaves * (kLanes >> a.shift), wide = kEmbedGroups << a.shift;
-  const dim3 grid((a.n + rows - 1) / rows, (a.groups + wide - 1) / wide);
+  const uint64_t most = max_grid(kEmbedWaves * kLanes) * rows;   // tokens of one launch
   return with_type(type, [&](auto t) {
     const auto kernel = streamed ? embed_kernel<decltype(t), true> : embed_kernel<decltype(t), false>;
-    kernel<<<grid, kEmbedWaves * kLanes, 0, (hipStream_t)stream>>>(a);
+    for (uint64_t at = 0; at < n; at += most) {
+      a.n = (uint32_t)std::min(most, n - at);
+      a.tokens = (const uint8_t*)d_tokens + at * token_bytes;
+      a.out = (uint8_t*)d_out + at * hidden * type_bytes(type);
+      const dim3 grid((a.n + rows - 1) / rows, (a.groups + wide - 1) / wide);
+      kernel<<<grid, kEmbedWaves * kLanes, 0, (hipStream_t)stream>>>(a);
+    }
     return launched();
   });
 }
@@ -901,7 +908,10 @@ int ec_embed_grad(const void* d_tokens, int token_bytes, uint64_t n, const void*
   a.join_columns = (hidden + kLanes * 4 - 1) / (kLanes * 4);
   const uint64_t join_blocks =
       a.tiles > 1 ? (uint64_t)(a.tiles + kJoinTiles - 2) / kJoinTiles * a.join_columns : 0;
-  if (sum_blocks + all_zero > 0x7fffffffull || join_blocks + all_zero > 0x7fffffffull)
+  // each launch as if it took all zeros along
+  const auto past = [&](uint64_t blocks, uint64_t lanes) { return (blocks + all_zero) * lanes >= 1ull << 32; };
+  if (past(sum_blocks, kSumWaves * kLanes) || past(join_blocks, kJoinWaves * kLanes) ||
+      past(w.sort_tiles, w.small ? kSmallLanes : kSortLanes))
     return EC_ERANGE;
   a.sum_blocks = (uint32_t)sum_blocks;
   a.join_blocks = (uint32_t)join_blocks;

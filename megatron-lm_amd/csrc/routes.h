@@ -113,7 +113,7 @@ constexpr bool batch_table_reached(int m) {
   return false;
 }
 
-// Workgroups of one launch at most; more work loops in the kernel.  HIP refuses
+// Workgroups of one launch at most; more work loops in the kernel or takes another launch.  HIP refuses
 // a grid of 2^32 lanes and more.
 constexpr uint64_t max_grid(uint64_t lanes) {
   constexpr uint64_t kMax = 1u << 24;
