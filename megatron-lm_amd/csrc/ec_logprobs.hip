@@ -21,6 +21,7 @@
 
 #include "ec_types.h"
 #include "fastdiv.h"
+#include "routes.h"
 
 namespace ec {
 namespace {
@@ -452,17 +453,27 @@ int ec_token_logprobs(const void* d_logits, int type, uint64_t rows, uint64_t vo
   a.groups = (uint32_t)((vocab + per_group - 1) / per_group);
   const bool streamed = rows * vocab * type_bytes(type) > kStreamBytes;
   const bool wide = rows <= kFewRows || a.groups >= kWideGroups;
-  const dim3 grid((uint32_t)rows);
+  const uint64_t most = max_grid(wide ? kWideLanes : kShortLanes);   // rows of one launch
   const hipStream_t st = (hipStream_t)stream;
   return with_type(type, [&](auto t) {
     typedef decltype(t) T;
     const auto go = [&](auto entropy, auto tops, auto stream_) {
       constexpr bool E = decltype(entropy)::value, K = decltype(tops)::value;
       constexpr bool S = decltype(stream_)::value;
-      if (wide)
-        logprob_kernel<T, kWideLanes, E, K, S><<<grid, kWideLanes, 0, st>>>(a);
-      else
-        logprob_kernel<T, kShortLanes, E, K, S><<<grid, kShortLanes, 0, st>>>(a);
+      for (uint64_t at = 0; at < rows; at += most) {
+        const dim3 grid((uint32_t)std::min(most, rows - at));
+        a.logits = (const T*)d_logits + at * row_stride;
+        a.targets = d_targets + at;
+        a.logprobs = d_logprobs + at;
+        a.lse = d_lse + at;
+        if (E) a.entropy = d_entropy + at;
+        if (K) a.top_logprobs = d_top_logprobs + at * top;
+        if (K) a.top_tokens = d_top_tokens + at * top;
+        if (wide)
+          logprob_kernel<T, kWideLanes, E, K, S><<<grid, kWideLanes, 0, st>>>(a);
+        else
+          logprob_kernel<T, kShortLanes, E, K, S><<<grid, kShortLanes, 0, st>>>(a);
+      }
       return launched();
     };
     const std::true_type yes;
@@ -492,8 +503,7 @@ int ec_token_logprobs_grad(const void* d_logits, int type, uint64_t rows, uint64
   const bool streamed = rows * vocab * type_bytes(type) > kStreamBytes;
   a.slabs = (a.groups + kGradLanes - 1) / kGradLanes;
   a.by_slabs = make_fastdiv(a.slabs);
-  if (rows * a.slabs > 0x7fffffffull) return EC_ERANGE;
-  const uint32_t grid = (uint32_t)rows * a.slabs;
+  const uint64_t most = max_grid(kGradLanes) / a.slabs;   // rows of one launch; a row has at most 2^21
   const hipStream_t st = (hipStream_t)stream;
   return with_type(type, [&](auto t) {
     typedef decltype(t) T;
@@ -501,7 +511,19 @@ int ec_token_logprobs_grad(const void* d_logits, int type, uint64_t rows, uint64
                                               : logprob_grad_kernel<T, true, false>
                                    : streamed ? logprob_grad_kernel<T, false, true>
                                               : logprob_grad_kernel<T, false, false>;
-    kernel<<<grid, kGradLanes, 0, st>>>(a);
+    for (uint64_t at = 0; at < rows; at += most) {
+      const uint32_t grid = (uint32_t)(std::min(most, rows - at) * a.slabs);
+      a.logits = (const T*)d_logits + at * row_stride;
+      a.out = (T*)d_dlogits + at * out_stride;
+      a.targets = d_targets + at;
+      a.lse = d_lse + at;
+      a.dlogprobs = d_dlogprobs + at;
+      if (d_dentropy) {
+        a.entropy = d_entropy + at;
+        a.dentropy = d_dentropy + at;
+      }
+      kernel<<<grid, kGradLanes, 0, st>>>(a);
+    }
     return launched();
   });
 }

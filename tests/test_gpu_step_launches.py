@@ -28,3 +28,24 @@ def test_embed_of_more_tokens_than_a_launch(pkg, dev):
     assert torch.equal(out[rows], want)
     del out
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("entropy,top", [(False, 0), (True, 2)])
+def test_logprobs_of_more_rows_than_a_launch(pkg, dev, entropy, top):
+    """More rows of three logits than a launch takes in any form; the gradient's rows run over two and three launches."""
+    room(16)
+    n, few = (1 << 25) + 7, 1013
+    base = torch.randn(few, 3, generator=gen("rows")).to(dev)
+    goal = torch.randint(-1, 4, (few,), generator=gen("goals")).to(dev)
+    at = torch.arange(n, device=dev) % few
+    x, target = base.bfloat16()[at], goal[at]
+    want = pkg.token_logprobs(base.bfloat16(), goal, entropy=entropy, top=top)
+    r = pkg.token_logprobs(x, target, entropy=entropy, top=top)
+    for got, some in zip(r, want):
+        if some is not None:
+            assert torch.equal(got, some[at])
+    kw = dict(entropy=r.entropy, dentropy=r.lse) if entropy else {}
+    some = dict(entropy=want.entropy, dentropy=want.lse) if entropy else {}
+    d = pkg.token_logprobs_grad(base.bfloat16(), goal, want.lse, want.logprobs, **some)
+    assert torch.equal(pkg.token_logprobs_grad(x, target, r.lse, r.logprobs, **kw), d[at])
+    torch.cuda.empty_cache()
