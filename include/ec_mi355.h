@@ -450,7 +450,7 @@ typedef struct {
 /* *d_norm = the norm of grad_scale * g over all elements g of n_items pieces
  * (d_items is a device array), in fp32: the square root of the sum of squares,
  * taken in fp64, or the largest magnitude.  A NaN or infinity among the
- * elements makes the norm NaN or infinity.  n_items 0: 0. */
+ * elements makes the norm NaN or infinity.  n_items 0: 0; EC_ERANGE for more than 2^28. */
 int ec_grad_norm(const ec_grad_item* d_items, uint32_t n_items, float grad_scale, int norm,
                  void* d_work, float* d_norm, ec_stream_t stream);
 

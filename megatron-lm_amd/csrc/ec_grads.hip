@@ -14,6 +14,7 @@
 #include <cmath>
 
 #include "ec_types.h"
+#include "routes.h"
 
 namespace ec {
 namespace {
@@ -218,7 +219,7 @@ __global__ void __launch_bounds__(kBlockLanes) grad_clip_kernel(
   });
 }
 
-constexpr uint32_t kMaxPieces = 1u << 28;   // the clip's grid
+constexpr uint32_t kMaxPieces = 1u << 28;   // of 16384 elements: more than any memory
 
 int check_list(const ec_grad_item* items, uint32_t n, float scale, int norm, const void* work,
                const float* out) {
@@ -255,10 +256,9 @@ int run_norm(const ec_grad_item* items, uint32_t n, float scale, double* parts, 
 template <int NORM>
 int run_clip(const ec_grad_item* items, uint32_t n, float scale, float max_norm, const float* given,
              double* parts, float* norm, hipStream_t st) {
-  const uint32_t blocks = std::max(1u, n) * kSplit;
   if (n && n <= kFewPieces && !given) {
     const uint32_t n_parts = run_parts<NORM>(items, n, parts, st);
-    grad_clip_kernel<NORM, true, false><<<blocks, kBlockLanes, 0, st>>>(
+    grad_clip_kernel<NORM, true, false><<<n * kSplit, kBlockLanes, 0, st>>>(
         items, n, parts, n_parts, scale, max_norm, given, norm);
     return launched();
   }
@@ -269,7 +269,14 @@ int run_clip(const ec_grad_item* items, uint32_t n, float scale, float max_norm,
   }
   const auto kernel = n > kManyPieces ? grad_clip_kernel<NORM, false, true>
                                       : grad_clip_kernel<NORM, false, false>;
-  kernel<<<blocks, kBlockLanes, 0, st>>>(items, n, parts, 0, scale, max_norm, given, norm);
+  // what a launch takes at most, from the list's end; an empty list's norm is still written
+  constexpr uint32_t kMost = (uint32_t)(max_grid(kBlockLanes) / kSplit);
+  do {
+    const uint32_t some = std::min(n, kMost);
+    n -= some;
+    kernel<<<std::max(1u, some) * kSplit, kBlockLanes, 0, st>>>(items + n, some, parts, 0, scale, max_norm,
+                                                                given, norm);
+  } while (n);
   return launched();
 }
 
