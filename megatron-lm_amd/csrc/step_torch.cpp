@@ -4,6 +4,7 @@
 // Each function returns the status of the C call first, for the caller to turn into
 // its error type, then what it allocated.
 #include <torch/extension.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
 #include <algorithm>
@@ -86,6 +87,8 @@ Rows rows_of(const Tensor& t, const char* what, const c10::Device* device) {
                         "rows that do not overlap");
 }
 
+// torch's current stream of the operands' device, for a call under a DeviceGuard: the
+// default stream's handle is null, which is that of whatever device is current.
 ec_stream_t stream_of(const c10::Device& device) {
   return reinterpret_cast<ec_stream_t>(c10::hip::getCurrentHIPStream(device.index()).stream());
 }
@@ -129,6 +132,7 @@ py::tuple embed(const Tensor& tokens, const Tensor& table, double scale, int64_t
                           shape_text(table.sizes()));
   const Rows rows = rows_of(table, "table", nullptr);
   const c10::Device device = table.device();
+  const c10::DeviceGuard guard(device);
   check_dense(tokens, "tokens", &device);
   const int bytes = token_bytes(tokens);
   const auto shape = with_last(tokens.sizes(), (int64_t)rows.width);
@@ -159,6 +163,7 @@ py::tuple embed_grad(const Tensor& tokens, const Tensor& dout, int64_t vocab, do
   const int type = type_code(dout, "dout");
   const Rows rows = rows_of(dout, "dout", nullptr);
   const c10::Device device = dout.device();
+  const c10::DeviceGuard guard(device);
   check_dense(tokens, "tokens", &device);
   const int bytes = token_bytes(tokens);
   if (vocab < 0) throw py::value_error("vocab_size must not be negative");
@@ -197,6 +202,7 @@ py::tuple token_logprobs(const Tensor& logits, const Tensor& targets, double sca
   const int type = type_code(logits, "logits");
   const Rows rows = rows_of(logits, "logits", nullptr);
   const c10::Device device = logits.device();
+  const c10::DeviceGuard guard(device);
   check_dense(targets, "targets", &device);
   check_type(targets, "targets", at::kLong);
   const auto lead = logits.sizes().slice(0, logits.dim() - 1);
@@ -230,6 +236,7 @@ py::tuple token_logprobs_grad(const Tensor& logits, const Tensor& targets, const
   const int type = type_code(logits, "logits");
   const Rows rows = rows_of(logits, "logits", nullptr);
   const c10::Device device = logits.device();
+  const c10::DeviceGuard guard(device);
   const auto lead = logits.sizes().slice(0, logits.dim() - 1);
   check_dense(targets, "targets", &device);
   check_type(targets, "targets", at::kLong);
@@ -339,6 +346,7 @@ Tensor grad_items(const std::vector<Tensor>& grads, const std::optional<std::vec
 py::tuple grad_call(const Tensor& items, double grad_scale, int64_t norm,
                     std::optional<double> max_norm, std::optional<Tensor> given) {
   const c10::Device device = items.device();
+  const c10::DeviceGuard guard(device);
   const auto opts = at::TensorOptions().device(device);
   const Tensor work = at::empty({EC_GRAD_WORK}, opts.dtype(at::kByte));
   const Tensor result = at::empty({}, opts.dtype(at::kFloat));
