@@ -12,6 +12,7 @@
 // The C ABI (include/ec_mi355.h) stays free of torch types; this module is a
 // client of it, like the ctypes binding, and links libec_mi355.so.
 #include <torch/extension.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
 #include <cstdint>
@@ -71,6 +72,8 @@ py::tuple shard_call(int64_t op, const std::string& coeff, int64_t m,
                             std::to_string(nb));
     in_ptrs[j] = static_cast<const uint8_t*>(shards[j].data_ptr());
   }
+  // (a default stream's handle is null, which is that of whatever device is current)
+  const c10::DeviceGuard guard(device);
   std::vector<at::Tensor> outs;
   if (out.has_value()) {
     outs = *out;

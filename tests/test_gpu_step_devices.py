@@ -1,4 +1,4 @@
-"""Step operators on tensors of a device that is not the current one.  One device shows only that the calls keep the
+"""Step operators and flat-shard calls on tensors of a device that is not the current one.  One device shows only that the calls keep the
 current one; the rest needs two."""
 import pytest
 import torch
@@ -21,7 +21,9 @@ def everything(pkg, dev):
     out = [e, pkg.embed_grad(tok, e, 70), *r, d, lst.norm(), lst.clip(0.5), table, x, pkg.grad_norm([x])]
     leaf = table.detach().requires_grad_()
     pkg.token_logprobs(pkg.embed(tok[:30], leaf), target % 40).logprobs.sum().backward()
-    return [t.cpu() for t in out + [leaf.grad]]
+    shards = [torch.randint(0, 256, (5000,), dtype=torch.uint8, generator=g).to(dev) for _ in range(4)]
+    coded = [pkg.xor_encode(shards), *pkg.rs_encode(shards, 2)]
+    return [t.cpu() for t in out + coded + [leaf.grad]]
 
 
 @pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two devices")
@@ -35,5 +37,5 @@ def test_on_a_device_that_is_not_current(pkg, dev):
 
 def test_the_current_device_stays(pkg, dev):
     before = torch.cuda.current_device()
-    assert len(everything(pkg, dev)) == 14
+    assert len(everything(pkg, dev)) == 17
     assert torch.cuda.current_device() == before
