@@ -107,6 +107,12 @@ bool share(const void* a, const Rows& ra, uint64_t wa, const void* b, const Rows
   return !(d >= ra.width * wa && d + rb.width * wb <= pitch);
 }
 
+// A caller's tensor was written: as after torch's own in-place operations, a backward pass that
+// saved it before raises.
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 void check_apart(bool together, const char* a, const char* b) {
   if (together) throw py::value_error(std::string(a) + " shares memory with " + b);
 }
@@ -155,6 +161,7 @@ py::tuple embed(const Tensor& tokens, const Tensor& table, double scale, int64_t
           ? EC_ERANGE
           : ec_embed(tokens.data_ptr(), bytes, n, table.data_ptr(), type, rows.n,
                      (uint32_t)rows.width, rows.stride, start, (float)scale, result.data_ptr(), st);
+  if (out.has_value()) written(result);
   return py::make_tuple(status, result);
 }
 
@@ -194,6 +201,7 @@ py::tuple embed_grad(const Tensor& tokens, const Tensor& dout, int64_t vocab, do
                                    rows.stride, (uint64_t)vocab, hidden, start, (float)scale,
                                    grad.data_ptr(), (int)grad_type, g.stride, accumulate,
                                    work.data_ptr(), need, stream_of(device));
+  if (out.has_value()) written(grad);
   return py::make_tuple(status, grad, work);
 }
 
@@ -270,12 +278,18 @@ py::tuple token_logprobs_grad(const Tensor& logits, const Tensor& targets, const
   const int status = ec_token_logprobs_grad(
       logits.data_ptr(), type, rows.n, rows.width, rows.stride, targets.data_ptr<int64_t>(), l, g,
       h, dh, (float)scale, result.data_ptr(), o.stride, stream_of(device));
+  if (out.has_value()) written(result);
   return py::make_tuple(status, result);
 }
 
+// The tensors that a clip of a list writes.
+struct Written {
+  std::vector<Tensor> tensors;
+};
+
 // The pieces of a list of gradients, as the bytes of an ec_grad_item array (a CPU
-// tensor), and whether any lie elsewhere than they are read.
-Tensor grad_items(const std::vector<Tensor>& grads, const std::optional<std::vector<Tensor>>& out) {
+// tensor), and the tensors that a clip writes.
+py::tuple grad_items(const std::vector<Tensor>& grads, const std::optional<std::vector<Tensor>>& out) {
   if (out && out->size() != grads.size())
     throw py::value_error("out: expected " + std::to_string(grads.size()) + " tensors, got " +
                           std::to_string(out->size()));
@@ -339,11 +353,11 @@ Tensor grad_items(const std::vector<Tensor>& grads, const std::optional<std::vec
   }
   const Tensor bytes = at::empty({(int64_t)(items.size() * sizeof(ec_grad_item))}, at::kByte);
   if (!items.empty()) std::memcpy(bytes.data_ptr(), items.data(), items.size() * sizeof(ec_grad_item));
-  return bytes;
+  return py::make_tuple(bytes, Written{out ? *out : grads});
 }
 
 // ec_grad_norm (max_norm empty) or ec_grad_clip over an uploaded list.
-py::tuple grad_call(const Tensor& items, double grad_scale, int64_t norm,
+py::tuple grad_call(const Tensor& items, const Written& list, double grad_scale, int64_t norm,
                     std::optional<double> max_norm, std::optional<Tensor> given) {
   const c10::Device device = items.device();
   const c10::DeviceGuard guard(device);
@@ -364,6 +378,7 @@ py::tuple grad_call(const Tensor& items, double grad_scale, int64_t norm,
     }
     status = ec_grad_clip(d, n, (float)grad_scale, (int)norm, (float)*max_norm, g, work.data_ptr(),
                           result.data_ptr<float>(), st);
+    for (const Tensor& t : list.tensors) written(t);
   } else {
     status = ec_grad_norm(d, n, (float)grad_scale, (int)norm, work.data_ptr(),
                           result.data_ptr<float>(), st);
@@ -385,7 +400,8 @@ void bind_step(py::module_& mod) {
   mod.def("token_logprobs_grad", &token_logprobs_grad, py::arg("logits"), py::arg("targets"),
           py::arg("lse"), py::arg("dlogprobs"), py::arg("entropy"), py::arg("dentropy"),
           py::arg("scale"), py::arg("out") = none);
+  py::class_<Written>(mod, "Written");
   mod.def("grad_items", &grad_items, py::arg("grads"), py::arg("out") = none);
-  mod.def("grad_call", &grad_call, py::arg("items"), py::arg("grad_scale"), py::arg("norm"),
+  mod.def("grad_call", &grad_call, py::arg("items"), py::arg("list"), py::arg("grad_scale"), py::arg("norm"),
           py::arg("max_norm") = none, py::arg("given") = none);
 }

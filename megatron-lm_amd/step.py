@@ -204,7 +204,7 @@ class GradList:
     def __init__(self, grads: Sequence[torch.Tensor], out: Optional[Sequence[torch.Tensor]] = None):
         self.grads = list(grads)
         self.out = None if out is None else list(out)
-        items = _lib.shards().grad_items(self.grads, self.out)
+        items, self._written = _lib.shards().grad_items(self.grads, self.out)
         self.device = self.grads[0].device if self.grads else \
             torch.device("cuda", torch.cuda.current_device())
         with torch.cuda.device(self.device):
@@ -218,7 +218,8 @@ class GradList:
             on = torch.cuda.current_stream(self.device) if stream is None else stream
             on.wait_event(self.uploaded)
             _hold(on, self._items)
-        return _call(what, _lib.shards().grad_call, self._items, stream, self._items, *args)[0]
+        return _call(what, _lib.shards().grad_call, self._items, stream, self._items, self._written,
+                     *args)[0]
 
     def norm(self, norm_type: float = 2.0, *, grad_scale: float = 1.0, stream=None) -> torch.Tensor:
         """The norm of grad_scale times all elements, a 0-d fp32 tensor: the square root of the sum
