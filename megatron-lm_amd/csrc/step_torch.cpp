@@ -288,8 +288,10 @@ struct Written {
 };
 
 // The pieces of a list of gradients, as the bytes of an ec_grad_item array (a CPU
-// tensor), and the tensors that a clip writes.
-py::tuple grad_items(const std::vector<Tensor>& grads, const std::optional<std::vector<Tensor>>& out) {
+// tensor), and the tensors that a clip writes; clips false: a list for norms only, whose tensors
+// may overlap.
+py::tuple grad_items(const std::vector<Tensor>& grads, const std::optional<std::vector<Tensor>>& out,
+                     bool clips) {
   if (out && out->size() != grads.size())
     throw py::value_error("out: expected " + std::to_string(grads.size()) + " tensors, got " +
                           std::to_string(out->size()));
@@ -319,7 +321,7 @@ py::tuple grad_items(const std::vector<Tensor>& grads, const std::optional<std::
     const uint64_t n = (uint64_t)src.numel();
     const uint64_t from = reinterpret_cast<uint64_t>(src.data_ptr());
     const uint64_t to = reinterpret_cast<uint64_t>(dst.data_ptr());
-    if (n) {
+    if (n && clips) {
       read.push_back({from, from + n * src.element_size(), i});
       written.push_back({to, to + n * dst.element_size(), i});
     }
@@ -353,7 +355,7 @@ py::tuple grad_items(const std::vector<Tensor>& grads, const std::optional<std::
   }
   const Tensor bytes = at::empty({(int64_t)(items.size() * sizeof(ec_grad_item))}, at::kByte);
   if (!items.empty()) std::memcpy(bytes.data_ptr(), items.data(), items.size() * sizeof(ec_grad_item));
-  return py::make_tuple(bytes, Written{out ? *out : grads});
+  return py::make_tuple(bytes, Written{!clips ? std::vector<Tensor>() : out ? *out : grads});
 }
 
 // ec_grad_norm (max_norm empty) or ec_grad_clip over an uploaded list.
@@ -401,7 +403,8 @@ void bind_step(py::module_& mod) {
           py::arg("lse"), py::arg("dlogprobs"), py::arg("entropy"), py::arg("dentropy"),
           py::arg("scale"), py::arg("out") = none);
   py::class_<Written>(mod, "Written");
-  mod.def("grad_items", &grad_items, py::arg("grads"), py::arg("out") = none);
+  mod.def("grad_items", &grad_items, py::arg("grads"), py::arg("out") = none,
+          py::arg("clips") = true);
   mod.def("grad_call", &grad_call, py::arg("items"), py::arg("list"), py::arg("grad_scale"), py::arg("norm"),
           py::arg("max_norm") = none, py::arg("given") = none);
 }

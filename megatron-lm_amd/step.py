@@ -201,10 +201,12 @@ class GradList:
     counts, any of the types: bf16 gradients into fp32 ones), or in place; no two of the tensors
     written may overlap.  The list keeps the tensors alive; gradients that are replaced by other tensors need a new list."""
 
+    _clips = True
+
     def __init__(self, grads: Sequence[torch.Tensor], out: Optional[Sequence[torch.Tensor]] = None):
         self.grads = list(grads)
         self.out = None if out is None else list(out)
-        items, self._written = _lib.shards().grad_items(self.grads, self.out)
+        items, self._written = _lib.shards().grad_items(self.grads, self.out, self._clips)
         self.device = self.grads[0].device if self.grads else \
             torch.device("cuda", torch.cuda.current_device())
         with torch.cuda.device(self.device):
@@ -240,10 +242,16 @@ class GradList:
                          _norm_code(norm_type), float(max_norm), norm)
 
 
+class _NormList(GradList):
+    """A list that is only read: its tensors may overlap."""
+    _clips = False
+
+
 def grad_norm(grads: Sequence[torch.Tensor], norm_type: float = 2.0, *, grad_scale: float = 1.0,
               stream=None) -> torch.Tensor:
-    """``GradList(grads).norm(...)``, for a list that is used once."""
-    return GradList(grads).norm(norm_type, grad_scale=grad_scale, stream=stream)
+    """``GradList(grads).norm(...)``, for a list that is used once.  Nothing is written, so the tensors
+    may overlap, and one that is in the list twice counts twice."""
+    return _NormList(grads).norm(norm_type, grad_scale=grad_scale, stream=stream)
 
 
 def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float = 2.0, *,
