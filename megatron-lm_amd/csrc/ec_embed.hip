@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(kEmbedWaves * kLanes) embed_kernel(const Embed
 // sorted tokens: workgroups that write zeros ride along in the sort's launches, which
 // leave the memory idle, and in the sums' launch.  Each takes the rows of 32 to 256 KiB and learns
 // which of them occur from bits that the sort's first launch collected (one bit per row
-// and tile of tokens), or, for few tokens, from the tokens themselves.
+// and span of the sort's tokens), or, for few tokens, from the tokens themselves.
 enum ZeroMode : int { kZeroSeen, kZeroScan, kZeroAll };
 
 struct Tokens {
@@ -113,10 +113,10 @@ struct Tokens {
 
 struct ZeroArgs {
   uint8_t* grad;
-  const uint32_t* seen;      // [tiles][words]
+  const uint32_t* seen;      // [spans][words]
   uint64_t stride;           // of the rows, in bytes
   FastDiv by_row;            // by row_bytes
-  uint32_t row_bytes, words, tiles;
+  uint32_t row_bytes, words, spans;
   int shift;                 // a workgroup's rows: 32 << shift
   uint32_t first, blocks;    // workgroups before this launch's, and in it
   int mode;
@@ -187,8 +187,8 @@ __device__ __forceinline__ void zero_block(const ZeroArgs& z, const Tokens& tok,
     const uint32_t w = t & (words - 1);
     uint32_t found = 0;
     if (w0 + w < z.words)
-      for (uint32_t tile = t >> z.shift; tile < z.tiles; tile += kAll >> z.shift)
-        found |= gp(z.seen)[(uint64_t)tile * z.words + w0 + w];
+      for (uint32_t span = t >> z.shift; span < z.spans; span += kAll >> z.shift)
+        found |= gp(z.seen)[(uint64_t)span * z.words + w0 + w];
     if (found) atomicOr(&bits[w], found);
   } else if (z.mode == kZeroScan) {
     for (uint32_t i = t; i < tok.n; i += kAll * 8) {
@@ -227,10 +227,10 @@ struct SortArgs {
   const uint32_t* pos;
   uint32_t* keys_out;
   uint32_t* pos_out;
-  uint32_t* counts;        // [tiles][2^bits]
-  uint32_t* seen;          // the first pass: [tiles][words], a bit for each row that occurs
+  uint32_t* counts;        // [spans][2^bits]
+  uint32_t* seen;          // the first pass: [spans][words], a bit for each row that occurs
   ZeroArgs zero;
-  uint32_t n, tiles, words;
+  uint32_t n, spans, walk, words;   // a span is `walk` tiles
   int shift, bits, passes;
 };
 
@@ -350,40 +350,46 @@ __global__ void __launch_bounds__(kSmallLanes) sort_small_kernel(const SortArgs 
 }
 
 // More tokens: digits of at most 9 bits (two of 8 for a vocabulary of 50304, two of 9
-// up to 2^18), a pass of two launches.  Each workgroup counts the digits of its
-// tile; then each sums the counts of the tiles before its own (and of the smaller
-// digits) and scatters its tile.  Bound by the latency of a few dependent loads: 5 and 7.5 us
+// below 2^18), a pass of two launches.  Each workgroup counts the digits of its
+// span; then each sums the counts of the spans before its own (and of the smaller
+// digits) and scatters its span.  Bound by the latency of a few dependent loads: 5 and 7.5 us
 // for 65536 tokens (7 and 20 with tiles of 4096 and each load waited for by itself).
+// A span is one tile, or, of more than kMaxSpans tiles (2^20 tokens), as many as leave that many
+// spans, one after the other: every workgroup reads the counts of all, which with a span
+// for each tile grew with the tokens' square.
 constexpr int kSortLanes = 512;
 constexpr int kSortWaves = kSortLanes / kLanes;
 constexpr int kSortSteps = 4;                        // items per lane
 constexpr uint32_t kSortTile = kSortLanes * kSortSteps;
 constexpr int kMaxDigit = 9;                         // a lane for each value
+constexpr uint32_t kMaxSpans = 512;                  // two workgroups a CU
 constexpr uint32_t kCountsAhead = 32;
 
 __global__ void __launch_bounds__(kSortLanes) sort_count_kernel(const SortArgs a) {
   __shared__ uint32_t count[1 << kMaxDigit];
   extern __shared__ uint32_t seen[];   // the first pass: `words` of them
-  if (blockIdx.x >= a.tiles)
-    return zero_block<kSortWaves>(a.zero, a.tok, blockIdx.x - a.tiles);
+  if (blockIdx.x >= a.spans)
+    return zero_block<kSortWaves>(a.zero, a.tok, blockIdx.x - a.spans);
   const uint32_t bins = 1u << a.bits, t = threadIdx.x;
   const uint32_t words = a.seen ? a.words : 0;
   count[t] = 0;
   for (uint32_t w = t; w < words; w += kSortLanes) seen[w] = 0;
   __syncthreads();
-  const uint32_t base = blockIdx.x * kSortTile;
-  uint32_t key[kSortSteps];
+  for (uint32_t tile = 0; tile < a.walk; ++tile) {
+    const uint32_t base = (blockIdx.x * a.walk + tile) * kSortTile;
+    uint32_t key[kSortSteps];
 #pragma unroll
-  for (int s = 0; s < kSortSteps; ++s) {
-    const uint32_t i = base + s * kSortLanes + t;
-    key[s] = i < a.n ? sort_key(a, i) : 0;
-  }
-#pragma unroll
-  for (int s = 0; s < kSortSteps; ++s)
-    if (base + s * kSortLanes + t < a.n) {
-      atomicAdd(&count[(key[s] >> a.shift) & (bins - 1)], 1u);
-      if (words && key[s] < (uint32_t)a.tok.vocab) atomicOr(&seen[key[s] / 32], 1u << (key[s] % 32));
+    for (int s = 0; s < kSortSteps; ++s) {
+      const uint32_t i = base + s * kSortLanes + t;
+      key[s] = i < a.n ? sort_key(a, i) : 0;
     }
+#pragma unroll
+    for (int s = 0; s < kSortSteps; ++s)
+      if (base + s * kSortLanes + t < a.n) {
+        atomicAdd(&count[(key[s] >> a.shift) & (bins - 1)], 1u);
+        if (words && key[s] < (uint32_t)a.tok.vocab) atomicOr(&seen[key[s] / 32], 1u << (key[s] % 32));
+      }
+  }
   __syncthreads();
   if (t < bins) gp(a.counts)[(uint64_t)blockIdx.x * bins + t] = count[t];
   for (uint32_t w = t; w < words; w += kSortLanes)
@@ -393,27 +399,30 @@ __global__ void __launch_bounds__(kSortLanes) sort_count_kernel(const SortArgs a
 __global__ void __launch_bounds__(kSortLanes) sort_scatter_kernel(const SortArgs a) {
   __shared__ uint32_t count[kSortWaves][1 << kMaxDigit];
   __shared__ uint32_t sums[kSortWaves];
-  if (blockIdx.x >= a.tiles)
-    return zero_block<kSortWaves>(a.zero, a.tok, blockIdx.x - a.tiles);
+  if (blockIdx.x >= a.spans)
+    return zero_block<kSortWaves>(a.zero, a.tok, blockIdx.x - a.spans);
   const uint32_t bins = 1u << a.bits, t = threadIdx.x, lane = t % kLanes, wave = t / kLanes;
   // the wave's items: 64 consecutive ones per step; all loads are issued up front
-  const uint32_t base = blockIdx.x * kSortTile + wave * (kLanes * kSortSteps) + lane;
+  uint32_t base = blockIdx.x * a.walk * kSortTile + wave * (kLanes * kSortSteps) + lane;
   uint32_t key[kSortSteps], at[kSortSteps], rank[kSortSteps];
+  const auto load_tile = [&] {
 #pragma unroll
-  for (int s = 0; s < kSortSteps; ++s) {
-    const uint32_t i = base + s * kLanes;
-    key[s] = i < a.n ? sort_key(a, i) : 0;
-    at[s] = !a.keys || i >= a.n ? i : gp(a.pos)[i];
-  }
-  // lane t owns digit t: how many of it lie in the tiles before this one, and in all
+    for (int s = 0; s < kSortSteps; ++s) {
+      const uint32_t i = base + s * kLanes;
+      key[s] = i < a.n ? sort_key(a, i) : 0;
+      at[s] = !a.keys || i >= a.n ? i : gp(a.pos)[i];
+    }
+  };
+  load_tile();
+  // lane t owns digit t: how many of it lie in the spans before this one, and in all
   uint32_t here = 0, all = 0;
   if (t < bins) {
     const global<uint32_t>* c = gp((const uint32_t*)a.counts) + t;
-    for (uint32_t b = 0; b < a.tiles; b += kCountsAhead) {
+    for (uint32_t b = 0; b < a.spans; b += kCountsAhead) {
       uint32_t v[kCountsAhead];
 #pragma unroll
       for (uint32_t u = 0; u < kCountsAhead; ++u)
-        v[u] = b + u < a.tiles ? c[(uint64_t)(b + u) * bins] : 0;
+        v[u] = b + u < a.spans ? c[(uint64_t)(b + u) * bins] : 0;
 #pragma unroll
       for (uint32_t u = 0; u < kCountsAhead; ++u) {
         here += b + u < blockIdx.x ? v[u] : 0;
@@ -421,25 +430,35 @@ __global__ void __launch_bounds__(kSortLanes) sort_scatter_kernel(const SortArgs
       }
     }
   }
-  for (int w = 0; w < kSortWaves; ++w) count[w][t] = 0;
-  __syncthreads();
+  uint32_t next = here;   // where the tile's first item of digit t goes
+  for (uint32_t tile = 0;;) {
+    for (int w = 0; w < kSortWaves; ++w) count[w][t] = 0;
+    __syncthreads();
 #pragma unroll
-  for (int s = 0; s < kSortSteps; ++s)
-    rank[s] = rank_in_wave(count[wave], (key[s] >> a.shift) & (bins - 1), a.bits,
-                           base + s * kLanes < a.n);
-  uint32_t next = scan_block<kSortWaves>(all, sums) + here;   // its barrier: all counts are there
-  for (int w = 0; w < kSortWaves; ++w) {
-    const uint32_t c = count[w][t];
-    count[w][t] = next;
-    next += c;
-  }
-  __syncthreads();
+    for (int s = 0; s < kSortSteps; ++s)
+      rank[s] = rank_in_wave(count[wave], (key[s] >> a.shift) & (bins - 1), a.bits,
+                             base + s * kLanes < a.n);
+    if (tile == 0)   // (a barrier in each branch: all counts are there)
+      next += scan_block<kSortWaves>(all, sums);
+    else
+      __syncthreads();
+    for (int w = 0; w < kSortWaves; ++w) {
+      const uint32_t c = count[w][t];
+      count[w][t] = next;
+      next += c;
+    }
+    __syncthreads();
 #pragma unroll
-  for (int s = 0; s < kSortSteps; ++s) {
-    if (base + s * kLanes >= a.n) continue;
-    const uint32_t to = count[wave][(key[s] >> a.shift) & (bins - 1)] + rank[s];
-    gp(a.keys_out)[to] = key[s];
-    gp(a.pos_out)[to] = at[s];
+    for (int s = 0; s < kSortSteps; ++s) {
+      if (base + s * kLanes >= a.n) continue;
+      const uint32_t to = count[wave][(key[s] >> a.shift) & (bins - 1)] + rank[s];
+      gp(a.keys_out)[to] = key[s];
+      gp(a.pos_out)[to] = at[s];
+    }
+    if (++tile == a.walk) break;
+    base += kSortTile;
+    load_tile();
+    __syncthreads();   // the counts have been read
   }
 }
 
@@ -749,7 +768,7 @@ constexpr uint64_t kMaxSeen = 1u << 18;
 
 struct Work {
   uint64_t keys[2], pos[2], counts, seen, parts, bytes;
-  uint32_t sort_tiles, sum_tiles, words;
+  uint32_t sort_spans, walk, sum_tiles, words;
   int passes, bits;
   bool small;
 };
@@ -760,7 +779,9 @@ Work work_of(uint64_t n, uint64_t vocab, uint32_t hidden) {
   const int all = bits_of(vocab), digit = w.small ? kSmallBits : kMaxDigit;
   w.passes = (all + digit - 1) / digit;
   w.bits = (all + w.passes - 1) / w.passes;
-  w.sort_tiles = (uint32_t)((n + kSortTile - 1) / kSortTile);
+  const uint64_t tiles = (n + kSortTile - 1) / kSortTile;
+  w.walk = (uint32_t)((tiles + kMaxSpans - 1) / kMaxSpans);
+  w.sort_spans = w.walk ? (uint32_t)((tiles + w.walk - 1) / w.walk) : 0;
   w.sum_tiles = (uint32_t)((n + tile_for(n) - 1) / tile_for(n));
   w.words = w.small || vocab > kMaxSeen ? 0 : (uint32_t)((vocab + 31) / 32);
   uint64_t at = 0;
@@ -773,8 +794,8 @@ Work work_of(uint64_t n, uint64_t vocab, uint32_t hidden) {
     w.keys[i] = take(4 * n);
     w.pos[i] = take(4 * n);
   }
-  if (!w.small) w.counts = take(4ull * w.sort_tiles << w.bits);
-  w.seen = take(4ull * w.sort_tiles * w.words);
+  if (!w.small) w.counts = take(4ull * w.sort_spans << w.bits);
+  w.seen = take(4ull * w.sort_spans * w.words);
   w.parts = take(8ull * w.sum_tiles * hidden);
   w.bytes = at;
   return w;
@@ -860,7 +881,7 @@ int ec_embed_grad(const void* d_tokens, int token_bytes, uint64_t n, const void*
   z.stride = grad_stride * type_bytes(grad_type);
   z.row_bytes = hidden * type_bytes(grad_type);
   z.words = w.words;
-  z.tiles = w.sort_tiles;
+  z.spans = w.sort_spans;
   z.mode = w.small ? kZeroScan : w.words ? kZeroSeen : kZeroAll;
   z.by_row = make_fastdiv(z.row_bytes);
   const uint64_t span = std::min(kMostSpan, std::max(kLeastSpan, vocab * z.row_bytes / kZeroSpans));
@@ -911,7 +932,7 @@ int ec_embed_grad(const void* d_tokens, int token_bytes, uint64_t n, const void*
   // each launch as if it took all zeros along
   const auto past = [&](uint64_t blocks, uint64_t lanes) { return (blocks + all_zero) * lanes >= 1ull << 32; };
   if (past(sum_blocks, kSumWaves * kLanes) || past(join_blocks, kJoinWaves * kLanes) ||
-      past(w.sort_tiles, w.small ? kSmallLanes : kSortLanes))
+      past(w.sort_spans, w.small ? kSmallLanes : kSortLanes))
     return EC_ERANGE;
   a.sum_blocks = (uint32_t)sum_blocks;
   a.join_blocks = (uint32_t)join_blocks;
@@ -919,7 +940,8 @@ int ec_embed_grad(const void* d_tokens, int token_bytes, uint64_t n, const void*
   SortArgs s = {};
   s.tok = tok;
   s.n = (uint32_t)n;
-  s.tiles = w.sort_tiles;
+  s.spans = w.sort_spans;
+  s.walk = w.walk;
   s.words = w.words;
   s.bits = w.bits;
   s.passes = w.passes;
@@ -942,10 +964,10 @@ int ec_embed_grad(const void* d_tokens, int token_bytes, uint64_t n, const void*
     // none are collected all rows are zeroed, and before the sums write theirs
     uint32_t extra = p || z.mode == kZeroAll ? sort_zeros() : 0;
     s.zero = z;
-    sort_count_kernel<<<s.tiles + extra, kSortLanes, s.seen ? 4 * w.words : 0, st>>>(s);
+    sort_count_kernel<<<s.spans + extra, kSortLanes, s.seen ? 4 * w.words : 0, st>>>(s);
     extra = z.mode == kZeroAll && p + 1 == w.passes ? zeros(0) : sort_zeros();
     s.zero = z;
-    sort_scatter_kernel<<<s.tiles + extra, kSortLanes, 0, st>>>(s);
+    sort_scatter_kernel<<<s.spans + extra, kSortLanes, 0, st>>>(s);
   }
 
   const uint32_t behind = join_blocks ? with_join : 0;   // zeros that the join takes along

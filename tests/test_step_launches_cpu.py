@@ -17,3 +17,12 @@ def test_embed_grad_past_a_launch(pkg):
     assert call(1 << 30, 1000, 1 << 13, kind=0) == big
     assert call(16, (1 << 31) - 1, 1 << 14) == big           # the zeros beside the small sort's 1024 lanes
     assert call(1 << 14, (1 << 31) - 1, 1 << 14) == big      # beside the large one's 512
+
+
+def test_the_sorts_memory_does_not_grow_with_the_tokens(pkg):
+    """Besides 16 bytes a token and the sums' two parts for each 32 tokens: each workgroup of the sort reads all
+    counts, so their number has a limit."""
+    ws = pkg._lib.lib().ec_embed_grad_workspace
+    for vocab in (50_304, 262_143, 1 << 30):
+        sizes = [ws(n, vocab, 1) - 16 * n - 8 * (n // 32) for n in (1 << 20, 1 << 24, 1 << 30)]
+        assert sizes[0] == sizes[1] == sizes[2] <= 512 * 4 * (512 + 8192), sizes
