@@ -66,3 +66,23 @@ def test_what_is_only_read_keeps_its_version(pkg, dev):
     lst.clip(1.0)
     pkg.grad_norm([t])
     loss.backward()
+
+
+def test_views_of_one_buffer(pkg, dev):
+    """A list of a buffer's pieces: the buffer, its other views and what shares its version were written; others were not."""
+    flat = torch.randn(40, device=dev)
+    other = torch.randn(8, device=dev)
+    pieces = list(flat.split([8, 20, 12])) + [flat.detach()[:0]]
+    lst = pkg.GradList(pieces + [other])
+    for t in (flat, flat[30:], flat.view(5, 8), pieces[1], flat.detach(), other):
+        weight = torch.ones_like(t, requires_grad=True)
+        loss = (t * weight).sum()
+        lst.clip(1e-3)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    kept, loss = saved(dev, 8)
+    lst.clip(1e-3)
+    loss.backward()
+    before = flat._version
+    lst.norm()
+    assert flat._version == before
