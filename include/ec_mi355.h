@@ -356,6 +356,7 @@ int ec_stage_last_stats(ec_stage_stats* out);
  * the vocabulary and its gradient, and the norm of the gradient list, whose
  * finiteness says whether the step, and a snapshot of it, is sound.
  *
+ * The stream's device is the current one.
  * Common rules.  `type` is EC_F32, EC_BF16 or EC_F16.  Arithmetic is in fp32
  * (sums of squares in fp64) and a result is rounded once, where it is stored.
  * Addresses need only the alignment of their elements; rows whose starts are
@@ -377,8 +378,9 @@ int ec_embed(const void* d_tokens, int token_bytes, uint64_t n, const void* d_ta
 /* Device memory ec_embed_grad needs at d_work, in bytes. */
 uint64_t ec_embed_grad_workspace(uint64_t n, uint64_t vocab, uint32_t hidden);
 
-/* grad[v] = scale * SUM over i with tokens[i] - vocab_start = v of dout[i], the
- * positions added in ascending order of a fixed grouping; tokens outside the slice add nothing.
+/* grad[v] = scale * SUM over i with tokens[i] - vocab_start = v of dout[i]; tokens outside the
+ * slice add nothing.  Positions are added in ascending order within tiles of 16 or 32 sorted
+ * ones, and the sums of a run over several tiles in a fixed grouping.
  * dout is [n, hidden] of `type`, rows dout_stride apart; grad is [vocab,
  * hidden] of `grad_type` (EC_F32 or `type`), rows grad_stride apart.
  * accumulate 0: every row is written, zeros for a token that does not occur;
@@ -406,8 +408,10 @@ int ec_embed_grad(const void* d_tokens, int token_bytes, uint64_t n, const void*
  * fp32 outputs, 64-bit signed targets and indices.  -infinity is a masked
  * logit: probability 0.  A row of nothing else has lse and log-probabilities of
  * -infinity and entropy 0.  A row with a NaN or +infinity has NaN in lse,
- * log-probabilities and entropy; its indices order NaN last.  One pass over
- * the logits.  EC_ERANGE for rows or vocab >= 2^31. */
+ * log-probabilities and entropy; its indices order NaN last.  lse is the largest
+ * logit's z as fp32 rounds it, plus a rounded term.  The logits are those of the whole
+ * vocabulary (the gradient of a slice's would need to know a target that lies in another
+ * one).  One pass over the logits.  EC_ERANGE for rows or vocab >= 2^31. */
 int ec_token_logprobs(const void* d_logits, int type, uint64_t rows, uint64_t vocab,
                       uint64_t row_stride, const int64_t* d_targets, float scale,
                       float* d_logprobs, float* d_lse, float* d_entropy, int top,
@@ -422,8 +426,8 @@ int ec_token_logprobs(const void* d_logits, int type, uint64_t rows, uint64_t vo
  * themselves.  A masked logit's gradient is 0, and so is the whole row's where
  * lse is -infinity or below -2^127 / log2 e * min(1, scale) (a row of nothing but masked
  * logits, the lowest value of fp32 or bf16 as a mask included; that of fp16 is a logit
- * like others).  A row with a NaN or +infinity has NaN gradients, and a logit whose z
- * overflows to +infinity has one. */
+ * like others).  Where lse is NaN so are the row's gradients; where z of the largest logit
+ * overflows, lse is +infinity, and that logit's gradient is NaN. */
 int ec_token_logprobs_grad(const void* d_logits, int type, uint64_t rows, uint64_t vocab,
                            uint64_t row_stride, const int64_t* d_targets, const float* d_lse,
                            const float* d_dlogprobs, const float* d_entropy,

@@ -35,7 +35,8 @@ __device__ __forceinline__ int64_t row_of(const void* tokens, int token_bytes, u
 //
 // Bound by memory: 32768 tokens of 2048 bf16 in 32 us, 134 MB written and 77 MB read (each
 // XCD reads the rows of its own tokens: 6.6 TB/s).  One, two or eight groups a lane took
-// 51, 49 and 44 us where four took 42 (cached stores): the token's load is waited for once.
+// 51, 49 and 44 us where four took 42 (cached stores, four tables in turn): the token's load is
+// waited for once.
 struct EmbedArgs {
   const void* tokens;
   const void* table;
@@ -50,9 +51,9 @@ struct EmbedArgs {
 constexpr int kEmbedGroups = 4;
 constexpr int kEmbedWaves = 4;
 // Results of at least this many bytes, in rows of at least a KiB, are streamed past the
-// caches: 32768 rows of 2048 bf16 39.3 -> 36.3 us, of 2047 47.2 -> 40.9, 65536 of 512 21.6 ->
-// 19.2, 16384 of 4096 fp32 78.6 -> 70.4; but 131072 of 33 fp16, whose rows share lines, 6.2
-// -> 11.4.
+// caches (a call, four tables in turn): 32768 rows of 2048 bf16 40.5 -> 37.0 us, of 2047 48.2 ->
+// 40.1, 65536 of 512 21.6 -> 17.2, 16384 of 4096 fp32 78.2 -> 70.7; but 131072 of 33 fp16, whose
+// rows share lines, 6.7 -> 10.7.
 constexpr uint64_t kEmbedStream = 64u << 20;
 constexpr uint32_t kEmbedStreamGroups = 64;
 
@@ -474,8 +475,9 @@ __global__ void __launch_bounds__(kSortLanes) sort_scatter_kernel(const SortArgs
 //
 // Bound by memory, gathered rows of 4 KiB at that: 65536 tokens of 2048 bf16, with the zeros
 // that ride along, in 95 us, 274 MB read and 294 MB written (6.0 TB/s).  The sums go through
-// the caches, in whole lines (Columns): the whole call takes 134 us; whole lines streamed
-// 156, a lane's 8 fp32 as two stores of half lines 143.
+// the caches, in whole lines (Columns): the whole call takes 134 us into one gradient buffer (143
+// into another one each time); whole lines streamed 156, a lane's 8 fp32 as two stores of half
+// lines 143.
 //
 // Tiles of 16 where there are few: more waves share the gathers' latency (tiles of 8 /
 // 16 / 32, us for the whole call: 67 tokens of 64 bf16 15.7 16.7 19.4; 2048 of 1999 fp32

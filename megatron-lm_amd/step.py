@@ -5,8 +5,8 @@ protects: ``embed`` and ``embed_grad`` (rows of the embedding table by token, an
 the table's gradient), ``token_logprobs`` and ``token_logprobs_grad`` (the loss over
 the vocabulary: log probabilities of given tokens, entropy, the likeliest tokens),
 and ``grad_norm`` / ``clip_grads`` / ``GradList`` (the global norm of a gradient list
-and its clipping).  The norm says whether a step is sound: one that is not
-finite is skipped, and so is the snapshot after it; and the log probabilities of a
+and its clipping).  The norm says whether a step is sound: where it is not finite a loop
+skips the update, and the snapshot after it; and the log probabilities of a
 probe batch say whether a loaded state answers as the saved one did.
 
 Every function takes HIP tensors of float32, bfloat16 or float16, computes in
@@ -101,7 +101,8 @@ def embed_grad(tokens: torch.Tensor, dout: torch.Tensor, vocab_size: int, *, sca
     ``dout`` ([*tokens.shape, hidden]) over the positions of its token.
 
     ``dtype`` is float32 (the default) or dout's, or that of ``out``.  The tokens are
-    sorted and each row's positions added in order, in fp32, without atomics.
+    sorted and each row's positions added in fp32, without atomics: in ascending order within tiles
+    of 16 or 32 sorted positions, then a long run's tiles in a fixed grouping.
     ``accumulate`` adds to ``out`` and leaves the rows of tokens that do not occur untouched
     (a micro-batch's part of a gradient buffer); otherwise they are zeros."""
     dtype = torch.float32 if dtype is None else dtype
@@ -117,9 +118,9 @@ def embed_grad(tokens: torch.Tensor, dout: torch.Tensor, vocab_size: int, *, sca
 class TokenLogprobs(NamedTuple):
     """What ``token_logprobs`` returns, fp32 (and int64 tokens), in the shape of the targets."""
     logprobs: torch.Tensor                 # of the targets; 0 where there is none
-    lse: torch.Tensor                      # log of the sum of exp(scale * logits)
+    lse: torch.Tensor                      # log of the sum of exp(scale * logits); no gradient
     entropy: Optional[torch.Tensor]
-    top_logprobs: Optional[torch.Tensor]   # [..., top], descending
+    top_logprobs: Optional[torch.Tensor]   # [..., top], descending; no gradient
     top_tokens: Optional[torch.Tensor]     # [..., top], equal ones by ascending index
 
 
@@ -150,8 +151,13 @@ class _TokenLogprobs(torch.autograd.Function):
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, scale: float = 1.0,
                    entropy: bool = False, top: int = 0, stream=None) -> TokenLogprobs:
     """Log probabilities of ``targets`` (int64, the logits' leading shape) under the softmax of
-    scale * ``logits`` ([..., vocabulary], rows may be strided), in one pass over the logits, and
-    on request the entropy and the ``top`` (at most MAX_TOP) likeliest tokens.
+    scale * ``logits`` ([..., vocabulary], contiguous, or two-dimensional with strided rows), in one
+    pass over the logits, and on request the entropy and the ``top`` (at most MAX_TOP) likeliest tokens.
+
+    With gradients enabled the log probabilities and the entropy are differentiable; ``lse`` and the
+    alternatives are constants, so a term of the loss made from them (a penalty on lse) has
+    no gradient.  The logits are those of the whole vocabulary: of a rank's slice the values are the
+    slice's own, and a target in another slice would count as ignored, with no gradient for this one.
 
     A target outside the vocabulary (an ignored position) has log probability 0.  Logits
     of -infinity are masked; a row of nothing else has log probability and lse -infinity and
@@ -177,7 +183,7 @@ def token_logprobs_grad(logits: torch.Tensor, targets: torch.Tensor, lse: torch.
                         out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
     """The gradient with respect to the logits, from the gradients of ``token_logprobs``' log
     probabilities and (``dentropy``, together with the ``entropy`` it returned) entropies, in the
-    logits' type.  ``out`` may be the logits themselves.  Ignored positions have no part in
+    logits' type.  Probabilities are exp(scale * logits - ``lse``), at most 1.  ``out`` may be the logits themselves.  Ignored positions have no part in
     ``dlogprobs``; masked logits, and rows of nothing else, have gradient 0."""
     return _call("ec_token_logprobs_grad", _lib.shards().token_logprobs_grad, logits, stream,
                  logits, targets, lse, dlogprobs, entropy, dentropy, _positive(scale, "scale"),
@@ -199,7 +205,8 @@ class GradList:
     once for ``norm`` and ``clip``: a training loop keeps its gradient buffers, and the list of
     their pieces stays on the device.  ``clip`` writes to the tensors of ``out`` (same element
     counts, any of the types: bf16 gradients into fp32 ones), or in place; no two of the tensors
-    written may overlap.  The list keeps the tensors alive; gradients that are replaced by other tensors need a new list."""
+    written may overlap.  The list keeps the tensors alive; gradients that are replaced by other tensors need a new
+    list.  Making one costs 0.3 to 2 us a tensor on the host (and an upload), more than the calls on small ones."""
 
     _clips = True
 
