@@ -356,8 +356,7 @@ int ec_stage_last_stats(ec_stage_stats* out);
  * the vocabulary and its gradient, and the norm of the gradient list, whose
  * finiteness says whether the step, and a snapshot of it, is sound.
  *
- * The stream's device is the current one.
- * Common rules.  `type` is EC_F32, EC_BF16 or EC_F16.  Arithmetic is in fp32
+ * Common rules.  The stream's device is the current one.  `type` is EC_F32, EC_BF16 or EC_F16.  Arithmetic is in fp32
  * (sums of squares in fp64) and a result is rounded once, where it is stored.
  * Addresses need only the alignment of their elements; rows whose starts are
  * 16-byte aligned run fastest.  Row strides are in elements; the elements of
