@@ -467,6 +467,103 @@ int ec_grad_clip(const ec_grad_item* d_items, uint32_t n_items, float grad_scale
                  float max_norm, const float* d_given, void* d_work, float* d_norm,
                  ec_stream_t stream);
 
+/* ---- operators of a block and of its matrices' update ----------------- */
+
+/* The activation of a gated feed-forward: g * sigmoid(g); g * Phi(g) with the normal distribution
+ * function Phi; and its tanh form, g / 2 (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))). */
+#define EC_ACT_SILU 0
+#define EC_ACT_GELU 1
+#define EC_ACT_GELU_TANH 2
+
+/* Device memory that ec_gated_ff (grad 0) or ec_gated_ff_grad (grad 1) needs at d_work for these
+ * operands, in bytes, 16-byte aligned: rows that are not 16-byte aligned, or not a multiple of 16 bytes long
+ * or apart, are copied there first; the gradients of both projections lie there. 0 for operands
+ * that the call refuses. */
+uint64_t ec_gated_ff_workspace(const void* d_x, uint64_t x_stride, const void* d_gate,
+                               uint64_t gate_stride, const void* d_up, uint64_t up_stride, int type,
+                               uint64_t n, uint32_t width, uint32_t inner, int grad);
+
+/* h[i][f] = act(g) * u, g = SUM_k x[i][k] gate[f][k] and u = SUM_k x[i][k] up[f][k], for n
+ * rows x of `width` and weights [inner][width], all of `type` (the weights may be the halves of
+ * one buffer). The sums and the activation are in fp32, on the matrix cores; h is rounded once.
+ * EC_ERANGE for n >= 2^31, width or inner > 2^19, or a launch of 2^32 lanes. */
+int ec_gated_ff(const void* d_x, uint64_t x_stride, const void* d_gate, uint64_t gate_stride,
+                const void* d_up, uint64_t up_stride, int type, uint64_t n, uint32_t width,
+                uint32_t inner, int activation, void* d_h, uint64_t h_stride, void* d_work,
+                uint64_t work_bytes, ec_stream_t stream);
+
+/* The gradients of ec_gated_ff: with dg = dh u act'(g) and du = dh act(g),
+ *   dx = dg gate + du up,  dgate = dg' x,  dup = du' x
+ * g and u are computed again. dx is of `type`; dgate and dup are of grad_type (EC_F32 or
+ * `type`), written, or added to where accumulate is 1. dx, or both others, may be null: not
+ * computed. dg and du are rounded to `type` for the products (with 256 rows and fewer they keep
+ * their rounding error as a second part); sums are in fp32, each result is rounded once. n 0: dgate
+ * and dup are zeros, or left as they are. */
+int ec_gated_ff_grad(const void* d_dh, uint64_t dh_stride, const void* d_x, uint64_t x_stride,
+                     const void* d_gate, uint64_t gate_stride, const void* d_up, uint64_t up_stride,
+                     int type, uint64_t n, uint32_t width, uint32_t inner, int activation, void* d_dx,
+                     uint64_t dx_stride, void* d_dgate, uint64_t dgate_stride, void* d_dup,
+                     uint64_t dup_stride, int grad_type, int accumulate, void* d_work,
+                     uint64_t work_bytes, ec_stream_t stream);
+
+/* Newton-Schulz steps that ec_orthogonalize takes at most. */
+#define EC_MAX_STEPS 64
+
+/* Device memory that ec_orthogonalize needs at d_work, in bytes, 16-byte aligned; 0 where the
+ * call refuses the sizes or has nothing to do. */
+uint64_t ec_orthogonalize_workspace(uint64_t batch, uint64_t rows, uint64_t cols);
+
+/* out = keep * base + scale * X for each of `batch` matrices x of [rows][cols], where X is x / (|x| + eps),
+ * |x| the root of the sum of its squares, after `steps` steps
+ *   X <- a X + (b A + c A A) X,  A = X X'
+ * (or X' X from the right, the same for rows > cols) with {a, b, c} = coefficients, three values on the host of magnitude
+ * up to 1024: each singular value s of X becomes a s + b s^3 + c s^5. base null: out = scale * X; base may be out.
+ * base and out are of out_type. Row strides and the distances from matrix to matrix are in elements.
+ * Products are of values of 22 bits, in fp32 sums, and |x| is summed in fp64. The iterates' magnitudes have to
+ * stay below 15 (values past it become infinite): with coefficients that keep [0, 1.2] in itself they are below 1.5.
+ * A matrix with a value that is not finite gives NaN; one of zeros gives keep * base. A matrix whose |x| is
+ * far below eps keeps fewer bits. EC_ERANGE for rows, cols or batch > 65536, steps past
+ * EC_MAX_STEPS or below 1, or a launch of 2^32 lanes. */
+int ec_orthogonalize(const void* d_x, int type, uint64_t batch, uint64_t rows, uint64_t cols,
+                     uint64_t x_stride, uint64_t x_matrix, int steps, const float* coefficients,
+                     float eps, float scale, const void* d_base, uint64_t base_stride,
+                     uint64_t base_matrix, float keep, void* d_out, int out_type, uint64_t out_stride,
+                     uint64_t out_matrix, void* d_work, uint64_t work_bytes, ec_stream_t stream);
+
+/* For n rows of `width` (at most 16384), with rms(v) = sqrt(mean(v^2) + eps):
+ *   u = branch, or branch_weight * branch / rms(branch) where branch_weight is not null
+ *   sum = residual + scale * gate * u
+ *   normed = weight * sum / rms(sum), of the sum before it is rounded; where weight is not null
+ * and d_rstd, d_branch_rstd (may be null) the factors 1 / rms. All but those are of `type`. gate is
+ * [gate_rows][width], gate_rows a divisor of n: row g goes with the n / gate_rows rows of u from g * n / gate_rows
+ * on; null: 1. branch null (with gate and branch_weight null): only normed is computed, and d_sum is not
+ * used. sum may be residual or branch; normed is contiguous. EC_ERANGE for n >= 2^31 or width > 16384. */
+int ec_residual_norm(const void* d_residual, uint64_t residual_stride, const void* d_branch,
+                     uint64_t branch_stride, int type, uint64_t n, uint32_t width, const void* d_gate,
+                     uint64_t gate_rows, float scale, const void* d_branch_weight,
+                     const void* d_weight, float eps, void* d_sum, uint64_t sum_stride, void* d_normed,
+                     float* d_rstd, float* d_branch_rstd, ec_stream_t stream);
+
+/* Device memory that ec_residual_norm_grad needs at d_work, in bytes, 16-byte aligned. */
+uint64_t ec_residual_norm_grad_workspace(uint64_t n, uint32_t width, uint64_t gate_rows);
+
+/* The gradients of ec_residual_norm from those of sum and normed, the sum, and the factors it left:
+ *   dresidual = dsum + (t - s mean(t s)) rstd, t = weight * dnormed, s = sum * rstd
+ *   dgate = SUM scale * dresidual * u over its rows
+ *   dbranch = the gradient of branch by du = scale * gate * dresidual, as dresidual's by t
+ *   dbranch_weight = SUM du * branch * branch_rstd, dweight = SUM dnormed * s over all rows
+ * dresidual and dbranch are contiguous, of `type`; dgate [gate_rows][width], dbranch_weight and dweight are fp32.
+ * dsum null: 0; weight (with dnormed, sum, rstd, dweight) null: no norm of the sum. The sums over
+ * rows have fixed places. n 0: the sums are zeros. */
+int ec_residual_norm_grad(const void* d_dsum, uint64_t dsum_stride, const void* d_dnormed,
+                          uint64_t dnormed_stride, const void* d_sum, uint64_t sum_stride,
+                          const void* d_branch, uint64_t branch_stride, int type, uint64_t n,
+                          uint32_t width, const float* d_rstd, const float* d_branch_rstd,
+                          const void* d_gate, uint64_t gate_rows, float scale,
+                          const void* d_branch_weight, const void* d_weight, void* d_dresidual,
+                          void* d_dbranch, float* d_dgate, float* d_dbranch_weight, float* d_dweight,
+                          void* d_work, uint64_t work_bytes, ec_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

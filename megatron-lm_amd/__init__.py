@@ -16,9 +16,13 @@ Modules:
   args     --non-persistent-ckpt-type in_memory: flags, validation, checkpointing context
   step     operators of the training step around the saves: embedding lookup and its gradient,
            log probabilities over the vocabulary and their gradient, gradient norm and clipping
+  block    operators of a block between the two and of its matrices' update: the gated feed-forward
+           and the norms around it with their gradients, orthogonalised updates
 """
 from . import _lib
 from ._lib import ECError, ECLibraryMissing, SingularError
+from .block import (GatedGrads, ResidualNorm, ResidualNormGrads, gated_ff, gated_ff_grad, orthogonalize,
+                    residual_norm, residual_norm_grad)
 from .codec import (ShardPlan, cauchy_matrix, decode_matrix, gf_inv, gf_invert, gf_mul, matvec,
                     reconstruct, rs_encode, side_stream, xor_encode)
 from .layout import ParitySet, StripeLayout, decode, encode, update
@@ -32,6 +36,8 @@ __all__ = [
     "StripeLayout", "ParitySet", "encode", "decode", "update",
     "GradList", "TokenLogprobs", "clip_grads", "embed", "embed_grad", "grad_norm", "token_logprobs",
     "token_logprobs_grad",
+    "GatedGrads", "ResidualNorm", "ResidualNormGrads", "gated_ff", "gated_ff_grad", "orthogonalize",
+    "residual_norm", "residual_norm_grad",
 ]
 
 

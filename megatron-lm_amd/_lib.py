@@ -53,6 +53,14 @@ EXPORTS = (
     "ec_token_logprobs_grad",
     "ec_grad_norm",
     "ec_grad_clip",
+    "ec_gated_ff_workspace",
+    "ec_gated_ff",
+    "ec_gated_ff_grad",
+    "ec_orthogonalize_workspace",
+    "ec_orthogonalize",
+    "ec_residual_norm",
+    "ec_residual_norm_grad_workspace",
+    "ec_residual_norm_grad",
 )
 
 
@@ -170,6 +178,27 @@ def lib() -> ctypes.CDLL:
     L.ec_grad_norm.argtypes = [_vp, _u32, _f, _i, _vp, _vp, _vp]
     L.ec_grad_clip.restype = _i
     L.ec_grad_clip.argtypes = [_vp, _u32, _f, _i, _f, _vp, _vp, _vp, _vp]
+    L.ec_gated_ff_workspace.restype = _u64
+    L.ec_gated_ff_workspace.argtypes = [_vp, _u64, _vp, _u64, _vp, _u64, _i, _u64, _u32, _u32, _i]
+    L.ec_gated_ff.restype = _i
+    L.ec_gated_ff.argtypes = [_vp, _u64, _vp, _u64, _vp, _u64, _i, _u64, _u32, _u32, _i, _vp, _u64, _vp,
+                              _u64, _vp]
+    L.ec_gated_ff_grad.restype = _i
+    L.ec_gated_ff_grad.argtypes = [_vp, _u64, _vp, _u64, _vp, _u64, _vp, _u64, _i, _u64, _u32, _u32, _i,
+                                   _vp, _u64, _vp, _u64, _vp, _u64, _i, _i, _vp, _u64, _vp]
+    L.ec_orthogonalize_workspace.restype = _u64
+    L.ec_orthogonalize_workspace.argtypes = [_u64, _u64, _u64]
+    L.ec_orthogonalize.restype = _i
+    L.ec_orthogonalize.argtypes = [_vp, _i, _u64, _u64, _u64, _u64, _u64, _i, _vp, _f, _f, _vp, _u64, _u64,
+                                   _f, _vp, _i, _u64, _u64, _vp, _u64, _vp]
+    L.ec_residual_norm.restype = _i
+    L.ec_residual_norm.argtypes = [_vp, _u64, _vp, _u64, _i, _u64, _u32, _vp, _u64, _f, _vp, _vp, _f, _vp,
+                                   _u64, _vp, _vp, _vp, _vp]
+    L.ec_residual_norm_grad_workspace.restype = _u64
+    L.ec_residual_norm_grad_workspace.argtypes = [_u64, _u32, _u64]
+    L.ec_residual_norm_grad.restype = _i
+    L.ec_residual_norm_grad.argtypes = [_vp, _u64, _vp, _u64, _vp, _u64, _vp, _u64, _i, _u64, _u32, _vp, _vp,
+                                        _vp, _u64, _f, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _u64, _vp]
     _lib = L
     return L
 

@@ -1,0 +1,337 @@
+// ec_ff.hip — ec_gated_ff and ec_gated_ff_grad: act(x Wg') * (x Wu') and its gradients.
+//
+// Forward: one product whose second operand is both weights' rows in turns, 32 of each, so that a
+// wave holds the gate and the up projection of the same outputs in its accumulators and
+// neither of them goes to memory.
+//
+// Backward: the same product again, whose epilogue turns g, u and dh into dg = dh u act'(g) and
+// du = dh act(g) ([n][2 inner] in the workspace), then dx = dg Wg + du Wu and dW = d' x as two products
+// more, 12 n width inner operations in all.  Computing the projections again costs 4 of
+// them and keeps 2 n inner values from being stored between the passes.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "ec_gemm.h"
+#include "ec_pack.h"
+
+namespace ec {
+namespace {
+
+struct Act {
+  float value, slope;
+};
+
+// The activation and its derivative at g, both from one exponential (or the error function).
+__device__ __forceinline__ Act activate(float g, int act) {
+  if (act == EC_ACT_GELU) {
+    const float p = 0.5f * erfcf(-0.70710678f * g);
+    return {g * p, p + g * 0.39894228f * expf(-0.5f * g * g)};
+  }
+  // silu and the tanh form of gelu are g * sigmoid(z), z = g or 2 sqrt(2 / pi) (g + 0.044715 g^3)
+  float z = g, dz = 1.0f;
+  if (act == EC_ACT_GELU_TANH) {
+    const float c = 1.59576912f, g2 = g * g;
+    z = c * g * (1.0f + 0.044715f * g2);
+    dz = c * (1.0f + 3.0f * 0.044715f * g2);
+  }
+  const float s = 1.0f / (1.0f + expf(-z));
+  // far out z' may overflow where s (1 - s) is 0
+  const float bend = s * (1.0f - s);
+  return {g * s, s + (bend > 0.0f ? g * bend * dz : 0.0f)};
+}
+
+struct FfArgs {
+  Operand x, w_gate, w_up;
+  uint32_t n, width, inner, act;
+  uint32_t tiles_m, tiles_n;
+  char* h;
+  uint64_t h_stride;
+  const char* dh;        // backward
+  uint64_t dh_stride;
+  char* d;               // [n][2 padded] of T, and the second parts behind it
+  uint32_t padded;
+  uint64_t low;          // elements from a value of d to its second part; 0: none
+};
+
+template <class S, typename T, bool GRAD>
+__global__ void __launch_bounds__(S::kLanes) ff_kernel(FfArgs p) {
+  __shared__ __attribute__((aligned(1024))) char lds[S::kLds];
+  uint32_t tm, tn;
+  tile_at(xcd_order(blockIdx.x, gridDim.x), p.tiles_m, p.tiles_n, tm, tn);
+  Acc<S> acc;
+  acc.clear();
+  product<S, T, false, false, true>(acc, (local<char>*)lds, p.x, p.w_gate, p.w_up, tm * S::BM,
+                                    tn * S::BN, p.width);
+  // of each 64 columns of the tile the first 32 are gates, the others the ups
+  static_assert(S::WN == 64, "a wave holds both projections of its 32 outputs");
+  const uint32_t l = threadIdx.x % 64, w = threadIdx.x / 64;
+  const uint32_t m0 = tm * S::BM + w / S::kWavesN * S::WM + l % 16;
+  const uint32_t f0 = tn * (S::BN / 2) + w % S::kWavesN * 32 + l / 16 * 4;
+#pragma unroll
+  for (int i = 0; i < S::MI; ++i) {
+    const uint32_t m = m0 + i * 16;
+    if (m >= p.n) continue;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t f = f0 + j * 16;
+      const f4 g = acc.v[i][j], u = acc.v[i][j + 2];
+      if constexpr (!GRAD) {
+        f4 h;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) h[e] = activate(g[e], p.act).value * u[e];
+        store4<T>((T*)p.h + m * p.h_stride, f, p.inner, h);
+      } else {
+        const f4 dh = load4<T>((const T*)p.dh + m * p.dh_stride, f, p.inner);
+        f4 dg, du;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const Act a = activate(g[e], p.act);
+          const bool in = f + e < p.inner;   // zeros in the padding, which is summed over
+          dg[e] = in ? dh[e] * u[e] * a.slope : 0.0f;
+          du[e] = in ? dh[e] * a.value : 0.0f;
+        }
+        T* row = (T*)p.d + (uint64_t)m * 2 * p.padded;
+        store4<T>(row, f, p.padded, dg);
+        store4<T>(row + p.padded, f, p.padded, du);
+        if (p.low) {
+          f4 lg, lu;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            lg[e] = dg[e] - (float)(T)dg[e];
+            lu[e] = du[e] - (float)(T)du[e];
+          }
+          store4<T>(row + p.low, f, p.padded, lg);
+          store4<T>(row + p.low + p.padded, f, p.padded, lu);
+        }
+      }
+    }
+  }
+}
+
+// C = the sum of up to four products, all across in their second operand.
+struct SumArgs {
+  Operand a[4], b[4];
+  uint32_t parts, K, M, N;
+  uint32_t tiles_m, tiles_n;
+  char* out[2];   // blockIdx.y's
+  uint64_t out_stride[2];
+  uint64_t a_step;   // bytes from blockIdx.y = 0's first operand to 1's
+  int accumulate;
+};
+
+template <class S, typename T, typename O, bool ACROSS_A>
+__global__ void __launch_bounds__(S::kLanes) sum_kernel(SumArgs p) {
+  __shared__ __attribute__((aligned(1024))) char lds[S::kLds];
+  uint32_t tm, tn;
+  tile_at(xcd_order(blockIdx.x, gridDim.x), p.tiles_m, p.tiles_n, tm, tn);
+  Acc<S> acc;
+  acc.clear();
+  for (uint32_t i = 0; i < p.parts; ++i) {
+    Operand a = p.a[i];
+    a.p += blockIdx.y * p.a_step;
+    product<S, T, ACROSS_A, true, false>(acc, (local<char>*)lds, a, p.b[i], p.b[i], tm * S::BM,
+                                         tn * S::BN, p.K);
+  }
+  O* out = (O*)p.out[blockIdx.y];
+  const uint64_t stride = p.out_stride[blockIdx.y];
+  acc.each([&](uint32_t m, uint32_t n, f4 v) {
+    m += tm * S::BM;
+    n += tn * S::BN;
+    if (m >= p.M || n >= p.N) return;
+    O* row = out + m * stride;
+    if (p.accumulate) v += load4<O>(row, n, p.N);
+    store4<O>(row, n, p.N, v);
+  });
+}
+
+struct FfWork {
+  uint64_t x, w_gate, w_up, d, total;   // offsets; kNone: read in place
+  bool low;
+};
+constexpr uint64_t kNone = ~0ull;
+constexpr uint32_t kMostWidth = 1u << 19;
+
+// Up to this many rows the gradients of the projections keep a second part, the first one's
+// rounding error, and the products take it along: the roundings of few rows do not
+// average out, and the products cost little there.
+constexpr uint64_t kFewRows = 256;
+
+struct FfCall {
+  const void *x, *w_gate, *w_up;
+  uint64_t x_stride, gate_stride, up_stride, n;
+  uint32_t width, inner;
+  int type;
+};
+
+FfWork ff_work(const FfCall& c, bool grad) {
+  const uint32_t b = type_bytes(c.type);
+  const uint64_t row = up_to((uint64_t)c.width * b, 16);
+  FfWork w = {kNone, kNone, kNone, kNone, 0, false};
+  const auto take = [&](uint64_t bytes) {
+    const uint64_t at = w.total;
+    w.total += part(bytes);
+    return at;
+  };
+  if (!readable(c.x, c.width, c.x_stride, b)) w.x = take(c.n * row);
+  if (!readable(c.w_gate, c.width, c.gate_stride, b)) w.w_gate = take(c.inner * row);
+  if (!readable(c.w_up, c.width, c.up_stride, b)) w.w_up = take(c.inner * row);
+  if (grad) {
+    w.low = c.type != EC_F32 && c.n <= kFewRows;
+    w.d = take(c.n * 2 * up_to(c.inner, 8) * b * (w.low ? 2 : 1));
+  }
+  return w;
+}
+
+template <typename T>
+Operand in_place(const void* p, uint64_t stride, uint64_t rows, uint32_t width, uint64_t at, char* work,
+                 hipStream_t st) {
+  if (at == kNone) return {(const char*)p, stride * sizeof(T), (uint32_t)rows};
+  pack<T>((const T*)p, stride, rows, width, (T*)(work + at), st);
+  return {work + at, up_to(width, Group<T>::kN) * sizeof(T), (uint32_t)rows};
+}
+
+template <typename T, bool GRAD>
+void run_ff(FfArgs& p, hipStream_t st) {
+  with_shape<false>([&](uint64_t side) { return tiles_of(p.n, 2ull * p.inner, side); }, [&](auto s) {
+    typedef decltype(s) S;
+    p.tiles_m = (p.n + S::BM - 1) / S::BM;
+    p.tiles_n = (p.inner + S::BN / 2 - 1) / (S::BN / 2);
+    ff_kernel<S, T, GRAD><<<p.tiles_m * p.tiles_n, S::kLanes, 0, st>>>(p);
+  });
+}
+
+template <typename T, typename O, bool ACROSS_A>
+void run_sum(SumArgs& p, uint32_t outs, hipStream_t st) {
+  with_shape<false>([&](uint64_t side) { return outs * tiles_of(p.M, p.N, side); }, [&](auto s) {
+    typedef decltype(s) S;
+    p.tiles_m = (p.M + S::BM - 1) / S::BM;
+    p.tiles_n = (p.N + S::BN - 1) / S::BN;
+    sum_kernel<S, T, O, ACROSS_A><<<dim3(p.tiles_m * p.tiles_n, outs), S::kLanes, 0, st>>>(p);
+  });
+}
+
+int check_call(const FfCall& c, int act) {
+  if (!known_type(c.type) || act < EC_ACT_SILU || act > EC_ACT_GELU_TANH) return EC_EINVAL;
+  if (!c.width || !c.inner) return EC_EINVAL;
+  if (c.x_stride < c.width || c.gate_stride < c.width || c.up_stride < c.width) return EC_EINVAL;
+  if (!c.w_gate || !c.w_up || (c.n && !c.x)) return EC_EINVAL;
+  if (c.n >= 1ull << 31 || c.width > kMostWidth || c.inner > kMostWidth) return EC_ERANGE;
+  // a launch takes less than 2^32 lanes
+  if (tiles_of(c.n, 2ull * c.inner, Middle::BM) >= (1ull << 32) / Middle::kLanes) return EC_ERANGE;
+  return EC_OK;
+}
+
+int check_work(const void* work, uint64_t have, uint64_t need) {
+  if (have < need || (need && !work)) return EC_EINVAL;
+  return (uintptr_t)work & 15u ? EC_EALIGN : EC_OK;
+}
+
+}  // namespace
+}  // namespace ec
+
+using namespace ec;
+
+extern "C" {
+
+uint64_t ec_gated_ff_workspace(const void* d_x, uint64_t x_stride, const void* d_gate, uint64_t gate_stride,
+                               const void* d_up, uint64_t up_stride, int type, uint64_t n, uint32_t width,
+                               uint32_t inner, int grad) {
+  const FfCall c = {d_x, d_gate, d_up, x_stride, gate_stride, up_stride, n, width, inner, type};
+  return check_call(c, EC_ACT_SILU) == EC_OK ? ff_work(c, grad != 0).total : 0;
+}
+
+int ec_gated_ff(const void* d_x, uint64_t x_stride, const void* d_gate, uint64_t gate_stride,
+                const void* d_up, uint64_t up_stride, int type, uint64_t n, uint32_t width,
+                uint32_t inner, int activation, void* d_h, uint64_t h_stride, void* d_work,
+                uint64_t work_bytes, ec_stream_t stream) {
+  const FfCall c = {d_x, d_gate, d_up, x_stride, gate_stride, up_stride, n, width, inner, type};
+  if (const int st = check_call(c, activation)) return st;
+  if (h_stride < inner || (n && !d_h)) return EC_EINVAL;
+  const FfWork w = ff_work(c, false);
+  if (const int st = check_work(d_work, work_bytes, w.total)) return st;
+  if (!n) return EC_OK;
+  const auto st = (hipStream_t)stream;
+  return with_type(type, [&](auto t) {
+    typedef decltype(t) T;
+    char* work = (char*)d_work;
+    FfArgs p = {};
+    p.x = in_place<T>(d_x, x_stride, n, width, w.x, work, st);
+    p.w_gate = in_place<T>(d_gate, gate_stride, inner, width, w.w_gate, work, st);
+    p.w_up = in_place<T>(d_up, up_stride, inner, width, w.w_up, work, st);
+    p.n = (uint32_t)n, p.width = width, p.inner = inner, p.act = (uint32_t)activation;
+    p.h = (char*)d_h, p.h_stride = h_stride;
+    run_ff<T, false>(p, st);
+    return launched();
+  });
+}
+
+int ec_gated_ff_grad(const void* d_dh, uint64_t dh_stride, const void* d_x, uint64_t x_stride,
+                     const void* d_gate, uint64_t gate_stride, const void* d_up, uint64_t up_stride,
+                     int type, uint64_t n, uint32_t width, uint32_t inner, int activation, void* d_dx,
+                     uint64_t dx_stride, void* d_dgate, uint64_t dgate_stride, void* d_dup,
+                     uint64_t dup_stride, int grad_type, int accumulate, void* d_work,
+                     uint64_t work_bytes, ec_stream_t stream) {
+  const FfCall c = {d_x, d_gate, d_up, x_stride, gate_stride, up_stride, n, width, inner, type};
+  if (const int st = check_call(c, activation)) return st;
+  if (dh_stride < inner || (n && !d_dh) || (d_dx && dx_stride < width)) return EC_EINVAL;
+  if (!d_dgate != !d_dup || (!d_dx && !d_dgate)) return EC_EINVAL;
+  if (d_dgate && (dgate_stride < width || dup_stride < width)) return EC_EINVAL;
+  if (grad_type != EC_F32 && grad_type != type) return EC_EINVAL;
+  const FfWork w = ff_work(c, true);
+  if (const int st = check_work(d_work, work_bytes, w.total)) return st;
+  if (!n && (!d_dgate || accumulate)) return EC_OK;
+  const auto st = (hipStream_t)stream;
+  return with_type(type, [&](auto t) {
+    typedef decltype(t) T;
+    char* work = (char*)d_work;
+    FfArgs p = {};
+    p.n = (uint32_t)n, p.width = width, p.inner = inner, p.act = (uint32_t)activation;
+    p.padded = (uint32_t)up_to(inner, 8);
+    const uint64_t d_row = 2ull * p.padded;
+    if (n) {
+      p.x = in_place<T>(d_x, x_stride, n, width, w.x, work, st);
+      p.w_gate = in_place<T>(d_gate, gate_stride, inner, width, w.w_gate, work, st);
+      p.w_up = in_place<T>(d_up, up_stride, inner, width, w.w_up, work, st);
+      p.dh = (const char*)d_dh, p.dh_stride = dh_stride;
+      p.d = work + w.d;
+      p.low = w.low ? n * d_row : 0;
+      run_ff<T, true>(p, st);
+    }
+    const uint64_t ld = d_row * sizeof(T), half = p.padded * sizeof(T), low = p.low * sizeof(T);
+    if (d_dx && n) {
+      SumArgs s = {};
+      s.parts = p.low ? 4 : 2;
+      for (uint32_t i = 0; i < s.parts; ++i) {
+        s.a[i] = {p.d + i % 2 * half + i / 2 * low, ld, p.n};
+        s.b[i] = i % 2 ? p.w_up : p.w_gate;
+        s.b[i].rows = width;
+      }
+      s.K = inner, s.M = p.n, s.N = width;
+      s.out[0] = (char*)d_dx, s.out_stride[0] = dx_stride;
+      run_sum<T, T, false>(s, 1, st);
+    }
+    if (d_dgate) {
+      SumArgs s = {};
+      s.parts = !n ? 0 : p.low ? 2 : 1;
+      for (uint32_t i = 0; i < s.parts; ++i) {
+        s.a[i] = {p.d + i * low, ld, inner};
+        s.b[i] = p.x;
+        s.b[i].rows = width;
+      }
+      s.a_step = half;
+      s.K = p.n, s.M = inner, s.N = width;
+      s.out[0] = (char*)d_dgate, s.out_stride[0] = dgate_stride;
+      s.out[1] = (char*)d_dup, s.out_stride[1] = dup_stride;
+      s.accumulate = accumulate;
+      if (grad_type == EC_F32)
+        run_sum<T, float, true>(s, 2, st);
+      else
+        run_sum<T, T, true>(s, 2, st);
+    }
+    return launched();
+  });
+}
+
+}  // extern "C"

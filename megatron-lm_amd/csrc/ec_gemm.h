@@ -1,0 +1,400 @@
+// ec_gemm.h — matrix products on the matrix cores for ec_ff.hip and ec_ortho.hip.
+//
+// C[m][n] = sum over k of A(m, k) * B(n, k).  A workgroup computes a BM x BN tile, a wave a
+// WM x WN part of it, in fp32 accumulators.  A step of the loop over k covers 128 bytes of a
+// row: 64 16-bit values, 32 fp32 ones, or 32 pairs (below).  Its BM + BN rows go from memory
+// straight to LDS (buffer_load ... lds, 16 bytes a lane), one step ahead of the products, and
+// from LDS to fragments of 16 rows by 16 bytes a lane.
+//
+// An operand lies in memory in one of two ways: along k ([rows][k], the tile in LDS is
+// [rows][128 bytes]), or across it ([k][rows], the tile is [k][rows], and the 16-bit fragments are
+// transposed on the way out of LDS, by ds_read_b64_tr_b16: of 16 lanes that give the
+// addresses of four times 16 values, lane i gets the four i-th ones).  So no operand is
+// ever transposed in memory.  16-byte chunks are exchanged within their row of the tile by an
+// exclusive or with a function of the row, so that neither form of reading meets bank conflicts.
+//
+// Ends: the buffer's size bounds the reads, which give zeros past it; chunks past the end of a row are
+// pointed there.  So operands are 16-byte aligned, rows a multiple of 16 bytes apart, and the
+// dimension along a row a multiple of 16 bytes (or padded to one, with zeros if it is k).
+//
+// Pairs: a value as the sum of two fp16 ones, 22 bits of significand: eight high parts, then the
+// eight low parts, in 32 bytes.  A product of two pairs takes three of the matrix cores' products
+// (the low parts' is below the fp32 accumulator's rounding), at 3/16 of the time of fp32 products.
+#pragma once
+
+#include "ec_types.h"
+#include "routes.h"
+
+namespace ec {
+namespace {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef int i4 __attribute__((ext_vector_type(4)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef short s8 __attribute__((ext_vector_type(8)));
+
+template <typename T>
+using local = __attribute__((address_space(3))) T;
+
+struct pair_t {   // 4 bytes of a matrix of pairs
+  uint32_t bits;
+};
+
+constexpr int kRowBytes = 128;   // of a step along k
+constexpr uint32_t kNowhere = 0x80000000u;   // an offset past any buffer below
+
+template <typename T>
+struct Kind {   // bf16, fp16
+  static constexpr int kBytes = 2, kSubs = 2, kParts = 1;
+};
+template <>
+struct Kind<float> {
+  static constexpr int kBytes = 4, kSubs = 2, kParts = 1;
+};
+template <>
+struct Kind<pair_t> {
+  static constexpr int kBytes = 4, kSubs = 1, kParts = 2;
+};
+
+template <typename T>
+struct Frag {
+  s8 part[Kind<T>::kParts];
+};
+
+// acc[m = lane % 16][n = 4 (lane / 16) + i] += A B: the second operand's rows go along the accumulators
+// of a lane, so that a lane stores four neighbours of a row of C.
+template <typename T>
+__device__ __forceinline__ void mma(f4& acc, const Frag<T>& a, const Frag<T>& b) {
+  typedef bf16_t __attribute__((ext_vector_type(8))) b8;
+  typedef fp16_t __attribute__((ext_vector_type(8))) h8;
+  if constexpr (__is_same(T, bf16_t)) {
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, b.part[0]),
+                                                  __builtin_bit_cast(b8, a.part[0]), acc, 0, 0, 0);
+  } else if constexpr (__is_same(T, fp16_t)) {
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, b.part[0]),
+                                                 __builtin_bit_cast(h8, a.part[0]), acc, 0, 0, 0);
+  } else if constexpr (__is_same(T, float)) {
+    const f4 x = __builtin_bit_cast(f4, a.part[0]), y = __builtin_bit_cast(f4, b.part[0]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(y[e], x[e], acc, 0, 0, 0);
+  } else {
+    const h8 ah = __builtin_bit_cast(h8, a.part[0]), al = __builtin_bit_cast(h8, a.part[1]);
+    const h8 bh = __builtin_bit_cast(h8, b.part[0]), bl = __builtin_bit_cast(h8, b.part[1]);
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(bl, ah, acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(bh, al, acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(bh, ah, acc, 0, 0, 0);
+  }
+}
+
+// The exclusive or on the 16-byte chunks of row k of a tile across k.
+template <typename T>
+__device__ __forceinline__ uint32_t across_swizzle(uint32_t k, uint32_t chunks) {
+  if constexpr (__is_same(T, float)) return (k >> 2 & 3) * 4 & (chunks - 1);
+  return ((k & 3) | (k >> 1 & 4)) * (Kind<T>::kParts == 2 ? 4 : 2) & (chunks - 1);
+}
+
+// Fragment `block` (16 rows of the operand) of sub-step `sub` of a tile of ROWS rows.
+template <typename T, int ROWS, bool ACROSS>
+__device__ __forceinline__ Frag<T> read_frag(const local<char>* tile, int block, int sub) {
+  const uint32_t l = threadIdx.x % 64, i = l % 16, q = l / 16;
+  Frag<T> f;
+  if constexpr (!ACROSS) {
+    const local<char>* row = tile + (block * 16 + i) * kRowBytes;
+    if constexpr (Kind<T>::kParts == 2) {
+      f.part[0] = *(const local<s8>*)(row + (2 * q ^ (i & 7)) * 16);
+      f.part[1] = *(const local<s8>*)(row + ((2 * q + 1) ^ (i & 7)) * 16);
+    } else {
+      f.part[0] = *(const local<s8>*)(row + ((sub * 4 + q) ^ (i & 7)) * 16);
+    }
+  } else if constexpr (__is_same(T, float)) {
+    f4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t k = sub * 16 + 4 * q + e;
+      const uint32_t chunk = (block * 4 + i / 4) ^ across_swizzle<T>(k, ROWS / 4);
+      v[e] = *(const local<float>*)(tile + k * (ROWS * 4) + chunk * 16 + i % 4 * 4);
+    }
+    f.part[0] = __builtin_bit_cast(s8, v);
+  } else {
+    constexpr int P = Kind<T>::kParts;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      s4 half[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t k = sub * 32 + 8 * q + 4 * h + i / 4;
+        const uint32_t chunk = ((block * 2 + i % 4 / 2) * P + p) ^
+                               across_swizzle<T>(k, ROWS * Kind<T>::kBytes / 16);
+        half[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (local<s4>*)(tile + k * (ROWS * Kind<T>::kBytes) + chunk * 16 + i % 2 * 8));
+      }
+      f.part[p] = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+  return f;
+}
+
+// A value that is the same in every lane, for the scalar unit: buffers are described by scalars.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// An operand: `rows` of it and K values along k; consecutive rows of memory are ld bytes apart.
+struct Operand {
+  const char* p;
+  uint64_t ld;
+  uint32_t rows;
+};
+
+// 16 bytes a lane from the buffer at byte `offset` to LDS at `lds` + 16 * lane.  The nop stands
+// between the write of m0 and its use.  (m0 is reserved: the compiler keeps nothing in it.)
+__device__ __forceinline__ void to_lds(uint32_t lds, uint32_t offset, const i4& buffer) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(lds), "v"(offset), "s"(buffer)
+               : "memory");
+}
+
+__device__ __forceinline__ uint32_t lds_address(const local<char>* p) { return (uint32_t)(uintptr_t)p; }
+
+// Brings the ROWS rows of an operand's tile to LDS step by step.  DUAL: 32 rows of a first operand,
+// 32 of a second one, and so on.
+template <typename T, int ROWS, int WAVES, bool ACROSS, bool DUAL>
+struct Loader {
+  static_assert(!(ACROSS && DUAL), "only operands along k are taken in turns");
+  static constexpr int kLoads = ROWS * kRowBytes / (WAVES * 1024);
+  static constexpr int kStep = kRowBytes / Kind<T>::kBytes;
+  uint32_t offset[kLoads];
+  uint64_t base, other;
+  uint64_t ld;
+  // bytes along k not yet brought, or rows across it; signed, as a saturating difference would
+  // leave the scalar unit
+  int32_t left;
+  uint32_t last_row;   // byte offset of the tile's last row of memory, where it bounds the buffer
+  uint32_t row_bytes;  // ACROSS: bytes of the tile's part of a row
+  uint32_t wave;
+
+  // up to the end of the last 16 bytes, or eight pairs
+  static __device__ __forceinline__ uint32_t whole(uint32_t bytes) {
+    constexpr uint32_t unit = 16 * Kind<T>::kParts;
+    return (bytes + unit - 1) & ~(unit - 1);
+  }
+
+  __device__ __forceinline__ void init(const Operand& a, const Operand& b, uint32_t row0, uint32_t k,
+                                       uint32_t w) {
+    const uint32_t l = threadIdx.x % 64;
+    wave = w;
+    ld = a.ld;
+    if constexpr (!ACROSS) {
+      const uint32_t first = DUAL ? row0 / 2 : row0, most = DUAL ? ROWS / 2 : ROWS;
+      base = (uint64_t)(uintptr_t)a.p + first * a.ld;
+      other = DUAL ? (uint64_t)(uintptr_t)b.p + first * b.ld : 0;
+      left = (int32_t)whole(k * Kind<T>::kBytes);
+      last_row = (min(most, a.rows - first) - 1) * (uint32_t)ld;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const uint32_t r = (i * WAVES + wave) * 8 + l / 8;
+        const uint32_t from = DUAL ? r / 64 * 32 + r % 32 : r;
+        offset[i] = from * (uint32_t)ld + ((l % 8) ^ (r & 7)) * 16;
+      }
+    } else {
+      base = (uint64_t)(uintptr_t)a.p + (uint64_t)row0 * Kind<T>::kBytes;
+      left = (int32_t)k;
+      row_bytes = whole(min((uint32_t)ROWS, a.rows - row0) * Kind<T>::kBytes);
+      constexpr uint32_t chunks = ROWS * Kind<T>::kBytes / 16;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const uint32_t slot = (i * WAVES + wave) * 64 + l, r = slot / chunks;
+        const uint32_t c = slot % chunks ^ across_swizzle<T>(r, chunks);
+        offset[i] = c * 16 < row_bytes ? r * (uint32_t)ld + c * 16 : kNowhere;
+      }
+    }
+  }
+
+  static __device__ __forceinline__ i4 buffer(uint64_t at, uint32_t bytes) {
+    return i4{(int)(uint32_t)at, (int)((uint32_t)(at >> 32) & 0xffffu), (int)bytes, 0x00020000};
+  }
+
+  // The next step's tile, to LDS at `lds`; as often as there are steps.
+  __device__ __forceinline__ void issue(uint32_t lds) {
+    uint32_t bytes;
+    if constexpr (!ACROSS) {
+      if (left < kRowBytes) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+          const uint32_t r = (i * WAVES + wave) * 8 + threadIdx.x % 64 / 8;
+          if (((threadIdx.x % 8) ^ (r & 7)) * 16 >= (uint32_t)left) offset[i] = kNowhere;
+        }
+      }
+      bytes = last_row + (uint32_t)left;
+      left -= kRowBytes;
+    } else {
+      bytes = (uint32_t)(min(left, kStep) - 1) * (uint32_t)ld + row_bytes;
+      left -= kStep;
+    }
+    const i4 one = buffer(base, bytes), two = buffer(other, bytes);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const uint32_t at = lds + (i * WAVES + wave) * 1024;
+      if constexpr (DUAL) {
+        const bool second = (i * WAVES + wave) / 4 & 1;
+        to_lds(at, offset[i], second ? two : one);
+      } else {
+        to_lds(at, offset[i], one);
+      }
+    }
+    const uint64_t step = ACROSS ? kStep * ld : kRowBytes;
+    base += step;
+    if (DUAL) other += step;
+  }
+};
+
+// A tile's geometry: BM x BN by waves of WM x WN.
+template <int BM_, int BN_, int WM_, int WN_>
+struct Shape {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
+  static constexpr int kWavesN = BN / WN, kWaves = (BM / WM) * kWavesN, kLanes = kWaves * 64;
+  static constexpr int MI = WM / 16, NI = WN / 16;
+  static constexpr int kStage = (BM + BN) * kRowBytes, kLds = 2 * kStage;
+};
+
+typedef Shape<256, 256, 128, 64> Large;    // 8 waves, a workgroup per CU
+typedef Shape<128, 128, 64, 64> Middle;    // 4 waves, two workgroups per CU
+typedef Shape<64, 64, 32, 32> Small;       // 4 waves, five workgroups per CU
+
+template <class S>
+struct Acc {
+  f4 v[S::MI][S::NI];
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < S::MI; ++i)
+#pragma unroll
+      for (int j = 0; j < S::NI; ++j) v[i][j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  // f(m, n, value): row m and columns n ... n + 3 of the tile.
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    const uint32_t l = threadIdx.x % 64, w = threadIdx.x / 64;
+    const uint32_t m0 = w / S::kWavesN * S::WM + l % 16, n0 = w % S::kWavesN * S::WN + l / 16 * 4;
+#pragma unroll
+    for (int i = 0; i < S::MI; ++i)
+#pragma unroll
+      for (int j = 0; j < S::NI; ++j) f(m0 + i * 16, n0 + j * 16, v[i][j]);
+  }
+};
+
+// Every load of this wave to LDS has landed and its reads of LDS are done, and the same holds
+// for the other waves.
+__device__ __forceinline__ void stage_barrier() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// acc += A B over K values along k, for the tile at (m0, n0); b2 is the second operand of a DUAL product.
+template <class S, typename T, bool ACROSS_A, bool ACROSS_B, bool DUAL>
+__device__ __forceinline__ void product(Acc<S>& acc, local<char>* lds, const Operand& a,
+                                        const Operand& b, const Operand& b2, uint32_t m0, uint32_t n0,
+                                        uint32_t K) {
+  Loader<T, S::BM, S::kWaves, ACROSS_A, false> la;
+  Loader<T, S::BN, S::kWaves, ACROSS_B, DUAL> lb;
+  const uint32_t wave = uniform(threadIdx.x / 64);
+  la.init(a, a, m0, K, wave);
+  lb.init(b, b2, n0, K, wave);
+  constexpr uint32_t step = kRowBytes / Kind<T>::kBytes;
+  const uint32_t steps = (K + step - 1) / step;
+  const int blockA = wave / S::kWavesN * S::MI, blockB = wave % S::kWavesN * S::NI;
+  const uint32_t at = lds_address(lds);
+  stage_barrier();   // what was in LDS before is read
+  la.issue(at);
+  lb.issue(at + S::BM * kRowBytes);
+  for (uint32_t s = 0; s < steps; ++s) {
+    stage_barrier();
+    if (s + 1 < steps) {
+      const uint32_t next = at + ((s + 1) & 1) * S::kStage;
+      la.issue(next);
+      lb.issue(next + S::BM * kRowBytes);
+    }
+    const local<char>* tile = lds + (s & 1) * S::kStage;
+#pragma unroll
+    for (int sub = 0; sub < Kind<T>::kSubs; ++sub) {
+      Frag<T> fa[S::MI], fb[S::NI];
+#pragma unroll
+      for (int j = 0; j < S::NI; ++j)
+        fb[j] = read_frag<T, S::BN, ACROSS_B>(tile + S::BM * kRowBytes, blockB + j, sub);
+#pragma unroll
+      for (int i = 0; i < S::MI; ++i) fa[i] = read_frag<T, S::BM, ACROSS_A>(tile, blockA + i, sub);
+#pragma unroll
+      for (int i = 0; i < S::MI; ++i)
+#pragma unroll
+        for (int j = 0; j < S::NI; ++j) mma<T>(acc.v[i][j], fa[i], fb[j]);
+    }
+  }
+}
+
+// Which tile a workgroup computes.  Workgroups go to the 8 XCDs in turns, each with an L2 of
+// its own: each XCD gets a run of tiles, in strips of kStrip tiles of rows, so that those at work
+// together share rows of both operands.
+constexpr uint32_t kXcds = 8, kStrip = 8;
+
+__device__ __forceinline__ uint32_t xcd_order(uint32_t b, uint32_t n) {
+  const uint32_t x = b % kXcds, whole = n / kXcds, more = n % kXcds;
+  return x * whole + min(x, more) + b / kXcds;
+}
+
+__device__ __forceinline__ void tile_at(uint32_t t, uint32_t tiles_m, uint32_t tiles_n, uint32_t& m,
+                                        uint32_t& n) {
+  const uint32_t strip = t / (kStrip * tiles_n), in = t % (kStrip * tiles_n);
+  const uint32_t high = min(kStrip, tiles_m - strip * kStrip);
+  m = uniform(strip * kStrip + in % high);
+  n = uniform(in / high);
+}
+
+// The shape for m x n results: the one whose workgroups, dealt to the CUs in turns, take least time.
+// A tile of four times the area takes a CU four times as long, less the better use of what it loads.
+constexpr uint64_t kCus = 256;
+
+inline uint64_t tiles_of(uint64_t m, uint64_t n, uint64_t side) {
+  return (m + side - 1) / side * ((n + side - 1) / side);
+}
+
+// f(S()) with the shape for `tiles(side)` tiles of side x side; the small one only where SMALL.
+template <bool SMALL, typename F, typename G>
+void with_shape(F tiles, G f) {
+  const auto cost = [&](uint64_t side, uint64_t area) { return (tiles(side) + kCus - 1) / kCus * area; };
+  const uint64_t large = cost(256, 400), middle = cost(128, 120), small = cost(64, 45);
+  if constexpr (SMALL) {
+    if (small < large && small < middle) return f(Small());
+  }
+  if (middle < large) return f(Middle());
+  return f(Large());
+}
+
+// Four neighbours of a row, at column n of `cols`.
+template <typename T>
+__device__ __forceinline__ void store4(T* row, uint32_t n, uint32_t cols, const f4& v) {
+  typedef T __attribute__((ext_vector_type(4))) t4;
+  typedef T __attribute__((ext_vector_type(4), aligned(sizeof(T)))) any4;
+  if (n + 4 <= cols) {
+    *(global<any4>*)(uintptr_t)(row + n) = __builtin_convertvector(v, t4);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < cols) gp(row)[n + e] = (T)v[e];
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ f4 load4(const T* row, uint32_t n, uint32_t cols) {
+  typedef T __attribute__((ext_vector_type(4), aligned(sizeof(T)))) any4;
+  f4 v = {};
+  if (n + 4 <= cols) {
+    v = __builtin_convertvector(*(const global<any4>*)(uintptr_t)(row + n), f4);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < cols) v[e] = (float)gp(row)[n + e];
+  }
+  return v;
+}
+
+}  // namespace
+}  // namespace ec

@@ -149,11 +149,13 @@ int64_t current_stream(int64_t device) {
 
 }  // namespace
 
-void bind_step(py::module_& mod);   // step_torch.cpp
+void bind_step(py::module_& mod);    // step_torch.cpp
+void bind_block(py::module_& mod);   // block_torch.cpp
 
 PYBIND11_MODULE(_ec_shards, mod) {
-  mod.doc() = "torch-tensor binding of the flat-shard and training-step calls of libec_mi355.so";
+  mod.doc() = "torch-tensor binding of the flat-shard, training-step and block calls of libec_mi355.so";
   bind_step(mod);
+  bind_block(mod);
   mod.attr("XOR") = static_cast<int64_t>(kXor);
   mod.attr("ENCODE") = static_cast<int64_t>(kEncode);
   mod.attr("DECODE") = static_cast<int64_t>(kDecode);
