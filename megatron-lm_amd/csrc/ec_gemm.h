@@ -213,37 +213,39 @@ struct Loader {
     return i4{(int)(uint32_t)at, (int)((uint32_t)(at >> 32) & 0xffffu), (int)bytes, 0x00020000};
   }
 
-  // The next step's tile, to LDS at `lds`; as often as there are steps.
-  __device__ __forceinline__ void issue(uint32_t lds) {
-    uint32_t bytes;
+  i4 one, two;         // what begin() describes: the next step's tile
+  uint32_t to;         // and where it goes in LDS
+  bool in;             // whether the lane's chunk of its rows is before their end
+
+  // The next step's tile, to LDS at `lds`: begin(), then every bring(i).  At most two steps past the last.
+  __device__ __forceinline__ void begin(uint32_t lds) {
+    uint32_t bytes;   // 0 past the last step
     if constexpr (!ACROSS) {
-      if (left < kRowBytes) {
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-          const uint32_t r = (i * WAVES + wave) * 8 + threadIdx.x % 64 / 8;
-          if (((threadIdx.x % 8) ^ (r & 7)) * 16 >= (uint32_t)left) offset[i] = kNowhere;
-        }
-      }
-      bytes = last_row + (uint32_t)left;
+      // each of a lane's rows is brought the same chunk of
+      in = ((threadIdx.x % 8) ^ (threadIdx.x / 8 % 8)) * 16 < (uint32_t)max(left, 0);
+      bytes = left > 0 ? last_row + (uint32_t)left : 0;
       left -= kRowBytes;
     } else {
-      bytes = (uint32_t)(min(left, kStep) - 1) * (uint32_t)ld + row_bytes;
+      bytes = left > 0 ? (uint32_t)(min(left, kStep) - 1) * (uint32_t)ld + row_bytes : 0;
       left -= kStep;
     }
-    const i4 one = buffer(base, bytes), two = buffer(other, bytes);
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const uint32_t at = lds + (i * WAVES + wave) * 1024;
-      if constexpr (DUAL) {
-        const bool second = (i * WAVES + wave) / 4 & 1;
-        to_lds(at, offset[i], second ? two : one);
-      } else {
-        to_lds(at, offset[i], one);
-      }
-    }
+    one = buffer(base, bytes);
+    if (DUAL) two = buffer(other, bytes);
+    to = lds + wave * 1024;
     const uint64_t step = ACROSS ? kStep * ld : kRowBytes;
     base += step;
     if (DUAL) other += step;
+  }
+
+  __device__ __forceinline__ void bring(int i) {
+    const bool second = DUAL && ((i * WAVES + wave) / 4 & 1);
+    to_lds(to + i * WAVES * 1024, ACROSS || in ? offset[i] : kNowhere, second ? two : one);
+  }
+
+  __device__ __forceinline__ void issue(uint32_t lds) {
+    begin(lds);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) bring(i);
   }
 };
 
@@ -289,45 +291,117 @@ __device__ __forceinline__ void stage_barrier() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
+// The compiler would put the reads of a group right before their use, to save registers.
+__device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0); }
+
+__device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// A wave's way through a step: kSubs sub-steps of kParts groups of its rows each.  Two groups' fragments are in
+// registers: that which is multiplied and the next one, which is read meanwhile.
+template <class S, typename T, bool ACROSS_A, bool ACROSS_B>
+struct Groups {
+  static constexpr int kParts = S::MI >= 4 ? 2 * Kind<T>::kParts : 2;
+  static constexpr int kRows = S::MI / kParts, kGroups = Kind<T>::kSubs * kParts;
+  static_assert(kGroups % 2 == 0, "the groups' fragments take turns");
+  Frag<T> a[2][kRows], b[2][S::NI];
+  int blockA, blockB;
+
+  // Group g of a tile; the second operand's fragments go to b[turn].
+  __device__ __forceinline__ void read(const local<char>* tile, int g, int turn) {
+    const int sub = g / kParts, at = g % kParts;
+    if (at == 0) {
+#pragma unroll
+      for (int j = 0; j < S::NI; ++j)
+        b[turn][j] = read_frag<T, S::BN, ACROSS_B>(tile + S::BM * kRowBytes, blockB + j, sub);
+    }
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+      a[g & 1][i] = read_frag<T, S::BM, ACROSS_A>(tile, blockA + at * kRows + i, sub);
+  }
+
+  // acc += A B for group g, with between(i) behind each row of products.
+  template <typename F>
+  __device__ __forceinline__ void multiply(Acc<S>& acc, int g, int turn, F between) const {
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+#pragma unroll
+      for (int j = 0; j < S::NI; ++j) mma<T>(acc.v[g % kParts * kRows + i][j], a[g & 1][i], b[turn][j]);
+      between(i);
+    }
+  }
+};
+
 // acc += A B over K values along k, for the tile at (m0, n0); b2 is the second operand of a DUAL product.
+//
+// A step's tile is read group by group, each while the one before is multiplied.  Before the last group is
+// multiplied comes the step's barrier, behind which the tile's place in LDS is free and the next tile has
+// landed: the next tile's first group is read, and the loads of the tile after that go out one by one between
+// the products (all at once they fill the queue, and the waves stand).  So products cover both latencies.
+// The steps past the last one bring zeros, which nobody multiplies.
 template <class S, typename T, bool ACROSS_A, bool ACROSS_B, bool DUAL>
 __device__ __forceinline__ void product(Acc<S>& acc, local<char>* lds, const Operand& a,
                                         const Operand& b, const Operand& b2, uint32_t m0, uint32_t n0,
                                         uint32_t K) {
-  Loader<T, S::BM, S::kWaves, ACROSS_A, false> la;
-  Loader<T, S::BN, S::kWaves, ACROSS_B, DUAL> lb;
+  typedef Loader<T, S::BM, S::kWaves, ACROSS_A, false> LoadA;
+  typedef Loader<T, S::BN, S::kWaves, ACROSS_B, DUAL> LoadB;
+  typedef Groups<S, T, ACROSS_A, ACROSS_B> G;
+  LoadA la;
+  LoadB lb;
   const uint32_t wave = uniform(threadIdx.x / 64);
   la.init(a, a, m0, K, wave);
   lb.init(b, b2, n0, K, wave);
   constexpr uint32_t step = kRowBytes / Kind<T>::kBytes;
   const uint32_t steps = (K + step - 1) / step;
-  const int blockA = wave / S::kWavesN * S::MI, blockB = wave % S::kWavesN * S::NI;
   const uint32_t at = lds_address(lds);
+  G g;
+  g.blockA = wave / S::kWavesN * S::MI, g.blockB = wave % S::kWavesN * S::NI;
+  const auto one_step = [&](uint32_t s, int parity) {
+    const local<char>* tile = lds + (s & 1) * S::kStage;
+    const local<char>* next = lds + ((s + 1) & 1) * S::kStage;
+    // which of b's halves a sub-step's fragments are in
+    const auto turn = [&](int group) { return Kind<T>::kSubs == 1 ? parity : group / G::kParts; };
+#pragma unroll
+    for (int i = 0; i < G::kGroups; ++i) {
+      if (i + 1 < G::kGroups) {
+        g.read(tile, i + 1, turn(i + 1));
+        keep_order();
+        g.multiply(acc, i, turn(i), [](int) {});
+        keep_order();
+      } else {
+        stage_barrier();
+        g.read(next, 0, Kind<T>::kSubs == 1 ? parity ^ 1 : 0);
+        keep_order();
+        const uint32_t to = at + (s & 1) * S::kStage;
+        la.begin(to);
+        lb.begin(to + S::BM * kRowBytes);
+        constexpr int kAll = LoadA::kLoads + LoadB::kLoads, kEach = (kAll + G::kRows - 1) / G::kRows;
+        g.multiply(acc, i, turn(i), [&](int row) {
+#pragma unroll
+          for (int l = row * kEach; l < (row + 1) * kEach && l < kAll; ++l) {
+            if (l < LoadA::kLoads)
+              la.bring(l);
+            else
+              lb.bring(l - LoadA::kLoads);
+          }
+          keep_order();
+        });
+      }
+    }
+  };
   stage_barrier();   // what was in LDS before is read
   la.issue(at);
   lb.issue(at + S::BM * kRowBytes);
+  stage_barrier();
+  la.issue(at + S::kStage);
+  lb.issue(at + S::kStage + S::BM * kRowBytes);
+  g.read(lds, 0, 0);
   for (uint32_t s = 0; s < steps; ++s) {
-    stage_barrier();
-    if (s + 1 < steps) {
-      const uint32_t next = at + ((s + 1) & 1) * S::kStage;
-      la.issue(next);
-      lb.issue(next + S::BM * kRowBytes);
-    }
-    const local<char>* tile = lds + (s & 1) * S::kStage;
-#pragma unroll
-    for (int sub = 0; sub < Kind<T>::kSubs; ++sub) {
-      Frag<T> fa[S::MI], fb[S::NI];
-#pragma unroll
-      for (int j = 0; j < S::NI; ++j)
-        fb[j] = read_frag<T, S::BN, ACROSS_B>(tile + S::BM * kRowBytes, blockB + j, sub);
-#pragma unroll
-      for (int i = 0; i < S::MI; ++i) fa[i] = read_frag<T, S::BM, ACROSS_A>(tile, blockA + i, sub);
-#pragma unroll
-      for (int i = 0; i < S::MI; ++i)
-#pragma unroll
-        for (int j = 0; j < S::NI; ++j) mma<T>(acc.v[i][j], fa[i], fb[j]);
+    one_step(s, 0);
+    if constexpr (Kind<T>::kSubs == 1) {
+      if (++s < steps) one_step(s, 1);
     }
   }
+  loads_done();   // none to LDS is under way when the workgroup gives it back
 }
 
 // Which tile a workgroup computes.  Workgroups go to the 8 XCDs in turns, each with an L2 of
