@@ -519,7 +519,8 @@ uint64_t ec_orthogonalize_workspace(uint64_t batch, uint64_t rows, uint64_t cols
  * (or X' X from the right, the same for rows > cols) with {a, b, c} = coefficients, three values on the host of magnitude
  * up to 1024: each singular value s of X becomes a s + b s^3 + c s^5. base null: out = scale * X; base may be out.
  * base and out are of out_type. Row strides and the distances from matrix to matrix are in elements.
- * Products are of values of 22 bits, in fp32 sums, and |x| is summed in fp64. The iterates' magnitudes have to
+ * Products are of values of 22 bits, in fp32 sums, and |x| is summed in fp64; where out is bf16 and rows and cols are 64 or
+ * more, products are of 11 bits, added to a X with 22: about 1e-3 of the result. The iterates' magnitudes have to
  * stay below 15 (values past it become infinite): with coefficients that keep [0, 1.2] in itself they are below 1.5.
  * A matrix with a value that is not finite gives NaN; one of zeros gives keep * base. A matrix whose |x| is
  * far below eps keeps fewer bits. EC_ERANGE for rows, cols or batch > 65536, steps past

@@ -209,7 +209,8 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Sequence[flo
 
     A weight update in place: ``orthogonalize(momentum, scale=-lr, base=weight, keep=1 - lr * decay, out=weight)``.
     The result is of ``out``'s type, or ``dtype``, or the base's, or x's; base and out are of the same.  Products
-    are of values of 22 bits with fp32 sums, whatever the types.  The coefficients are of magnitude up to 1024 and have to keep the
+    are of values of 22 bits with fp32 sums; for a bf16 result with 64 or more rows and columns of
+    11 bits, added to a X with 22, which leaves about 1e-3 of the result.  The coefficients are of magnitude up to 1024 and have to keep the
     iterates' entries below 15.  A value that is not finite makes its matrix NaN."""
     steps = int(steps)
     if not 1 <= steps <= 64:

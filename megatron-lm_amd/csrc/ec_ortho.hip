@@ -6,9 +6,18 @@
 // and above the diagonal are computed, and written twice.
 //
 // Small singular values grow by `a` a step, and so do the rounding errors of what is
-// stored in between: with 16-bit matrices 0.2 % (fp16) or 2 % (bf16) of the result after five
-// steps.  So the matrices in between are pairs of fp16 values (22 bits, ec_gemm.h), and the result is as
-// good as that of fp32 products, at a third of the fp16 rate instead of the fp32 products' sixteenth.
+// stored in between: with X, A and B in 16 bits 0.2 % (fp16) or 2 % (bf16) of the result after five
+// steps.  There are two kinds of steps:
+// - exact ones: all matrices are pairs of fp16 values (22 bits, ec_gemm.h).  The result is as good as that of
+//   fp32 products (4.5e-7 off after five steps), at a third of the fp16 rate instead of a sixteenth.
+// - fast ones: the products are of fp16 values, but X = a X + (b A + c A A) X, and the X that a stands before
+//   has a second fp16 part.  What small singular values consist of is that first term; the
+//   products' errors are small where they are.  Five of them leave 0.8e-3 to 1.1e-3 of the result (without the second
+//   part 1.9e-3 to 2.5e-3), against 1.7e-3 by the rounding to bf16; an update of a single nonzero row, whose
+//   roundings do not average out, has 2e-3 to 4e-3.
+// A bf16 result takes fast steps, from kFastSide rows and columns on (smaller matrices are bound by the launches, and
+// their roundings average out less); an fp16 or fp32 one exact steps.
+//
 // What is stored is 2^12 times the value: X and A have entries of at most about 1.5 (the norm
 // bounds them), and ordinary ones of 1 / sqrt(columns) and less.
 #include <hip/hip_runtime.h>
@@ -77,49 +86,50 @@ __device__ __forceinline__ void split(float v, fp16_t& high, fp16_t& low) {
 typedef fp16_t __attribute__((ext_vector_type(4))) h4;
 typedef fp16_t __attribute__((ext_vector_type(8))) h8;
 
-// Columns n ... n + 3 (n a multiple of 4) of a row of pairs, or of fp16 values.
+// Columns n ... n + 3 (n a multiple of 4) of a row of pairs; or of one of fp16 values, of a matrix whose second parts
+// are `low_at` bytes behind (0: it has none).
 template <typename K>
-__device__ __forceinline__ void put4(char* row, uint32_t n, const f4& v) {
-  if constexpr (__is_same(K, pair_t)) {
-    h4 high, low;
+__device__ __forceinline__ void put4(char* row, uint32_t n, const f4& v, uint64_t low_at) {
+  h4 high, low;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      fp16_t h, l;
-      split(v[e], h, l);
-      high[e] = h;
-      low[e] = l;
-    }
+  for (int e = 0; e < 4; ++e) {
+    fp16_t h, l;
+    split(v[e], h, l);
+    high[e] = h;
+    low[e] = l;
+  }
+  if constexpr (Kind<K>::kParts == 2) {
     global<char>* to = gp(row) + n / 8 * 32 + n % 8 * 2;
     *(global<h4>*)to = high;
     *(global<h4>*)(to + 16) = low;
   } else {
-    *(global<h4>*)(gp(row) + n * 2) = __builtin_convertvector(v, h4);
+    *(global<h4>*)(gp(row) + n * 2) = high;
+    if (low_at) *(global<h4>*)(gp(row) + n * 2 + low_at) = low;
   }
 }
 
 template <typename K>
-__device__ __forceinline__ f4 get4(const char* row, uint32_t n) {
-  if constexpr (__is_same(K, pair_t)) {
-    const global<char>* from = gp(row) + n / 8 * 32 + n % 8 * 2;
-    return __builtin_convertvector(*(const global<h4>*)from, f4) +
-           __builtin_convertvector(*(const global<h4>*)(from + 16), f4);
-  } else {
-    return __builtin_convertvector(*(const global<h4>*)(gp(row) + n * 2), f4);
-  }
+__device__ __forceinline__ f4 get4(const char* row, uint32_t n, uint64_t low_at) {
+  constexpr bool kPairs = Kind<K>::kParts == 2;
+  const global<char>* from = gp(row) + (kPairs ? n / 8 * 32 + n % 8 * 2 : n * 2);
+  f4 v = __builtin_convertvector(*(const global<h4>*)from, f4);
+  if (kPairs || low_at) v += __builtin_convertvector(*(const global<h4>*)(from + (kPairs ? 16 : low_at)), f4);
+  return v;
 }
 
-// x / (|x| + eps) as pairs, 8 elements a lane, with zeros behind a row's end.  |x| comes from the partial sums
-// in order, in every workgroup.
-template <typename T>
+// x / (|x| + eps) as a matrix of K, 8 elements a lane, with zeros behind a row's end.  |x| comes from the partial
+// sums in order, in every workgroup.
+template <typename T, typename K>
 __global__ void __launch_bounds__(kLanes) scale_kernel(const T* x, uint64_t stride, uint64_t matrix,
                                                        uint32_t rows, uint32_t cols, const double* parts,
-                                                       uint32_t n_parts, double eps, char* out) {
+                                                       uint32_t n_parts, double eps, char* out, uint64_t low_at) {
   double sum = 0.0;
   for (uint32_t i = 0; i < n_parts; ++i) sum += gp(parts)[blockIdx.y * kMostParts + i];
   const double by = (double)(1 << kStored) / (__builtin_sqrt(sum) + eps);
   const T* from = x + blockIdx.y * matrix;
   const uint32_t groups = (cols + 7) / 8, all = rows * groups;
-  char* to = out + (uint64_t)blockIdx.y * all * 32;
+  constexpr uint32_t kGroup = 8 * Kind<K>::kBytes;
+  char* to = out + (uint64_t)blockIdx.y * all * kGroup;
   for (uint32_t g = blockIdx.x * kLanes + threadIdx.x; g < all; g += gridDim.x * kLanes) {
     const uint32_t row = g / groups, at = g % groups * 8;
     const T* p = from + row * stride;
@@ -134,9 +144,9 @@ __global__ void __launch_bounds__(kLanes) scale_kernel(const T* x, uint64_t stri
       high[e] = h;
       low[e] = l;
     }
-    global<char>* q = gp(to) + (uint64_t)g * 32;
+    global<char>* q = gp(to) + (uint64_t)g * kGroup;
     *(global<h8>*)q = high;
-    *(global<h8>*)(q + 16) = low;
+    *(global<h8>*)(q + (Kind<K>::kParts == 2 ? 16 : low_at)) = low;
   }
 }
 
@@ -149,14 +159,15 @@ struct NsArgs {
   char* out;
   uint64_t out_ld, out_matrix;   // bytes
   float by;                      // the result: by * product
-  const char* add;               // POLY: + linear * add + diagonal * I
+  uint64_t out_low;              // from a value to its second part, in bytes
+  const char* add;               // + linear * add + diagonal * I, add a matrix like the product
+  uint64_t add_ld, add_matrix, add_low;
   float linear, diagonal;
   Matrices base;                 // LAST: + keep * base, or none
   float keep;
 };
 
-// What becomes of a product: a symmetric matrix of K, one plus a polynomial's other terms, a matrix of
-// K, or the result.
+// What becomes of a product: A, B, the next X, or the result.
 enum { kGram, kPoly, kNext, kLast };
 
 template <class S, typename In, bool ACROSS_A, bool ACROSS_B, int WHAT, typename Out>
@@ -179,36 +190,37 @@ __global__ void __launch_bounds__(S::kLanes) ns_kernel(NsArgs p) {
   acc.clear();
   product<S, In, ACROSS_A, ACROSS_B, false>(acc, (local<char>*)lds, a, b, b, tm * S::BM, tn * S::BN, p.K);
   char* out = p.out + matrix * p.out_matrix;
+  const uint32_t padded = (p.N + 7) & ~7u;
+  const auto value = [&](uint32_t m, uint32_t n, f4 v) {
+    v *= p.by;
+    if (WHAT != kGram && p.add) {
+      if (m < p.M && n < padded)
+        v += p.linear * get4<In>(p.add + matrix * p.add_matrix + m * p.add_ld, n, p.add_low);
+    }
+    if constexpr (WHAT == kPoly) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (m == n + e) v[e] += p.diagonal;
+    }
+    return v;
+  };
   if constexpr (WHAT == kLast) {
     const uint64_t first = matrix * p.base.matrix;
     acc.each([&](uint32_t m, uint32_t n, f4 v) {
       m += tm * S::BM;
       n += tn * S::BN;
       if (m >= p.M || n >= p.N) return;
-      v *= p.by;
+      v = value(m, n, v);
       if (p.base.p) v += p.keep * load4<Out>((const Out*)p.base.p + first + m * p.base.stride, n, p.N);
       store4<Out>((Out*)(out + m * p.out_ld), n, p.N, v);
     });
   } else {
-    const uint32_t padded = (p.N + 7) & ~7u;
-    const auto value = [&](uint32_t m, uint32_t n, f4 v) {
-      v *= p.by;
-      if constexpr (WHAT == kPoly) {
-        if (m < p.M && n < padded) {
-          v += p.linear * get4<In>(p.add + matrix * p.out_matrix + m * p.out_ld, n);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (m == n + e) v[e] += p.diagonal;
-        }
-      }
-      return v;
-    };
     if (!kSymmetric || tm == tn) {
       acc.each([&](uint32_t m, uint32_t n, f4 v) {
         m += tm * S::BM;
         n += tn * S::BN;
         v = value(m, n, v);
-        if (m < p.M && n < padded) put4<Out>(out + m * p.out_ld, n, v);
+        if (m < p.M && n < padded) put4<Out>(out + m * p.out_ld, n, v, p.out_low);
       });
     } else {
       // and the mirrored tile, 16 x 16 at a time turned round in the wave's part of LDS
@@ -220,7 +232,7 @@ __global__ void __launch_bounds__(S::kLanes) ns_kernel(NsArgs p) {
         m += tm * S::BM;
         n += tn * S::BN;
         v = value(m, n, v);
-        if (m < p.M && n < padded) put4<Out>(out + m * p.out_ld, n, v);
+        if (m < p.M && n < padded) put4<Out>(out + m * p.out_ld, n, v, p.out_low);
         *(local<f4>*)(turn + l % 16 * kRow + l / 16 * 4) = v;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -231,7 +243,7 @@ __global__ void __launch_bounds__(S::kLanes) ns_kernel(NsArgs p) {
         __builtin_amdgcn_wave_barrier();
         // the block's rows are at m - l % 16, its columns at n - 4 (l / 16)
         const uint32_t row = n - l / 16 * 4 + l % 16, col = m - l % 16 + l / 16 * 4;
-        if (row < p.N && col < padded) put4<Out>(out + row * p.out_ld, col, w);
+        if (row < p.N && col < padded) put4<Out>(out + row * p.out_ld, col, w, p.out_low);
       });
     }
   }
@@ -294,56 +306,87 @@ struct Call {
   float a, b, c, eps, scale, keep;
 };
 
-template <bool TALL>
-int run_steps(const Plan& p, const Call& c, char* work, hipStream_t st) {
-  const auto matrix = [&](uint64_t at, uint32_t rows, uint32_t cols) {
-    return Operand{work + at, up_to(cols, 8) * 4, rows};
-  };
-  // stored times 2^at so that a I + b A + c A A stays below fp16's largest value
-  const float most = std::fabs(c.a) + 2.0f * std::fabs(c.b) + 4.0f * std::fabs(c.c);
+constexpr uint32_t kFastSide = 64;
+
+bool fast(const Plan& p, int out_type) { return out_type == EC_BF16 && p.side >= kFastSide; }
+
+// A matrix of K in the workspace, the bytes of one of the batch, and those to its second parts.
+struct Stored {
+  Operand m;
+  uint64_t matrix, low;
+};
+
+template <typename K>
+Stored stored(char* at, uint32_t batch, uint32_t rows, uint32_t cols, bool low) {
+  Stored s;
+  s.m = {at, up_to(cols, 8) * Kind<K>::kBytes, rows};
+  s.matrix = s.m.ld * rows;
+  s.low = Kind<K>::kParts == 1 && low ? s.matrix * batch : 0;
+  return s;
+}
+
+// Step s: the next step's X, or the result.
+template <bool TALL, typename In>
+int run_step(const Plan& p, const Call& c, char* work, int s, hipStream_t st) {
+  constexpr bool kFast = Kind<In>::kParts == 1;
+  const Stored x = stored<In>(work + p.x[s & 1], p.batch, p.rows, p.cols, true);
+  const Stored gram = stored<In>(work + p.gram, p.batch, p.side, p.side, false);
+  const Stored poly = stored<In>(work + p.poly, p.batch, p.side, p.side, false);
+  // stored times 2^at so that (a I +) b A + c A A stays below fp16's largest value
+  const float most = (kFast ? 0.0f : std::fabs(c.a)) + 2.0f * std::fabs(c.b) + 4.0f * std::fabs(c.c);
   int at = kStored;
   while (at > 0 && std::ldexp(most, at) > 32768.0f) --at;
+
+  NsArgs n = {};
+  n.a = n.b = x.m;
+  n.a.rows = n.b.rows = p.side;
+  n.a_matrix = n.b_matrix = x.matrix;
+  n.K = p.other, n.M = n.N = p.side;
+  n.out = work + p.gram, n.out_ld = gram.m.ld, n.out_matrix = gram.matrix;
+  n.by = std::ldexp(1.0f, -kStored);
+  if (const int e = run_ns<In, TALL, TALL, kGram, In>(n, p.batch, st)) return e;
+
+  n.a = n.b = gram.m;
+  n.a_matrix = n.b_matrix = gram.matrix;
+  n.K = p.side;
+  n.out = work + p.poly;
+  n.add = work + p.gram, n.add_ld = gram.m.ld, n.add_matrix = gram.matrix;
+  n.by = c.c * std::ldexp(1.0f, at - 2 * kStored);
+  n.linear = c.b * std::ldexp(1.0f, at - kStored);
+  n.diagonal = kFast ? 0.0f : c.a * std::ldexp(1.0f, at);
+  if (const int e = run_ns<In, false, false, kPoly, In>(n, p.batch, st)) return e;
+
+  // B X, X across; or X B, X along
+  n.a = TALL ? x.m : poly.m, n.b = TALL ? poly.m : x.m;
+  n.a.rows = p.rows, n.b.rows = p.cols;
+  n.a_matrix = TALL ? x.matrix : poly.matrix, n.b_matrix = TALL ? poly.matrix : x.matrix;
+  n.M = p.rows, n.N = p.cols;
+  n.add = kFast ? x.m.p : nullptr, n.add_ld = x.m.ld, n.add_matrix = x.matrix, n.add_low = x.low;
+  if (s + 1 < c.steps) {
+    n.out = work + p.x[(s + 1) & 1], n.out_ld = x.m.ld, n.out_matrix = x.matrix, n.out_low = x.low;
+    n.by = std::ldexp(1.0f, -at);
+    n.linear = c.a;
+    return run_ns<In, false, !TALL, kNext, In>(n, p.batch, st);
+  }
+  const uint32_t w = type_bytes(c.out_type);
+  n.out = c.out, n.out_ld = c.out_stride * w, n.out_matrix = c.out_matrix * w;
+  n.by = c.scale * std::ldexp(1.0f, -at - kStored);
+  n.linear = c.scale * c.a * std::ldexp(1.0f, -kStored);
+  n.base = c.base, n.keep = c.keep;
+  if constexpr (kFast)
+    return run_ns<In, false, !TALL, kLast, bf16_t>(n, p.batch, st);
+  else
+    return with_type(c.out_type, [&](auto o) {
+      return run_ns<In, false, !TALL, kLast, decltype(o)>(n, p.batch, st);
+    });
+}
+
+template <bool TALL>
+int run_steps(const Plan& p, const Call& c, char* work, hipStream_t st) {
   for (int s = 0; s < c.steps; ++s) {
-    const Operand x = matrix(p.x[s & 1], p.rows, p.cols);
-    const uint64_t xm = x.ld * p.rows;
-    Operand gram = matrix(p.gram, p.side, p.side), poly = matrix(p.poly, p.side, p.side);
-    const uint64_t gm = gram.ld * p.side;
-    NsArgs n = {};
-    n.a = n.b = x;
-    n.a.rows = n.b.rows = p.side;
-    n.a_matrix = n.b_matrix = xm;
-    n.K = p.other, n.M = n.N = p.side;
-    n.out = work + p.gram, n.out_ld = gram.ld, n.out_matrix = gm;
-    n.by = std::ldexp(1.0f, -kStored);
-    if (const int e = run_ns<pair_t, TALL, TALL, kGram, pair_t>(n, p.batch, st)) return e;
-    n.a = n.b = gram;
-    n.a_matrix = n.b_matrix = gm;
-    n.K = p.side;
-    n.out = work + p.poly;
-    n.add = work + p.gram;
-    n.by = c.c * std::ldexp(1.0f, at - 2 * kStored);
-    n.linear = c.b * std::ldexp(1.0f, at - kStored);
-    n.diagonal = c.a * std::ldexp(1.0f, at);
-    if (const int e = run_ns<pair_t, false, false, kPoly, pair_t>(n, p.batch, st)) return e;
-    // X = B X, X across; or X B, X along
-    n.a = TALL ? x : poly, n.b = TALL ? poly : x;
-    n.a.rows = p.rows, n.b.rows = p.cols;
-    n.a_matrix = TALL ? xm : gm, n.b_matrix = TALL ? gm : xm;
-    n.M = p.rows, n.N = p.cols;
-    if (s + 1 < c.steps) {
-      n.out = work + p.x[(s + 1) & 1], n.out_ld = x.ld, n.out_matrix = xm;
-      n.by = std::ldexp(1.0f, -at);
-      if (const int e = run_ns<pair_t, false, !TALL, kNext, pair_t>(n, p.batch, st)) return e;
-    } else {
-      const uint32_t w = type_bytes(c.out_type);
-      n.out = c.out, n.out_ld = c.out_stride * w, n.out_matrix = c.out_matrix * w;
-      n.by = c.scale * std::ldexp(1.0f, -at - kStored);
-      n.base = c.base, n.keep = c.keep;
-      const int e = with_type(c.out_type, [&](auto o) {
-        return run_ns<pair_t, false, !TALL, kLast, decltype(o)>(n, p.batch, st);
-      });
-      if (e) return e;
-    }
+    const int e = fast(p, c.out_type) ? run_step<TALL, fp16_t>(p, c, work, s, st)
+                                      : run_step<TALL, pair_t>(p, c, work, s, st);
+    if (e) return e;
   }
   return EC_OK;
 }
@@ -391,9 +434,14 @@ int ec_orthogonalize(const void* d_x, int type, uint64_t batch, uint64_t rows, u
     typedef decltype(t) T;
     square_kernel<T><<<dim3(parts, (uint32_t)batch), kLanes, 0, st>>>(
         (const T*)d_x, dense ? kPiece : x_stride, x_matrix, pieces, total, dense ? kPiece : (uint32_t)cols, sums);
-    scale_kernel<T><<<dim3(grid, (uint32_t)batch), kLanes, 0, st>>>(
-        (const T*)d_x, x_stride, x_matrix, (uint32_t)rows, (uint32_t)cols, sums, parts, (double)eps,
-        work + p.x[0]);
+    if (fast(p, out_type)) {
+      const Stored x = stored<fp16_t>(work + p.x[0], p.batch, p.rows, p.cols, true);
+      scale_kernel<T, fp16_t><<<dim3(grid, (uint32_t)batch), kLanes, 0, st>>>(
+          (const T*)d_x, x_stride, x_matrix, p.rows, p.cols, sums, parts, (double)eps, work + p.x[0], x.low);
+    } else {
+      scale_kernel<T, pair_t><<<dim3(grid, (uint32_t)batch), kLanes, 0, st>>>(
+          (const T*)d_x, x_stride, x_matrix, p.rows, p.cols, sums, parts, (double)eps, work + p.x[0], 0);
+    }
     return EC_OK;
   });
   Call c = {};
