@@ -84,46 +84,42 @@ __global__ void __launch_bounds__(S::kLanes) ff_kernel(FfArgs p) {
   // of each 64 columns of the tile the first 32 are gates, the others the ups
   static_assert(S::WN == 64, "a wave holds both projections of its 32 outputs");
   const uint32_t l = threadIdx.x % 64, w = threadIdx.x / 64;
-  const uint32_t m0 = tm * S::BM + w / S::kWavesN * S::WM + l % 16;
-  const uint32_t f0 = tn * (S::BN / 2) + w % S::kWavesN * 32 + l / 16 * 4;
+  const uint32_t m0 = tm * S::BM + w / S::kWavesN * S::WM + l % 16 / 4 * 8 + l % 4;
+  const uint32_t f = tn * (S::BN / 2) + w % S::kWavesN * 32 + l / 16 * 8;
   with_activation(p.act, [&](auto which) {
     constexpr int ACT = decltype(which)::value;
 #pragma unroll
     for (int i = 0; i < S::MI; ++i) {
-      const uint32_t m = m0 + i * 16;
+      const uint32_t m = m0 + i / 2 * 32 + i % 2 * 4;
       if (m >= p.n) continue;
+      const f8 g = acc.pair(i, 0), u = acc.pair(i, 2);
+      if constexpr (!GRAD) {
+        f8 h;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint32_t f = f0 + j * 16;
-        const f4 g = acc.v[i][j], u = acc.v[i][j + 2];
-        if constexpr (!GRAD) {
-          f4 h;
+        for (int e = 0; e < 8; ++e) h[e] = activate<ACT>(g[e]).value * u[e];
+        store8<T>((T*)p.h + m * p.h_stride, f, p.inner, h);
+      } else {
+        const f8 dh = load8<T>((const T*)p.dh + m * p.dh_stride, f, p.inner);
+        f8 dg, du;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) h[e] = activate<ACT>(g[e]).value * u[e];
-          store4<T>((T*)p.h + m * p.h_stride, f, p.inner, h);
-        } else {
-          const f4 dh = load4<T>((const T*)p.dh + m * p.dh_stride, f, p.inner);
-          f4 dg, du;
+        for (int e = 0; e < 8; ++e) {
+          const Act a = activate<ACT>(g[e]);
+          const bool in = f + e < p.inner;   // zeros in the padding, which is summed over
+          dg[e] = in ? dh[e] * u[e] * a.slope : 0.0f;
+          du[e] = in ? dh[e] * a.value : 0.0f;
+        }
+        T* row = (T*)p.d + (uint64_t)m * 2 * p.padded;
+        store8<T>(row, f, p.padded, dg);
+        store8<T>(row + p.padded, f, p.padded, du);
+        if (p.low) {
+          f8 lg, lu;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const Act a = activate<ACT>(g[e]);
-            const bool in = f + e < p.inner;   // zeros in the padding, which is summed over
-            dg[e] = in ? dh[e] * u[e] * a.slope : 0.0f;
-            du[e] = in ? dh[e] * a.value : 0.0f;
+          for (int e = 0; e < 8; ++e) {
+            lg[e] = dg[e] - (float)(T)dg[e];
+            lu[e] = du[e] - (float)(T)du[e];
           }
-          T* row = (T*)p.d + (uint64_t)m * 2 * p.padded;
-          store4<T>(row, f, p.padded, dg);
-          store4<T>(row + p.padded, f, p.padded, du);
-          if (p.low) {
-            f4 lg, lu;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              lg[e] = dg[e] - (float)(T)dg[e];
-              lu[e] = du[e] - (float)(T)du[e];
-            }
-            store4<T>(row + p.low, f, p.padded, lg);
-            store4<T>(row + p.low + p.padded, f, p.padded, lu);
-          }
+          store8<T>(row + p.low, f, p.padded, lg);
+          store8<T>(row + p.low + p.padded, f, p.padded, lu);
         }
       }
     }
@@ -156,13 +152,13 @@ __global__ void __launch_bounds__(S::kLanes) sum_kernel(SumArgs p) {
   }
   O* out = (O*)p.out[blockIdx.y];
   const uint64_t stride = p.out_stride[blockIdx.y];
-  acc.each([&](uint32_t m, uint32_t n, f4 v) {
+  acc.each([&](uint32_t m, uint32_t n, f8 v) {
     m += tm * S::BM;
     n += tn * S::BN;
     if (m >= p.M || n >= p.N) return;
     O* row = out + m * stride;
-    if (p.accumulate) v += load4<O>(row, n, p.N);
-    store4<O>(row, n, p.N, v);
+    if (p.accumulate) v += load8<O>(row, n, p.N);
+    store8<O>(row, n, p.N, v);
   });
 }
 

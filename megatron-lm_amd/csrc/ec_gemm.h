@@ -29,6 +29,7 @@ namespace ec {
 namespace {
 
 typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f8 __attribute__((ext_vector_type(8)));
 typedef int i4 __attribute__((ext_vector_type(4)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef short s8 __attribute__((ext_vector_type(8)));
@@ -86,47 +87,52 @@ __device__ __forceinline__ void mma(f4& acc, const Frag<T>& a, const Frag<T>& b)
   }
 }
 
-// The exclusive or on the 16-byte chunks of row k of a tile across k.
+// Which of a wave's 32 rows fragment h (0, 1) of a pair of fragments holds in lane i of 16:
+// 8 (i / 4) + 4 h + i % 4, so that both accumulators of a lane together are eight neighbours of a row of C,
+// 64 bytes of four lanes.
+
+// The exclusive or on the 16-byte chunks of row r of a tile along k: i % 8 for the row above.
+__device__ __forceinline__ uint32_t along_swizzle(uint32_t r) { return (r & 3) | (r >> 1 & 4); }
+
+// That of row k of a tile across k: the rows that are read together, four neighbours, or for fp32 four that are
+// four apart, are exchanged into different banks.
 template <typename T>
 __device__ __forceinline__ uint32_t across_swizzle(uint32_t k, uint32_t chunks) {
-  if constexpr (__is_same(T, float)) return (k >> 2 & 3) * 4 & (chunks - 1);
-  return ((k & 3) | (k >> 1 & 4)) * (Kind<T>::kParts == 2 ? 4 : 2) & (chunks - 1);
+  const uint32_t f = __is_same(T, float) ? k >> 2 & 3 : along_swizzle(k);
+  return (Kind<T>::kBytes == 4 ? (f >> 1) * 8 | (f & 1) : f * 4) & (chunks - 1);
 }
 
-// Fragment `block` (16 rows of the operand) of sub-step `sub` of a tile of ROWS rows.
+// Fragment `block` (of 16 rows of the operand) of sub-step `sub` of a tile of ROWS rows.
 template <typename T, int ROWS, bool ACROSS>
 __device__ __forceinline__ Frag<T> read_frag(const local<char>* tile, int block, int sub) {
-  const uint32_t l = threadIdx.x % 64, i = l % 16, q = l / 16;
+  constexpr int P = Kind<T>::kParts;
+  const uint32_t l = threadIdx.x % 64, i = l % 16, q = l / 16, pair = block / 2 * 32, h = block % 2;
   Frag<T> f;
   if constexpr (!ACROSS) {
-    const local<char>* row = tile + (block * 16 + i) * kRowBytes;
-    if constexpr (Kind<T>::kParts == 2) {
-      f.part[0] = *(const local<s8>*)(row + (2 * q ^ (i & 7)) * 16);
-      f.part[1] = *(const local<s8>*)(row + ((2 * q + 1) ^ (i & 7)) * 16);
-    } else {
-      f.part[0] = *(const local<s8>*)(row + ((sub * 4 + q) ^ (i & 7)) * 16);
-    }
+    const local<char>* row = tile + (pair + i / 4 * 8 + h * 4 + i % 4) * kRowBytes;
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+      f.part[p] = *(const local<s8>*)(row + (((sub * 4 + q) * P + p) ^ (i & 7)) * 16);
   } else if constexpr (__is_same(T, float)) {
     f4 v;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const uint32_t k = sub * 16 + 4 * q + e;
-      const uint32_t chunk = (block * 4 + i / 4) ^ across_swizzle<T>(k, ROWS / 4);
+      const uint32_t chunk = (pair / 4 + i / 4 * 2 + h) ^ across_swizzle<T>(k, ROWS / 4);
       v[e] = *(const local<float>*)(tile + k * (ROWS * 4) + chunk * 16 + i % 4 * 4);
     }
     f.part[0] = __builtin_bit_cast(s8, v);
   } else {
-    constexpr int P = Kind<T>::kParts;
 #pragma unroll
     for (int p = 0; p < P; ++p) {
       s4 half[2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t k = sub * 32 + 8 * q + 4 * h + i / 4;
-        const uint32_t chunk = ((block * 2 + i % 4 / 2) * P + p) ^
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t k = sub * 32 + 8 * q + 4 * e + i / 4;
+        const uint32_t chunk = ((pair / 8 + i % 4) * P + p) ^
                                across_swizzle<T>(k, ROWS * Kind<T>::kBytes / 16);
-        half[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (local<s4>*)(tile + k * (ROWS * Kind<T>::kBytes) + chunk * 16 + i % 2 * 8));
+        half[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (local<s4>*)(tile + k * (ROWS * Kind<T>::kBytes) + chunk * 16 + h * 8));
       }
       f.part[p] = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
     }
@@ -178,6 +184,12 @@ struct Loader {
     return (bytes + unit - 1) & ~(unit - 1);
   }
 
+  // Along k, the chunk of its rows that a lane brings: they are a multiple of 16 rows apart.
+  __device__ __forceinline__ uint32_t chunk() const {
+    static_assert(WAVES % 2 == 0, "rows of one swizzle");
+    return (threadIdx.x % 8) ^ along_swizzle(wave * 8 + threadIdx.x % 64 / 8);
+  }
+
   __device__ __forceinline__ void init(const Operand& a, const Operand& b, uint32_t row0, uint32_t k,
                                        uint32_t w) {
     const uint32_t l = threadIdx.x % 64;
@@ -193,7 +205,7 @@ struct Loader {
       for (int i = 0; i < kLoads; ++i) {
         const uint32_t r = (i * WAVES + wave) * 8 + l / 8;
         const uint32_t from = DUAL ? r / 64 * 32 + r % 32 : r;
-        offset[i] = from * (uint32_t)ld + ((l % 8) ^ (r & 7)) * 16;
+        offset[i] = from * (uint32_t)ld + chunk() * 16;
       }
     } else {
       base = (uint64_t)(uintptr_t)a.p + (uint64_t)row0 * Kind<T>::kBytes;
@@ -221,8 +233,7 @@ struct Loader {
   __device__ __forceinline__ void begin(uint32_t lds) {
     uint32_t bytes;   // 0 past the last step
     if constexpr (!ACROSS) {
-      // each of a lane's rows is brought the same chunk of
-      in = ((threadIdx.x % 8) ^ (threadIdx.x / 8 % 8)) * 16 < (uint32_t)max(left, 0);
+      in = chunk() * 16 < (uint32_t)max(left, 0);
       bytes = left > 0 ? last_row + (uint32_t)left : 0;
       left -= kRowBytes;
     } else {
@@ -273,15 +284,20 @@ struct Acc {
       for (int j = 0; j < S::NI; ++j) v[i][j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  // f(m, n, value): row m and columns n ... n + 3 of the tile.
+  // f(m, n, values): row m and columns n ... n + 7 of the tile.
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
-    const uint32_t l = threadIdx.x % 64, w = threadIdx.x / 64;
-    const uint32_t m0 = w / S::kWavesN * S::WM + l % 16, n0 = w % S::kWavesN * S::WN + l / 16 * 4;
+    const uint32_t l = threadIdx.x % 64, w = threadIdx.x / 64, i = l % 16;
+    const uint32_t m0 = w / S::kWavesN * S::WM + i / 4 * 8 + i % 4;
+    const uint32_t n0 = w % S::kWavesN * S::WN + l / 16 * 8;
 #pragma unroll
-    for (int i = 0; i < S::MI; ++i)
+    for (int r = 0; r < S::MI; ++r)
 #pragma unroll
-      for (int j = 0; j < S::NI; ++j) f(m0 + i * 16, n0 + j * 16, v[i][j]);
+      for (int j = 0; j < S::NI; j += 2) f(m0 + r / 2 * 32 + r % 2 * 4, n0 + j * 16, pair(r, j));
+  }
+
+  __device__ __forceinline__ f8 pair(int r, int j) const {
+    return __builtin_shufflevector(v[r][j], v[r][j + 1], 0, 1, 2, 3, 4, 5, 6, 7);
   }
 };
 
@@ -442,29 +458,29 @@ void with_shape(F tiles, G f) {
   return f(Large());
 }
 
-// Four neighbours of a row, at column n of `cols`.
+// Eight neighbours of a row, at column n of `cols`.
 template <typename T>
-__device__ __forceinline__ void store4(T* row, uint32_t n, uint32_t cols, const f4& v) {
-  typedef T __attribute__((ext_vector_type(4))) t4;
-  typedef T __attribute__((ext_vector_type(4), aligned(sizeof(T)))) any4;
-  if (n + 4 <= cols) {
-    *(global<any4>*)(uintptr_t)(row + n) = __builtin_convertvector(v, t4);
+__device__ __forceinline__ void store8(T* row, uint32_t n, uint32_t cols, const f8& v) {
+  typedef T __attribute__((ext_vector_type(8))) t8;
+  typedef T __attribute__((ext_vector_type(8), aligned(sizeof(T)))) any8;
+  if (n + 8 <= cols) {
+    *(global<any8>*)(uintptr_t)(row + n) = __builtin_convertvector(v, t8);
   } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+    for (int e = 0; e < 8; ++e)
       if (n + e < cols) gp(row)[n + e] = (T)v[e];
   }
 }
 
 template <typename T>
-__device__ __forceinline__ f4 load4(const T* row, uint32_t n, uint32_t cols) {
-  typedef T __attribute__((ext_vector_type(4), aligned(sizeof(T)))) any4;
-  f4 v = {};
-  if (n + 4 <= cols) {
-    v = __builtin_convertvector(*(const global<any4>*)(uintptr_t)(row + n), f4);
+__device__ __forceinline__ f8 load8(const T* row, uint32_t n, uint32_t cols) {
+  typedef T __attribute__((ext_vector_type(8), aligned(sizeof(T)))) any8;
+  f8 v = {};
+  if (n + 8 <= cols) {
+    v = __builtin_convertvector(*(const global<any8>*)(uintptr_t)(row + n), f8);
   } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+    for (int e = 0; e < 8; ++e)
       if (n + e < cols) v[e] = (float)gp(row)[n + e];
   }
   return v;

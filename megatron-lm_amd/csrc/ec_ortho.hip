@@ -83,37 +83,34 @@ __device__ __forceinline__ void split(float v, fp16_t& high, fp16_t& low) {
   low = (fp16_t)(v - (float)high);
 }
 
-typedef fp16_t __attribute__((ext_vector_type(4))) h4;
 typedef fp16_t __attribute__((ext_vector_type(8))) h8;
 
-// Columns n ... n + 3 (n a multiple of 4) of a row of pairs; or of one of fp16 values, of a matrix whose second parts
+// Columns n ... n + 7 (n a multiple of 8) of a row of pairs; or of one of fp16 values, of a matrix whose second parts
 // are `low_at` bytes behind (0: it has none).
 template <typename K>
-__device__ __forceinline__ void put4(char* row, uint32_t n, const f4& v, uint64_t low_at) {
-  h4 high, low;
+__device__ __forceinline__ void put8(char* row, uint32_t n, const f8& v, uint64_t low_at) {
+  h8 high, low;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
+  for (int e = 0; e < 8; ++e) {
     fp16_t h, l;
     split(v[e], h, l);
     high[e] = h;
     low[e] = l;
   }
-  if constexpr (Kind<K>::kParts == 2) {
-    global<char>* to = gp(row) + n / 8 * 32 + n % 8 * 2;
-    *(global<h4>*)to = high;
-    *(global<h4>*)(to + 16) = low;
-  } else {
-    *(global<h4>*)(gp(row) + n * 2) = high;
-    if (low_at) *(global<h4>*)(gp(row) + n * 2 + low_at) = low;
-  }
+  global<char>* to = gp(row) + n * Kind<K>::kBytes;
+  *(global<h8>*)to = high;
+  if (Kind<K>::kParts == 2)
+    *(global<h8>*)(to + 16) = low;
+  else if (low_at)
+    *(global<h8>*)(to + low_at) = low;
 }
 
 template <typename K>
-__device__ __forceinline__ f4 get4(const char* row, uint32_t n, uint64_t low_at) {
-  constexpr bool kPairs = Kind<K>::kParts == 2;
-  const global<char>* from = gp(row) + (kPairs ? n / 8 * 32 + n % 8 * 2 : n * 2);
-  f4 v = __builtin_convertvector(*(const global<h4>*)from, f4);
-  if (kPairs || low_at) v += __builtin_convertvector(*(const global<h4>*)(from + (kPairs ? 16 : low_at)), f4);
+__device__ __forceinline__ f8 get8(const char* row, uint32_t n, uint64_t low_at) {
+  const global<char>* from = gp(row) + n * Kind<K>::kBytes;
+  f8 v = __builtin_convertvector(*(const global<h8>*)from, f8);
+  if (Kind<K>::kParts == 2 || low_at)
+    v += __builtin_convertvector(*(const global<h8>*)(from + (Kind<K>::kParts == 2 ? 16 : low_at)), f8);
   return v;
 }
 
@@ -132,21 +129,10 @@ __global__ void __launch_bounds__(kLanes) scale_kernel(const T* x, uint64_t stri
   char* to = out + (uint64_t)blockIdx.y * all * kGroup;
   for (uint32_t g = blockIdx.x * kLanes + threadIdx.x; g < all; g += gridDim.x * kLanes) {
     const uint32_t row = g / groups, at = g % groups * 8;
-    const T* p = from + row * stride;
-    const f4 a = load4<T>(p, at, cols);
-    f4 b = {};
-    if (at + 4 < cols) b = load4<T>(p, at + 4, cols);
-    h8 high, low;
+    f8 v = load8<T>(from + row * stride, at, cols);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      fp16_t h, l;
-      split((float)((double)(e < 4 ? a[e % 4] : b[e % 4]) * by), h, l);
-      high[e] = h;
-      low[e] = l;
-    }
-    global<char>* q = gp(to) + (uint64_t)g * kGroup;
-    *(global<h8>*)q = high;
-    *(global<h8>*)(q + (Kind<K>::kParts == 2 ? 16 : low_at)) = low;
+    for (int e = 0; e < 8; ++e) v[e] = (float)((double)v[e] * by);
+    put8<K>(to + (uint64_t)g * kGroup, 0, v, low_at);
   }
 }
 
@@ -191,60 +177,73 @@ __global__ void __launch_bounds__(S::kLanes) ns_kernel(NsArgs p) {
   product<S, In, ACROSS_A, ACROSS_B, false>(acc, (local<char>*)lds, a, b, b, tm * S::BM, tn * S::BN, p.K);
   char* out = p.out + matrix * p.out_matrix;
   const uint32_t padded = (p.N + 7) & ~7u;
-  const auto value = [&](uint32_t m, uint32_t n, f4 v) {
+  const auto value = [&](uint32_t m, uint32_t n, f8 v) {
     v *= p.by;
     if (WHAT != kGram && p.add) {
       if (m < p.M && n < padded)
-        v += p.linear * get4<In>(p.add + matrix * p.add_matrix + m * p.add_ld, n, p.add_low);
+        v += p.linear * get8<In>(p.add + matrix * p.add_matrix + m * p.add_ld, n, p.add_low);
     }
     if constexpr (WHAT == kPoly) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int e = 0; e < 8; ++e)
         if (m == n + e) v[e] += p.diagonal;
     }
     return v;
   };
+  const uint32_t m0 = tm * S::BM, n0 = tn * S::BN;
   if constexpr (WHAT == kLast) {
     const uint64_t first = matrix * p.base.matrix;
-    acc.each([&](uint32_t m, uint32_t n, f4 v) {
-      m += tm * S::BM;
-      n += tn * S::BN;
+    acc.each([&](uint32_t m, uint32_t n, f8 v) {
+      m += m0;
+      n += n0;
       if (m >= p.M || n >= p.N) return;
       v = value(m, n, v);
-      if (p.base.p) v += p.keep * load4<Out>((const Out*)p.base.p + first + m * p.base.stride, n, p.N);
-      store4<Out>((Out*)(out + m * p.out_ld), n, p.N, v);
+      if (p.base.p) v += p.keep * load8<Out>((const Out*)p.base.p + first + m * p.base.stride, n, p.N);
+      store8<Out>((Out*)(out + m * p.out_ld), n, p.N, v);
+    });
+  } else if (!kSymmetric || tm == tn) {
+    acc.each([&](uint32_t m, uint32_t n, f8 v) {
+      m += m0;
+      n += n0;
+      v = value(m, n, v);
+      if (m < p.M && n < padded) put8<Out>(out + m * p.out_ld, n, v, p.out_low);
     });
   } else {
-    if (!kSymmetric || tm == tn) {
-      acc.each([&](uint32_t m, uint32_t n, f4 v) {
-        m += tm * S::BM;
-        n += tn * S::BN;
-        v = value(m, n, v);
-        if (m < p.M && n < padded) put4<Out>(out + m * p.out_ld, n, v, p.out_low);
-      });
-    } else {
-      // and the mirrored tile, 16 x 16 at a time turned round in the wave's part of LDS
-      stage_barrier();
-      constexpr uint32_t kRow = 20;
-      local<float>* turn = (local<float>*)(local<char>*)lds + threadIdx.x / 64 * (16 * kRow);
-      const uint32_t l = threadIdx.x % 64;
-      acc.each([&](uint32_t m, uint32_t n, f4 v) {
-        m += tm * S::BM;
-        n += tn * S::BN;
-        v = value(m, n, v);
-        if (m < p.M && n < padded) put4<Out>(out + m * p.out_ld, n, v, p.out_low);
-        *(local<f4>*)(turn + l % 16 * kRow + l / 16 * 4) = v;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        f4 w;
+    // and the mirrored tile, 32 x 32 at a time turned round in the wave's part of LDS
+    stage_barrier();
+    constexpr uint32_t kRow = 36;
+    local<float>* turn = (local<float>*)(local<char>*)lds + threadIdx.x / 64 * (32 * kRow);
+    static_assert(S::kWaves * 32 * kRow * 4 <= S::kLds, "a part for each wave");
+    const uint32_t l = threadIdx.x % 64, w = threadIdx.x / 64, i = l % 16;
+    const uint32_t mw = m0 + w / S::kWavesN * S::WM, nw = n0 + w % S::kWavesN * S::WN;
+    const auto in_step = [] {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    };
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = turn[(l / 16 * 4 + e) * kRow + l % 16];
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        // the block's rows are at m - l % 16, its columns at n - 4 (l / 16)
-        const uint32_t row = n - l / 16 * 4 + l % 16, col = m - l % 16 + l / 16 * 4;
-        if (row < p.N && col < padded) put4<Out>(out + row * p.out_ld, col, w, p.out_low);
-      });
+    for (int r = 0; r < S::MI; r += 2) {
+#pragma unroll
+      for (int j = 0; j < S::NI; j += 2) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t mr = i / 4 * 8 + h * 4 + i % 4, nr = l / 16 * 8;
+          const uint32_t m = mw + r * 16 + mr, n = nw + j * 16 + nr;
+          const f8 v = value(m, n, acc.pair(r + h, j));
+          if (m < p.M && n < padded) put8<Out>(out + m * p.out_ld, n, v, p.out_low);
+          *(local<f4>*)(turn + mr * kRow + nr) = __builtin_shufflevector(v, v, 0, 1, 2, 3);
+          *(local<f4>*)(turn + mr * kRow + nr + 4) = __builtin_shufflevector(v, v, 4, 5, 6, 7);
+        }
+        in_step();
+        const uint32_t row = nw + j * 16 + l / 2, col = mw + r * 16 + l % 2 * 16;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          f8 v;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = turn[(l % 2 * 16 + h * 8 + e) * kRow + l / 2];
+          if (row < p.N && col + h * 8 < padded) put8<Out>(out + row * p.out_ld, col + h * 8, v, p.out_low);
+        }
+        in_step();
+      }
     }
   }
 }
