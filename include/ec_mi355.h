@@ -523,7 +523,7 @@ uint64_t ec_orthogonalize_workspace(uint64_t batch, uint64_t rows, uint64_t cols
  * more, products are of 11 bits, added to a X with 22: about 1e-3 of the result. The iterates' magnitudes have to
  * stay below 15 (values past it become infinite): with coefficients that keep [0, 1.2] in itself they are below 1.5.
  * A matrix with a value that is not finite gives NaN; one of zeros gives keep * base. A matrix whose |x| is
- * far below eps keeps fewer bits. EC_ERANGE for rows, cols or batch > 65536, steps past
+ * far below eps keeps fewer bits. EC_ERANGE for rows or cols > 65536, batch > 65535, steps past
  * EC_MAX_STEPS or below 1, or a launch of 2^32 lanes. */
 int ec_orthogonalize(const void* d_x, int type, uint64_t batch, uint64_t rows, uint64_t cols,
                      uint64_t x_stride, uint64_t x_matrix, int steps, const float* coefficients,

@@ -229,7 +229,7 @@ struct Loader {
   uint32_t to;         // and where it goes in LDS
   bool in;             // whether the lane's chunk of its rows is before their end
 
-  // The next step's tile, to LDS at `lds`: begin(), then every bring(i).  At most two steps past the last.
+  // The next step's tile, to LDS at `lds`: begin(), then every bring(i).  At most kStages steps past the last.
   __device__ __forceinline__ void begin(uint32_t lds) {
     uint32_t bytes;   // 0 past the last step
     if constexpr (!ACROSS) {
@@ -260,18 +260,20 @@ struct Loader {
   }
 };
 
-// A tile's geometry: BM x BN by waves of WM x WN.
-template <int BM_, int BN_, int WM_, int WN_>
+// A tile's geometry: BM x BN by waves of WM x WN, STAGES steps of it in LDS.  The smaller a tile, the sooner a step is
+// multiplied, so small ones are brought from further ahead.
+template <int BM_, int BN_, int WM_, int WN_, int STAGES_>
 struct Shape {
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, kStages = STAGES_;
   static constexpr int kWavesN = BN / WN, kWaves = (BM / WM) * kWavesN, kLanes = kWaves * 64;
   static constexpr int MI = WM / 16, NI = WN / 16;
-  static constexpr int kStage = (BM + BN) * kRowBytes, kLds = 2 * kStage;
+  static constexpr int kStage = (BM + BN) * kRowBytes, kLds = kStages * kStage;
 };
 
-typedef Shape<256, 256, 128, 64> Large;    // 8 waves, a workgroup per CU
-typedef Shape<128, 128, 64, 64> Middle;    // 4 waves, two workgroups per CU
-typedef Shape<64, 64, 32, 32> Small;       // 4 waves, five workgroups per CU
+typedef Shape<256, 256, 128, 64, 2> Large;    // 8 waves, a workgroup per CU
+typedef Shape<128, 128, 64, 64, 2> Middle;    // 4 waves, two workgroups per CU
+typedef Shape<64, 128, 32, 64, 3> Flat;       // 4 waves, two workgroups per CU
+typedef Shape<64, 64, 32, 32, 3> Small;       // 4 waves, three workgroups per CU
 
 template <class S>
 struct Acc {
@@ -301,10 +303,11 @@ struct Acc {
   }
 };
 
-// Every load of this wave to LDS has landed and its reads of LDS are done, and the same holds
-// for the other waves.
+// All of this wave's loads to LDS but the last LATER ones have landed and its reads of LDS are done, and the same
+// holds for the other waves.
+template <int LATER = 0>
 __device__ __forceinline__ void stage_barrier() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LATER) : "memory");
 }
 
 // The compiler would put the reads of a group right before their use, to save registers.
@@ -371,25 +374,26 @@ __device__ __forceinline__ void product(Acc<S>& acc, local<char>* lds, const Ope
   const uint32_t at = lds_address(lds);
   G g;
   g.blockA = wave / S::kWavesN * S::MI, g.blockB = wave % S::kWavesN * S::NI;
-  const auto one_step = [&](uint32_t s, int parity) {
-    const local<char>* tile = lds + (s & 1) * S::kStage;
-    const local<char>* next = lds + ((s + 1) & 1) * S::kStage;
+  // loads of the stages behind the one that is waited for
+  constexpr int kLater = (S::kStages - 2) * (LoadA::kLoads + LoadB::kLoads);
+  uint32_t here = 0;   // the step's place in LDS
+  const auto one_step = [&](int parity) {
+    const uint32_t ahead = here + S::kStage < (uint32_t)S::kLds ? here + S::kStage : 0;
     // which of b's halves a sub-step's fragments are in
     const auto turn = [&](int group) { return Kind<T>::kSubs == 1 ? parity : group / G::kParts; };
 #pragma unroll
     for (int i = 0; i < G::kGroups; ++i) {
       if (i + 1 < G::kGroups) {
-        g.read(tile, i + 1, turn(i + 1));
+        g.read(lds + here, i + 1, turn(i + 1));
         keep_order();
         g.multiply(acc, i, turn(i), [](int) {});
         keep_order();
       } else {
-        stage_barrier();
-        g.read(next, 0, Kind<T>::kSubs == 1 ? parity ^ 1 : 0);
+        stage_barrier<kLater>();
+        g.read(lds + ahead, 0, Kind<T>::kSubs == 1 ? parity ^ 1 : 0);
         keep_order();
-        const uint32_t to = at + (s & 1) * S::kStage;
-        la.begin(to);
-        lb.begin(to + S::BM * kRowBytes);
+        la.begin(at + here);
+        lb.begin(at + here + S::BM * kRowBytes);
         constexpr int kAll = LoadA::kLoads + LoadB::kLoads, kEach = (kAll + G::kRows - 1) / G::kRows;
         g.multiply(acc, i, turn(i), [&](int row) {
 #pragma unroll
@@ -403,18 +407,20 @@ __device__ __forceinline__ void product(Acc<S>& acc, local<char>* lds, const Ope
         });
       }
     }
+    here = ahead;
   };
   stage_barrier();   // what was in LDS before is read
-  la.issue(at);
-  lb.issue(at + S::BM * kRowBytes);
-  stage_barrier();
-  la.issue(at + S::kStage);
-  lb.issue(at + S::kStage + S::BM * kRowBytes);
+#pragma unroll
+  for (int s = 0; s < S::kStages; ++s) {
+    la.issue(at + s * S::kStage);
+    lb.issue(at + s * S::kStage + S::BM * kRowBytes);
+  }
+  stage_barrier<(S::kStages - 1) * (LoadA::kLoads + LoadB::kLoads)>();
   g.read(lds, 0, 0);
   for (uint32_t s = 0; s < steps; ++s) {
-    one_step(s, 0);
+    one_step(0);
     if constexpr (Kind<T>::kSubs == 1) {
-      if (++s < steps) one_step(s, 1);
+      if (++s < steps) one_step(1);
     }
   }
   loads_done();   // none to LDS is under way when the workgroup gives it back
@@ -439,21 +445,33 @@ __device__ __forceinline__ void tile_at(uint32_t t, uint32_t tiles_m, uint32_t t
 }
 
 // The shape for m x n results: the one whose workgroups, dealt to the CUs in turns, take least time.
-// A tile of four times the area takes a CU four times as long, less the better use of what it loads.
 constexpr uint64_t kCus = 256;
 
-inline uint64_t tiles_of(uint64_t m, uint64_t n, uint64_t side) {
-  return (m + side - 1) / side * ((n + side - 1) / side);
+inline uint64_t tiles_of(uint64_t m, uint64_t n, uint64_t bm, uint64_t bn) {
+  return (m + bm - 1) / bm * ((n + bn - 1) / bn);
 }
 
-// f(S()) with the shape for `tiles(side)` tiles of side x side; the small one only where SMALL.
-template <bool SMALL, typename F, typename G>
+// What a turn of one tile to each CU costs, by its shape.  16-bit products of smaller tiles are bound by what comes from
+// L2, 64 bytes a clock and CU; others by the matrix cores.
+template <class S, typename T>
+constexpr uint64_t cost_of() {
+  constexpr bool narrow = Kind<T>::kBytes == 2;
+  if (__is_same(S, Large)) return 400;
+  if (__is_same(S, Middle)) return narrow ? 165 : 120;
+  if (__is_same(S, Flat)) return narrow ? 110 : 70;
+  return narrow ? 70 : 42;
+}
+
+template <class S, typename T, typename F>
+uint64_t turns(F tiles) {
+  return (tiles(S()) + kCus - 1) / kCus * cost_of<S, T>();
+}
+
+// f(S()) with the best of Large, Middle and Least for `tiles(S())` tiles.
+template <typename T, class Least, typename F, typename G>
 void with_shape(F tiles, G f) {
-  const auto cost = [&](uint64_t side, uint64_t area) { return (tiles(side) + kCus - 1) / kCus * area; };
-  const uint64_t large = cost(256, 400), middle = cost(128, 120), small = cost(64, 45);
-  if constexpr (SMALL) {
-    if (small < large && small < middle) return f(Small());
-  }
+  const uint64_t large = turns<Large, T>(tiles), middle = turns<Middle, T>(tiles), least = turns<Least, T>(tiles);
+  if (least < large && least < middle) return f(Least());
   if (middle < large) return f(Middle());
   return f(Large());
 }

@@ -50,6 +50,12 @@ __device__ __forceinline__ float team_sum(float v, int& turn) {
   return v;
 }
 
+// A lane's groups of a row as they lie in memory: half the registers of 16-bit values, for rows that are under way.
+template <typename T, int V>
+struct Raw {
+  typename Group<T>::vec x[V];
+};
+
 // V groups of a row, one after another R lanes apart: group v of lane l is at (v R + l) kN.
 template <typename T, int R, int V>
 struct Row {
@@ -61,21 +67,30 @@ struct Row {
   }
 
   template <bool STREAM>
-  __device__ __forceinline__ void load(const T* p, uint32_t width) {
+  __device__ __forceinline__ static Raw<T, V> fetch(const T* p, uint32_t width) {
+    Raw<T, V> raw;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const uint32_t i = at(v);
-      typename Group<T>::vec raw = {};
+      raw.x[v] = {};
       if (i + kN <= width) {
-        raw = load_group<T, STREAM>(p + i);
+        raw.x[v] = load_group<T, STREAM>(p + i);
       } else {
 #pragma unroll
         for (int e = 0; e < kN; ++e)
-          if (i + e < width) raw[e] = gp(p)[i + e];
+          if (i + e < width) raw.x[v][e] = gp(p)[i + e];
       }
-#pragma unroll
-      for (int e = 0; e < kN; ++e) x[v][e] = (float)raw[e];
     }
+    return raw;
+  }
+
+  __device__ __forceinline__ void take(const Raw<T, V>& raw) {
+    each([&](int v, int e) { x[v][e] = (float)raw.x[v][e]; });
+  }
+
+  template <bool STREAM>
+  __device__ __forceinline__ void load(const T* p, uint32_t width) {
+    take(fetch<STREAM>(p, width));
   }
 
   template <typename O, bool STREAM>
@@ -202,17 +217,26 @@ __global__ void __launch_bounds__(block_lanes<R>()) norm_grad_kernel(GradArgs p)
   }
   const float mean = 1.0f / (float)p.width;
   int turn = 0;
+  // the next row's values are under way while a row is summed
+  Raw<T, V> d_raw = {}, y_raw = {}, z_raw = {}, x_raw = {};
+  const auto fetch = [&](uint64_t row) {
+    if (p.dsum) d_raw = row_t::template fetch<true>((const T*)p.dsum + row * p.dsum_stride, p.width);
+    if (p.branch) y_raw = row_t::template fetch<true>((const T*)p.branch + row * p.branch_stride, p.width);
+    if (p.weight) {
+      z_raw = row_t::template fetch<true>((const T*)p.dnormed + row * p.dnormed_stride, p.width);
+      x_raw = row_t::template fetch<true>((const T*)p.sum + row * p.sum_stride, p.width);
+    }
+  };
+  constexpr bool kAhead = R < 1024;
+  if (kAhead && first < last) fetch(first);
   for (uint64_t row = first; row < last; ++row) {
+    if (!kAhead) fetch(row);
     if (p.gate && kKeep && (row == first || row % p.gate_share == 0))
       factors(gate, (const T*)p.gate + row / p.gate_share * p.width);
-    row_t d, y;
-    d.fill(0.0f);
-    if (p.dsum) d.template load<true>((const T*)p.dsum + row * p.dsum_stride, p.width);
-    if (p.branch) y.template load<true>((const T*)p.branch + row * p.branch_stride, p.width);
+    row_t d, y, dz, x;
+    d.take(d_raw), y.take(y_raw), dz.take(z_raw), x.take(x_raw);
+    if (kAhead && row + 1 < last) fetch(row + 1);
     if (p.weight) {
-      row_t dz, x;
-      dz.template load<true>((const T*)p.dnormed + row * p.dnormed_stride, p.width);
-      x.template load<true>((const T*)p.sum + row * p.sum_stride, p.width);
       const float root = gp(p.rstd)[row];
       float s = 0.0f;
       if (!kKeep) factors(w, p.weight);
@@ -312,7 +336,9 @@ void with_team(uint32_t width, F f) {
     f(std::integral_constant<int, 1024>(), std::integral_constant<int, 4>());
 }
 
-constexpr uint64_t kMostTeams = 1024;
+// Teams for n rows: each row its own up to 256 (one for each CU), then four rows a team and more, as the partials are
+// as large as the rows (1023 rows of 1999 fp32: 26 us with one row a team), and 1024 at most.
+constexpr uint64_t kMostTeams = 1024, kLeastTeams = 256, kTeamRows = 4;
 
 struct Split {
   uint64_t teams, per_gate, rows, gates;
@@ -322,14 +348,15 @@ struct Split {
 // Teams for n rows, of which gate_share each share a row of the gate.
 Split split_rows(uint64_t n, uint64_t gate_share) {
   Split s = {};
+  const uint64_t most = std::min(kMostTeams, std::max(kLeastTeams, n / kTeamRows));
   s.gates = n / gate_share;
-  s.direct = s.gates > kMostTeams / 2;
+  s.direct = s.gates > most / 2;
   if (s.direct) {   // a run of whole gate rows each
-    const uint64_t gates = (s.gates + kMostTeams - 1) / kMostTeams;
+    const uint64_t gates = (s.gates + most - 1) / most;
     s.rows = gates * gate_share;
     s.teams = (s.gates + gates - 1) / gates;
   } else {
-    s.per_gate = std::max<uint64_t>(1, std::min(gate_share, kMostTeams / s.gates));
+    s.per_gate = std::max<uint64_t>(1, std::min(gate_share, most / s.gates));
     s.rows = (gate_share + s.per_gate - 1) / s.per_gate;
     s.per_gate = (gate_share + s.rows - 1) / s.rows;
     s.teams = s.gates * s.per_gate;

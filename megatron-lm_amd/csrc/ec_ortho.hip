@@ -33,16 +33,27 @@ namespace ec {
 namespace {
 
 constexpr int kLanes = 256;
-constexpr uint32_t kMostParts = 64;       // of a matrix's sum of squares
+constexpr uint32_t kMostParts = 1024;     // of a matrix's sum of squares
 constexpr uint32_t kPiece = 8192;         // elements of a contiguous matrix that are summed at a time
 constexpr int kStored = 12;               // matrices are stored times 2^12
 constexpr uint32_t kMostSide = 1u << 16;
-constexpr uint32_t kMostBatch = 1u << 16;
+constexpr uint32_t kMostBatch = 65535;
 
 struct Matrices {
   const char* p;
   uint64_t stride, matrix;   // elements from row to row, from matrix to matrix
 };
+
+__device__ __forceinline__ double block_sum(double v) {
+  __shared__ double shared[kLanes / 64];
+#pragma unroll
+  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+  if (threadIdx.x % 64 == 0) shared[threadIdx.x / 64] = v;
+  __syncthreads();
+  v = shared[0];
+  for (int w = 1; w < kLanes / 64; ++w) v += shared[w];
+  return v;
+}
 
 template <typename T>
 __global__ void __launch_bounds__(kLanes) square_kernel(const T* x, uint64_t stride, uint64_t matrix,
@@ -66,15 +77,8 @@ __global__ void __launch_bounds__(kLanes) square_kernel(const T* x, uint64_t str
       sum = __builtin_fma(v, v, sum);
     }
   }
-  __shared__ double shared[kLanes / 64];
-#pragma unroll
-  for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-  if (threadIdx.x % 64 == 0) shared[threadIdx.x / 64] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < kLanes / 64; ++w) sum += shared[w];
-    gp(parts)[blockIdx.y * kMostParts + blockIdx.x] = sum;
-  }
+  sum = block_sum(sum);
+  if (threadIdx.x == 0) gp(parts)[blockIdx.y * kMostParts + blockIdx.x] = sum;
 }
 
 // Two fp16 values whose sum is v to 22 bits.
@@ -121,7 +125,8 @@ __global__ void __launch_bounds__(kLanes) scale_kernel(const T* x, uint64_t stri
                                                        uint32_t rows, uint32_t cols, const double* parts,
                                                        uint32_t n_parts, double eps, char* out, uint64_t low_at) {
   double sum = 0.0;
-  for (uint32_t i = 0; i < n_parts; ++i) sum += gp(parts)[blockIdx.y * kMostParts + i];
+  for (uint32_t i = threadIdx.x; i < n_parts; i += kLanes) sum += gp(parts)[blockIdx.y * kMostParts + i];
+  sum = block_sum(sum);
   const double by = (double)(1 << kStored) / (__builtin_sqrt(sum) + eps);
   const T* from = x + blockIdx.y * matrix;
   const uint32_t groups = (cols + 7) / 8, all = rows * groups;
@@ -252,15 +257,15 @@ template <typename In, bool ACROSS_A, bool ACROSS_B, int WHAT, typename Out>
 int run_ns(NsArgs& p, uint32_t batch, hipStream_t st) {
   constexpr bool kSymmetric = WHAT == kGram || WHAT == kPoly;
   int status = EC_OK;
-  const auto tiles = [&](uint64_t side) {
-    const uint64_t n = (p.N + side - 1) / side;
-    return kSymmetric ? n * (n + 1) / 2 * batch : tiles_of(p.M, p.N, side) * batch;
+  const auto tiles = [&](auto s) -> uint64_t {
+    const uint64_t n = (p.N + s.BN - 1) / s.BN;
+    return kSymmetric ? n * (n + 1) / 2 * batch : tiles_of(p.M, p.N, s.BM, s.BN) * batch;
   };
-  with_shape<true>(tiles, [&](auto s) {
+  with_shape<In, Small>(tiles, [&](auto s) {
     typedef decltype(s) S;
     p.tiles_m = (p.M + S::BM - 1) / S::BM;
     p.tiles_n = (p.N + S::BN - 1) / S::BN;
-    p.tiles = (uint32_t)(tiles(S::BM) / batch);
+    p.tiles = (uint32_t)(tiles(s) / batch);
     if ((uint64_t)p.tiles * batch >= (1ull << 32) / S::kLanes)
       status = EC_ERANGE;
     else
@@ -425,7 +430,8 @@ int ec_orthogonalize(const void* d_x, int type, uint64_t batch, uint64_t rows, u
   const bool dense = x_stride == cols;
   const uint64_t total = rows * cols;
   const uint64_t pieces = dense ? (total + kPiece - 1) / kPiece : rows;
-  const uint32_t parts = (uint32_t)std::min<uint64_t>(kMostParts, pieces);
+  // enough workgroups in all to keep the memory busy
+  const uint32_t parts = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(1, 2 * kMostParts / batch), std::min<uint64_t>(kMostParts, pieces));
   double* sums = (double*)(work + p.parts);
   const uint64_t blocks = (rows * ((cols + 7) / 8) + kLanes - 1) / kLanes;
   const uint32_t grid = (uint32_t)std::min<uint64_t>(blocks, std::max<uint64_t>(1, 8192 / batch));
