@@ -77,15 +77,31 @@ __global__ void __launch_bounds__(S::kLanes) ff_kernel(FfArgs p) {
   __shared__ __attribute__((aligned(1024))) char lds[S::kLds];
   uint32_t tm, tn;
   tile_at(xcd_order(blockIdx.x, gridDim.x), p.tiles_m, p.tiles_n, tm, tn);
-  Acc<S> acc;
-  acc.clear();
-  product<S, T, false, false, true>(acc, (local<char>*)lds, p.x, p.w_gate, p.w_up, tm * S::BM,
-                                    tn * S::BN, p.width);
   // of each 64 columns of the tile the first 32 are gates, the others the ups
   static_assert(S::WN == 64, "a wave holds both projections of its 32 outputs");
   const uint32_t l = threadIdx.x % 64, w = threadIdx.x / 64;
   const uint32_t m0 = tm * S::BM + w / S::kWavesN * S::WM + l % 16 / 4 * 8 + l % 4;
   const uint32_t f = tn * (S::BN / 2) + w % S::kWavesN * 32 + l / 16 * 8;
+  // dh is under way during the product; past its ends some other value, which is not used
+  typedef T __attribute__((ext_vector_type(8), aligned(sizeof(T)))) any8;
+  T __attribute__((ext_vector_type(8))) dhs[GRAD ? S::MI : 1];
+  if constexpr (GRAD) {
+    const bool whole = (tn + 1) * (S::BN / 2) <= p.inner;
+#pragma unroll
+    for (int i = 0; i < S::MI; ++i) {
+      const T* row = (const T*)p.dh + min(m0 + i / 2 * 32 + i % 2 * 4, p.n - 1) * p.dh_stride;
+      if (whole) {
+        dhs[i] = *(const global<any8>*)(uintptr_t)(row + f);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dhs[i][e] = gp(row)[min(f + e, p.inner - 1)];
+      }
+    }
+  }
+  Acc<S> acc;
+  acc.clear();
+  product<S, T, false, false, true>(acc, (local<char>*)lds, p.x, p.w_gate, p.w_up, tm * S::BM,
+                                    tn * S::BN, p.width);
   with_activation(p.act, [&](auto which) {
     constexpr int ACT = decltype(which)::value;
 #pragma unroll
@@ -99,7 +115,7 @@ __global__ void __launch_bounds__(S::kLanes) ff_kernel(FfArgs p) {
         for (int e = 0; e < 8; ++e) h[e] = activate<ACT>(g[e]).value * u[e];
         store8<T>((T*)p.h + m * p.h_stride, f, p.inner, h);
       } else {
-        const f8 dh = load8<T>((const T*)p.dh + m * p.dh_stride, f, p.inner);
+        const f8 dh = __builtin_convertvector(dhs[i], f8);
         f8 dg, du;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -227,10 +243,9 @@ struct SumArgs {
   char* out[2];   // blockIdx.y's
   uint64_t out_stride[2];
   uint64_t a_step;   // bytes from blockIdx.y = 0's first operand to 1's
-  int accumulate;
 };
 
-template <class S, typename T, typename O, bool ACROSS_A>
+template <class S, typename T, typename O, bool ACROSS_A, bool ACCUMULATE>
 __global__ void __launch_bounds__(S::kLanes) sum_kernel(SumArgs p) {
   __shared__ __attribute__((aligned(1024))) char lds[S::kLds];
   uint32_t tm, tn;
@@ -245,14 +260,17 @@ __global__ void __launch_bounds__(S::kLanes) sum_kernel(SumArgs p) {
   }
   O* out = (O*)p.out[blockIdx.y];
   const uint64_t stride = p.out_stride[blockIdx.y];
-  acc.each([&](uint32_t m, uint32_t n, f8 v) {
-    m += tm * S::BM;
-    n += tn * S::BN;
-    if (m >= p.M || n >= p.N) return;
-    O* row = out + m * stride;
-    if (p.accumulate) v += load8<O>(row, n, p.N);
-    store8<O>(row, n, p.N, v);
-  });
+  const uint32_t m0 = tm * S::BM, n0 = tn * S::BN;
+  const auto put = [&](uint32_t m, uint32_t n, const f8& v) {
+    m += m0;
+    n += n0;
+    if (m < p.M && n < p.N) store8<O>(out + m * stride, n, p.N, v);
+  };
+  if constexpr (ACCUMULATE)
+    acc.each_with([&](uint32_t m, uint32_t n) { return load8(out + min(m0 + m, p.M - 1) * stride, n0 + n, p.N); },
+                  [&](uint32_t m, uint32_t n, const f8& v, const f8& x) { put(m, n, v + x); });
+  else
+    acc.each(put);
 }
 
 // Rows up to which few_kernel takes the forward pass. 2048 -> 8192 bf16, eight sets of weights in turns, us: 1 row 14.9,
@@ -325,13 +343,13 @@ void run_ff(FfArgs& p, hipStream_t st) {
   });
 }
 
-template <typename T, typename O, bool ACROSS_A>
+template <typename T, typename O, bool ACROSS_A, bool ACCUMULATE>
 void run_sum(SumArgs& p, uint32_t outs, hipStream_t st) {
   with_shape<T, Small>([&](auto s) { return outs * tiles_of(p.M, p.N, s.BM, s.BN); }, [&](auto s) {
     typedef decltype(s) S;
     p.tiles_m = (p.M + S::BM - 1) / S::BM;
     p.tiles_n = (p.N + S::BN - 1) / S::BN;
-    sum_kernel<S, T, O, ACROSS_A><<<dim3(p.tiles_m * p.tiles_n, outs), S::kLanes, 0, st>>>(p);
+    sum_kernel<S, T, O, ACROSS_A, ACCUMULATE><<<dim3(p.tiles_m * p.tiles_n, outs), S::kLanes, 0, st>>>(p);
   });
 }
 
@@ -436,7 +454,7 @@ int ec_gated_ff_grad(const void* d_dh, uint64_t dh_stride, const void* d_x, uint
       }
       s.K = inner, s.M = p.n, s.N = width;
       s.out[0] = (char*)d_dx, s.out_stride[0] = dx_stride;
-      run_sum<T, T, false>(s, 1, st);
+      run_sum<T, T, false, false>(s, 1, st);
     }
     if (d_dgate) {
       SumArgs s = {};
@@ -450,11 +468,11 @@ int ec_gated_ff_grad(const void* d_dh, uint64_t dh_stride, const void* d_x, uint
       s.K = p.n, s.M = inner, s.N = width;
       s.out[0] = (char*)d_dgate, s.out_stride[0] = dgate_stride;
       s.out[1] = (char*)d_dup, s.out_stride[1] = dup_stride;
-      s.accumulate = accumulate;
-      if (grad_type == EC_F32)
-        run_sum<T, float, true>(s, 2, st);
-      else
-        run_sum<T, T, true>(s, 2, st);
+      const auto run = [&](auto o) {
+        typedef decltype(o) O;
+        accumulate ? run_sum<T, O, true, true>(s, 2, st) : run_sum<T, O, true, false>(s, 2, st);
+      };
+      grad_type == EC_F32 ? run(float()) : run(T());
     }
     return launched();
   });

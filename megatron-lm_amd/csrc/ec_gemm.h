@@ -298,6 +298,50 @@ struct Acc {
       for (int j = 0; j < S::NI; j += 2) f(m0 + r / 2 * 32 + r % 2 * 4, n0 + j * 16, pair(r, j));
   }
 
+  // The values become f(m, n).
+  template <typename F>
+  __device__ __forceinline__ void start(F f) {
+    const uint32_t l = threadIdx.x % 64, w = threadIdx.x / 64, i = l % 16;
+    const uint32_t m0 = w / S::kWavesN * S::WM + i / 4 * 8 + i % 4;
+    const uint32_t n0 = w % S::kWavesN * S::WN + l / 16 * 8;
+#pragma unroll
+    for (int r = 0; r < S::MI; ++r) {
+#pragma unroll
+      for (int j = 0; j < S::NI; j += 2) {
+        const f8 x = f(m0 + r / 2 * 32 + r % 2 * 4, n0 + j * 16);
+        v[r][j] = __builtin_shufflevector(x, x, 0, 1, 2, 3);
+        v[r][j + 1] = __builtin_shufflevector(x, x, 4, 5, 6, 7);
+      }
+      if (r % 4 == 3) __builtin_amdgcn_sched_barrier(0);   // all at once would take too many registers
+    }
+  }
+
+  // g(m, n, values, f(m, n)), where f loads and g stores: the loads are two rows ahead, as the compiler would not
+  // let them overtake a store.
+  template <typename F, typename G>
+  __device__ __forceinline__ void each_with(F f, G g) const {
+    const uint32_t l = threadIdx.x % 64, w = threadIdx.x / 64, i = l % 16;
+    const uint32_t m0 = w / S::kWavesN * S::WM + i / 4 * 8 + i % 4;
+    const uint32_t n0 = w % S::kWavesN * S::WN + l / 16 * 8;
+    constexpr int kAhead = 2;
+    const auto m = [&](int r) { return m0 + r / 2 * 32 + r % 2 * 4; };
+    f8 x[kAhead][S::NI / 2];
+#pragma unroll
+    for (int r = -kAhead; r < S::MI; ++r) {
+      f8 now[S::NI / 2];
+#pragma unroll
+      for (int j = 0; j < S::NI; j += 2) {
+        const int at = (r + kAhead) % kAhead;
+        now[j / 2] = x[at][j / 2];
+        if (r + kAhead < S::MI) x[at][j / 2] = f(m(r + kAhead), n0 + j * 16);
+      }
+#pragma unroll
+      for (int j = 0; j < S::NI; j += 2)
+        if (r >= 0) g(m(r), n0 + j * 16, pair(r, j), now[j / 2]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+
   __device__ __forceinline__ f8 pair(int r, int j) const {
     return __builtin_shufflevector(v[r][j], v[r][j + 1], 0, 1, 2, 3, 4, 5, 6, 7);
   }
@@ -476,6 +520,12 @@ void with_shape(F tiles, G f) {
   return f(Large());
 }
 
+template <typename T>
+__device__ __forceinline__ f8 load8(const T* p) {
+  typedef T __attribute__((ext_vector_type(8), aligned(sizeof(T)))) any8;
+  return __builtin_convertvector(*(const global<any8>*)(uintptr_t)p, f8);
+}
+
 // Eight neighbours of a row, at column n of `cols`.
 template <typename T>
 __device__ __forceinline__ void store8(T* row, uint32_t n, uint32_t cols, const f8& v) {
@@ -492,10 +542,9 @@ __device__ __forceinline__ void store8(T* row, uint32_t n, uint32_t cols, const 
 
 template <typename T>
 __device__ __forceinline__ f8 load8(const T* row, uint32_t n, uint32_t cols) {
-  typedef T __attribute__((ext_vector_type(8), aligned(sizeof(T)))) any8;
   f8 v = {};
   if (n + 8 <= cols) {
-    v = __builtin_convertvector(*(const global<any8>*)(uintptr_t)(row + n), f8);
+    v = load8(row + n);
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)

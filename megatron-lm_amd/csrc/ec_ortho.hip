@@ -10,11 +10,11 @@
 // steps.  There are two kinds of steps:
 // - exact ones: all matrices are pairs of fp16 values (22 bits, ec_gemm.h).  The result is as good as that of
 //   fp32 products (4.5e-7 off after five steps), at a third of the fp16 rate instead of a sixteenth.
-// - fast ones: the products are of fp16 values, but X = a X + (b A + c A A) X, and the X that a stands before
-//   has a second fp16 part.  What small singular values consist of is that first term; the
-//   products' errors are small where they are.  Five of them leave 0.8e-3 to 1.1e-3 of the result (without the second
-//   part 1.9e-3 to 2.5e-3), against 1.7e-3 by the rounding to bf16; an update of a single nonzero row, whose
-//   roundings do not average out, has 2e-3 to 4e-3.
+// - fast ones: the products are of fp16 values, but all but the last two steps take X = a X + (b A + c A A) X, and
+//   the X that a stands before has a second fp16 part.  What small singular values consist of is that first
+//   term; the products' errors are small where they are.  Five steps leave 0.7e-3 to 0.8e-3 of the result
+//   (with second parts in the last two steps too 0.8e-3 to 1.1e-3, without any 1.9e-3 to 2.5e-3), against 1.7e-3 by the
+//   rounding to bf16; an update of a single nonzero row, whose roundings do not average out, has 2e-3 to 4e-3.
 // A bf16 result takes fast steps, from kFastSide rows and columns on (smaller matrices are bound by the launches, and
 // their roundings average out less); an fp16 or fp32 one exact steps.
 //
@@ -33,6 +33,7 @@ namespace ec {
 namespace {
 
 constexpr int kLanes = 256;
+constexpr int kAhead = 4;
 constexpr uint32_t kMostParts = 1024;     // of a matrix's sum of squares
 constexpr uint32_t kPiece = 8192;         // elements of a contiguous matrix that are summed at a time
 constexpr int kStored = 12;               // matrices are stored times 2^12
@@ -66,10 +67,18 @@ __global__ void __launch_bounds__(kLanes) square_kernel(const T* x, uint64_t str
     const T* p = base + i * stride;
     const uint32_t n = (uint32_t)min((uint64_t)width, total - i * width);
     const uint32_t groups = n / G::kN;
-    for (uint32_t g = threadIdx.x; g < groups; g += kLanes) {
-      const typename G::wide v = widen<T>(load_group<T, false>(p + g * G::kN));
+    for (uint32_t g = threadIdx.x; g < groups; g += kLanes * kAhead) {
+      typename G::vec v[kAhead];
 #pragma unroll
-      for (int e = 0; e < G::kN; ++e) sum = __builtin_fma((double)v[e], (double)v[e], sum);
+      for (int u = 0; u < kAhead; ++u)   // without conditions, so that all are in flight together
+        v[u] = load_group<T, false>(p + (uint64_t)min(g + u * kLanes, groups - 1) * G::kN);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (g + u * kLanes < groups) {
+          const typename G::wide w = widen<T>(v[u]);
+#pragma unroll
+          for (int e = 0; e < G::kN; ++e) sum = __builtin_fma((double)w[e], (double)w[e], sum);
+        }
     }
     const uint32_t rest = groups * G::kN + threadIdx.x;
     if (rest < n) {
@@ -151,9 +160,9 @@ struct NsArgs {
   uint64_t out_ld, out_matrix;   // bytes
   float by;                      // the result: by * product
   uint64_t out_low;              // from a value to its second part, in bytes
-  const char* add;               // + linear * add + diagonal * I, add a matrix like the product
+  const char* add;               // a matrix like the result: by * (linear * add + product), or none
   uint64_t add_ld, add_matrix, add_low;
-  float linear, diagonal;
+  float linear, diagonal;        // POLY: + diagonal * I
   Matrices base;                 // LAST: + keep * base, or none
   float keep;
 };
@@ -177,17 +186,22 @@ __global__ void __launch_bounds__(S::kLanes) ns_kernel(NsArgs p) {
   Operand a = p.a, b = p.b;
   a.p += matrix * p.a_matrix;
   b.p += matrix * p.b_matrix;
+  const uint32_t m0 = tm * S::BM, n0 = tn * S::BN, padded = (p.N + 7) & ~7u;
+  // at places past the ends some other value, which is not stored
+  const auto added = [&](uint32_t m, uint32_t n) {
+    return p.linear * get8<In>(p.add + matrix * p.add_matrix + min(m0 + m, p.M - 1) * p.add_ld,
+                               min(n0 + n, padded - 8), p.add_low);
+  };
+  constexpr bool kStarts = WHAT == kPoly || (WHAT != kGram && Kind<In>::kParts == 1);
   Acc<S> acc;
-  acc.clear();
-  product<S, In, ACROSS_A, ACROSS_B, false>(acc, (local<char>*)lds, a, b, b, tm * S::BM, tn * S::BN, p.K);
+  if (kStarts && p.add)
+    acc.start(added);
+  else
+    acc.clear();
+  product<S, In, ACROSS_A, ACROSS_B, false>(acc, (local<char>*)lds, a, b, b, m0, n0, p.K);
   char* out = p.out + matrix * p.out_matrix;
-  const uint32_t padded = (p.N + 7) & ~7u;
   const auto value = [&](uint32_t m, uint32_t n, f8 v) {
     v *= p.by;
-    if (WHAT != kGram && p.add) {
-      if (m < p.M && n < padded)
-        v += p.linear * get8<In>(p.add + matrix * p.add_matrix + m * p.add_ld, n, p.add_low);
-    }
     if constexpr (WHAT == kPoly) {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
@@ -195,23 +209,27 @@ __global__ void __launch_bounds__(S::kLanes) ns_kernel(NsArgs p) {
     }
     return v;
   };
-  const uint32_t m0 = tm * S::BM, n0 = tn * S::BN;
   if constexpr (WHAT == kLast) {
-    const uint64_t first = matrix * p.base.matrix;
-    acc.each([&](uint32_t m, uint32_t n, f8 v) {
+    const auto put = [&](uint32_t m, uint32_t n, const f8& v) {
       m += m0;
       n += n0;
-      if (m >= p.M || n >= p.N) return;
-      v = value(m, n, v);
-      if (p.base.p) v += p.keep * load8<Out>((const Out*)p.base.p + first + m * p.base.stride, n, p.N);
-      store8<Out>((Out*)(out + m * p.out_ld), n, p.N, v);
-    });
+      if (m < p.M && n < p.N) store8<Out>((Out*)(out + m * p.out_ld), n, p.N, v);
+    };
+    if (p.base.p) {
+      const Out* base = (const Out*)p.base.p + matrix * p.base.matrix;
+      acc.each_with(
+          [&](uint32_t m, uint32_t n) {
+            return load8(base + min(m0 + m, p.M - 1) * p.base.stride, n0 + n, p.N);
+          },
+          [&](uint32_t m, uint32_t n, const f8& v, const f8& x) { put(m, n, p.by * v + p.keep * x); });
+    } else {
+      acc.each([&](uint32_t m, uint32_t n, const f8& v) { put(m, n, p.by * v); });
+    }
   } else if (!kSymmetric || tm == tn) {
     acc.each([&](uint32_t m, uint32_t n, f8 v) {
       m += m0;
       n += n0;
-      v = value(m, n, v);
-      if (m < p.M && n < padded) put8<Out>(out + m * p.out_ld, n, v, p.out_low);
+      if (m < p.M && n < padded) put8<Out>(out + m * p.out_ld, n, value(m, n, v), p.out_low);
     });
   } else {
     // and the mirrored tile, 32 x 32 at a time turned round in the wave's part of LDS
@@ -311,6 +329,7 @@ struct Call {
 };
 
 constexpr uint32_t kFastSide = 64;
+constexpr int kPlainSteps = 2;   // the last fast steps, whose X has no second part
 
 bool fast(const Plan& p, int out_type) { return out_type == EC_BF16 && p.side >= kFastSide; }
 
@@ -333,11 +352,13 @@ Stored stored(char* at, uint32_t batch, uint32_t rows, uint32_t cols, bool low) 
 template <bool TALL, typename In>
 int run_step(const Plan& p, const Call& c, char* work, int s, hipStream_t st) {
   constexpr bool kFast = Kind<In>::kParts == 1;
+  // X has a second part, and a step adds a X by itself, up to the last steps
+  const bool adds = kFast && s + kPlainSteps < c.steps, next_adds = kFast && s + 1 + kPlainSteps < c.steps;
   const Stored x = stored<In>(work + p.x[s & 1], p.batch, p.rows, p.cols, true);
   const Stored gram = stored<In>(work + p.gram, p.batch, p.side, p.side, false);
   const Stored poly = stored<In>(work + p.poly, p.batch, p.side, p.side, false);
   // stored times 2^at so that (a I +) b A + c A A stays below fp16's largest value
-  const float most = (kFast ? 0.0f : std::fabs(c.a)) + 2.0f * std::fabs(c.b) + 4.0f * std::fabs(c.c);
+  const float most = (adds ? 0.0f : std::fabs(c.a)) + 2.0f * std::fabs(c.b) + 4.0f * std::fabs(c.c);
   int at = kStored;
   while (at > 0 && std::ldexp(most, at) > 32768.0f) --at;
 
@@ -355,9 +376,11 @@ int run_step(const Plan& p, const Call& c, char* work, int s, hipStream_t st) {
   n.K = p.side;
   n.out = work + p.poly;
   n.add = work + p.gram, n.add_ld = gram.m.ld, n.add_matrix = gram.matrix;
-  n.by = c.c * std::ldexp(1.0f, at - 2 * kStored);
-  n.linear = c.b * std::ldexp(1.0f, at - kStored);
-  n.diagonal = kFast ? 0.0f : c.a * std::ldexp(1.0f, at);
+  // c (b / c A + A A); where there is no A A, so little of it that it is rounded off
+  const float square = c.c != 0.0f ? c.c : 0x1p-60f;
+  n.by = square * std::ldexp(1.0f, at - 2 * kStored);
+  n.linear = c.b / square * std::ldexp(1.0f, kStored);
+  n.diagonal = adds ? 0.0f : c.a * std::ldexp(1.0f, at);
   if (const int e = run_ns<In, false, false, kPoly, In>(n, p.batch, st)) return e;
 
   // B X, X across; or X B, X along
@@ -365,17 +388,17 @@ int run_step(const Plan& p, const Call& c, char* work, int s, hipStream_t st) {
   n.a.rows = p.rows, n.b.rows = p.cols;
   n.a_matrix = TALL ? x.matrix : poly.matrix, n.b_matrix = TALL ? poly.matrix : x.matrix;
   n.M = p.rows, n.N = p.cols;
-  n.add = kFast ? x.m.p : nullptr, n.add_ld = x.m.ld, n.add_matrix = x.matrix, n.add_low = x.low;
+  n.add = adds ? x.m.p : nullptr, n.add_ld = x.m.ld, n.add_matrix = x.matrix, n.add_low = x.low;
+  n.linear = c.a * std::ldexp(1.0f, at);
   if (s + 1 < c.steps) {
-    n.out = work + p.x[(s + 1) & 1], n.out_ld = x.m.ld, n.out_matrix = x.matrix, n.out_low = x.low;
+    n.out = work + p.x[(s + 1) & 1], n.out_ld = x.m.ld, n.out_matrix = x.matrix;
+    n.out_low = next_adds ? x.low : 0;
     n.by = std::ldexp(1.0f, -at);
-    n.linear = c.a;
     return run_ns<In, false, !TALL, kNext, In>(n, p.batch, st);
   }
   const uint32_t w = type_bytes(c.out_type);
   n.out = c.out, n.out_ld = c.out_stride * w, n.out_matrix = c.out_matrix * w;
   n.by = c.scale * std::ldexp(1.0f, -at - kStored);
-  n.linear = c.scale * c.a * std::ldexp(1.0f, -kStored);
   n.base = c.base, n.keep = c.keep;
   if constexpr (kFast)
     return run_ns<In, false, !TALL, kLast, bf16_t>(n, p.batch, st);
@@ -440,7 +463,7 @@ int ec_orthogonalize(const void* d_x, int type, uint64_t batch, uint64_t rows, u
     square_kernel<T><<<dim3(parts, (uint32_t)batch), kLanes, 0, st>>>(
         (const T*)d_x, dense ? kPiece : x_stride, x_matrix, pieces, total, dense ? kPiece : (uint32_t)cols, sums);
     if (fast(p, out_type)) {
-      const Stored x = stored<fp16_t>(work + p.x[0], p.batch, p.rows, p.cols, true);
+      const Stored x = stored<fp16_t>(work + p.x[0], p.batch, p.rows, p.cols, steps > kPlainSteps);
       scale_kernel<T, fp16_t><<<dim3(grid, (uint32_t)batch), kLanes, 0, st>>>(
           (const T*)d_x, x_stride, x_matrix, p.rows, p.cols, sums, parts, (double)eps, work + p.x[0], x.low);
     } else {
