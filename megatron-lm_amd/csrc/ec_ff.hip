@@ -70,13 +70,30 @@ struct FfArgs {
   char* d;               // [n][2 padded] of T, and the second parts behind it
   uint32_t padded;
   uint64_t low;          // elements from a value of d to its second part; 0: none
+  Splits splits;
 };
 
-template <class S, typename T, bool GRAD>
-__global__ void __launch_bounds__(S::kLanes) ff_kernel(FfArgs p) {
+template <class S, typename T>
+__global__ void __launch_bounds__(S::kLanes) ff_part_kernel(FfArgs p) {
   __shared__ __attribute__((aligned(1024))) char lds[S::kLds];
+  const uint32_t tiles = p.tiles_m * p.tiles_n, t = xcd_order(blockIdx.x, gridDim.x), split = uniform(t / tiles);
   uint32_t tm, tn;
-  tile_at(xcd_order(blockIdx.x, gridDim.x), p.tiles_m, p.tiles_n, tm, tn);
+  tile_at(t % tiles, p.tiles_m, p.tiles_n, tm, tn);
+  Acc<S> acc;
+  acc.clear();
+  const uint32_t s0 = split * p.splits.steps;
+  product<S, T, false, false, true>(acc, (local<char>*)lds, from_step<T, false>(p.x, s0),
+                                    from_step<T, false>(p.w_gate, s0), from_step<T, false>(p.w_up, s0),
+                                    tm * S::BM, tn * S::BN, split_length<T>(p.splits, split, p.width));
+  store_part(acc, p.splits.parts, t);
+}
+
+template <class S, typename T, bool GRAD, bool JOIN>
+__global__ void __launch_bounds__(S::kLanes) ff_kernel(FfArgs p) {
+  __shared__ __attribute__((aligned(1024))) char lds[JOIN ? 16 : S::kLds];
+  const uint32_t t = xcd_order(blockIdx.x, gridDim.x);
+  uint32_t tm, tn;
+  tile_at(t, p.tiles_m, p.tiles_n, tm, tn);
   // of each 64 columns of the tile the first 32 are gates, the others the ups
   static_assert(S::WN == 64, "a wave holds both projections of its 32 outputs");
   const uint32_t l = threadIdx.x % 64, w = threadIdx.x / 64;
@@ -100,8 +117,11 @@ __global__ void __launch_bounds__(S::kLanes) ff_kernel(FfArgs p) {
   }
   Acc<S> acc;
   acc.clear();
-  product<S, T, false, false, true>(acc, (local<char>*)lds, p.x, p.w_gate, p.w_up, tm * S::BM,
-                                    tn * S::BN, p.width);
+  if constexpr (JOIN)
+    add_parts(acc, p.splits.parts, t, gridDim.x, p.splits.n);
+  else
+    product<S, T, false, false, true>(acc, (local<char>*)lds, p.x, p.w_gate, p.w_up, tm * S::BM,
+                                      tn * S::BN, p.width);
   with_activation(p.act, [&](auto which) {
     constexpr int ACT = decltype(which)::value;
 #pragma unroll
@@ -243,21 +263,45 @@ struct SumArgs {
   char* out[2];   // blockIdx.y's
   uint64_t out_stride[2];
   uint64_t a_step;   // bytes from blockIdx.y = 0's first operand to 1's
+  Splits splits;     // each takes its steps of every product
 };
 
-template <class S, typename T, typename O, bool ACROSS_A, bool ACCUMULATE>
-__global__ void __launch_bounds__(S::kLanes) sum_kernel(SumArgs p) {
+template <class S, typename T, bool ACROSS_A>
+__device__ __forceinline__ void sum_products(Acc<S>& acc, local<char>* lds, const SumArgs& p, uint32_t tm,
+                                             uint32_t tn, uint32_t split, uint32_t K) {
+  const uint32_t s0 = split * p.splits.steps;
+  for (uint32_t i = 0; i < p.parts; ++i) {
+    Operand a = from_step<T, ACROSS_A>(p.a[i], s0);
+    a.p += blockIdx.y * p.a_step;
+    const Operand b = from_step<T, true>(p.b[i], s0);
+    product<S, T, ACROSS_A, true, false>(acc, lds, a, b, b, tm * S::BM, tn * S::BN, K);
+  }
+}
+
+template <class S, typename T, bool ACROSS_A>
+__global__ void __launch_bounds__(S::kLanes) sum_part_kernel(SumArgs p) {
   __shared__ __attribute__((aligned(1024))) char lds[S::kLds];
+  const uint32_t tiles = p.tiles_m * p.tiles_n, t = xcd_order(blockIdx.x, gridDim.x), split = uniform(t / tiles);
   uint32_t tm, tn;
-  tile_at(xcd_order(blockIdx.x, gridDim.x), p.tiles_m, p.tiles_n, tm, tn);
+  tile_at(t % tiles, p.tiles_m, p.tiles_n, tm, tn);
   Acc<S> acc;
   acc.clear();
-  for (uint32_t i = 0; i < p.parts; ++i) {
-    Operand a = p.a[i];
-    a.p += blockIdx.y * p.a_step;
-    product<S, T, ACROSS_A, true, false>(acc, (local<char>*)lds, a, p.b[i], p.b[i], tm * S::BM,
-                                         tn * S::BN, p.K);
-  }
+  sum_products<S, T, ACROSS_A>(acc, (local<char>*)lds, p, tm, tn, split, split_length<T>(p.splits, split, p.K));
+  store_part(acc, p.splits.parts, (uint64_t)blockIdx.y * gridDim.x + t);
+}
+
+template <class S, typename T, typename O, bool ACROSS_A, bool ACCUMULATE, bool JOIN>
+__global__ void __launch_bounds__(S::kLanes) sum_kernel(SumArgs p) {
+  __shared__ __attribute__((aligned(1024))) char lds[JOIN ? 16 : S::kLds];
+  const uint32_t t = xcd_order(blockIdx.x, gridDim.x);
+  uint32_t tm, tn;
+  tile_at(t, p.tiles_m, p.tiles_n, tm, tn);
+  Acc<S> acc;
+  acc.clear();
+  if constexpr (JOIN)
+    add_parts(acc, p.splits.parts, (uint64_t)blockIdx.y * gridDim.x * p.splits.n + t, gridDim.x, p.splits.n);
+  else
+    sum_products<S, T, ACROSS_A>(acc, (local<char>*)lds, p, tm, tn, 0, p.K);
   O* out = (O*)p.out[blockIdx.y];
   const uint64_t stride = p.out_stride[blockIdx.y];
   const uint32_t m0 = tm * S::BM, n0 = tn * S::BN;
@@ -278,7 +322,7 @@ __global__ void __launch_bounds__(S::kLanes) sum_kernel(SumArgs p) {
 constexpr uint64_t kFewForward = 32;
 
 struct FfWork {
-  uint64_t x, w_gate, w_up, d, total;   // offsets; kNone: read in place
+  uint64_t x, w_gate, w_up, d, parts, total;   // offsets; kNone: read in place
   bool low;
 };
 constexpr uint64_t kNone = ~0ull;
@@ -296,10 +340,28 @@ struct FfCall {
   int type;
 };
 
+template <typename T>
+Choice choose_ff(uint64_t n, uint64_t width, uint64_t inner) {
+  return choose<T, Flat>([&](auto s) { return tiles_of(n, 2 * inner, s.BM, s.BN); }, steps_of<T>(width));
+}
+
+// An m x n sum of `parts` products over K, `outs` times.
+template <typename T>
+Choice choose_sum(uint64_t m, uint64_t n, uint64_t K, uint64_t parts, uint64_t outs) {
+  const uint64_t steps = std::max<uint64_t>(1, steps_of<T>(K));
+  Choice c = choose<T, Small>([&](auto s) { return outs * tiles_of(m, n, s.BM, s.BN); }, steps * parts);
+  c.splits.steps = (uint32_t)((steps + c.splits.n - 1) / c.splits.n);   // of each product
+  c.splits.n = (uint32_t)((steps + c.splits.steps - 1) / c.splits.steps);
+  return c;
+}
+
+// Products of the gradients with the low parts: twice as many.
+uint64_t low_parts(const FfWork& w) { return w.low ? 2 : 1; }
+
 FfWork ff_work(const FfCall& c, bool grad) {
   const uint32_t b = type_bytes(c.type);
   const uint64_t row = up_to((uint64_t)c.width * b, 16);
-  FfWork w = {kNone, kNone, kNone, kNone, 0, false};
+  FfWork w = {kNone, kNone, kNone, kNone, kNone, 0, false};
   const auto take = [&](uint64_t bytes) {
     const uint64_t at = w.total;
     w.total += part(bytes);
@@ -311,8 +373,19 @@ FfWork ff_work(const FfCall& c, bool grad) {
   if (!readable(c.w_up, c.width, c.up_stride, b)) w.w_up = take(c.inner * row);
   if (grad) {
     w.low = c.type != EC_F32 && c.n <= kFewRows;
-    w.d = take(c.n * 2 * up_to(c.inner, 8) * b * (w.low ? 2 : 1));
+    w.d = take(c.n * 2 * up_to(c.inner, 8) * b * low_parts(w));
   }
+  uint64_t bytes = 0;
+  with_type(c.type, [&](auto t) {
+    typedef decltype(t) T;
+    bytes = choose_ff<T>(c.n, c.width, c.inner).bytes;
+    if (grad) {
+      bytes = std::max(bytes, choose_sum<T>(c.n, c.width, c.inner, 2 * low_parts(w), 1).bytes);
+      bytes = std::max(bytes, choose_sum<T>(c.inner, c.width, c.n, low_parts(w), 2).bytes);
+    }
+    return EC_OK;
+  });
+  if (bytes) w.parts = take(bytes);
   return w;
 }
 
@@ -334,22 +407,40 @@ void run_few(const FfArgs& p, hipStream_t st) {
 }
 
 template <typename T, bool GRAD>
-void run_ff(FfArgs& p, hipStream_t st) {
-  with_shape<T, Flat>([&](auto s) { return tiles_of(p.n, 2ull * p.inner, s.BM, s.BN); }, [&](auto s) {
+void run_ff(FfArgs& p, char* parts, hipStream_t st) {
+  const Choice c = choose_ff<T>(p.n, p.width, p.inner);
+  p.splits = c.splits;
+  p.splits.parts = (float*)parts;
+  with_shape<Flat>(c, [&](auto s) {
     typedef decltype(s) S;
     p.tiles_m = (p.n + S::BM - 1) / S::BM;
     p.tiles_n = (p.inner + S::BN / 2 - 1) / (S::BN / 2);
-    ff_kernel<S, T, GRAD><<<p.tiles_m * p.tiles_n, S::kLanes, 0, st>>>(p);
+    const uint32_t tiles = p.tiles_m * p.tiles_n;
+    if (c.splits.n > 1) {
+      ff_part_kernel<S, T><<<tiles * c.splits.n, S::kLanes, 0, st>>>(p);
+      ff_kernel<S, T, GRAD, true><<<tiles, S::kLanes, 0, st>>>(p);
+    } else {
+      ff_kernel<S, T, GRAD, false><<<tiles, S::kLanes, 0, st>>>(p);
+    }
   });
 }
 
 template <typename T, typename O, bool ACROSS_A, bool ACCUMULATE>
-void run_sum(SumArgs& p, uint32_t outs, hipStream_t st) {
-  with_shape<T, Small>([&](auto s) { return outs * tiles_of(p.M, p.N, s.BM, s.BN); }, [&](auto s) {
+void run_sum(SumArgs& p, uint32_t outs, char* parts, hipStream_t st) {
+  const Choice c = choose_sum<T>(p.M, p.N, p.K, std::max(1u, p.parts), outs);
+  p.splits = c.splits;
+  p.splits.parts = (float*)parts;
+  with_shape<Small>(c, [&](auto s) {
     typedef decltype(s) S;
     p.tiles_m = (p.M + S::BM - 1) / S::BM;
     p.tiles_n = (p.N + S::BN - 1) / S::BN;
-    sum_kernel<S, T, O, ACROSS_A, ACCUMULATE><<<dim3(p.tiles_m * p.tiles_n, outs), S::kLanes, 0, st>>>(p);
+    const uint32_t tiles = p.tiles_m * p.tiles_n;
+    if (c.splits.n > 1) {
+      sum_part_kernel<S, T, ACROSS_A><<<dim3(tiles * c.splits.n, outs), S::kLanes, 0, st>>>(p);
+      sum_kernel<S, T, O, ACROSS_A, ACCUMULATE, true><<<dim3(tiles, outs), S::kLanes, 0, st>>>(p);
+    } else {
+      sum_kernel<S, T, O, ACROSS_A, ACCUMULATE, false><<<dim3(tiles, outs), S::kLanes, 0, st>>>(p);
+    }
   });
 }
 
@@ -406,7 +497,7 @@ int ec_gated_ff(const void* d_x, uint64_t x_stride, const void* d_gate, uint64_t
     if (n <= kFewForward)
       run_few<T>(p, st);
     else
-      run_ff<T, false>(p, st);
+      run_ff<T, false>(p, work + w.parts, st);
     return launched();
   });
 }
@@ -441,7 +532,7 @@ int ec_gated_ff_grad(const void* d_dh, uint64_t dh_stride, const void* d_x, uint
       p.dh = (const char*)d_dh, p.dh_stride = dh_stride;
       p.d = work + w.d;
       p.low = w.low ? n * d_row : 0;
-      run_ff<T, true>(p, st);
+      run_ff<T, true>(p, work + w.parts, st);
     }
     const uint64_t ld = d_row * sizeof(T), half = p.padded * sizeof(T), low = p.low * sizeof(T);
     if (d_dx && n) {
@@ -454,7 +545,7 @@ int ec_gated_ff_grad(const void* d_dh, uint64_t dh_stride, const void* d_x, uint
       }
       s.K = inner, s.M = p.n, s.N = width;
       s.out[0] = (char*)d_dx, s.out_stride[0] = dx_stride;
-      run_sum<T, T, false, false>(s, 1, st);
+      run_sum<T, T, false, false>(s, 1, work + w.parts, st);
     }
     if (d_dgate) {
       SumArgs s = {};
@@ -470,7 +561,8 @@ int ec_gated_ff_grad(const void* d_dh, uint64_t dh_stride, const void* d_x, uint
       s.out[1] = (char*)d_dup, s.out_stride[1] = dup_stride;
       const auto run = [&](auto o) {
         typedef decltype(o) O;
-        accumulate ? run_sum<T, O, true, true>(s, 2, st) : run_sum<T, O, true, false>(s, 2, st);
+        accumulate ? run_sum<T, O, true, true>(s, 2, work + w.parts, st)
+                   : run_sum<T, O, true, false>(s, 2, work + w.parts, st);
       };
       grad_type == EC_F32 ? run(float()) : run(T());
     }

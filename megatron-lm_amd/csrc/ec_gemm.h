@@ -22,6 +22,8 @@
 // (the low parts' is below the fp32 accumulator's rounding), at 3/16 of the time of fp32 products.
 #pragma once
 
+#include <algorithm>
+
 #include "ec_types.h"
 #include "routes.h"
 
@@ -488,36 +490,128 @@ __device__ __forceinline__ void tile_at(uint32_t t, uint32_t tiles_m, uint32_t t
   n = uniform(in / high);
 }
 
-// The shape for m x n results: the one whose workgroups, dealt to the CUs in turns, take least time.
+// Few tiles with a long way along k are split: each split's sums go to memory as they lie in the accumulators, in
+// fp32, and a second launch adds them in order and goes on as a product of one split would.
+struct Splits {
+  uint32_t n, steps;   // steps along k of each but the last; n 1: not split
+  float* parts;
+};
+
+template <class S>
+__device__ __forceinline__ float* part_at(float* parts, uint64_t tile) {
+  return parts + tile * (S::BM * S::BN) + threadIdx.x * 4;
+}
+
+template <class S>
+__device__ __forceinline__ void store_part(const Acc<S>& acc, float* parts, uint64_t tile) {
+  float* to = part_at<S>(parts, tile);
+#pragma unroll
+  for (int r = 0; r < S::MI; ++r)
+#pragma unroll
+    for (int j = 0; j < S::NI; ++j) *(global<f4>*)(uintptr_t)(to + (r * S::NI + j) * S::kLanes * 4) = acc.v[r][j];
+}
+
+// acc += the parts of `tile` of each split, `tiles` apart.
+template <class S>
+__device__ __forceinline__ void add_parts(Acc<S>& acc, float* parts, uint64_t tile, uint64_t tiles,
+                                          uint32_t splits) {
+  for (uint32_t s = 0; s < splits; ++s) {
+    const float* from = part_at<S>(parts, tile + s * tiles);
+#pragma unroll
+    for (int r = 0; r < S::MI; ++r) {
+#pragma unroll
+      for (int j = 0; j < S::NI; ++j)
+        acc.v[r][j] += *(const global<f4>*)(uintptr_t)(from + (r * S::NI + j) * S::kLanes * 4);
+      if (r % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+}
+
+// The part of an operand along or across k from step s0 on.
+template <typename T, bool ACROSS>
+__device__ __forceinline__ Operand from_step(Operand a, uint32_t s0) {
+  a.p += ACROSS ? (uint64_t)s0 * (kRowBytes / Kind<T>::kBytes) * a.ld : (uint64_t)s0 * kRowBytes;
+  return a;
+}
+
+// Values along k of a split, of K.
+template <typename T>
+__device__ __forceinline__ uint32_t split_length(const Splits& s, uint32_t split, uint32_t K) {
+  constexpr uint32_t step = kRowBytes / Kind<T>::kBytes;
+  const uint32_t from = split * s.steps * step;
+  return min(K - from, s.steps * step);
+}
+
 constexpr uint64_t kCus = 256;
 
 inline uint64_t tiles_of(uint64_t m, uint64_t n, uint64_t bm, uint64_t bn) {
   return (m + bm - 1) / bm * ((n + bn - 1) / bn);
 }
 
-// What a turn of one tile to each CU costs, by its shape.  16-bit products of smaller tiles are bound by what comes from
-// L2, 64 bytes a clock and CU; others by the matrix cores.
+// What a step takes a workgroup that has a CU for itself, and what a tile takes beside its steps, in ns as measured.
+// 16-bit products of small tiles are bound by what comes from L2 (64 bytes a clock and CU), others by the matrix cores.
 template <class S, typename T>
-constexpr uint64_t cost_of() {
-  constexpr bool narrow = Kind<T>::kBytes == 2;
-  if (__is_same(S, Large)) return 400;
-  if (__is_same(S, Middle)) return narrow ? 165 : 120;
-  if (__is_same(S, Flat)) return narrow ? 110 : 70;
-  return narrow ? 70 : 42;
+constexpr uint64_t step_ns() {
+  constexpr int at = __is_same(S, Large) ? 0 : __is_same(S, Middle) ? 1 : __is_same(S, Flat) ? 2 : 3;
+  constexpr uint64_t narrow[] = {1470, 610, 400, 260}, pairs[] = {2400, 720, 400, 250}, wide[] = {6800, 1720, 880, 450};
+  return __is_same(T, float) ? wide[at] : __is_same(T, pair_t) ? pairs[at] : narrow[at];
+}
+template <class S>
+constexpr uint64_t tile_ns() {
+  return __is_same(S, Large) ? 8000 : __is_same(S, Middle) ? 5000 : 3500;
 }
 
-template <class S, typename T, typename F>
-uint64_t turns(F tiles) {
-  return (tiles(S()) + kCus - 1) / kCus * cost_of<S, T>();
+struct Choice {
+  int shape;           // 0: Large, 1: Middle, 2: the least
+  Splits splits;
+  uint64_t bytes;      // of the parts
+  uint64_t ns;
+};
+
+constexpr uint64_t kMostPartBytes = 256u << 20;   // bytes of parts
+
+// The best shape and number of splits for `tiles(S())` tiles of `steps` steps: the CUs take the workgroups in
+// turns; parts are written and read at 5.5 KB a ns in all, and read at 35 bytes a ns by a workgroup, in a launch of 4 us.
+// (2048 -> 8192 bf16, dx of 256 rows: 8 large tiles in 32 splits 301 us, most of them in the join.)
+template <typename T, class Least, typename F>
+Choice choose(F tiles, uint64_t steps, bool may_split = true) {
+  Choice best = {};
+  best.ns = ~0ull;
+  steps = steps ? steps : 1;
+  const auto consider = [&](auto s, int shape) {
+    typedef decltype(s) S;
+    const uint64_t n = tiles(s);
+    for (uint64_t splits = 1; splits <= (may_split ? 32 : 1); splits += splits < 4 ? 1 : splits / 2) {
+      const uint64_t each = (steps + splits - 1) / splits;
+      if (splits > 1 && (each < 4 || n >= 2 * kCus)) break;
+      const uint64_t real = (steps + each - 1) / each, bytes = real > 1 ? n * real * S::BM * S::BN * 4 : 0;
+      if (bytes > kMostPartBytes) break;
+      const uint64_t turns = (n * real + kCus - 1) / kCus;
+      const uint64_t join = real == 1 ? 0 : 4000 + std::max(bytes * 2 / 5500, (n + kCus - 1) / kCus * (bytes / n) / 35);
+      const uint64_t ns = turns * (each * step_ns<S, T>() + tile_ns<S>()) + join;
+      if (ns < best.ns) best = {shape, {(uint32_t)real, (uint32_t)each, nullptr}, bytes, ns};
+    }
+  };
+  consider(Large(), 0);
+  consider(Middle(), 1);
+  consider(Least(), 2);
+  return best;
 }
 
-// f(S()) with the best of Large, Middle and Least for `tiles(S())` tiles.
-template <typename T, class Least, typename F, typename G>
-void with_shape(F tiles, G f) {
-  const uint64_t large = turns<Large, T>(tiles), middle = turns<Middle, T>(tiles), least = turns<Least, T>(tiles);
-  if (least < large && least < middle) return f(Least());
-  if (middle < large) return f(Middle());
-  return f(Large());
+template <class Least, typename G>
+void with_shape(const Choice& c, G f) {
+  if (c.shape == 0)
+    f(Large());
+  else if (c.shape == 1)
+    f(Middle());
+  else
+    f(Least());
+}
+
+template <typename T>
+uint64_t steps_of(uint64_t K) {
+  constexpr uint64_t step = kRowBytes / Kind<T>::kBytes;
+  return (K + step - 1) / step;
 }
 
 template <typename T>

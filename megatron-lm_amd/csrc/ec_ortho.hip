@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(kLanes) square_kernel(const T* x, uint64_t str
     }
   }
   sum = block_sum(sum);
-  if (threadIdx.x == 0) gp(parts)[blockIdx.y * kMostParts + blockIdx.x] = sum;
+  if (threadIdx.x == 0) gp(parts)[blockIdx.y * gridDim.x + blockIdx.x] = sum;
 }
 
 // Two fp16 values whose sum is v to 22 bits.
@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(kLanes) scale_kernel(const T* x, uint64_t stri
                                                        uint32_t rows, uint32_t cols, const double* parts,
                                                        uint32_t n_parts, double eps, char* out, uint64_t low_at) {
   double sum = 0.0;
-  for (uint32_t i = threadIdx.x; i < n_parts; i += kLanes) sum += gp(parts)[blockIdx.y * kMostParts + i];
+  for (uint32_t i = threadIdx.x; i < n_parts; i += kLanes) sum += gp(parts)[blockIdx.y * n_parts + i];
   sum = block_sum(sum);
   const double by = (double)(1 << kStored) / (__builtin_sqrt(sum) + eps);
   const T* from = x + blockIdx.y * matrix;
@@ -165,24 +165,50 @@ struct NsArgs {
   float linear, diagonal;        // POLY: + diagonal * I
   Matrices base;                 // LAST: + keep * base, or none
   float keep;
+  Splits splits;                 // GRAM
 };
+
+// A wave's LDS to turn a block of 32 x 32 round: rows of 36 meet no bank conflicts either way.
+constexpr uint32_t kTurnRow = 36, kTurn = 32 * kTurnRow;
 
 // What becomes of a product: A, B, the next X, or the result.
 enum { kGram, kPoly, kNext, kLast };
 
-template <class S, typename In, bool ACROSS_A, bool ACROSS_B, int WHAT, typename Out>
-__global__ void __launch_bounds__(S::kLanes) ns_kernel(NsArgs p) {
+// The t-th tile on and above the diagonal, column by column.
+__device__ __forceinline__ void upper_tile_at(uint32_t t, uint32_t& tm, uint32_t& tn) {
+  t = uniform(t);
+  for (tn = 0; (tn + 1) * (tn + 2) / 2 <= t;) ++tn;
+  tm = t - tn * (tn + 1) / 2;
+}
+
+// A split of A's product.
+template <class S, typename In, bool ACROSS>
+__global__ void __launch_bounds__(S::kLanes) gram_part_kernel(NsArgs p) {
   __shared__ __attribute__((aligned(1024))) char lds[S::kLds];
+  const uint32_t t = xcd_order(blockIdx.x, gridDim.x), all = gridDim.x / p.splits.n, split = uniform(t / all);
+  const uint32_t matrix = uniform(t % all / p.tiles);
+  uint32_t tm, tn;
+  upper_tile_at(t % all % p.tiles, tm, tn);
+  Operand a = from_step<In, ACROSS>(p.a, split * p.splits.steps), b = from_step<In, ACROSS>(p.b, split * p.splits.steps);
+  a.p += matrix * p.a_matrix;
+  b.p += matrix * p.b_matrix;
+  Acc<S> acc;
+  acc.clear();
+  product<S, In, ACROSS, ACROSS, false>(acc, (local<char>*)lds, a, b, b, tm * S::BM, tn * S::BN,
+                                        split_length<In>(p.splits, split, p.K));
+  store_part(acc, p.splits.parts, t);
+}
+
+template <class S, typename In, bool ACROSS_A, bool ACROSS_B, int WHAT, typename Out, bool JOIN>
+__global__ void __launch_bounds__(S::kLanes) ns_kernel(NsArgs p) {
+  __shared__ __attribute__((aligned(1024))) char lds[JOIN ? S::kWaves * kTurn * 4 : S::kLds];
   const uint32_t t = xcd_order(blockIdx.x, gridDim.x), matrix = uniform(t / p.tiles);
   uint32_t tm, tn;
   constexpr bool kSymmetric = WHAT == kGram || WHAT == kPoly;
-  if (kSymmetric) {   // the tiles above the diagonal, column by column
-    const uint32_t i = uniform(t % p.tiles);
-    for (tn = 0; (tn + 1) * (tn + 2) / 2 <= i;) ++tn;
-    tm = i - tn * (tn + 1) / 2;
-  } else {
+  if (kSymmetric)
+    upper_tile_at(t % p.tiles, tm, tn);
+  else
     tile_at(t % p.tiles, p.tiles_m, p.tiles_n, tm, tn);
-  }
   Operand a = p.a, b = p.b;
   a.p += matrix * p.a_matrix;
   b.p += matrix * p.b_matrix;
@@ -198,7 +224,10 @@ __global__ void __launch_bounds__(S::kLanes) ns_kernel(NsArgs p) {
     acc.start(added);
   else
     acc.clear();
-  product<S, In, ACROSS_A, ACROSS_B, false>(acc, (local<char>*)lds, a, b, b, m0, n0, p.K);
+  if constexpr (JOIN)
+    add_parts(acc, p.splits.parts, t, gridDim.x, p.splits.n);
+  else
+    product<S, In, ACROSS_A, ACROSS_B, false>(acc, (local<char>*)lds, a, b, b, m0, n0, p.K);
   char* out = p.out + matrix * p.out_matrix;
   const auto value = [&](uint32_t m, uint32_t n, f8 v) {
     v *= p.by;
@@ -234,9 +263,8 @@ __global__ void __launch_bounds__(S::kLanes) ns_kernel(NsArgs p) {
   } else {
     // and the mirrored tile, 32 x 32 at a time turned round in the wave's part of LDS
     stage_barrier();
-    constexpr uint32_t kRow = 36;
-    local<float>* turn = (local<float>*)(local<char>*)lds + threadIdx.x / 64 * (32 * kRow);
-    static_assert(S::kWaves * 32 * kRow * 4 <= S::kLds, "a part for each wave");
+    local<float>* turn = (local<float>*)(local<char>*)lds + threadIdx.x / 64 * kTurn;
+    static_assert(S::kWaves * kTurn * 4 <= S::kLds, "a part for each wave");
     const uint32_t l = threadIdx.x % 64, w = threadIdx.x / 64, i = l % 16;
     const uint32_t mw = m0 + w / S::kWavesN * S::WM, nw = n0 + w % S::kWavesN * S::WN;
     const auto in_step = [] {
@@ -253,8 +281,8 @@ __global__ void __launch_bounds__(S::kLanes) ns_kernel(NsArgs p) {
           const uint32_t m = mw + r * 16 + mr, n = nw + j * 16 + nr;
           const f8 v = value(m, n, acc.pair(r + h, j));
           if (m < p.M && n < padded) put8<Out>(out + m * p.out_ld, n, v, p.out_low);
-          *(local<f4>*)(turn + mr * kRow + nr) = __builtin_shufflevector(v, v, 0, 1, 2, 3);
-          *(local<f4>*)(turn + mr * kRow + nr + 4) = __builtin_shufflevector(v, v, 4, 5, 6, 7);
+          *(local<f4>*)(turn + mr * kTurnRow + nr) = __builtin_shufflevector(v, v, 0, 1, 2, 3);
+          *(local<f4>*)(turn + mr * kTurnRow + nr + 4) = __builtin_shufflevector(v, v, 4, 5, 6, 7);
         }
         in_step();
         const uint32_t row = nw + j * 16 + l / 2, col = mw + r * 16 + l % 2 * 16;
@@ -262,7 +290,7 @@ __global__ void __launch_bounds__(S::kLanes) ns_kernel(NsArgs p) {
         for (int h = 0; h < 2; ++h) {
           f8 v;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = turn[(l % 2 * 16 + h * 8 + e) * kRow + l / 2];
+          for (int e = 0; e < 8; ++e) v[e] = turn[(l % 2 * 16 + h * 8 + e) * kTurnRow + l / 2];
           if (row < p.N && col + h * 8 < padded) put8<Out>(out + row * p.out_ld, col + h * 8, v, p.out_low);
         }
         in_step();
@@ -271,36 +299,61 @@ __global__ void __launch_bounds__(S::kLanes) ns_kernel(NsArgs p) {
   }
 }
 
+// The tiles of M x N results, or (symmetric) those on and above the diagonal.
+template <class S>
+uint64_t ns_tiles(uint64_t m, uint64_t n, bool symmetric) {
+  const uint64_t wide = (n + S::BN - 1) / S::BN;
+  return symmetric ? wide * (wide + 1) / 2 : tiles_of(m, n, S::BM, S::BN);
+}
+
+template <typename In>
+Choice choose_ns(uint32_t m, uint32_t n, uint32_t K, uint32_t batch, int what) {
+  const bool symmetric = what == kGram || what == kPoly;
+  return choose<In, Small>([&](auto s) { return batch * ns_tiles<decltype(s)>(m, n, symmetric); }, steps_of<In>(K),
+                           what == kGram);   // only A's products are split
+}
+
 template <typename In, bool ACROSS_A, bool ACROSS_B, int WHAT, typename Out>
-int run_ns(NsArgs& p, uint32_t batch, hipStream_t st) {
+int run_ns(NsArgs& p, uint32_t batch, char* parts, hipStream_t st) {
   constexpr bool kSymmetric = WHAT == kGram || WHAT == kPoly;
   int status = EC_OK;
-  const auto tiles = [&](auto s) -> uint64_t {
-    const uint64_t n = (p.N + s.BN - 1) / s.BN;
-    return kSymmetric ? n * (n + 1) / 2 * batch : tiles_of(p.M, p.N, s.BM, s.BN) * batch;
-  };
-  with_shape<In, Small>(tiles, [&](auto s) {
+  const Choice c = choose_ns<In>(p.M, p.N, p.K, batch, WHAT);
+  p.splits = c.splits;
+  p.splits.parts = (float*)parts;
+  with_shape<Small>(c, [&](auto s) {
     typedef decltype(s) S;
     p.tiles_m = (p.M + S::BM - 1) / S::BM;
     p.tiles_n = (p.N + S::BN - 1) / S::BN;
-    p.tiles = (uint32_t)(tiles(s) / batch);
-    if ((uint64_t)p.tiles * batch >= (1ull << 32) / S::kLanes)
+    p.tiles = (uint32_t)ns_tiles<S>(p.M, p.N, kSymmetric);
+    const uint64_t all = (uint64_t)p.tiles * batch;
+    if (all >= (1ull << 32) / S::kLanes) {
       status = EC_ERANGE;
-    else
-      ns_kernel<S, In, ACROSS_A, ACROSS_B, WHAT, Out><<<p.tiles * batch, S::kLanes, 0, st>>>(p);
+      return;
+    }
+    if constexpr (WHAT == kGram) {
+      if (c.splits.n > 1) {
+        gram_part_kernel<S, In, ACROSS_A><<<(uint32_t)all * c.splits.n, S::kLanes, 0, st>>>(p);
+        ns_kernel<S, In, ACROSS_A, ACROSS_B, WHAT, Out, true><<<(uint32_t)all, S::kLanes, 0, st>>>(p);
+        return;
+      }
+    }
+    ns_kernel<S, In, ACROSS_A, ACROSS_B, WHAT, Out, false><<<(uint32_t)all, S::kLanes, 0, st>>>(p);
   });
   return status;
 }
 
 struct Plan {
   uint32_t batch, rows, cols, side, other;   // side: of the symmetric matrices
-  uint64_t parts, x[2], gram, poly, total;
+  uint32_t sums;                             // parts of a matrix's sum of squares
+  uint64_t parts, x[2], gram, poly, splits, total;
 };
 
 Plan plan_of(uint32_t batch, uint32_t rows, uint32_t cols) {
   Plan p = {};
   p.batch = batch, p.rows = rows, p.cols = cols;
   p.side = std::min(rows, cols), p.other = std::max(rows, cols);
+  // enough workgroups in all to keep the memory busy
+  p.sums = std::min(kMostParts, std::max(1u, 2 * kMostParts / batch));
   const auto take = [&](uint64_t bytes) {
     const uint64_t at = p.total;
     p.total += part(bytes);
@@ -308,9 +361,11 @@ Plan plan_of(uint32_t batch, uint32_t rows, uint32_t cols) {
   };
   const uint64_t x = (uint64_t)batch * rows * up_to(cols, 8) * 4;
   const uint64_t square = (uint64_t)batch * p.side * up_to(p.side, 8) * 4;
-  p.parts = take((uint64_t)batch * kMostParts * sizeof(double));
+  p.parts = take((uint64_t)batch * p.sums * sizeof(double));
   p.x[0] = take(x), p.x[1] = take(x);
   p.gram = take(square), p.poly = take(square);
+  p.splits = take(std::max(choose_ns<pair_t>(p.side, p.side, p.other, batch, kGram).bytes,
+                           choose_ns<fp16_t>(p.side, p.side, p.other, batch, kGram).bytes));
   return p;
 }
 
@@ -369,7 +424,7 @@ int run_step(const Plan& p, const Call& c, char* work, int s, hipStream_t st) {
   n.K = p.other, n.M = n.N = p.side;
   n.out = work + p.gram, n.out_ld = gram.m.ld, n.out_matrix = gram.matrix;
   n.by = std::ldexp(1.0f, -kStored);
-  if (const int e = run_ns<In, TALL, TALL, kGram, In>(n, p.batch, st)) return e;
+  if (const int e = run_ns<In, TALL, TALL, kGram, In>(n, p.batch, work + p.splits, st)) return e;
 
   n.a = n.b = gram.m;
   n.a_matrix = n.b_matrix = gram.matrix;
@@ -381,7 +436,7 @@ int run_step(const Plan& p, const Call& c, char* work, int s, hipStream_t st) {
   n.by = square * std::ldexp(1.0f, at - 2 * kStored);
   n.linear = c.b / square * std::ldexp(1.0f, kStored);
   n.diagonal = adds ? 0.0f : c.a * std::ldexp(1.0f, at);
-  if (const int e = run_ns<In, false, false, kPoly, In>(n, p.batch, st)) return e;
+  if (const int e = run_ns<In, false, false, kPoly, In>(n, p.batch, work + p.splits, st)) return e;
 
   // B X, X across; or X B, X along
   n.a = TALL ? x.m : poly.m, n.b = TALL ? poly.m : x.m;
@@ -394,17 +449,17 @@ int run_step(const Plan& p, const Call& c, char* work, int s, hipStream_t st) {
     n.out = work + p.x[(s + 1) & 1], n.out_ld = x.m.ld, n.out_matrix = x.matrix;
     n.out_low = next_adds ? x.low : 0;
     n.by = std::ldexp(1.0f, -at);
-    return run_ns<In, false, !TALL, kNext, In>(n, p.batch, st);
+    return run_ns<In, false, !TALL, kNext, In>(n, p.batch, work + p.splits, st);
   }
   const uint32_t w = type_bytes(c.out_type);
   n.out = c.out, n.out_ld = c.out_stride * w, n.out_matrix = c.out_matrix * w;
   n.by = c.scale * std::ldexp(1.0f, -at - kStored);
   n.base = c.base, n.keep = c.keep;
   if constexpr (kFast)
-    return run_ns<In, false, !TALL, kLast, bf16_t>(n, p.batch, st);
+    return run_ns<In, false, !TALL, kLast, bf16_t>(n, p.batch, work + p.splits, st);
   else
     return with_type(c.out_type, [&](auto o) {
-      return run_ns<In, false, !TALL, kLast, decltype(o)>(n, p.batch, st);
+      return run_ns<In, false, !TALL, kLast, decltype(o)>(n, p.batch, work + p.splits, st);
     });
 }
 
@@ -453,8 +508,7 @@ int ec_orthogonalize(const void* d_x, int type, uint64_t batch, uint64_t rows, u
   const bool dense = x_stride == cols;
   const uint64_t total = rows * cols;
   const uint64_t pieces = dense ? (total + kPiece - 1) / kPiece : rows;
-  // enough workgroups in all to keep the memory busy
-  const uint32_t parts = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(1, 2 * kMostParts / batch), std::min<uint64_t>(kMostParts, pieces));
+  const uint32_t parts = (uint32_t)std::min<uint64_t>(p.sums, pieces);
   double* sums = (double*)(work + p.parts);
   const uint64_t blocks = (rows * ((cols + 7) / 8) + kLanes - 1) / kLanes;
   const uint32_t grid = (uint32_t)std::min<uint64_t>(blocks, std::max<uint64_t>(1, 8192 / batch));

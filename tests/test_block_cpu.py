@@ -23,15 +23,16 @@ def test_gated_ff_refusals(pkg):
     assert call(n=0) == ok and call(n=0, x=None, h=None) == ok
     for bad in (dict(x=None), dict(g=None), dict(u=None), dict(h=None), dict(kind=3), dict(kind=-1), dict(act=3), dict(act=-1),
                 dict(xs=31), dict(gs=31), dict(us=31), dict(hs=47), dict(width=0, xs=0), dict(inner=0),
-                dict(x=ctypes.c_void_p(4098)), dict(xs=33), dict(width=31)):   # the last need a workspace
+                dict(n=99, x=ctypes.c_void_p(4098)), dict(n=99, xs=33), dict(n=99, width=31)):   # the last need a workspace
         assert call(**bad) == inval, bad
     for bad in (dict(n=1 << 31), dict(width=(1 << 19) + 1, xs=1 << 20, gs=1 << 20, us=1 << 20),
                 dict(inner=(1 << 19) + 1, hs=1 << 20), dict(n=(1 << 31) - 1, inner=1 << 19, hs=1 << 20)):
         assert call(**bad) == big, bad
-    need = L.ec_gated_ff_workspace(P, 31, P, 32, P, 32, 1, 4, 31, 48, 0)
-    assert need >= 4 * 64 + 2 * 48 * 64 and L.ec_gated_ff_workspace(P, 32, P, 32, P, 32, 1, 4, 32, 48, 0) == 0
-    assert call(width=31, xs=31, work=P, have=need - 1) == inval
-    assert call(width=31, xs=31, work=ODD, have=need) == align
+    need = L.ec_gated_ff_workspace(P, 31, P, 32, P, 32, 1, 99, 31, 48, 0)
+    assert need >= 99 * 64 + 2 * 48 * 64 and L.ec_gated_ff_workspace(P, 32, P, 32, P, 32, 1, 99, 32, 48, 0) == 0
+    assert L.ec_gated_ff_workspace(P, 31, P, 31, P, 31, 1, 4, 31, 48, 0) == 0   # few rows are read as they are
+    assert call(n=99, width=31, xs=31, work=P, have=need - 1) == inval
+    assert call(n=99, width=31, xs=31, work=ODD, have=need) == align
     assert L.ec_gated_ff_workspace(P, 32, P, 32, P, 32, 7, 4, 32, 48, 0) == 0
 
 
