@@ -162,9 +162,10 @@ def residual_norm(residual: torch.Tensor, branch: Optional[torch.Tensor] = None,
         normed = weight * residual' / rms(residual')    with ``weight`` (the norm before the next block)
 
     with rms(v) = sqrt(mean(v^2) + eps) over the last dimension, at most 16384 wide.  ``residual`` and ``branch``
-    are [..., width] of one type (contiguous, or two-dimensional with strided rows), the weights [width].  ``gate`` is [..., width]
-    with any number of rows that divides theirs, which share them evenly in order: one for all ([width]), one for each
-    sequence of [batch, length, width] ([batch, width] or [batch, 1, width]), or one for each row.  Without a
+    are [..., width] of one type (contiguous, or two-dimensional with strided rows), the weights [width].  ``gate`` has rows
+    that theirs share evenly, in order: one for all ([width]), one for each sequence of [batch, length, width] ([batch,
+    width] or [batch, 1, width]: the leading dimensions are the gate's), or one for each row; with two-dimensional rows
+    any number that divides theirs.  Without a
     ``branch`` only the norm is taken (a first block's).  normed is that of the sum before its rounding.
     ``out`` takes the sum, and may be the residual itself."""
     scale, eps = _finite(scale, "scale"), _finite(eps, "eps")

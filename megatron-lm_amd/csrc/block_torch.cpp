@@ -210,7 +210,8 @@ Tensor vector_of(const Tensor& t, const char* what, const Tensor& x, uint64_t wi
   return t;
 }
 
-// Rows of the gate: those of [..., width], which the rows of x share evenly, in order.
+// Rows of the gate: those of [..., width], which the rows of x share evenly, in order. Of more than two dimensions
+// x's leading ones have to be the gate's (and ones after them), so that none is taken for another.
 uint64_t gate_rows(const std::optional<Tensor>& gate, const Tensor& x, const Rows& rows) {
   if (!gate) return 1;
   const c10::Device device = x.device();
@@ -221,9 +222,14 @@ uint64_t gate_rows(const std::optional<Tensor>& gate, const Tensor& x, const Row
                           shape_text(gate->sizes()));
   uint64_t n = 1;
   for (int64_t d = 0; d + 1 < gate->dim(); ++d) n *= (uint64_t)gate->size(d);
-  if (rows.n ? (!n || rows.n % n) : false)
-    throw py::value_error("gate has " + std::to_string(n) + " rows, which " +
-                          std::to_string(rows.n) + " rows do not share evenly");
+  bool ones = false, fits = x.dim() <= 2 || gate->dim() <= x.dim();
+  for (int64_t d = 0; x.dim() > 2 && fits && d + 1 < gate->dim(); ++d) {
+    ones = ones || gate->size(d) != x.size(d);
+    fits = !ones || gate->size(d) == 1;
+  }
+  if (!fits || (rows.n && (!n || rows.n % n)))
+    throw py::value_error("gate of shape " + shape_text(gate->sizes()) + ": the rows of " +
+                          shape_text(x.sizes()) + " do not share its rows evenly, in order");
   return std::max<uint64_t>(n, 1);
 }
 

@@ -391,10 +391,20 @@ FfWork ff_work(const FfCall& c, bool grad) {
 
 template <typename T>
 Operand in_place(const void* p, uint64_t stride, uint64_t rows, uint32_t width, uint64_t at, char* work,
-                 hipStream_t st) {
+                 Packer<T>& packer) {
   if (at == kNone) return {(const char*)p, stride * sizeof(T), (uint32_t)rows};
-  pack<T>((const T*)p, stride, rows, width, (T*)(work + at), st);
+  packer.add((const T*)p, stride, rows, (T*)(work + at));
   return {work + at, up_to(width, Group<T>::kN) * sizeof(T), (uint32_t)rows};
+}
+
+// The call's operands, packed where they have to be.
+template <typename T>
+void place(FfArgs& p, const FfCall& c, const FfWork& w, char* work, hipStream_t st) {
+  Packer<T> packer(c.width);
+  p.x = in_place<T>(c.x, c.x_stride, c.n, c.width, w.x, work, packer);
+  p.w_gate = in_place<T>(c.w_gate, c.gate_stride, c.inner, c.width, w.w_gate, work, packer);
+  p.w_up = in_place<T>(c.w_up, c.up_stride, c.inner, c.width, w.w_up, work, packer);
+  packer.run(st);
 }
 
 template <typename T>
@@ -489,9 +499,7 @@ int ec_gated_ff(const void* d_x, uint64_t x_stride, const void* d_gate, uint64_t
     typedef decltype(t) T;
     char* work = (char*)d_work;
     FfArgs p = {};
-    p.x = in_place<T>(d_x, x_stride, n, width, w.x, work, st);
-    p.w_gate = in_place<T>(d_gate, gate_stride, inner, width, w.w_gate, work, st);
-    p.w_up = in_place<T>(d_up, up_stride, inner, width, w.w_up, work, st);
+    place<T>(p, c, w, work, st);
     p.n = (uint32_t)n, p.width = width, p.inner = inner, p.act = (uint32_t)activation;
     p.h = (char*)d_h, p.h_stride = h_stride;
     if (n <= kFewForward)
@@ -526,9 +534,7 @@ int ec_gated_ff_grad(const void* d_dh, uint64_t dh_stride, const void* d_x, uint
     p.padded = (uint32_t)up_to(inner, 8);
     const uint64_t d_row = 2ull * p.padded;
     if (n) {
-      p.x = in_place<T>(d_x, x_stride, n, width, w.x, work, st);
-      p.w_gate = in_place<T>(d_gate, gate_stride, inner, width, w.w_gate, work, st);
-      p.w_up = in_place<T>(d_up, up_stride, inner, width, w.w_up, work, st);
+      place<T>(p, c, w, work, st);
       p.dh = (const char*)d_dh, p.dh_stride = dh_stride;
       p.d = work + w.d;
       p.low = w.low ? n * d_row : 0;

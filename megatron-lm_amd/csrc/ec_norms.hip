@@ -25,11 +25,11 @@ namespace ec {
 namespace {
 
 constexpr uint32_t kMostWidth = 16384;
-constexpr int kTeamLanes = 256;   // of a workgroup of teams of 64 or 256 lanes
+constexpr int kTeamLanes = 256;   // of a workgroup of teams of 64 lanes
 
 template <int R>
 constexpr int block_lanes() {
-  return R > kTeamLanes ? R : kTeamLanes;
+  return R > 64 ? R : kTeamLanes;
 }
 
 // The sum over a team's R lanes, in each of them.  `turn` alternates from call to call, so that a slot is
@@ -315,30 +315,36 @@ __global__ void __launch_bounds__(kJoinLanes) join_parts_kernel(JoinArgs p) {
   }
 }
 
-// The teams' lanes and groups for a row: one or two groups a lane, and teams no larger than that needs.
-// f(lanes, groups), as constants.
-template <typename T, typename F>
+// The teams' lanes and groups a lane for a row; f(lanes, groups), as constants.  Forward two groups a lane pay (16384 x
+// 1000 bf16 28.8 us against 33.6 with one, 8192 x 4096 47.3 against 48.6), backward one (fewer registers: 1024 x 4096
+// 21.0 us against 21.9).
+template <typename T, bool PAIRS, typename F>
 void with_team(uint32_t width, F f) {
   const uint32_t groups = (width + Group<T>::kN - 1) / Group<T>::kN;
+  const auto run = [&](auto lanes, auto per_lane) { f(lanes, per_lane); };
+  constexpr auto one = std::integral_constant<int, 1>();
   if (groups <= 64)
-    f(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
+    run(std::integral_constant<int, 64>(), one);
   else if (groups <= 128)
-    f(std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
+    run(std::integral_constant<int, PAIRS ? 64 : 128>(), std::integral_constant<int, PAIRS ? 2 : 1>());
   else if (groups <= 256)
-    f(std::integral_constant<int, 256>(), std::integral_constant<int, 1>());
+    run(std::integral_constant<int, 256>(), one);
   else if (groups <= 512)
-    f(std::integral_constant<int, 256>(), std::integral_constant<int, 2>());
+    run(std::integral_constant<int, PAIRS ? 256 : 512>(), std::integral_constant<int, PAIRS ? 2 : 1>());
   else if (groups <= 1024)
-    f(std::integral_constant<int, 1024>(), std::integral_constant<int, 1>());
+    run(std::integral_constant<int, 1024>(), one);
   else if (groups <= 2048)
-    f(std::integral_constant<int, 1024>(), std::integral_constant<int, 2>());
+    run(std::integral_constant<int, 1024>(), std::integral_constant<int, 2>());
   else if constexpr (sizeof(T) == 4)
-    f(std::integral_constant<int, 1024>(), std::integral_constant<int, 4>());
+    run(std::integral_constant<int, 1024>(), std::integral_constant<int, 4>());
 }
 
 // Teams for n rows: each row its own up to 256 (one for each CU), then four rows a team and more, as the partials are
-// as large as the rows (1023 rows of 1999 fp32: 26 us with one row a team), and 1024 at most.
-constexpr uint64_t kMostTeams = 1024, kLeastTeams = 256, kTeamRows = 4;
+// as large as the rows; and as many as the CUs hold (16384 x 2048 bf16: 1024 teams 83 us, 512 101; 16384 x 1000: 2048 teams
+// 63 us, 1024 82).
+constexpr uint64_t kLeastTeams = 256, kTeamRows = 4;
+
+constexpr uint64_t most_teams(uint32_t width) { return width <= 512 ? 4096 : width <= 1024 ? 2048 : 1024; }
 
 struct Split {
   uint64_t teams, per_gate, rows, gates;
@@ -346,9 +352,9 @@ struct Split {
 };
 
 // Teams for n rows, of which gate_share each share a row of the gate.
-Split split_rows(uint64_t n, uint64_t gate_share) {
+Split split_rows(uint64_t n, uint64_t gate_share, uint32_t width) {
   Split s = {};
-  const uint64_t most = std::min(kMostTeams, std::max(kLeastTeams, n / kTeamRows));
+  const uint64_t most = std::min(most_teams(width), std::max(kLeastTeams, n / kTeamRows));
   s.gates = n / gate_share;
   s.direct = s.gates > most / 2;
   if (s.direct) {   // a run of whole gate rows each
@@ -399,7 +405,7 @@ int ec_residual_norm(const void* d_residual, uint64_t residual_stride, const voi
   const auto st = (hipStream_t)stream;
   return with_type(type, [&](auto t) {
     typedef decltype(t) T;
-    with_team<T>(width, [&](auto lanes, auto groups) {
+    with_team<T, true>(width, [&](auto lanes, auto groups) {
       constexpr int R = decltype(lanes)::value, V = decltype(groups)::value;
       constexpr uint64_t kTeams = block_lanes<R>() / R;
       for (uint64_t row = 0; row < n;) {   // as many launches as the grid's limit asks for
@@ -422,7 +428,7 @@ int ec_residual_norm(const void* d_residual, uint64_t residual_stride, const voi
 
 uint64_t ec_residual_norm_grad_workspace(uint64_t n, uint32_t width, uint64_t gate_rows) {
   if (check_rows(EC_F32, n, width, gate_rows) != EC_OK || !n) return 0;
-  return 3 * split_rows(n, n / std::max<uint64_t>(1, gate_rows)).teams * width * sizeof(float);
+  return 3 * split_rows(n, n / std::max<uint64_t>(1, gate_rows), width).teams * width * sizeof(float);
 }
 
 int ec_residual_norm_grad(const void* d_dsum, uint64_t dsum_stride, const void* d_dnormed,
@@ -450,7 +456,7 @@ int ec_residual_norm_grad(const void* d_dsum, uint64_t dsum_stride, const void* 
     if (!d_work || work_bytes < ec_residual_norm_grad_workspace(n, width, gate_rows)) return EC_EINVAL;
     if ((uintptr_t)d_work & 15u) return EC_EALIGN;
   }
-  const Split s = n ? split_rows(n, n / gate_rows) : Split{0, 1, 0, gate_rows, false};
+  const Split s = n ? split_rows(n, n / gate_rows, width) : Split{0, 1, 0, gate_rows, false};
   float* parts = (float*)d_work;
   const uint64_t area = s.teams * width;
   GradArgs p = {};
@@ -469,7 +475,7 @@ int ec_residual_norm_grad(const void* d_dsum, uint64_t dsum_stride, const void* 
   if (n)
     with_type(type, [&](auto t) {
       typedef decltype(t) T;
-      with_team<T>(width, [&](auto lanes, auto groups) {
+      with_team<T, false>(width, [&](auto lanes, auto groups) {
         constexpr int R = decltype(lanes)::value, V = decltype(groups)::value;
         constexpr uint64_t kTeams = block_lanes<R>() / R;
         norm_grad_kernel<T, R, V><<<(uint32_t)((s.teams + kTeams - 1) / kTeams), block_lanes<R>(), 0, st>>>(p);

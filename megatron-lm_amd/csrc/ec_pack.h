@@ -19,36 +19,60 @@ inline bool readable(const void* p, uint64_t width, uint64_t stride, uint32_t by
 
 constexpr int kPackLanes = 256;
 
+// What is packed in one launch, blockIdx.y's each.
+template <typename T>
+struct PackArgs {
+  const T* src[3];
+  uint64_t stride[3], rows[3];
+  T* dst[3];
+  uint32_t width, groups;
+};
+
 // 16 bytes of the result a lane.
 template <typename T>
-__global__ void __launch_bounds__(kPackLanes) pack_kernel(const T* src, uint64_t stride, uint64_t rows,
-                                                          uint32_t width, uint32_t groups, T* dst) {
+__global__ void __launch_bounds__(kPackLanes) pack_kernel(PackArgs<T> p) {
   typedef Group<T> G;
-  const uint64_t n = rows * groups;
+  const T* src = p.src[blockIdx.y];
+  const uint64_t stride = p.stride[blockIdx.y], n = p.rows[blockIdx.y] * p.groups;
+  T* dst = p.dst[blockIdx.y];
   for (uint64_t g = (uint64_t)blockIdx.x * kPackLanes + threadIdx.x; g < n;
        g += (uint64_t)gridDim.x * kPackLanes) {
-    const uint64_t row = g / groups;
-    const uint32_t at = (uint32_t)(g % groups) * G::kN;
+    const uint64_t row = g / p.groups;
+    const uint32_t at = (uint32_t)(g % p.groups) * G::kN;
     const T* from = src + row * stride + at;
     typename G::vec v = {};
-    if (at + G::kN <= width) {
+    if (at + G::kN <= p.width) {
       v = load_group<T, true>(from);
     } else {
 #pragma unroll
       for (int e = 0; e < G::kN; ++e)
-        if (at + e < width) v[e] = gp(from)[e];
+        if (at + e < p.width) v[e] = gp(from)[e];
     }
     store_group<T, false>(dst + g * G::kN, v);
   }
 }
 
+// Rows of one width, up to three times, in one launch.
 template <typename T>
-void pack(const T* src, uint64_t stride, uint64_t rows, uint32_t width, T* dst, hipStream_t st) {
-  const uint32_t groups = (uint32_t)(up_to(width, Group<T>::kN) / Group<T>::kN);
-  const uint64_t blocks = (rows * groups + kPackLanes - 1) / kPackLanes;
-  pack_kernel<T><<<(uint32_t)(blocks < 8192 ? blocks : 8192), kPackLanes, 0, st>>>(src, stride, rows, width,
-                                                                                  groups, dst);
-}
+struct Packer {
+  PackArgs<T> p = {};
+  uint32_t n = 0;
+  uint64_t most = 0;
+
+  explicit Packer(uint32_t width) {
+    p.width = width;
+    p.groups = (uint32_t)(up_to(width, Group<T>::kN) / Group<T>::kN);
+  }
+  void add(const T* src, uint64_t stride, uint64_t rows, T* dst) {
+    p.src[n] = src, p.stride[n] = stride, p.rows[n] = rows, p.dst[n] = dst;
+    most = rows > most ? rows : most;
+    ++n;
+  }
+  void run(hipStream_t st) const {
+    const uint64_t blocks = (most * p.groups + kPackLanes - 1) / kPackLanes;
+    if (n) pack_kernel<T><<<dim3((uint32_t)(blocks < 8192 ? blocks : 8192), n), kPackLanes, 0, st>>>(p);
+  }
+};
 
 }  // namespace
 }  // namespace ec
