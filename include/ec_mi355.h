@@ -510,7 +510,7 @@ int ec_gated_ff_grad(const void* d_dh, uint64_t dh_stride, const void* d_x, uint
 #define EC_MAX_STEPS 64
 
 /* Device memory that ec_orthogonalize needs at d_work, in bytes, 16-byte aligned; 0 where the
- * call refuses the sizes or has nothing to do. */
+ * call refuses the sizes, has nothing to do, or takes matrices of at most 128 x 128. */
 uint64_t ec_orthogonalize_workspace(uint64_t batch, uint64_t rows, uint64_t cols);
 
 /* out = keep * base + scale * X for each of `batch` matrices x of [rows][cols], where X is x / (|x| + eps),

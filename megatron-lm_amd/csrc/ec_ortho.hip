@@ -40,19 +40,23 @@ constexpr int kStored = 12;               // matrices are stored times 2^12
 constexpr uint32_t kMostSide = 1u << 16;
 constexpr uint32_t kMostBatch = 65535;
 
+constexpr uint32_t kFastSide = 64;
+constexpr int kPlainSteps = 2;   // the last fast steps, whose X has no second part
+
 struct Matrices {
   const char* p;
   uint64_t stride, matrix;   // elements from row to row, from matrix to matrix
 };
 
+template <int LANES>
 __device__ __forceinline__ double block_sum(double v) {
-  __shared__ double shared[kLanes / 64];
+  __shared__ double shared[LANES / 64];
 #pragma unroll
   for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
   if (threadIdx.x % 64 == 0) shared[threadIdx.x / 64] = v;
   __syncthreads();
   v = shared[0];
-  for (int w = 1; w < kLanes / 64; ++w) v += shared[w];
+  for (int w = 1; w < LANES / 64; ++w) v += shared[w];
   return v;
 }
 
@@ -86,7 +90,7 @@ __global__ void __launch_bounds__(kLanes) square_kernel(const T* x, uint64_t str
       sum = __builtin_fma(v, v, sum);
     }
   }
-  sum = block_sum(sum);
+  sum = block_sum<kLanes>(sum);
   if (threadIdx.x == 0) gp(parts)[blockIdx.y * gridDim.x + blockIdx.x] = sum;
 }
 
@@ -135,7 +139,7 @@ __global__ void __launch_bounds__(kLanes) scale_kernel(const T* x, uint64_t stri
                                                        uint32_t n_parts, double eps, char* out, uint64_t low_at) {
   double sum = 0.0;
   for (uint32_t i = threadIdx.x; i < n_parts; i += kLanes) sum += gp(parts)[blockIdx.y * n_parts + i];
-  sum = block_sum(sum);
+  sum = block_sum<kLanes>(sum);
   const double by = (double)(1 << kStored) / (__builtin_sqrt(sum) + eps);
   const T* from = x + blockIdx.y * matrix;
   const uint32_t groups = (cols + 7) / 8, all = rows * groups;
@@ -342,6 +346,206 @@ int run_ns(NsArgs& p, uint32_t batch, char* parts, hipStream_t st) {
   return status;
 }
 
+// A matrix of at most D x D: one workgroup takes all steps, with everything in LDS, one launch instead of seventeen.  A tall
+// matrix is taken transposed.  A matrix lies there as D-row tiles along k, one behind another; B takes A's place and
+// the next X that of X, when all waves have read them.
+struct SmallArgs {
+  Matrices x, base;
+  char* out;
+  uint64_t out_stride, out_matrix;   // elements
+  uint32_t rows, cols, steps;
+  float a, b, c, scale, keep;
+  double eps;
+  int at_added, at_plain;            // B is stored times 2^at: in steps that add a X, in others
+};
+
+constexpr int kSmallSide = 128;
+
+template <typename K, int D>
+struct Resident {
+  static constexpr int kBlock = D * kRowBytes, kBlocks = D * Kind<K>::kBytes / kRowBytes, kSize = kBlock * kBlocks;
+
+  // 16-byte chunk c of row r
+  __device__ __forceinline__ static uint32_t chunk_at(uint32_t r, uint32_t c) {
+    return c / 8 * kBlock + r * kRowBytes + ((c % 8) ^ along_swizzle(r)) * 16;
+  }
+  __device__ __forceinline__ static void put(local<char>* m, local<char>* low, uint32_t row, uint32_t n, const f8& v) {
+    h8 h, l;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      fp16_t x, y;
+      split(v[e], x, y);
+      h[e] = x;
+      l[e] = y;
+    }
+    if constexpr (Kind<K>::kParts == 2) {
+      *(local<h8>*)(m + chunk_at(row, n / 4)) = h;
+      *(local<h8>*)(m + chunk_at(row, n / 4 + 1)) = l;
+    } else {
+      *(local<h8>*)(m + chunk_at(row, n / 8)) = h;
+      if (low) *(local<h8>*)(low + chunk_at(row, n / 8)) = l;
+    }
+  }
+  __device__ __forceinline__ static f8 get(const local<char>* m, const local<char>* low, uint32_t row, uint32_t n) {
+    if constexpr (Kind<K>::kParts == 2)
+      return __builtin_convertvector(*(const local<h8>*)(m + chunk_at(row, n / 4)), f8) +
+             __builtin_convertvector(*(const local<h8>*)(m + chunk_at(row, n / 4 + 1)), f8);
+    f8 v = __builtin_convertvector(*(const local<h8>*)(m + chunk_at(row, n / 8)), f8);
+    if (low) v += __builtin_convertvector(*(const local<h8>*)(low + chunk_at(row, n / 8)), f8);
+    return v;
+  }
+  // The fragment whose rows are the matrix's columns and whose k its rows, of step k0 / 32: read_frag's across k.
+  __device__ __forceinline__ static Frag<K> turned(const local<char>* m, int block, uint32_t k0) {
+    constexpr int P = Kind<K>::kParts;
+    const uint32_t l = threadIdx.x % 64, i = l % 16, q = l / 16;
+    Frag<K> f;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      s4 half[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t k = k0 + 8 * q + 4 * e + i / 4;
+        half[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (local<s4>*)(m + chunk_at(k, (block / 2 * 4 + i % 4) * P + p) + block % 2 * 8));
+      }
+      f.part[p] = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    return f;
+  }
+};
+
+// Waves: four for 64 x 64, eight for 128 x 128, so that one's products cover another's reads.
+template <int D>
+using SmallShape = Shape<D, D, D / 2, D == 128 ? D / 4 : D / 2, 2>;
+
+template <typename T, typename Out, typename K, int D>
+__global__ void __launch_bounds__(SmallShape<D>::kLanes) small_kernel(SmallArgs p) {
+  typedef Resident<K, D> R;
+  typedef SmallShape<D> S;
+  constexpr bool kFast = Kind<K>::kParts == 1;
+  __shared__ __attribute__((aligned(1024))) char lds[R::kSize * (kFast ? 3 : 2)];
+  local<char>* x = (local<char>*)lds;
+  local<char>* a = x + R::kSize;
+  local<char>* low = kFast ? a + R::kSize : nullptr;
+  const uint32_t matrix = blockIdx.x, wave = threadIdx.x / 64;
+  const int blockA = wave / S::kWavesN * S::MI, blockB = wave % S::kWavesN * S::NI;
+  const bool tall = p.rows > p.cols;
+  {   // X = x / (|x| + eps), groups of 8 along x's rows
+    const T* from = (const T*)p.x.p + matrix * p.x.matrix;
+    constexpr int kGroups = D * D / 8 / S::kLanes;
+    f8 v[kGroups];
+    double sum = 0.0;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      const uint32_t at = g * S::kLanes + threadIdx.x, row = at / (D / 8), col = at % (D / 8) * 8;
+      v[g] = f8{};
+      if (row < p.rows) v[g] = load8(from + row * p.x.stride, col, p.cols);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum = __builtin_fma((double)v[g][e], (double)v[g][e], sum);
+    }
+    const double by = (double)(1 << kStored) / (__builtin_sqrt(block_sum<S::kLanes>(sum)) + p.eps);
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      const uint32_t at = g * S::kLanes + threadIdx.x, row = at / (D / 8), col = at % (D / 8) * 8;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[g][e] = (float)((double)v[g][e] * by);
+      if (!tall) {
+        R::put(x, low, row, col, v[g]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          fp16_t h, l;
+          split(v[g][e], h, l);
+          const uint32_t c = row / 8 * Kind<K>::kParts, in = row % 8 * 2;
+          *(local<fp16_t>*)(x + R::chunk_at(col + e, c) + in) = h;
+          *(local<fp16_t>*)((kFast ? low : x) + R::chunk_at(col + e, kFast ? c : c + 1) + in) = l;
+        }
+      }
+    }
+  }
+  // acc += the product with the second matrix's rows, or (TURNED) its columns, of what is `first` along k
+  Acc<S> acc;
+  const auto multiply = [&](const local<char>* first, const local<char>* second, auto turned) {
+    constexpr bool kTurned = decltype(turned)::value;
+#pragma unroll
+    for (int t = 0; t < R::kBlocks; ++t) {
+#pragma unroll
+      for (int sub = 0; sub < Kind<K>::kSubs; ++sub) {
+        Frag<K> fa[S::MI], fb[S::NI];
+#pragma unroll
+        for (int j = 0; j < S::NI; ++j) {
+          if constexpr (kTurned)
+            fb[j] = R::turned(second, blockB + j, (t * Kind<K>::kSubs + sub) * 32);
+          else
+            fb[j] = read_frag<K, D, false>(second + t * R::kBlock, blockB + j, sub);
+        }
+#pragma unroll
+        for (int i = 0; i < S::MI; ++i) fa[i] = read_frag<K, D, false>(first + t * R::kBlock, blockA + i, sub);
+#pragma unroll
+        for (int i = 0; i < S::MI; ++i)
+#pragma unroll
+          for (int j = 0; j < S::NI; ++j) mma<K>(acc.v[i][j], fa[i], fb[j]);
+      }
+    }
+  };
+  const float one = __builtin_ldexpf(1.0f, -kStored);
+  const float square = p.c != 0.0f ? p.c : 0x1p-60f;   // as in run_step
+  for (uint32_t s = 0; s < p.steps; ++s) {
+    const bool adds = kFast && s + kPlainSteps < p.steps;
+    const int at = adds ? p.at_added : p.at_plain;
+    __syncthreads();
+    acc.clear();
+    multiply(x, x, std::false_type());
+    acc.each([&](uint32_t m, uint32_t n, f8 v) { R::put(a, nullptr, m, n, one * v); });
+    __syncthreads();
+    acc.start([&](uint32_t m, uint32_t n) {
+      return p.b / square * __builtin_ldexpf(1.0f, kStored) * R::get(a, nullptr, m, n);
+    });
+    multiply(a, a, std::false_type());
+    __syncthreads();
+    const float by = square * __builtin_ldexpf(1.0f, at - 2 * kStored);
+    const float diagonal = adds ? 0.0f : p.a * __builtin_ldexpf(1.0f, at);
+    acc.each([&](uint32_t m, uint32_t n, f8 v) {
+      v *= by;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (m == n + e) v[e] += diagonal;
+      R::put(a, nullptr, m, n, v);
+    });
+    __syncthreads();
+    if (adds)
+      acc.start([&](uint32_t m, uint32_t n) { return p.a * __builtin_ldexpf(1.0f, at) * R::get(x, low, m, n); });
+    else
+      acc.clear();
+    multiply(a, x, std::true_type());
+    const float down = __builtin_ldexpf(1.0f, -at);
+    if (s + 1 < p.steps) {
+      __syncthreads();
+      acc.each([&](uint32_t m, uint32_t n, f8 v) { R::put(x, low, m, n, down * v); });
+      continue;
+    }
+    const float scale = p.scale * down * one;
+    Out* out = (Out*)p.out + matrix * p.out_matrix;
+    const Out* base = (const Out*)p.base.p + matrix * p.base.matrix;
+    acc.each([&](uint32_t m, uint32_t n, f8 v) {
+      v *= scale;
+      if (!tall) {
+        if (m >= p.rows || n >= p.cols) return;
+        if (p.base.p) v += p.keep * load8(base + m * p.base.stride, n, p.cols);
+        store8<Out>(out + m * p.out_stride, n, p.cols, v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (n + e >= p.rows || m >= p.cols) continue;
+          float w = v[e];
+          if (p.base.p) w += p.keep * (float)gp(base)[(n + e) * p.base.stride + m];
+          gp(out)[(n + e) * p.out_stride + m] = (Out)w;
+        }
+      }
+    });
+  }
+}
+
 struct Plan {
   uint32_t batch, rows, cols, side, other;   // side: of the symmetric matrices
   uint32_t sums;                             // parts of a matrix's sum of squares
@@ -383,10 +587,9 @@ struct Call {
   float a, b, c, eps, scale, keep;
 };
 
-constexpr uint32_t kFastSide = 64;
-constexpr int kPlainSteps = 2;   // the last fast steps, whose X has no second part
-
 bool fast(const Plan& p, int out_type) { return out_type == EC_BF16 && p.side >= kFastSide; }
+
+bool small(uint64_t rows, uint64_t cols) { return std::max(rows, cols) <= kSmallSide; }
 
 // A matrix of K in the workspace, the bytes of one of the batch, and those to its second parts.
 struct Stored {
@@ -403,6 +606,13 @@ Stored stored(char* at, uint32_t batch, uint32_t rows, uint32_t cols, bool low) 
   return s;
 }
 
+int stored_at(const Call& c, bool adds) {
+  const float most = (adds ? 0.0f : std::fabs(c.a)) + 2.0f * std::fabs(c.b) + 4.0f * std::fabs(c.c);
+  int at = kStored;
+  while (at > 0 && std::ldexp(most, at) > 32768.0f) --at;
+  return at;
+}
+
 // Step s: the next step's X, or the result.
 template <bool TALL, typename In>
 int run_step(const Plan& p, const Call& c, char* work, int s, hipStream_t st) {
@@ -413,9 +623,7 @@ int run_step(const Plan& p, const Call& c, char* work, int s, hipStream_t st) {
   const Stored gram = stored<In>(work + p.gram, p.batch, p.side, p.side, false);
   const Stored poly = stored<In>(work + p.poly, p.batch, p.side, p.side, false);
   // stored times 2^at so that (a I +) b A + c A A stays below fp16's largest value
-  const float most = (adds ? 0.0f : std::fabs(c.a)) + 2.0f * std::fabs(c.b) + 4.0f * std::fabs(c.c);
-  int at = kStored;
-  while (at > 0 && std::ldexp(most, at) > 32768.0f) --at;
+  const int at = stored_at(c, adds);
 
   NsArgs n = {};
   n.a = n.b = x.m;
@@ -473,6 +681,20 @@ int run_steps(const Plan& p, const Call& c, char* work, hipStream_t st) {
   return EC_OK;
 }
 
+template <typename T, typename Out, typename K>
+void run_small(const Plan& p, const Call& c, hipStream_t st) {
+  SmallArgs a = {};
+  a.x = c.x, a.base = c.base;
+  a.out = c.out, a.out_stride = c.out_stride, a.out_matrix = c.out_matrix;
+  a.rows = p.rows, a.cols = p.cols, a.steps = (uint32_t)c.steps;
+  a.a = c.a, a.b = c.b, a.c = c.c, a.scale = c.scale, a.keep = c.keep, a.eps = (double)c.eps;
+  a.at_added = stored_at(c, true), a.at_plain = stored_at(c, false);
+  if (p.other <= kSmallSide / 2)
+    small_kernel<T, Out, K, kSmallSide / 2><<<p.batch, SmallShape<kSmallSide / 2>::kLanes, 0, st>>>(a);
+  else
+    small_kernel<T, Out, K, kSmallSide><<<p.batch, SmallShape<kSmallSide>::kLanes, 0, st>>>(a);
+}
+
 }  // namespace
 }  // namespace ec
 
@@ -481,7 +703,7 @@ using namespace ec;
 extern "C" {
 
 uint64_t ec_orthogonalize_workspace(uint64_t batch, uint64_t rows, uint64_t cols) {
-  if (!batch || check_sizes(batch, rows, cols) != EC_OK) return 0;
+  if (!batch || check_sizes(batch, rows, cols) != EC_OK || small(rows, cols)) return 0;
   return plan_of((uint32_t)batch, (uint32_t)rows, (uint32_t)cols).total;
 }
 
@@ -500,10 +722,34 @@ int ec_orthogonalize(const void* d_x, int type, uint64_t batch, uint64_t rows, u
   if (!batch) return EC_OK;
   if (!d_x || !d_out) return EC_EINVAL;
   const Plan p = plan_of((uint32_t)batch, (uint32_t)rows, (uint32_t)cols);
-  if (!d_work || work_bytes < p.total) return EC_EINVAL;
+  if (!small(rows, cols) && (!d_work || work_bytes < p.total)) return EC_EINVAL;
   if ((uintptr_t)d_work & 15u) return EC_EALIGN;
   char* work = (char*)d_work;
   const auto st = (hipStream_t)stream;
+  Call c = {};
+  c.x = {(const char*)d_x, x_stride, x_matrix};
+  c.base = {(const char*)d_base, base_stride, base_matrix};
+  c.out = (char*)d_out, c.out_stride = out_stride, c.out_matrix = out_matrix;
+  c.out_type = out_type, c.steps = steps;
+  c.a = coefficients[0], c.b = coefficients[1], c.c = coefficients[2];
+  c.eps = eps, c.scale = scale, c.keep = keep;
+  if (small(rows, cols)) {
+    with_type(type, [&](auto t) {
+      return with_type(out_type, [&](auto o) {
+        typedef decltype(t) T;
+        typedef decltype(o) Out;
+        if constexpr (__is_same(Out, bf16_t)) {
+          if (fast(p, out_type)) {
+            run_small<T, Out, fp16_t>(p, c, st);
+            return EC_OK;
+          }
+        }
+        run_small<T, Out, pair_t>(p, c, st);
+        return EC_OK;
+      });
+    });
+    return launched();
+  }
   // rows without gaps are summed as one
   const bool dense = x_stride == cols;
   const uint64_t total = rows * cols;
@@ -526,12 +772,6 @@ int ec_orthogonalize(const void* d_x, int type, uint64_t batch, uint64_t rows, u
     }
     return EC_OK;
   });
-  Call c = {};
-  c.base = {(const char*)d_base, base_stride, base_matrix};
-  c.out = (char*)d_out, c.out_stride = out_stride, c.out_matrix = out_matrix;
-  c.out_type = out_type, c.steps = steps;
-  c.a = coefficients[0], c.b = coefficients[1], c.c = coefficients[2];
-  c.scale = scale, c.keep = keep;
   const int e = rows > cols ? run_steps<true>(p, c, work, st) : run_steps<false>(p, c, work, st);
   return e ? e : launched();
 }

@@ -58,16 +58,17 @@ def test_orthogonalize_refusals(pkg):
     L, ok, inval, big, align = _codes(pkg)
     abc = (ctypes.c_float * 3)(3.4445, -4.775, 2.0315)
 
-    def call(x=P, kind=1, batch=2, rows=30, cols=50, xs=50, xm=1500, steps=5, coef=abc, eps=1e-7, scale=1.0, base=None, bs=0,
-             bm=0, keep=1.0, out=P, okind=0, os=50, om=1500, work=P, have=1 << 24):
+    def call(x=P, kind=1, batch=2, rows=130, cols=150, xs=150, xm=19500, steps=5, coef=abc, eps=1e-7, scale=1.0, base=None,
+             bs=0, bm=0, keep=1.0, out=P, okind=0, os=150, om=19500, work=P, have=1 << 28):
         return L.ec_orthogonalize(x, kind, batch, rows, cols, xs, xm, steps, coef, eps, scale, base, bs, bm, keep, out, okind,
                                   os, om, work, have, None)
 
     assert call(batch=0) == ok and call(batch=0, x=None, out=None, work=None) == ok
-    need = L.ec_orthogonalize_workspace(2, 30, 50)
-    assert need >= 2 * (2 * 2 * 30 * 56 + 2 * 2 * 30 * 32)
-    for bad in (dict(x=None), dict(out=None), dict(kind=4), dict(okind=-1), dict(rows=0), dict(cols=0), dict(xs=49), dict(os=49),
-                dict(base=P, bs=49), dict(eps=0.0), dict(eps=NAN), dict(eps=INF), dict(scale=INF), dict(keep=NAN), dict(coef=None),
+    need = L.ec_orthogonalize_workspace(2, 130, 150)
+    assert need >= 2 * 4 * (2 * 130 * 152 + 2 * 130 * 136)
+    assert L.ec_orthogonalize_workspace(2, 128, 128) == 0   # small ones need none
+    for bad in (dict(x=None), dict(out=None), dict(kind=4), dict(okind=-1), dict(rows=0), dict(cols=0), dict(xs=149), dict(os=149),
+                dict(base=P, bs=149), dict(eps=0.0), dict(eps=NAN), dict(eps=INF), dict(scale=INF), dict(keep=NAN), dict(coef=None),
                 dict(coef=(ctypes.c_float * 3)(1, NAN, 0)), dict(coef=(ctypes.c_float * 3)(1, 1025, 0)), dict(work=None),
                 dict(have=need - 1)):
         assert call(**bad) == inval, bad
