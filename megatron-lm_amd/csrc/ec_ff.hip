@@ -74,7 +74,7 @@ struct FfArgs {
 };
 
 template <class S, typename T>
-__global__ void __launch_bounds__(S::kLanes) ff_part_kernel(FfArgs p) {
+__global__ void __launch_bounds__(S::kLanes, S::kPerSimd) ff_part_kernel(FfArgs p) {
   __shared__ __attribute__((aligned(1024))) char lds[S::kLds];
   const uint32_t tiles = p.tiles_m * p.tiles_n, t = xcd_order(blockIdx.x, gridDim.x), split = uniform(t / tiles);
   uint32_t tm, tn;
@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(S::kLanes) ff_part_kernel(FfArgs p) {
 }
 
 template <class S, typename T, bool GRAD, bool JOIN>
-__global__ void __launch_bounds__(S::kLanes) ff_kernel(FfArgs p) {
+__global__ void __launch_bounds__(S::kLanes, S::kPerSimd) ff_kernel(FfArgs p) {
   __shared__ __attribute__((aligned(1024))) char lds[JOIN ? 16 : S::kLds];
   const uint32_t t = xcd_order(blockIdx.x, gridDim.x);
   uint32_t tm, tn;
@@ -279,7 +279,7 @@ __device__ __forceinline__ void sum_products(Acc<S>& acc, local<char>* lds, cons
 }
 
 template <class S, typename T, bool ACROSS_A>
-__global__ void __launch_bounds__(S::kLanes) sum_part_kernel(SumArgs p) {
+__global__ void __launch_bounds__(S::kLanes, S::kPerSimd) sum_part_kernel(SumArgs p) {
   __shared__ __attribute__((aligned(1024))) char lds[S::kLds];
   const uint32_t tiles = p.tiles_m * p.tiles_n, t = xcd_order(blockIdx.x, gridDim.x), split = uniform(t / tiles);
   uint32_t tm, tn;
@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(S::kLanes) sum_part_kernel(SumArgs p) {
 }
 
 template <class S, typename T, typename O, bool ACROSS_A, bool ACCUMULATE, bool JOIN>
-__global__ void __launch_bounds__(S::kLanes) sum_kernel(SumArgs p) {
+__global__ void __launch_bounds__(S::kLanes, S::kPerSimd) sum_kernel(SumArgs p) {
   __shared__ __attribute__((aligned(1024))) char lds[JOIN ? 16 : S::kLds];
   const uint32_t t = xcd_order(blockIdx.x, gridDim.x);
   uint32_t tm, tn;
@@ -421,7 +421,7 @@ void run_ff(FfArgs& p, char* parts, hipStream_t st) {
   const Choice c = choose_ff<T>(p.n, p.width, p.inner);
   p.splits = c.splits;
   p.splits.parts = (float*)parts;
-  with_shape<Flat>(c, [&](auto s) {
+  with_shape<T, Flat>(c, [&](auto s) {
     typedef decltype(s) S;
     p.tiles_m = (p.n + S::BM - 1) / S::BM;
     p.tiles_n = (p.inner + S::BN / 2 - 1) / (S::BN / 2);
@@ -440,7 +440,7 @@ void run_sum(SumArgs& p, uint32_t outs, char* parts, hipStream_t st) {
   const Choice c = choose_sum<T>(p.M, p.N, p.K, std::max(1u, p.parts), outs);
   p.splits = c.splits;
   p.splits.parts = (float*)parts;
-  with_shape<Small>(c, [&](auto s) {
+  with_shape<T, Small>(c, [&](auto s) {
     typedef decltype(s) S;
     p.tiles_m = (p.M + S::BM - 1) / S::BM;
     p.tiles_n = (p.N + S::BN - 1) / S::BN;

@@ -19,7 +19,10 @@
 //
 // Pairs: a value as the sum of two fp16 ones, 22 bits of significand: eight high parts, then the
 // eight low parts, in 32 bytes.  A product of two pairs takes three of the matrix cores' products
-// (the low parts' is below the fp32 accumulator's rounding), at 3/16 of the time of fp32 products.
+// (the low parts' is below the fp32 accumulator's rounding), at 3/16 of the time of fp32 products.  The matrix
+// cores truncate where they add to an accumulator, so the two small products have accumulators of their own, which
+// are added at the end: five Newton-Schulz steps on 1001 x 777 are 3.5e-6 off with one accumulator, 2.1e-6 with two, and
+// those of fp32 products 2.3e-6.
 #pragma once
 
 #include <algorithm>
@@ -80,13 +83,17 @@ __device__ __forceinline__ void mma(f4& acc, const Frag<T>& a, const Frag<T>& b)
     const f4 x = __builtin_bit_cast(f4, a.part[0]), y = __builtin_bit_cast(f4, b.part[0]);
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(y[e], x[e], acc, 0, 0, 0);
-  } else {
-    const h8 ah = __builtin_bit_cast(h8, a.part[0]), al = __builtin_bit_cast(h8, a.part[1]);
-    const h8 bh = __builtin_bit_cast(h8, b.part[0]), bl = __builtin_bit_cast(h8, b.part[1]);
-    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(bl, ah, acc, 0, 0, 0);
-    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(bh, al, acc, 0, 0, 0);
-    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(bh, ah, acc, 0, 0, 0);
   }
+}
+
+// The same of pairs: what the high parts give, and the rest.
+__device__ __forceinline__ void mma_pairs(f4& acc, f4& rest, const Frag<pair_t>& a, const Frag<pair_t>& b) {
+  typedef fp16_t __attribute__((ext_vector_type(8))) h8;
+  const h8 ah = __builtin_bit_cast(h8, a.part[0]), al = __builtin_bit_cast(h8, a.part[1]);
+  const h8 bh = __builtin_bit_cast(h8, b.part[0]), bl = __builtin_bit_cast(h8, b.part[1]);
+  rest = __builtin_amdgcn_mfma_f32_16x16x32_f16(bl, ah, rest, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(bh, ah, acc, 0, 0, 0);
+  rest = __builtin_amdgcn_mfma_f32_16x16x32_f16(bh, al, rest, 0, 0, 0);
 }
 
 // Which of a wave's 32 rows fragment h (0, 1) of a pair of fragments holds in lane i of 16:
@@ -269,6 +276,7 @@ struct Shape {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, kStages = STAGES_;
   static constexpr int kWavesN = BN / WN, kWaves = (BM / WM) * kWavesN, kLanes = kWaves * 64;
   static constexpr int MI = WM / 16, NI = WN / 16;
+  static constexpr int kPerSimd = 2;   // waves, at least
   static constexpr int kStage = (BM + BN) * kRowBytes, kLds = kStages * kStage;
 };
 
@@ -286,6 +294,13 @@ struct Acc {
     for (int i = 0; i < S::MI; ++i)
 #pragma unroll
       for (int j = 0; j < S::NI; ++j) v[i][j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  __device__ __forceinline__ void add(const Acc& x) {
+#pragma unroll
+    for (int i = 0; i < S::MI; ++i)
+#pragma unroll
+      for (int j = 0; j < S::NI; ++j) v[i][j] += x.v[i][j];
   }
 
   // f(m, n, values): row m and columns n ... n + 7 of the tile.
@@ -384,13 +399,19 @@ struct Groups {
       a[g & 1][i] = read_frag<T, S::BM, ACROSS_A>(tile, blockA + at * kRows + i, sub);
   }
 
-  // acc += A B for group g, with between(i) behind each row of products.
+  // acc += A B for group g (of pairs acc + rest), with between(i) behind each row of products.
   template <typename F>
-  __device__ __forceinline__ void multiply(Acc<S>& acc, int g, int turn, F between) const {
+  __device__ __forceinline__ void multiply(Acc<S>& acc, Acc<S>& rest, int g, int turn, F between) const {
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
+      const int r = g % kParts * kRows + i;
 #pragma unroll
-      for (int j = 0; j < S::NI; ++j) mma<T>(acc.v[g % kParts * kRows + i][j], a[g & 1][i], b[turn][j]);
+      for (int j = 0; j < S::NI; ++j) {
+        if constexpr (Kind<T>::kParts == 2)
+          mma_pairs(acc.v[r][j], rest.v[r][j], a[g & 1][i], b[turn][j]);
+        else
+          mma<T>(acc.v[r][j], a[g & 1][i], b[turn][j]);
+      }
       between(i);
     }
   }
@@ -420,6 +441,8 @@ __device__ __forceinline__ void product(Acc<S>& acc, local<char>* lds, const Ope
   const uint32_t at = lds_address(lds);
   G g;
   g.blockA = wave / S::kWavesN * S::MI, g.blockB = wave % S::kWavesN * S::NI;
+  Acc<S> rest;   // of pairs
+  if (Kind<T>::kParts == 2) rest.clear();
   // loads of the stages behind the one that is waited for
   constexpr int kLater = (S::kStages - 2) * (LoadA::kLoads + LoadB::kLoads);
   uint32_t here = 0;   // the step's place in LDS
@@ -432,7 +455,7 @@ __device__ __forceinline__ void product(Acc<S>& acc, local<char>* lds, const Ope
       if (i + 1 < G::kGroups) {
         g.read(lds + here, i + 1, turn(i + 1));
         keep_order();
-        g.multiply(acc, i, turn(i), [](int) {});
+        g.multiply(acc, rest, i, turn(i), [](int) {});
         keep_order();
       } else {
         stage_barrier<kLater>();
@@ -441,7 +464,7 @@ __device__ __forceinline__ void product(Acc<S>& acc, local<char>* lds, const Ope
         la.begin(at + here);
         lb.begin(at + here + S::BM * kRowBytes);
         constexpr int kAll = LoadA::kLoads + LoadB::kLoads, kEach = (kAll + G::kRows - 1) / G::kRows;
-        g.multiply(acc, i, turn(i), [&](int row) {
+        g.multiply(acc, rest, i, turn(i), [&](int row) {
 #pragma unroll
           for (int l = row * kEach; l < (row + 1) * kEach && l < kAll; ++l) {
             if (l < LoadA::kLoads)
@@ -469,6 +492,7 @@ __device__ __forceinline__ void product(Acc<S>& acc, local<char>* lds, const Ope
       if (++s < steps) one_step(1);
     }
   }
+  if (Kind<T>::kParts == 2) acc.add(rest);
   loads_done();   // none to LDS is under way when the workgroup gives it back
 }
 
@@ -553,7 +577,7 @@ inline uint64_t tiles_of(uint64_t m, uint64_t n, uint64_t bm, uint64_t bn) {
 template <class S, typename T>
 constexpr uint64_t step_ns() {
   constexpr int at = __is_same(S, Large) ? 0 : __is_same(S, Middle) ? 1 : __is_same(S, Flat) ? 2 : 3;
-  constexpr uint64_t narrow[] = {1470, 610, 400, 260}, pairs[] = {2400, 720, 400, 250}, wide[] = {6800, 1720, 880, 450};
+  constexpr uint64_t narrow[] = {1470, 610, 400, 260}, pairs[] = {0, 720, 400, 250}, wide[] = {6800, 1720, 880, 450};
   return __is_same(T, float) ? wide[at] : __is_same(T, pair_t) ? pairs[at] : narrow[at];
 }
 template <class S>
@@ -592,20 +616,19 @@ Choice choose(F tiles, uint64_t steps, bool may_split = true) {
       if (ns < best.ns) best = {shape, {(uint32_t)real, (uint32_t)each, nullptr}, bytes, ns};
     }
   };
-  consider(Large(), 0);
+  if constexpr (!__is_same(T, pair_t)) consider(Large(), 0);   // pairs' accumulators would not fit
   consider(Middle(), 1);
   consider(Least(), 2);
   return best;
 }
 
-template <class Least, typename G>
+template <typename T, class Least, typename G>
 void with_shape(const Choice& c, G f) {
-  if (c.shape == 0)
-    f(Large());
-  else if (c.shape == 1)
-    f(Middle());
-  else
-    f(Least());
+  if constexpr (!__is_same(T, pair_t)) {
+    if (c.shape == 0) return f(Large());
+  }
+  if (c.shape == 1) return f(Middle());
+  return f(Least());
 }
 
 template <typename T>

@@ -187,7 +187,7 @@ __device__ __forceinline__ void upper_tile_at(uint32_t t, uint32_t& tm, uint32_t
 
 // A split of A's product.
 template <class S, typename In, bool ACROSS>
-__global__ void __launch_bounds__(S::kLanes) gram_part_kernel(NsArgs p) {
+__global__ void __launch_bounds__(S::kLanes, S::kPerSimd) gram_part_kernel(NsArgs p) {
   __shared__ __attribute__((aligned(1024))) char lds[S::kLds];
   const uint32_t t = xcd_order(blockIdx.x, gridDim.x), all = gridDim.x / p.splits.n, split = uniform(t / all);
   const uint32_t matrix = uniform(t % all / p.tiles);
@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(S::kLanes) gram_part_kernel(NsArgs p) {
 }
 
 template <class S, typename In, bool ACROSS_A, bool ACROSS_B, int WHAT, typename Out, bool JOIN>
-__global__ void __launch_bounds__(S::kLanes) ns_kernel(NsArgs p) {
+__global__ void __launch_bounds__(S::kLanes, S::kPerSimd) ns_kernel(NsArgs p) {
   __shared__ __attribute__((aligned(1024))) char lds[JOIN ? S::kWaves * kTurn * 4 : S::kLds];
   const uint32_t t = xcd_order(blockIdx.x, gridDim.x), matrix = uniform(t / p.tiles);
   uint32_t tm, tn;
@@ -324,7 +324,7 @@ int run_ns(NsArgs& p, uint32_t batch, char* parts, hipStream_t st) {
   const Choice c = choose_ns<In>(p.M, p.N, p.K, batch, WHAT);
   p.splits = c.splits;
   p.splits.parts = (float*)parts;
-  with_shape<Small>(c, [&](auto s) {
+  with_shape<In, Small>(c, [&](auto s) {
     typedef decltype(s) S;
     p.tiles_m = (p.M + S::BM - 1) / S::BM;
     p.tiles_n = (p.N + S::BN - 1) / S::BN;
@@ -467,6 +467,8 @@ __global__ void __launch_bounds__(SmallShape<D>::kLanes) small_kernel(SmallArgs 
   Acc<S> acc;
   const auto multiply = [&](const local<char>* first, const local<char>* second, auto turned) {
     constexpr bool kTurned = decltype(turned)::value;
+    Acc<S> rest;   // of pairs
+    if (!kFast) rest.clear();
 #pragma unroll
     for (int t = 0; t < R::kBlocks; ++t) {
 #pragma unroll
@@ -484,9 +486,15 @@ __global__ void __launch_bounds__(SmallShape<D>::kLanes) small_kernel(SmallArgs 
 #pragma unroll
         for (int i = 0; i < S::MI; ++i)
 #pragma unroll
-          for (int j = 0; j < S::NI; ++j) mma<K>(acc.v[i][j], fa[i], fb[j]);
+          for (int j = 0; j < S::NI; ++j) {
+            if constexpr (kFast)
+              mma<K>(acc.v[i][j], fa[i], fb[j]);
+            else
+              mma_pairs(acc.v[i][j], rest.v[i][j], fa[i], fb[j]);
+          }
       }
     }
+    if (!kFast) acc.add(rest);
   };
   const float one = __builtin_ldexpf(1.0f, -kStored);
   const float square = p.c != 0.0f ? p.c : 0x1p-60f;   // as in run_step
