@@ -203,6 +203,61 @@ struct GradArgs {
   uint64_t teams, per_gate, rows;   // teams for a row of the gate; rows of a team
 };
 
+// A lane's sums over rows, of V groups: in registers, or for the longest rows in LDS, four neighbours at a time so that
+// lanes meet no bank conflicts.
+template <typename T, int R, int V, bool LDS>
+struct Sums {
+  typedef Row<T, R, V> row_t;
+  row_t r;
+  float* at;
+
+  __device__ __forceinline__ void clear(float* lds) {
+    at = lds + threadIdx.x * 4;
+    fill();
+  }
+  __device__ __forceinline__ void fill() {
+    if constexpr (LDS) {
+#pragma unroll
+      for (int i = 0; i < V * row_t::kN / 4; ++i) *(v4*)(at + i * R * 4) = v4{0.0f, 0.0f, 0.0f, 0.0f};
+    } else {
+      r.fill(0.0f);
+    }
+  }
+  // += f(v, e)
+  template <typename F>
+  __device__ __forceinline__ void add(F f) {
+    if constexpr (LDS) {
+#pragma unroll
+      for (int i = 0; i < V * row_t::kN / 4; ++i) {
+        v4 s = *(v4*)(at + i * R * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] += f(i * 4 / row_t::kN, i * 4 % row_t::kN + e);
+        *(v4*)(at + i * R * 4) = s;
+      }
+    } else {
+      row_t::each([&](int v, int e) { r.x[v][e] += f(v, e); });
+    }
+  }
+  __device__ __forceinline__ void store(float* to, uint32_t width) {
+    if constexpr (LDS) {
+#pragma unroll
+      for (int i = 0; i < V * row_t::kN / 4; ++i) {
+        const v4 s = *(v4*)(at + i * R * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t c = row_t::at(i * 4 / row_t::kN) + i * 4 % row_t::kN + e;
+          if (c < width) gp(to)[c] = s[e];
+        }
+      }
+    } else {
+      r.template store<float, false>(to, width);
+    }
+  }
+
+ private:
+  typedef float v4 __attribute__((ext_vector_type(4)));
+};
+
 // The rows of a team: a part of those of one row of the gate, or those of some.
 template <typename T, int R, int V>
 __global__ void __launch_bounds__(block_lanes<R>()) norm_grad_kernel(GradArgs p) {
@@ -214,11 +269,15 @@ __global__ void __launch_bounds__(block_lanes<R>()) norm_grad_kernel(GradArgs p)
                                     : team * p.rows;
   const uint64_t past = p.per_gate ? (team / p.per_gate + 1) * p.gate_share : p.n;
   const uint64_t last = min(min(first + p.rows, past), p.n);
-  row_t dweight, dbranch_weight, dgate, w, bw, gate;
-  dweight.fill(0.0f), dbranch_weight.fill(0.0f), dgate.fill(0.0f);
+  row_t w, bw, gate;
   w.fill(0.0f), bw.fill(1.0f), gate.fill(1.0f);
-  // the longest rows' factors are read again for each row, for want of registers
-  constexpr bool kKeep = R * V * row_t::kN <= 8192;
+  // the longest rows' factors are read again for each row, and two of their sums are in LDS, for want of registers (2048 x
+  // 16384 bf16 186 us, 333 with all in registers, which spills)
+  constexpr bool kKeep = R < 1024 || V == 1, kLong = R == 1024 && V * row_t::kN > 8;
+  __shared__ float long_sums[kLong ? 2 * R * V * row_t::kN : 1];
+  Sums<T, R, V, kLong> dbranch_weight, dgate;
+  Sums<T, R, V, false> dweight;
+  dbranch_weight.clear(long_sums), dgate.clear(long_sums + (kLong ? R * V * row_t::kN : 0)), dweight.clear(nullptr);
   const auto factors = [&](row_t& to, const void* from) {
     if (from) to.template load<false>((const T*)from, p.width);
   };
@@ -230,9 +289,12 @@ __global__ void __launch_bounds__(block_lanes<R>()) norm_grad_kernel(GradArgs p)
   int turn = 0;
   // the next row's values are under way while a row is summed
   Raw<T, V> d_raw = {}, y_raw = {}, z_raw = {}, x_raw = {};
+  const auto branch_of = [&](uint64_t row) {
+    return row_t::template fetch<true>((const T*)p.branch + row * p.branch_stride, p.width);
+  };
   const auto fetch = [&](uint64_t row) {
     if (p.dsum) d_raw = row_t::template fetch<true>((const T*)p.dsum + row * p.dsum_stride, p.width);
-    if (p.branch) y_raw = row_t::template fetch<true>((const T*)p.branch + row * p.branch_stride, p.width);
+    if (p.branch && !kLong) y_raw = branch_of(row);
     if (p.weight) {
       z_raw = row_t::template fetch<true>((const T*)p.dnormed + row * p.dnormed_stride, p.width);
       x_raw = row_t::template fetch<true>((const T*)p.sum + row * p.sum_stride, p.width);
@@ -245,7 +307,8 @@ __global__ void __launch_bounds__(block_lanes<R>()) norm_grad_kernel(GradArgs p)
     if (p.gate && kKeep && (row == first || row % p.gate_share == 0))
       factors(gate, (const T*)p.gate + row / p.gate_share * p.width);
     row_t d, y, dz, x;
-    d.take(d_raw), y.take(y_raw), dz.take(z_raw), x.take(x_raw);
+    d.take(d_raw), dz.take(z_raw), x.take(x_raw);
+    if (!kLong) y.take(y_raw);
     if (kAhead && row + 1 < last) fetch(row + 1);
     if (p.weight) {
       const float root = gp(p.rstd)[row];
@@ -253,7 +316,7 @@ __global__ void __launch_bounds__(block_lanes<R>()) norm_grad_kernel(GradArgs p)
       if (!kKeep) factors(w, p.weight);
       row_t::each([&](int v, int e) {
         x.x[v][e] *= root;
-        dweight.x[v][e] = __builtin_fmaf(dz.x[v][e], x.x[v][e], dweight.x[v][e]);
+        dweight.r.x[v][e] = __builtin_fmaf(dz.x[v][e], x.x[v][e], dweight.r.x[v][e]);
         dz.x[v][e] *= w.x[v][e];
         s = __builtin_fmaf(dz.x[v][e], x.x[v][e], s);
       });
@@ -262,6 +325,7 @@ __global__ void __launch_bounds__(block_lanes<R>()) norm_grad_kernel(GradArgs p)
     }
     d.template store<T, false>((T*)p.dresidual + row * p.width, p.width);
     if (p.branch) {
+      if (kLong) y.take(branch_of(row));
       const float root = p.branch_weight ? gp(p.branch_rstd)[row] : 1.0f;
       float s = 0.0f;
       if (!kKeep) {
@@ -270,11 +334,13 @@ __global__ void __launch_bounds__(block_lanes<R>()) norm_grad_kernel(GradArgs p)
       }
       row_t::each([&](int v, int e) {
         y.x[v][e] *= root;
-        const float by = p.scale * d.x[v][e];
-        dgate.x[v][e] = __builtin_fmaf(by, y.x[v][e] * bw.x[v][e], dgate.x[v][e]);
-        const float g = by * gate.x[v][e];
-        dbranch_weight.x[v][e] = __builtin_fmaf(g, y.x[v][e], dbranch_weight.x[v][e]);
-        d.x[v][e] = g * bw.x[v][e];
+        d.x[v][e] *= p.scale;
+      });
+      if (p.gate_parts || p.dgate) dgate.add([&](int v, int e) { return d.x[v][e] * (y.x[v][e] * bw.x[v][e]); });
+      row_t::each([&](int v, int e) { d.x[v][e] *= gate.x[v][e]; });
+      if (p.branch_parts) dbranch_weight.add([&](int v, int e) { return d.x[v][e] * y.x[v][e]; });
+      row_t::each([&](int v, int e) {
+        d.x[v][e] *= bw.x[v][e];
         s = __builtin_fmaf(d.x[v][e], y.x[v][e], s);
       });
       if (p.branch_weight) {
@@ -283,15 +349,14 @@ __global__ void __launch_bounds__(block_lanes<R>()) norm_grad_kernel(GradArgs p)
       }
       d.template store<T, false>((T*)p.dbranch + row * p.width, p.width);
       if (p.dgate && (row + 1) % p.gate_share == 0) {
-        dgate.template store<float, false>(p.dgate + row / p.gate_share * p.width, p.width);
-        dgate.fill(0.0f);
+        dgate.store(p.dgate + row / p.gate_share * p.width, p.width);
+        dgate.fill();
       }
     }
   }
-  if (p.gate_parts) dgate.template store<float, false>(p.gate_parts + team * p.width, p.width);
-  if (p.branch_parts)
-    dbranch_weight.template store<float, false>(p.branch_parts + team * p.width, p.width);
-  if (p.weight_parts) dweight.template store<float, false>(p.weight_parts + team * p.width, p.width);
+  if (p.gate_parts) dgate.store(p.gate_parts + team * p.width, p.width);
+  if (p.branch_parts) dbranch_weight.store(p.branch_parts + team * p.width, p.width);
+  if (p.weight_parts) dweight.store(p.weight_parts + team * p.width, p.width);
 }
 
 // out[i] = the sum of `each` rows of parts from row i * each on, 64 columns a workgroup, 16 rows at a time.
