@@ -572,8 +572,10 @@ inline uint64_t tiles_of(uint64_t m, uint64_t n, uint64_t bm, uint64_t bn) {
   return (m + bm - 1) / bm * ((n + bn - 1) / bn);
 }
 
-// What a step takes a workgroup that has a CU for itself, and what a tile takes beside its steps, in ns as measured.
-// 16-bit products of small tiles are bound by what comes from L2 (64 bytes a clock and CU), others by the matrix cores.
+// What a step takes a CU full of such workgroups for each of them, and what a tile takes beside its steps, in ns as
+// measured. 16-bit products of small tiles are bound by what comes from L2 (64 bytes a clock and CU), others by the matrix
+// cores. A workgroup of four waves that has a CU for itself takes a quarter longer (2048 x 2048 pairs over 2048: 136
+// middle tiles 63 us, 528 small ones 49).
 template <class S, typename T>
 constexpr uint64_t step_ns() {
   constexpr int at = __is_same(S, Large) ? 0 : __is_same(S, Middle) ? 1 : __is_same(S, Flat) ? 2 : 3;
@@ -612,7 +614,8 @@ Choice choose(F tiles, uint64_t steps, bool may_split = true) {
       if (bytes > kMostPartBytes) break;
       const uint64_t turns = (n * real + kCus - 1) / kCus;
       const uint64_t join = real == 1 ? 0 : 4000 + std::max(bytes * 2 / 5500, (n + kCus - 1) / kCus * (bytes / n) / 35);
-      const uint64_t ns = turns * (each * step_ns<S, T>() + tile_ns<S>()) + join;
+      const uint64_t step = step_ns<S, T>() * (turns == 1 && S::kWaves == 4 ? 5 : 4) / 4;
+      const uint64_t ns = turns * (each * step + tile_ns<S>()) + join;
       if (ns < best.ns) best = {shape, {(uint32_t)real, (uint32_t)each, nullptr}, bytes, ns};
     }
   };

@@ -84,7 +84,8 @@ def test_a_block_in_a_step(pkg, dev, dtype):
     want.backward()
     # eight roundings of the chain's tensors, each half a step, in the mean square of many values
     near = 8 * (UNIT[dtype] if dtype != torch.float32 else 64 * E)
-    assert abs(float(got) - float(want)) <= near * abs(float(want))
+    got, want = float(got.detach()), float(want.detach())
+    assert abs(got - want) <= near * abs(want)
     for k, leaf in leaves.items():
         far = (leaf.grad.double().cpu() - exact[k].grad).norm() / exact[k].grad.norm()
         assert float(far) <= near, (k, float(far))
