@@ -477,8 +477,8 @@ int ec_grad_clip(const ec_grad_item* d_items, uint32_t n_items, float grad_scale
 
 /* Device memory that ec_gated_ff (grad 0) or ec_gated_ff_grad (grad 1) needs at d_work for these
  * operands, in bytes, 16-byte aligned: rows that are not 16-byte aligned, or not a multiple of 16 bytes long
- * or apart, are copied there first; the gradients of both projections lie there. 0 for operands
- * that the call refuses. */
+ * or apart, and weights whose strides differ, are copied there first; so do the gradients of both projections and
+ * partial sums. 0 for operands that the call refuses. */
 uint64_t ec_gated_ff_workspace(const void* d_x, uint64_t x_stride, const void* d_gate,
                                uint64_t gate_stride, const void* d_up, uint64_t up_stride, int type,
                                uint64_t n, uint32_t width, uint32_t inner, int grad);
@@ -486,7 +486,8 @@ uint64_t ec_gated_ff_workspace(const void* d_x, uint64_t x_stride, const void* d
 /* h[i][f] = act(g) * u, g = SUM_k x[i][k] gate[f][k] and u = SUM_k x[i][k] up[f][k], for n
  * rows x of `width` and weights [inner][width], all of `type` (the weights may be the halves of
  * one buffer). The sums and the activation are in fp32, on the matrix cores; h is rounded once.
- * EC_ERANGE for n >= 2^31, width or inner > 2^19, or a launch of 2^32 lanes. */
+ * EC_ERANGE for n >= 2^31, width or inner > 2^19, or 2^23 tiles of 128 x 128 (of h with its two projections, of x, or of both
+ * weights): launches of 2^32 lanes. */
 int ec_gated_ff(const void* d_x, uint64_t x_stride, const void* d_gate, uint64_t gate_stride,
                 const void* d_up, uint64_t up_stride, int type, uint64_t n, uint32_t width,
                 uint32_t inner, int activation, void* d_h, uint64_t h_stride, void* d_work,

@@ -369,8 +369,12 @@ FfWork ff_work(const FfCall& c, bool grad) {
   };
   if (!grad && c.n <= kFewForward) return w;   // read as they are
   if (!readable(c.x, c.width, c.x_stride, b)) w.x = take(c.n * row);
-  if (!readable(c.w_gate, c.width, c.gate_stride, b)) w.w_gate = take(c.inner * row);
-  if (!readable(c.w_up, c.width, c.up_stride, b)) w.w_up = take(c.inner * row);
+  // the two weights are read in turns, so their rows have to be equally far apart
+  if (c.gate_stride != c.up_stride || !readable(c.w_gate, c.width, c.gate_stride, b) ||
+      !readable(c.w_up, c.width, c.up_stride, b)) {
+    w.w_gate = take(c.inner * row);
+    w.w_up = take(c.inner * row);
+  }
   if (grad) {
     w.low = c.type != EC_F32 && c.n <= kFewRows;
     w.d = take(c.n * 2 * up_to(c.inner, 8) * b * low_parts(w));
@@ -460,8 +464,12 @@ int check_call(const FfCall& c, int act) {
   if (c.x_stride < c.width || c.gate_stride < c.width || c.up_stride < c.width) return EC_EINVAL;
   if (!c.w_gate || !c.w_up || (c.n && !c.x)) return EC_EINVAL;
   if (c.n >= 1ull << 31 || c.width > kMostWidth || c.inner > kMostWidth) return EC_ERANGE;
-  // a launch takes less than 2^32 lanes
-  if (tiles_of(c.n, 2ull * c.inner, Middle::BM, Middle::BN) >= (1ull << 32) / Middle::kLanes) return EC_ERANGE;
+  // a launch takes less than 2^32 lanes, whichever tiles are chosen
+  constexpr uint64_t kMostTiles = 1u << 23;
+  if (tiles_of(c.n, 2ull * c.inner, Middle::BM, Middle::BN) >= kMostTiles ||
+      tiles_of(c.n, c.width, Middle::BM, Middle::BN) >= kMostTiles ||
+      2 * tiles_of(c.inner, c.width, Middle::BM, Middle::BN) >= kMostTiles)
+    return EC_ERANGE;
   return EC_OK;
 }
 

@@ -171,7 +171,7 @@ __device__ __forceinline__ void to_lds(uint32_t lds, uint32_t offset, const i4& 
 __device__ __forceinline__ uint32_t lds_address(const local<char>* p) { return (uint32_t)(uintptr_t)p; }
 
 // Brings the ROWS rows of an operand's tile to LDS step by step.  DUAL: 32 rows of a first operand,
-// 32 of a second one, and so on.
+// 32 of a second one, and so on; both with the same number of rows, equally far apart.
 template <typename T, int ROWS, int WAVES, bool ACROSS, bool DUAL>
 struct Loader {
   static_assert(!(ACROSS && DUAL), "only operands along k are taken in turns");

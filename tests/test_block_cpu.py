@@ -26,12 +26,15 @@ def test_gated_ff_refusals(pkg):
                 dict(n=99, x=ctypes.c_void_p(4098)), dict(n=99, xs=33), dict(n=99, width=31)):   # the last need a workspace
         assert call(**bad) == inval, bad
     for bad in (dict(n=1 << 31), dict(width=(1 << 19) + 1, xs=1 << 20, gs=1 << 20, us=1 << 20),
-                dict(inner=(1 << 19) + 1, hs=1 << 20), dict(n=(1 << 31) - 1, inner=1 << 19, hs=1 << 20)):
+                dict(inner=(1 << 19) + 1, hs=1 << 20), dict(n=(1 << 31) - 1, inner=1 << 19, hs=1 << 20),
+                dict(n=1 << 30), dict(inner=1 << 19, width=1 << 19, xs=1 << 19, gs=1 << 19, us=1 << 19, hs=1 << 19)):
         assert call(**bad) == big, bad
     need = L.ec_gated_ff_workspace(P, 31, P, 32, P, 32, 1, 99, 31, 48, 0)
     assert need >= 99 * 64 + 2 * 48 * 64 and L.ec_gated_ff_workspace(P, 32, P, 32, P, 32, 1, 99, 32, 48, 0) == 0
     assert L.ec_gated_ff_workspace(P, 31, P, 31, P, 31, 1, 4, 31, 48, 0) == 0   # few rows are read as they are
     assert call(n=99, width=31, xs=31, work=P, have=need - 1) == inval
+    # weights of different strides are copied, both
+    assert L.ec_gated_ff_workspace(P, 32, P, 32, P, 40, 1, 99, 32, 48, 0) >= 2 * 48 * 64 and call(n=99, us=40) == inval
     assert call(n=99, width=31, xs=31, work=ODD, have=need) == align
     assert L.ec_gated_ff_workspace(P, 32, P, 32, P, 32, 7, 4, 32, 48, 0) == 0
 

@@ -141,6 +141,25 @@ def test_strides_and_addresses(pkg, dev, dtype, n):
             assert int((b == 7.0).sum()) >= inner * pad
 
 
+@types
+@pytest.mark.parametrize("n", [7, 90, 300])
+def test_weights_of_different_strides(pkg, dev, dtype, n):
+    """Each weight with rows as far apart as its own buffer has them, one of them perhaps not to be read in place."""
+    width, inner = 64, 72
+    x, w, dh = operands(dtype, n, width, inner)
+    want, bound, _ = forward(x, w[:inner], w[inner:], "silu")
+    wants = gradients(dh, x, w[:inner], w[inner:], "silu", dtype, dtype)
+    for gate_pad, up_pad in ((0, 64), (192, 0), (8, 16), (0, 1), (3, 0)):
+        views = []
+        for t, pad in ((w[:inner], gate_pad), (w[inner:], up_pad)):
+            views.append(torch.full((inner, width + pad), 9.0, dtype=dtype, device=dev)[:, :width])
+            views[-1].copy_(t)
+        check(pkg.gated_ff(x.to(dev), *views), want, rounded(want, dtype, bound), "h")
+        got = pkg.gated_ff_grad(dh.to(dev), x.to(dev), *views)
+        for name, g, (value, most) in zip(got._fields, got, wants):
+            check(g, value, most, name)
+
+
 def test_leading_dimensions_and_one_side(pkg, dev):
     x, w, dh = (t.to(dev) for t in operands(torch.bfloat16, 6 * 5, 32, 48))
     g, u = w[:48], w[48:]
