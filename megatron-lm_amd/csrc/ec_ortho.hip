@@ -94,8 +94,11 @@ __global__ void __launch_bounds__(kLanes) square_kernel(const T* x, uint64_t str
   if (threadIdx.x == 0) gp(parts)[blockIdx.y * gridDim.x + blockIdx.x] = sum;
 }
 
-// Two fp16 values whose sum is v to 22 bits.
+// Two fp16 values whose sum is v to 22 bits.  v is made a value first: where it is a product, the compiler would
+// round the unrounded product to the `high` that the difference takes and the rounded one to the `high` that is
+// stored, which are a step of 11 bits apart in one of 2^14 elements (and left one matrix in 20 with 1e-5 of its result).
 __device__ __forceinline__ void split(float v, fp16_t& high, fp16_t& low) {
+  asm("" : "+v"(v));
   high = (fp16_t)v;
   low = (fp16_t)(v - (float)high);
 }
@@ -217,10 +220,12 @@ __global__ void __launch_bounds__(S::kLanes, S::kPerSimd) ns_kernel(NsArgs p) {
   a.p += matrix * p.a_matrix;
   b.p += matrix * p.b_matrix;
   const uint32_t m0 = tm * S::BM, n0 = tn * S::BN, padded = (p.N + 7) & ~7u;
-  // at places past the ends some other value, which is not stored
+  // zeros below the last row, which the mirrored tile has as columns of padding; past the columns some other value,
+  // which is not stored
   const auto added = [&](uint32_t m, uint32_t n) {
-    return p.linear * get8<In>(p.add + matrix * p.add_matrix + min(m0 + m, p.M - 1) * p.add_ld,
-                               min(n0 + n, padded - 8), p.add_low);
+    return (m0 + m < p.M ? p.linear : 0.0f) *
+           get8<In>(p.add + matrix * p.add_matrix + min(m0 + m, p.M - 1) * p.add_ld, min(n0 + n, padded - 8),
+                    p.add_low);
   };
   constexpr bool kStarts = WHAT == kPoly || (WHAT != kGram && Kind<In>::kParts == 1);
   Acc<S> acc;

@@ -81,6 +81,20 @@ def test_as_good_as_single_precision(pkg, dev, shape):
     assert float(far) <= 8 * float(single)
 
 
+@pytest.mark.parametrize("width", [8, 136])
+def test_each_element_of_22_bits(pkg, dev, width):
+    """One step of c A A X on positive matrices of 8 x 8 (and zeros behind them), where nothing cancels: each element of
+    the result has the relative errors of what it is made of.  X is in it five times, A twice, B once, each stored with 2^-22;
+    four products leave out the product of the second parts, 2^-22 of them; and each of their sums of 8 terms rounds 8
+    times, by at most a step, 2 E.  A stored element whose parts do not belong together would be 2^-11 off, an eighth of that here."""
+    x = torch.zeros(4096, 8, width)
+    x[:, :, :8] = 0.5 + torch.rand(4096, 8, 8, generator=gen("positive", width))
+    want = steps_of(x.double(), steps=1, abc=(0.0, 0.0, 1.9))
+    got = pkg.orthogonalize(x.to(dev), steps=1, coefficients=(0.0, 0.0, 1.9)).double().cpu()
+    most = 12 * 2.0 ** -22 + 4 * 8 * 2 * E
+    assert bool(((got - want).abs() <= most * want).all()), float(((got - want).abs() / want.clamp(min=1e-30)).max())
+
+
 def half(x):
     """As stored for a product: times 2^12 in fp16."""
     return (x * 4096).half().double() / 4096
