@@ -502,7 +502,7 @@ __global__ void __launch_bounds__(SmallShape<D>::kLanes) small_kernel(SmallArgs 
     if (!kFast) acc.add(rest);
   };
   const float one = __builtin_ldexpf(1.0f, -kStored);
-  const float square = p.c != 0.0f ? p.c : 0x1p-60f;   // as in run_step
+  const float square = __builtin_fabsf(p.c) > 0x1p-60f ? p.c : 0x1p-60f;   // as in run_step
   for (uint32_t s = 0; s < p.steps; ++s) {
     const bool adds = kFast && s + kPlainSteps < p.steps;
     const int at = adds ? p.at_added : p.at_plain;
@@ -652,8 +652,8 @@ int run_step(const Plan& p, const Call& c, char* work, int s, hipStream_t st) {
   n.K = p.side;
   n.out = work + p.poly;
   n.add = work + p.gram, n.add_ld = gram.m.ld, n.add_matrix = gram.matrix;
-  // c (b / c A + A A); where there is no A A, so little of it that it is rounded off
-  const float square = c.c != 0.0f ? c.c : 0x1p-60f;
+  // c (b / c A + A A); where there is no A A, or next to none, so little of it that it is rounded off and b / c is finite
+  const float square = std::fabs(c.c) > 0x1p-60f ? c.c : 0x1p-60f;
   n.by = square * std::ldexp(1.0f, at - 2 * kStored);
   n.linear = c.b / square * std::ldexp(1.0f, kStored);
   n.diagonal = adds ? 0.0f : c.a * std::ldexp(1.0f, at);

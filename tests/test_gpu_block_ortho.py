@@ -176,6 +176,14 @@ def test_steps_and_coefficients(pkg, dev, steps, abc):
     assert float((got - want).norm()) <= steps * 22 * stretch * (2.0 ** -22 + 20 * E) * 1.2 * math.sqrt(60)
 
 
+@pytest.mark.parametrize("cols", [100, 200])
+@pytest.mark.parametrize("least", [1e-36, -1e-30, 1e-20])
+def test_next_to_no_fifth_powers(pkg, dev, cols, least):
+    """A coefficient that is rounded off is as good as none: b over it is never taken."""
+    x = update(torch.float32, 60, cols).to(dev)
+    assert torch.equal(pkg.orthogonalize(x, coefficients=(1.5, -0.5, least)), pkg.orthogonalize(x, coefficients=(1.5, -0.5, 0.0)))
+
+
 def test_singular_values_go_towards_one(pkg, dev):
     x = torch.randn(128, 256, generator=gen("spread")).to(dev)
     s = torch.linalg.svdvals(pkg.orthogonalize(x).double())
