@@ -524,6 +524,8 @@ int ec_residual_norm_grad(const void* d_dsum, uint64_t dsum_stride, const void* 
   if ((d_dsum && dsum_stride < width) || (d_weight && (dnormed_stride < width || sum_stride < width)) ||
       (d_branch && branch_stride < width))
     return EC_EINVAL;
+  // without rows there may be any number of the gate's, whose gradients are zeros, as far as one launch goes
+  if (!n && gate_rows > max_grid(kJoinLanes) / ((width + 63) / 64) - 2) return EC_ERANGE;
   const auto st = (hipStream_t)stream;
   if (n) {
     if (!d_dresidual || (d_branch && !d_dbranch)) return EC_EINVAL;

@@ -110,7 +110,7 @@ def test_residual_norm_grad_refusals(pkg):
                 dict(dg=None), dict(gate=None), dict(bw=None), dict(w=None), dict(ds=None, w=None, dw=None), dict(scale=INF),
                 dict(work=None), dict(have=need - 1)):
         assert call(**bad) == inval, bad
-    assert call(work=ODD) == align and call(n=1 << 31, gates=1) == big
+    assert call(work=ODD) == align and call(n=1 << 31, gates=1) == big and call(n=0, gates=1 << 40) == big
     assert L.ec_residual_norm_grad_workspace(6, 64, 4) == 0
 
 
