@@ -94,29 +94,23 @@ __global__ void __launch_bounds__(kLanes) square_kernel(const T* x, uint64_t str
   if (threadIdx.x == 0) gp(parts)[blockIdx.y * gridDim.x + blockIdx.x] = sum;
 }
 
-// Two fp16 values whose sum is v to 22 bits.  v is made a value first: where it is a product, the compiler would
+typedef fp16_t __attribute__((ext_vector_type(8))) h8;
+
+// Two fp16 values whose sum is v to 22 bits.  `high` is made a value of its own: where v is a product, the compiler would
 // round the unrounded product to the `high` that the difference takes and the rounded one to the `high` that is
 // stored, which are a step of 11 bits apart in one of 2^14 elements (and left one matrix in 20 with 1e-5 of its result).
-__device__ __forceinline__ void split(float v, fp16_t& high, fp16_t& low) {
-  asm("" : "+v"(v));
-  high = (fp16_t)v;
-  low = (fp16_t)(v - (float)high);
+__device__ __forceinline__ void split(const f8& v, h8& high, h8& low) {
+  high = __builtin_convertvector(v, h8);
+  asm("" : "+v"(high));
+  low = __builtin_convertvector(v - __builtin_convertvector(high, f8), h8);
 }
-
-typedef fp16_t __attribute__((ext_vector_type(8))) h8;
 
 // Columns n ... n + 7 (n a multiple of 8) of a row of pairs; or of one of fp16 values, of a matrix whose second parts
 // are `low_at` bytes behind (0: it has none).
 template <typename K>
 __device__ __forceinline__ void put8(char* row, uint32_t n, const f8& v, uint64_t low_at) {
   h8 high, low;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    fp16_t h, l;
-    split(v[e], h, l);
-    high[e] = h;
-    low[e] = l;
-  }
+  split(v, high, low);
   global<char>* to = gp(row) + n * Kind<K>::kBytes;
   *(global<h8>*)to = high;
   if (Kind<K>::kParts == 2)
@@ -376,13 +370,7 @@ struct Resident {
   }
   __device__ __forceinline__ static void put(local<char>* m, local<char>* low, uint32_t row, uint32_t n, const f8& v) {
     h8 h, l;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      fp16_t x, y;
-      split(v[e], x, y);
-      h[e] = x;
-      l[e] = y;
-    }
+    split(v, h, l);
     if constexpr (Kind<K>::kParts == 2) {
       *(local<h8>*)(m + chunk_at(row, n / 4)) = h;
       *(local<h8>*)(m + chunk_at(row, n / 4 + 1)) = l;
@@ -457,13 +445,13 @@ __global__ void __launch_bounds__(SmallShape<D>::kLanes) small_kernel(SmallArgs 
       if (!tall) {
         R::put(x, low, row, col, v[g]);
       } else {
+        h8 h, l;
+        split(v[g], h, l);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          fp16_t h, l;
-          split(v[g][e], h, l);
           const uint32_t c = row / 8 * Kind<K>::kParts, in = row % 8 * 2;
-          *(local<fp16_t>*)(x + R::chunk_at(col + e, c) + in) = h;
-          *(local<fp16_t>*)((kFast ? low : x) + R::chunk_at(col + e, kFast ? c : c + 1) + in) = l;
+          *(local<fp16_t>*)(x + R::chunk_at(col + e, c) + in) = h[e];
+          *(local<fp16_t>*)((kFast ? low : x) + R::chunk_at(col + e, kFast ? c : c + 1) + in) = l[e];
         }
       }
     }

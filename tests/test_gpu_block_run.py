@@ -165,6 +165,43 @@ def test_two_graphs(pkg, dev):
             assert all(torch.equal(x, y) for x, y in zip(out, want))
 
 
+def test_a_captured_backward(pkg, dev):
+    """Forward and backward passes through autograd in one graph, replayed on new values between eager passes.  The leaves
+    of the graph are its own: no eager graph of them lives while it is captured."""
+    def pass_of(p):
+        z = pkg.residual_norm(p["x"], weight=p["first"]).normed
+        h = pkg.gated_ff(z, p["w_gate"], p["w_up"])
+        r = pkg.residual_norm(p["x"][:, :32], h[:, :32].contiguous(), gate=p["gate"], branch_weight=p["post"], weight=p["last"])
+        return torch.autograd.grad((r.residual, r.normed), list(p.values()), (p["x"].detach()[:, :32].contiguous(),) * 2)
+
+    def values(key):
+        g = gen("backward", key)
+        shapes = {"x": (40, 72), "first": (72,), "w_gate": (48, 72), "w_up": (48, 72), "gate": (5, 32), "post": (32,), "last": (32,)}
+        return {k: torch.randn(*s, generator=g).to(torch.bfloat16).to(dev) for k, s in shapes.items()}
+
+    side = torch.cuda.Stream(dev)
+    leaves = {k: v.requires_grad_() for k, v in values(0).items()}
+    side.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            pass_of(leaves)
+    torch.cuda.current_stream(dev).wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = pass_of(leaves)
+    for key in range(1, 4):
+        new = values(key)
+        with torch.no_grad():
+            for k, v in leaves.items():
+                v.copy_(new[k])
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = pass_of({k: v.requires_grad_() for k, v in new.items()})
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
 def test_past_32_bits(pkg, dev):
     """More than 2^32 elements of h, dh and the stream: the last rows are those of a call on them alone."""
     n, width, inner = 66000, 64, 65600
