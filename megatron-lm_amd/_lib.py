@@ -210,9 +210,9 @@ _shards_lock = threading.Lock()
 
 
 def shards():
-    """The torch-tensor binding of the flat-shard calls and the training-step
-    operators (``_ec_shards.so``, csrc/shards_torch.cpp and step_torch.cpp), which links
-    libec_mi355.so.  Raises
+    """The torch-tensor binding of the flat-shard calls, the training-step operators
+    and the block's (``_ec_shards.so``, csrc/shards_torch.cpp, step_torch.cpp and
+    block_torch.cpp), which links libec_mi355.so.  Raises
     ``ECLibraryMissing`` when it is not built; there is no fallback."""
     global _shards_mod
     if _shards_mod is not None:

@@ -21,7 +21,7 @@
 // eight low parts, in 32 bytes.  A product of two pairs takes three of the matrix cores' products
 // (the low parts' is below the fp32 accumulator's rounding), at 3/16 of the time of fp32 products.  The matrix
 // cores truncate where they add to an accumulator, so the two small products have accumulators of their own, which
-// are added at the end: five Newton-Schulz steps on 1001 x 777 are 3.5e-6 off with one accumulator, 2.1e-6 with two, and
+// are added at the end: five Newton-Schulz steps on 1001 x 777 are 3.5e-6 off with one accumulator, 2.0e-6 with two, and
 // those of fp32 products 2.3e-6.
 #pragma once
 

@@ -5,12 +5,12 @@
 //   sum = residual + scale * gate * u
 //   normed = weight * sum / rms(sum)
 //
-// A row is held in the registers of a team of 64, 256 or 1024 lanes, 16 bytes a lane and group,
+// A row is held in the registers of a team of 64 to 1024 lanes, 16 bytes a lane and group,
 // so that it is read once whatever is done with it.  The norms' sums go over
 // the wave by shuffles and over the team's waves through LDS.
 //
 // Backward, a team goes over a run of rows and keeps the sums over them, of the weights' and the
-// gate's gradients, in registers; each team leaves one row of partials, which a second launch
+// gate's gradients, in registers (those of the longest rows partly in LDS); each team leaves one row of partials, which a second launch
 // adds in order.  No atomics.
 #include <hip/hip_runtime.h>
 #include <stdint.h>

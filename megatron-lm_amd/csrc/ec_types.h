@@ -1,5 +1,5 @@
 // ec_types.h — element types and group accesses of the training-step kernels
-// (ec_embed.hip, ec_logprobs.hip, ec_grads.hip).
+// (ec_embed.hip, ec_logprobs.hip, ec_grads.hip) and the block's (ec_ff.hip, ec_norms.hip, ec_ortho.hip).
 //
 // A group is the 16 bytes one lane moves at once: 4 fp32 or 8 bf16 / fp16
 // elements, at any address that is a multiple of the element's size (the vector
