@@ -582,10 +582,14 @@ constexpr uint64_t step_ns() {
   constexpr uint64_t narrow[] = {1470, 610, 400, 260}, pairs[] = {0, 720, 400, 250}, wide[] = {6800, 1720, 880, 450};
   return __is_same(T, float) ? wide[at] : __is_same(T, pair_t) ? pairs[at] : narrow[at];
 }
+// Tiles of few steps are bound by what they write, in bursts that only other workgroups of the CU fill the pauses of (gradients of
+// 4096 rows 64 -> 1000 bf16 52 us with large tiles, 39 with middle ones).
 template <class S>
-constexpr uint64_t tile_ns() {
+constexpr uint64_t tile_ns(bool few_steps) {
+  if (few_steps) return __is_same(S, Large) ? 13000 : __is_same(S, Middle) ? 3500 : S::BN > 64 ? 2500 : 1500;
   return __is_same(S, Large) ? 8000 : __is_same(S, Middle) ? 5000 : 3500;
 }
+constexpr uint64_t kFewSteps = 4;
 
 struct Choice {
   int shape;           // 0: Large, 1: Middle, 2: the least
@@ -615,7 +619,7 @@ Choice choose(F tiles, uint64_t steps, bool may_split = true) {
       const uint64_t turns = (n * real + kCus - 1) / kCus;
       const uint64_t join = real == 1 ? 0 : 4000 + std::max(bytes * 2 / 5500, (n + kCus - 1) / kCus * (bytes / n) / 35);
       const uint64_t step = step_ns<S, T>() * (turns == 1 && S::kWaves == 4 ? 5 : 4) / 4;
-      const uint64_t ns = turns * (each * step + tile_ns<S>()) + join;
+      const uint64_t ns = turns * (each * step + tile_ns<S>(steps <= kFewSteps)) + join;
       if (ns < best.ns) best = {shape, {(uint32_t)real, (uint32_t)each, nullptr}, bytes, ns};
     }
   };
