@@ -268,42 +268,41 @@ struct SumArgs {
 
 template <class S, typename T, bool ACROSS_A>
 __device__ __forceinline__ void sum_products(Acc<S>& acc, local<char>* lds, const SumArgs& p, uint32_t tm,
-                                             uint32_t tn, uint32_t split, uint32_t K) {
+                                             uint32_t tn, uint32_t which, uint32_t split, uint32_t K) {
   const uint32_t s0 = split * p.splits.steps;
   for (uint32_t i = 0; i < p.parts; ++i) {
     Operand a = from_step<T, ACROSS_A>(p.a[i], s0);
-    a.p += blockIdx.y * p.a_step;
+    a.p += which * p.a_step;
     const Operand b = from_step<T, true>(p.b[i], s0);
     product<S, T, ACROSS_A, true, false>(acc, lds, a, b, b, tm * S::BM, tn * S::BN, K);
   }
 }
 
+// Workgroup t of a split's, or a result's `which`-th sum.
 template <class S, typename T, bool ACROSS_A>
-__global__ void __launch_bounds__(S::kLanes, S::kPerSimd) sum_part_kernel(SumArgs p) {
-  __shared__ __attribute__((aligned(1024))) char lds[S::kLds];
-  const uint32_t tiles = p.tiles_m * p.tiles_n, t = xcd_order(blockIdx.x, gridDim.x), split = uniform(t / tiles);
+__device__ __forceinline__ void sum_part(const SumArgs& p, local<char>* lds, uint32_t t, uint32_t which) {
+  const uint32_t tiles = p.tiles_m * p.tiles_n, split = uniform(t / tiles);
   uint32_t tm, tn;
   tile_at(t % tiles, p.tiles_m, p.tiles_n, tm, tn);
   Acc<S> acc;
   acc.clear();
-  sum_products<S, T, ACROSS_A>(acc, (local<char>*)lds, p, tm, tn, split, split_length<T>(p.splits, split, p.K));
-  store_part(acc, p.splits.parts, (uint64_t)blockIdx.y * gridDim.x + t);
+  sum_products<S, T, ACROSS_A>(acc, lds, p, tm, tn, which, split, split_length<T>(p.splits, split, p.K));
+  store_part(acc, p.splits.parts, (uint64_t)which * tiles * p.splits.n + t);
 }
 
 template <class S, typename T, typename O, bool ACROSS_A, bool ACCUMULATE, bool JOIN>
-__global__ void __launch_bounds__(S::kLanes, S::kPerSimd) sum_kernel(SumArgs p) {
-  __shared__ __attribute__((aligned(1024))) char lds[JOIN ? 16 : S::kLds];
-  const uint32_t t = xcd_order(blockIdx.x, gridDim.x);
+__device__ __forceinline__ void sum_tile(const SumArgs& p, local<char>* lds, uint32_t t, uint32_t which) {
   uint32_t tm, tn;
   tile_at(t, p.tiles_m, p.tiles_n, tm, tn);
+  const uint32_t tiles = p.tiles_m * p.tiles_n;
   Acc<S> acc;
   acc.clear();
   if constexpr (JOIN)
-    add_parts(acc, p.splits.parts, (uint64_t)blockIdx.y * gridDim.x * p.splits.n + t, gridDim.x, p.splits.n);
+    add_parts(acc, p.splits.parts, (uint64_t)which * tiles * p.splits.n + t, tiles, p.splits.n);
   else
-    sum_products<S, T, ACROSS_A>(acc, (local<char>*)lds, p, tm, tn, 0, p.K);
-  O* out = (O*)p.out[blockIdx.y];
-  const uint64_t stride = p.out_stride[blockIdx.y];
+    sum_products<S, T, ACROSS_A>(acc, lds, p, tm, tn, which, 0, p.K);
+  O* out = (O*)p.out[which];
+  const uint64_t stride = p.out_stride[which];
   const uint32_t m0 = tm * S::BM, n0 = tn * S::BN;
   const auto put = [&](uint32_t m, uint32_t n, const f8& v) {
     m += m0;
@@ -315,6 +314,37 @@ __global__ void __launch_bounds__(S::kLanes, S::kPerSimd) sum_kernel(SumArgs p) 
                   [&](uint32_t m, uint32_t n, const f8& v, const f8& x) { put(m, n, v + x); });
   else
     acc.each(put);
+}
+
+template <class S, typename T, bool ACROSS_A>
+__global__ void __launch_bounds__(S::kLanes, S::kPerSimd) sum_part_kernel(SumArgs p) {
+  __shared__ __attribute__((aligned(1024))) char lds[S::kLds];
+  sum_part<S, T, ACROSS_A>(p, (local<char>*)lds, xcd_order(blockIdx.x, gridDim.x), blockIdx.y);
+}
+
+template <class S, typename T, typename O, bool ACROSS_A, bool ACCUMULATE, bool JOIN>
+__global__ void __launch_bounds__(S::kLanes, S::kPerSimd) sum_kernel(SumArgs p) {
+  __shared__ __attribute__((aligned(1024))) char lds[JOIN ? 16 : S::kLds];
+  sum_tile<S, T, O, ACROSS_A, ACCUMULATE, JOIN>(p, (local<char>*)lds, xcd_order(blockIdx.x, gridDim.x), blockIdx.y);
+}
+
+// dx in small tiles (SPLIT: the splits of them) and both dW in tiles of S, in one launch: neither fills the CUs by itself
+// (777 rows 1001 -> 1333 fp16 22.4 us, 17.3 and 14.5 one after the other).
+template <class S, typename T, typename O, bool ACCUMULATE, bool SPLIT>
+__global__ void __launch_bounds__(S::kLanes, S::kPerSimd) sum_both_kernel(SumArgs x, SumArgs w) {
+  static_assert(S::kLanes == Small::kLanes, "one workgroup size");
+  __shared__ __attribute__((aligned(1024))) char lds[S::kLds > Small::kLds ? S::kLds : Small::kLds];
+  const uint32_t first = x.tiles_m * x.tiles_n * x.splits.n;
+  if (blockIdx.x < first) {
+    const uint32_t t = xcd_order(blockIdx.x, first);
+    if constexpr (SPLIT)
+      sum_part<Small, T, false>(x, (local<char>*)lds, t, 0);
+    else
+      sum_tile<Small, T, T, false, false, false>(x, (local<char>*)lds, t, 0);
+  } else {
+    const uint32_t tiles = w.tiles_m * w.tiles_n, t = xcd_order(blockIdx.x - first, 2 * tiles);
+    sum_tile<S, T, O, true, ACCUMULATE, false>(w, (local<char>*)lds, t % tiles, uniform(t / tiles));
+  }
 }
 
 // Rows up to which few_kernel takes the forward pass. 2048 -> 8192 bf16, eight sets of weights in turns, us: 1 row 14.9,
@@ -439,6 +469,13 @@ void run_ff(FfArgs& p, char* parts, hipStream_t st) {
   });
 }
 
+template <class S>
+uint32_t set_tiles(SumArgs& p) {
+  p.tiles_m = (p.M + S::BM - 1) / S::BM;
+  p.tiles_n = (p.N + S::BN - 1) / S::BN;
+  return p.tiles_m * p.tiles_n;
+}
+
 template <typename T, typename O, bool ACROSS_A, bool ACCUMULATE>
 void run_sum(SumArgs& p, uint32_t outs, char* parts, hipStream_t st) {
   const Choice c = choose_sum<T>(p.M, p.N, p.K, std::max(1u, p.parts), outs);
@@ -446,9 +483,7 @@ void run_sum(SumArgs& p, uint32_t outs, char* parts, hipStream_t st) {
   p.splits.parts = (float*)parts;
   with_shape<T, Small>(c, [&](auto s) {
     typedef decltype(s) S;
-    p.tiles_m = (p.M + S::BM - 1) / S::BM;
-    p.tiles_n = (p.N + S::BN - 1) / S::BN;
-    const uint32_t tiles = p.tiles_m * p.tiles_n;
+    const uint32_t tiles = set_tiles<S>(p);
     if (c.splits.n > 1) {
       sum_part_kernel<S, T, ACROSS_A><<<dim3(tiles * c.splits.n, outs), S::kLanes, 0, st>>>(p);
       sum_kernel<S, T, O, ACROSS_A, ACCUMULATE, true><<<dim3(tiles, outs), S::kLanes, 0, st>>>(p);
@@ -456,6 +491,35 @@ void run_sum(SumArgs& p, uint32_t outs, char* parts, hipStream_t st) {
       sum_kernel<S, T, O, ACROSS_A, ACCUMULATE, false><<<dim3(tiles, outs), S::kLanes, 0, st>>>(p);
     }
   });
+}
+
+// dx and both dW, in one launch (and dx's join) where dx takes small tiles, and dW such or middle ones and no splits; large
+// ones of few steps are no better than middle ones (tile_ns).
+template <typename T, typename O, bool ACCUMULATE>
+void run_sums(SumArgs& x, SumArgs& w, char* parts, hipStream_t st) {
+  Choice cx = choose_sum<T>(x.M, x.N, x.K, x.parts, 1), cw = choose_sum<T>(w.M, w.N, w.K, w.parts, 2);
+  if (cw.shape == 0 && steps_of<T>(w.K) * w.parts <= kFewSteps) cw.shape = 1;
+  const uint64_t tiles = tiles_of(x.M, x.N, Small::BM, Small::BN);
+  if (cx.shape != 2 || tiles * cx.splits.n > 2 * kCus || cw.shape == 0 || cw.splits.n > 1) {
+    run_sum<T, T, false, false>(x, 1, parts, st);
+    run_sum<T, O, true, ACCUMULATE>(w, 2, parts, st);
+    return;
+  }
+  x.splits = cx.splits, w.splits = cw.splits;
+  x.splits.parts = (float*)parts;
+  set_tiles<Small>(x);
+  const auto run = [&](auto s, auto split) {
+    typedef decltype(s) S;
+    const uint32_t blocks = (uint32_t)tiles * x.splits.n + 2 * set_tiles<S>(w);
+    sum_both_kernel<S, T, O, ACCUMULATE, decltype(split)::value><<<blocks, S::kLanes, 0, st>>>(x, w);
+  };
+  const auto with_tiles = [&](auto split) { cw.shape == 1 ? run(Middle(), split) : run(Small(), split); };
+  if (x.splits.n > 1) {
+    with_tiles(std::true_type());
+    sum_kernel<Small, T, T, false, false, true><<<(uint32_t)tiles, Small::kLanes, 0, st>>>(x);
+  } else {
+    with_tiles(std::false_type());
+  }
 }
 
 int check_call(const FfCall& c, int act) {
@@ -549,20 +613,18 @@ int ec_gated_ff_grad(const void* d_dh, uint64_t dh_stride, const void* d_x, uint
       run_ff<T, true>(p, work + w.parts, st);
     }
     const uint64_t ld = d_row * sizeof(T), half = p.padded * sizeof(T), low = p.low * sizeof(T);
+    SumArgs x = {}, s = {};   // dx, dW
     if (d_dx && n) {
-      SumArgs s = {};
-      s.parts = p.low ? 4 : 2;
-      for (uint32_t i = 0; i < s.parts; ++i) {
-        s.a[i] = {p.d + i % 2 * half + i / 2 * low, ld, p.n};
-        s.b[i] = i % 2 ? p.w_up : p.w_gate;
-        s.b[i].rows = width;
+      x.parts = p.low ? 4 : 2;
+      for (uint32_t i = 0; i < x.parts; ++i) {
+        x.a[i] = {p.d + i % 2 * half + i / 2 * low, ld, p.n};
+        x.b[i] = i % 2 ? p.w_up : p.w_gate;
+        x.b[i].rows = width;
       }
-      s.K = inner, s.M = p.n, s.N = width;
-      s.out[0] = (char*)d_dx, s.out_stride[0] = dx_stride;
-      run_sum<T, T, false, false>(s, 1, work + w.parts, st);
+      x.K = inner, x.M = p.n, x.N = width;
+      x.out[0] = (char*)d_dx, x.out_stride[0] = dx_stride;
     }
     if (d_dgate) {
-      SumArgs s = {};
       s.parts = !n ? 0 : p.low ? 2 : 1;
       for (uint32_t i = 0; i < s.parts; ++i) {
         s.a[i] = {p.d + i * low, ld, inner};
@@ -573,13 +635,18 @@ int ec_gated_ff_grad(const void* d_dh, uint64_t dh_stride, const void* d_x, uint
       s.K = p.n, s.M = inner, s.N = width;
       s.out[0] = (char*)d_dgate, s.out_stride[0] = dgate_stride;
       s.out[1] = (char*)d_dup, s.out_stride[1] = dup_stride;
-      const auto run = [&](auto o) {
-        typedef decltype(o) O;
-        accumulate ? run_sum<T, O, true, true>(s, 2, work + w.parts, st)
-                   : run_sum<T, O, true, false>(s, 2, work + w.parts, st);
-      };
-      grad_type == EC_F32 ? run(float()) : run(T());
     }
+    char* parts = work + w.parts;
+    const auto run = [&](auto o, auto add) {
+      typedef decltype(o) O;
+      constexpr bool kAdd = decltype(add)::value;
+      x.parts ? run_sums<T, O, kAdd>(x, s, parts, st) : run_sum<T, O, true, kAdd>(s, 2, parts, st);
+    };
+    const auto run_type = [&](auto o) { accumulate ? run(o, std::true_type()) : run(o, std::false_type()); };
+    if (!d_dgate)
+      run_sum<T, T, false, false>(x, 1, parts, st);
+    else
+      grad_type == EC_F32 ? run_type(float()) : run_type(T());
     return launched();
   });
 }

@@ -31,6 +31,29 @@ def test_split_sums(pkg, dev, dtype, n, width, inner):
         check(g, want + 1.0, bound + 2 * E * (want.abs() + 1.0), "dw added to ones")
 
 
+@types
+@pytest.mark.parametrize("n,width,inner", [(777, 501, 1333), (30, 1000, 2665), (200, 330, 500), (50, 512, 2050), (1, 4100, 700),
+                                           (520, 1030, 770)])
+def test_sums_in_one_launch(pkg, dev, dtype, n, width, inner):
+    """Both kinds of gradients in one launch, dx split or not, dW in middle or small tiles: as when they are asked for
+    one at a time, within the same bounds, and nothing beside the rows written."""
+    x, w, dh = operands(dtype, n, width, inner)
+    xd, wd, dhd = x.to(dev), w.to(dev), dh.to(dev)
+    for out in {dtype, torch.float32}:
+        wants = gradients(dh, x, w[:inner], w[inner:], "silu", dtype, out)
+        room = torch.full((2, inner, width + 9), 2.0, dtype=out, device=dev)
+        into = [room[0, :, :width], room[1, :, :width]]
+        both = pkg.gated_ff_grad(dhd, xd, wd[:inner], wd[inner:], out=into)
+        alone = [pkg.gated_ff_grad(dhd, xd, wd[:inner], wd[inner:], weights=False).dx,
+                 *pkg.gated_ff_grad(dhd, xd, wd[:inner], wd[inner:], inputs=False, dtype=out)[1:]]
+        for got in (both, alone):
+            for name, g, (want, bound) in zip(both._fields, got, wants):
+                check(g, want, bound, name)
+        assert bool((room[:, :, width:] == 2).all())
+        again = pkg.gated_ff_grad(dhd, xd, wd[:inner], wd[inner:], dtype=out)
+        assert all(torch.equal(a, b) for a, b in zip(both, again))
+
+
 @pytest.mark.parametrize("shape", [(40, 6000), (6000, 40), (130, 3000), (2, 3000, 100)], ids=str)
 @pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
 def test_split_grams(pkg, dev, shape, out):
