@@ -263,6 +263,7 @@ struct SumArgs {
   char* out[2];   // blockIdx.y's
   uint64_t out_stride[2];
   uint64_t a_step;   // bytes from blockIdx.y = 0's first operand to 1's
+  bool accumulate;   // added to what is there
   Splits splits;     // each takes its steps of every product
 };
 
@@ -290,7 +291,7 @@ __device__ __forceinline__ void sum_part(const SumArgs& p, local<char>* lds, uin
   store_part(acc, p.splits.parts, (uint64_t)which * tiles * p.splits.n + t);
 }
 
-template <class S, typename T, typename O, bool ACROSS_A, bool ACCUMULATE, bool JOIN>
+template <class S, typename T, typename O, bool ACROSS_A, bool JOIN>
 __device__ __forceinline__ void sum_tile(const SumArgs& p, local<char>* lds, uint32_t t, uint32_t which) {
   uint32_t tm, tn;
   tile_at(t, p.tiles_m, p.tiles_n, tm, tn);
@@ -309,7 +310,7 @@ __device__ __forceinline__ void sum_tile(const SumArgs& p, local<char>* lds, uin
     n += n0;
     if (m < p.M && n < p.N) store8<O>(out + m * stride, n, p.N, v);
   };
-  if constexpr (ACCUMULATE)
+  if (ACROSS_A && p.accumulate)
     acc.each_with([&](uint32_t m, uint32_t n) { return load8(out + min(m0 + m, p.M - 1) * stride, n0 + n, p.N); },
                   [&](uint32_t m, uint32_t n, const f8& v, const f8& x) { put(m, n, v + x); });
   else
@@ -322,15 +323,15 @@ __global__ void __launch_bounds__(S::kLanes, S::kPerSimd) sum_part_kernel(SumArg
   sum_part<S, T, ACROSS_A>(p, (local<char>*)lds, xcd_order(blockIdx.x, gridDim.x), blockIdx.y);
 }
 
-template <class S, typename T, typename O, bool ACROSS_A, bool ACCUMULATE, bool JOIN>
+template <class S, typename T, typename O, bool ACROSS_A, bool JOIN>
 __global__ void __launch_bounds__(S::kLanes, S::kPerSimd) sum_kernel(SumArgs p) {
   __shared__ __attribute__((aligned(1024))) char lds[JOIN ? 16 : S::kLds];
-  sum_tile<S, T, O, ACROSS_A, ACCUMULATE, JOIN>(p, (local<char>*)lds, xcd_order(blockIdx.x, gridDim.x), blockIdx.y);
+  sum_tile<S, T, O, ACROSS_A, JOIN>(p, (local<char>*)lds, xcd_order(blockIdx.x, gridDim.x), blockIdx.y);
 }
 
 // dx in small tiles (SPLIT: the splits of them) and both dW in tiles of S, in one launch: neither fills the CUs by itself
 // (777 rows 1001 -> 1333 fp16 22.4 us, 17.3 and 14.5 one after the other).
-template <class S, typename T, typename O, bool ACCUMULATE, bool SPLIT>
+template <class S, typename T, typename O, bool SPLIT>
 __global__ void __launch_bounds__(S::kLanes, S::kPerSimd) sum_both_kernel(SumArgs x, SumArgs w) {
   static_assert(S::kLanes == Small::kLanes, "one workgroup size");
   __shared__ __attribute__((aligned(1024))) char lds[S::kLds > Small::kLds ? S::kLds : Small::kLds];
@@ -340,10 +341,10 @@ __global__ void __launch_bounds__(S::kLanes, S::kPerSimd) sum_both_kernel(SumArg
     if constexpr (SPLIT)
       sum_part<Small, T, false>(x, (local<char>*)lds, t, 0);
     else
-      sum_tile<Small, T, T, false, false, false>(x, (local<char>*)lds, t, 0);
+      sum_tile<Small, T, T, false, false>(x, (local<char>*)lds, t, 0);
   } else {
     const uint32_t tiles = w.tiles_m * w.tiles_n, t = xcd_order(blockIdx.x - first, 2 * tiles);
-    sum_tile<S, T, O, true, ACCUMULATE, false>(w, (local<char>*)lds, t % tiles, uniform(t / tiles));
+    sum_tile<S, T, O, true, false>(w, (local<char>*)lds, t % tiles, uniform(t / tiles));
   }
 }
 
@@ -476,7 +477,7 @@ uint32_t set_tiles(SumArgs& p) {
   return p.tiles_m * p.tiles_n;
 }
 
-template <typename T, typename O, bool ACROSS_A, bool ACCUMULATE>
+template <typename T, typename O, bool ACROSS_A>
 void run_sum(SumArgs& p, uint32_t outs, char* parts, hipStream_t st) {
   const Choice c = choose_sum<T>(p.M, p.N, p.K, std::max(1u, p.parts), outs);
   p.splits = c.splits;
@@ -486,23 +487,23 @@ void run_sum(SumArgs& p, uint32_t outs, char* parts, hipStream_t st) {
     const uint32_t tiles = set_tiles<S>(p);
     if (c.splits.n > 1) {
       sum_part_kernel<S, T, ACROSS_A><<<dim3(tiles * c.splits.n, outs), S::kLanes, 0, st>>>(p);
-      sum_kernel<S, T, O, ACROSS_A, ACCUMULATE, true><<<dim3(tiles, outs), S::kLanes, 0, st>>>(p);
+      sum_kernel<S, T, O, ACROSS_A, true><<<dim3(tiles, outs), S::kLanes, 0, st>>>(p);
     } else {
-      sum_kernel<S, T, O, ACROSS_A, ACCUMULATE, false><<<dim3(tiles, outs), S::kLanes, 0, st>>>(p);
+      sum_kernel<S, T, O, ACROSS_A, false><<<dim3(tiles, outs), S::kLanes, 0, st>>>(p);
     }
   });
 }
 
 // dx and both dW, in one launch (and dx's join) where dx takes small tiles, and dW such or middle ones and no splits; large
 // ones of few steps are no better than middle ones (tile_ns).
-template <typename T, typename O, bool ACCUMULATE>
+template <typename T, typename O>
 void run_sums(SumArgs& x, SumArgs& w, char* parts, hipStream_t st) {
   Choice cx = choose_sum<T>(x.M, x.N, x.K, x.parts, 1), cw = choose_sum<T>(w.M, w.N, w.K, w.parts, 2);
   if (cw.shape == 0 && steps_of<T>(w.K) * w.parts <= kFewSteps) cw.shape = 1;
   const uint64_t tiles = tiles_of(x.M, x.N, Small::BM, Small::BN);
   if (cx.shape != 2 || tiles * cx.splits.n > 2 * kCus || cw.shape == 0 || cw.splits.n > 1) {
-    run_sum<T, T, false, false>(x, 1, parts, st);
-    run_sum<T, O, true, ACCUMULATE>(w, 2, parts, st);
+    run_sum<T, T, false>(x, 1, parts, st);
+    run_sum<T, O, true>(w, 2, parts, st);
     return;
   }
   x.splits = cx.splits, w.splits = cw.splits;
@@ -511,12 +512,12 @@ void run_sums(SumArgs& x, SumArgs& w, char* parts, hipStream_t st) {
   const auto run = [&](auto s, auto split) {
     typedef decltype(s) S;
     const uint32_t blocks = (uint32_t)tiles * x.splits.n + 2 * set_tiles<S>(w);
-    sum_both_kernel<S, T, O, ACCUMULATE, decltype(split)::value><<<blocks, S::kLanes, 0, st>>>(x, w);
+    sum_both_kernel<S, T, O, decltype(split)::value><<<blocks, S::kLanes, 0, st>>>(x, w);
   };
   const auto with_tiles = [&](auto split) { cw.shape == 1 ? run(Middle(), split) : run(Small(), split); };
   if (x.splits.n > 1) {
     with_tiles(std::true_type());
-    sum_kernel<Small, T, T, false, false, true><<<(uint32_t)tiles, Small::kLanes, 0, st>>>(x);
+    sum_kernel<Small, T, T, false, true><<<(uint32_t)tiles, Small::kLanes, 0, st>>>(x);
   } else {
     with_tiles(std::false_type());
   }
@@ -631,22 +632,20 @@ int ec_gated_ff_grad(const void* d_dh, uint64_t dh_stride, const void* d_x, uint
         s.b[i] = p.x;
         s.b[i].rows = width;
       }
-      s.a_step = half;
+      s.a_step = half, s.accumulate = accumulate;
       s.K = p.n, s.M = inner, s.N = width;
       s.out[0] = (char*)d_dgate, s.out_stride[0] = dgate_stride;
       s.out[1] = (char*)d_dup, s.out_stride[1] = dup_stride;
     }
     char* parts = work + w.parts;
-    const auto run = [&](auto o, auto add) {
+    const auto run = [&](auto o) {
       typedef decltype(o) O;
-      constexpr bool kAdd = decltype(add)::value;
-      x.parts ? run_sums<T, O, kAdd>(x, s, parts, st) : run_sum<T, O, true, kAdd>(s, 2, parts, st);
+      x.parts ? run_sums<T, O>(x, s, parts, st) : run_sum<T, O, true>(s, 2, parts, st);
     };
-    const auto run_type = [&](auto o) { accumulate ? run(o, std::true_type()) : run(o, std::false_type()); };
     if (!d_dgate)
-      run_sum<T, T, false, false>(x, 1, parts, st);
+      run_sum<T, T, false>(x, 1, parts, st);
     else
-      grad_type == EC_F32 ? run_type(float()) : run_type(T());
+      grad_type == EC_F32 ? run(float()) : run(T());
     return launched();
   });
 }
