@@ -398,7 +398,7 @@ FfWork ff_work(const FfCall& c, bool grad) {
     w.total += part(bytes);
     return at;
   };
-  if (!grad && c.n <= kFewForward) return w;   // read as they are
+  if (!c.n || (!grad && c.n <= kFewForward)) return w;   // none are read, or read as they are
   if (!readable(c.x, c.width, c.x_stride, b)) w.x = take(c.n * row);
   // the two weights are read in turns, so their rows have to be equally far apart
   if (c.gate_stride != c.up_stride || !readable(c.w_gate, c.width, c.gate_stride, b) ||

@@ -613,7 +613,7 @@ Choice choose(F tiles, uint64_t steps, bool may_split = true) {
     const uint64_t n = tiles(s);
     for (uint64_t splits = 1; splits <= (may_split ? 32 : 1); splits += splits < 4 ? 1 : splits / 2) {
       const uint64_t each = (steps + splits - 1) / splits;
-      if (splits > 1 && (each < 4 || n >= 2 * kCus)) break;
+      if (splits > 1 && (!n || each < 4 || n >= 2 * kCus)) break;   // (no tiles, no rows: nothing to split)
       const uint64_t real = (steps + each - 1) / each, bytes = real > 1 ? n * real * S::BM * S::BN * 4 : 0;
       if (bytes > kMostPartBytes) break;
       const uint64_t turns = (n * real + kCus - 1) / kCus;

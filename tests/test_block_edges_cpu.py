@@ -1,0 +1,19 @@
+"""The block operators' edges on the host, without a GPU: every call returns before any device work, so the addresses are
+never touched."""
+import ctypes
+
+import pytest
+
+P = ctypes.c_void_p(4096)
+
+
+@pytest.mark.parametrize("kind", [0, 1, 2], ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("width,inner", [(2048, 8192), (256, 256), (64, 512), (448, 64), (65, 4001), (1, 1)])
+def test_gated_ff_without_rows(pkg, kind, width, inner):
+    """No rows at widths whose sums are split along k with rows: no workspace, and nothing to do but the weights' zeros."""
+    L = pkg._lib.lib()
+    rows = (P, width, P, width, P, width, kind, 0, width, inner)
+    assert L.ec_gated_ff_workspace(*rows, 0) == L.ec_gated_ff_workspace(*rows, 1) == 0
+    assert L.ec_gated_ff(*rows, 0, P, inner, None, 0, None) == pkg._lib.EC_OK
+    assert L.ec_gated_ff_grad(P, inner, *rows, 0, P, width, P, width, P, width, kind, 1, None, 0, None) == pkg._lib.EC_OK
+    assert L.ec_gated_ff_grad(P, inner, *rows, 0, P, width, None, 0, None, 0, kind, 0, None, 0, None) == pkg._lib.EC_OK
