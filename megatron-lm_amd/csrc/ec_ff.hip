@@ -592,7 +592,7 @@ int ec_gated_ff_grad(const void* d_dh, uint64_t dh_stride, const void* d_x, uint
   const FfCall c = {d_x, d_gate, d_up, x_stride, gate_stride, up_stride, n, width, inner, type};
   if (const int st = check_call(c, activation)) return st;
   if (dh_stride < inner || (n && !d_dh) || (d_dx && dx_stride < width)) return EC_EINVAL;
-  if (!d_dgate != !d_dup || (!d_dx && !d_dgate)) return EC_EINVAL;
+  if (!d_dgate != !d_dup || (n && !d_dx && !d_dgate)) return EC_EINVAL;   // (a dx of no rows may have no address)
   if (d_dgate && (dgate_stride < width || dup_stride < width)) return EC_EINVAL;
   if (grad_type != EC_F32 && grad_type != type) return EC_EINVAL;
   const FfWork w = ff_work(c, true);

@@ -17,3 +17,15 @@ def test_gated_ff_without_rows(pkg, kind, width, inner):
     assert L.ec_gated_ff(*rows, 0, P, inner, None, 0, None) == pkg._lib.EC_OK
     assert L.ec_gated_ff_grad(P, inner, *rows, 0, P, width, P, width, P, width, kind, 1, None, 0, None) == pkg._lib.EC_OK
     assert L.ec_gated_ff_grad(P, inner, *rows, 0, P, width, None, 0, None, 0, kind, 0, None, 0, None) == pkg._lib.EC_OK
+
+
+@pytest.mark.parametrize("accumulate", [0, 1])
+def test_the_input_gradient_of_no_rows(pkg, accumulate):
+    """A dx without elements has no address: nothing asked for is refused where there are rows only."""
+    L = pkg._lib.lib()
+
+    def call(n):
+        return L.ec_gated_ff_grad(P, 48, P, 32, P, 32, P, 32, 1, n, 32, 48, 0, None, 32, None, 0, None, 0, 1, accumulate, P,
+                                  1 << 20, None)
+
+    assert call(0) == pkg._lib.EC_OK and call(4) == pkg._lib.EC_EINVAL
