@@ -18,8 +18,9 @@
 // A bf16 result takes fast steps, from kFastSide rows and columns on (smaller matrices are bound by the launches, and
 // their roundings average out less); an fp16 or fp32 one exact steps.
 //
-// What is stored is 2^12 times the value: X and A have entries of at most about 1.5 (the norm
-// bounds them), and ordinary ones of 1 / sqrt(columns) and less.
+// What is stored is 2^12 times the value, as ordinary entries are of 1 / sqrt(columns) and less: X has none above its largest
+// singular value, A none above that squared.  Those are 1 at first, for the norm, and with coefficients that orthogonalise about
+// 1.2 later.  Where the coefficients let them grow or shrink, the host follows them (exponents_of) and scales so that fp16 holds them.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -36,7 +37,8 @@ constexpr int kLanes = 256;
 constexpr int kAhead = 4;
 constexpr uint32_t kMostParts = 1024;     // of a matrix's sum of squares
 constexpr uint32_t kPiece = 8192;         // elements of a contiguous matrix that are summed at a time
-constexpr int kStored = 12;               // matrices are stored times 2^12
+constexpr int kStored = 12;               // matrices are stored times 2^12,
+constexpr int kMostStored = 42;           // or up to this where values shrink
 constexpr uint32_t kMostSide = 1u << 16;
 constexpr uint32_t kMostBatch = 65535;
 
@@ -92,6 +94,37 @@ __global__ void __launch_bounds__(kLanes) square_kernel(const T* x, uint64_t str
   }
   sum = block_sum<kLanes>(sum);
   if (threadIdx.x == 0) gp(parts)[blockIdx.y * gridDim.x + blockIdx.x] = sum;
+}
+
+// The exponents that a step's X, A, B and the next X (of a result 0) are stored with.
+struct Exponents {
+  int8_t x, gram, poly, next;
+};
+
+struct Coefficients {
+  float a, b, c;
+};
+
+// A step's factors between stored values.
+struct Factors {
+  float gram;       // of the product of X with itself: A
+  float poly;       // c, of ratio * A + A A, beside the diagonal: B
+  float ratio;      // b / c
+  float own;        // a, of the diagonal, or of an X that is added to B X
+  float next;       // of B X
+};
+
+__host__ __device__ __forceinline__ Factors factors_of(const Exponents& at, const Coefficients& k) {
+  Factors f;
+  f.gram = __builtin_ldexpf(1.0f, at.gram - 2 * at.x);
+  // where there is no A A, or next to none, so little of it that it is rounded off (as stored it is below 2^30) and b / c
+  // is finite
+  f.poly = k.c * __builtin_ldexpf(1.0f, at.poly - 2 * at.gram);
+  if (__builtin_fabsf(f.poly) < 0x1p-72f) f.poly = 0x1p-72f;
+  f.ratio = k.b * __builtin_ldexpf(1.0f, at.poly - at.gram) / f.poly;
+  f.own = k.a * __builtin_ldexpf(1.0f, at.poly);
+  f.next = __builtin_ldexpf(1.0f, at.next - at.poly - at.x);
+  return f;
 }
 
 typedef fp16_t __attribute__((ext_vector_type(8))) h8;
@@ -353,9 +386,10 @@ struct SmallArgs {
   char* out;
   uint64_t out_stride, out_matrix;   // elements
   uint32_t rows, cols, steps;
-  float a, b, c, scale, keep;
+  Coefficients k;
+  float scale, keep;
   double eps;
-  int at_added, at_plain;            // B is stored times 2^at: in steps that add a X, in others
+  Exponents at[EC_MAX_STEPS];
 };
 
 constexpr int kSmallSide = 128;
@@ -489,43 +523,35 @@ __global__ void __launch_bounds__(SmallShape<D>::kLanes) small_kernel(SmallArgs 
     }
     if (!kFast) acc.add(rest);
   };
-  const float one = __builtin_ldexpf(1.0f, -kStored);
-  const float square = __builtin_fabsf(p.c) > 0x1p-60f ? p.c : 0x1p-60f;   // as in run_step
   for (uint32_t s = 0; s < p.steps; ++s) {
     const bool adds = kFast && s + kPlainSteps < p.steps;
-    const int at = adds ? p.at_added : p.at_plain;
+    const Factors f = factors_of(p.at[s], p.k);
+    const float diagonal = adds ? 0.0f : f.own;
     __syncthreads();
     acc.clear();
     multiply(x, x, std::false_type());
-    acc.each([&](uint32_t m, uint32_t n, f8 v) { R::put(a, nullptr, m, n, one * v); });
+    acc.each([&](uint32_t m, uint32_t n, f8 v) { R::put(a, nullptr, m, n, f.gram * v); });
     __syncthreads();
-    acc.start([&](uint32_t m, uint32_t n) {
-      return p.b / square * __builtin_ldexpf(1.0f, kStored) * R::get(a, nullptr, m, n);
-    });
+    acc.start([&](uint32_t m, uint32_t n) { return f.ratio * R::get(a, nullptr, m, n); });
     multiply(a, a, std::false_type());
     __syncthreads();
-    const float by = square * __builtin_ldexpf(1.0f, at - 2 * kStored);
-    const float diagonal = adds ? 0.0f : p.a * __builtin_ldexpf(1.0f, at);
     acc.each([&](uint32_t m, uint32_t n, f8 v) {
-      v *= by;
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (m == n + e) v[e] += diagonal;
+      for (int e = 0; e < 8; ++e) v[e] = m == n + e ? __builtin_fmaf(v[e], f.poly, diagonal) : v[e] * f.poly;
       R::put(a, nullptr, m, n, v);
     });
     __syncthreads();
     if (adds)
-      acc.start([&](uint32_t m, uint32_t n) { return p.a * __builtin_ldexpf(1.0f, at) * R::get(x, low, m, n); });
+      acc.start([&](uint32_t m, uint32_t n) { return f.own * R::get(x, low, m, n); });
     else
       acc.clear();
     multiply(a, x, std::true_type());
-    const float down = __builtin_ldexpf(1.0f, -at);
     if (s + 1 < p.steps) {
       __syncthreads();
-      acc.each([&](uint32_t m, uint32_t n, f8 v) { R::put(x, low, m, n, down * v); });
+      acc.each([&](uint32_t m, uint32_t n, f8 v) { R::put(x, low, m, n, f.next * v); });
       continue;
     }
-    const float scale = p.scale * down * one;
+    const float scale = p.scale * f.next;
     Out* out = (Out*)p.out + matrix * p.out_matrix;
     const Out* base = (const Out*)p.base.p + matrix * p.base.matrix;
     acc.each([&](uint32_t m, uint32_t n, f8 v) {
@@ -585,7 +611,9 @@ struct Call {
   char* out;
   uint64_t out_stride, out_matrix;
   int type, out_type, steps;
-  float a, b, c, eps, scale, keep;
+  Coefficients k;
+  float eps, scale, keep;
+  Exponents at[EC_MAX_STEPS];
 };
 
 bool fast(const Plan& p, int out_type) { return out_type == EC_BF16 && p.side >= kFastSide; }
@@ -607,11 +635,48 @@ Stored stored(char* at, uint32_t batch, uint32_t rows, uint32_t cols, bool low) 
   return s;
 }
 
-int stored_at(const Call& c, bool adds) {
-  const float most = (adds ? 0.0f : std::fabs(c.a)) + 2.0f * std::fabs(c.b) + 4.0f * std::fabs(c.c);
+// The exponent that values up to `most` are stored with: at most half of what fp16 holds, as roundings may pass the bounds, and
+// so much that ordinary entries, a fraction of the largest, keep their second parts' bits.
+int stored_at(double most) {
   int at = kStored;
-  while (at > 0 && std::ldexp(most, at) > 32768.0f) --at;
+  while (std::ldexp(most, at) > 32768.0) --at;
+  while (std::ldexp(most, at) < 512.0 && at < kMostStored) ++at;
   return at;
+}
+
+// The largest singular value after a step from values in [0, most]: s (a + b s^2 + c s^4) at the end, or where
+// a + 3 b t + 5 c t^2 = 0, t = s^2.
+double largest_next(double a, double b, double c, double most) {
+  const auto at = [&](double s) { return std::fabs(s * (a + s * s * (b + c * s * s))); };
+  double next = at(most);
+  const auto turn = [&](double t) {
+    if (t > 0.0 && t < most * most) next = std::max(next, at(std::sqrt(t)));
+  };
+  const double root = std::sqrt(std::max(0.0, 9.0 * b * b - 20.0 * a * c));
+  const double q = -0.5 * (3.0 * b + std::copysign(root, b));   // both roots without cancellation
+  if (c != 0.0) turn(q / (5.0 * c));
+  if (q != 0.0) turn(a / q);
+  return next;
+}
+
+// Bounds of singular values are followed up to here: the factors stay within fp32's exponents.
+constexpr double kMostSingular = 1u << 20;
+
+// The exponents of all steps; `fast`: all but the last kPlainSteps add a X by themselves.
+void exponents_of(const Coefficients& k, int steps, bool fast, Exponents* to) {
+  const double a = k.a, b = k.b, c = k.c;
+  double most = 1.0;   // singular values of X
+  int x = kStored;
+  for (int s = 0; s < steps; ++s) {
+    const bool adds = fast && s + kPlainSteps < steps;
+    const double a_most = most * most, in_poly = std::max(2.0, a_most);
+    const int gram = stored_at(a_most);
+    const int poly = stored_at((adds ? 0.0 : std::fabs(a)) + in_poly * (std::fabs(b) + in_poly * std::fabs(c)));
+    most = std::min(largest_next(a, b, c, most), kMostSingular);
+    const int next = s + 1 < steps ? stored_at(most) : 0;
+    to[s] = {(int8_t)x, (int8_t)gram, (int8_t)poly, (int8_t)next};
+    x = next;
+  }
 }
 
 // Step s: the next step's X, or the result.
@@ -623,8 +688,7 @@ int run_step(const Plan& p, const Call& c, char* work, int s, hipStream_t st) {
   const Stored x = stored<In>(work + p.x[s & 1], p.batch, p.rows, p.cols, true);
   const Stored gram = stored<In>(work + p.gram, p.batch, p.side, p.side, false);
   const Stored poly = stored<In>(work + p.poly, p.batch, p.side, p.side, false);
-  // stored times 2^at so that (a I +) b A + c A A stays below fp16's largest value
-  const int at = stored_at(c, adds);
+  const Factors f = factors_of(c.at[s], c.k);
 
   NsArgs n = {};
   n.a = n.b = x.m;
@@ -632,7 +696,7 @@ int run_step(const Plan& p, const Call& c, char* work, int s, hipStream_t st) {
   n.a_matrix = n.b_matrix = x.matrix;
   n.K = p.other, n.M = n.N = p.side;
   n.out = work + p.gram, n.out_ld = gram.m.ld, n.out_matrix = gram.matrix;
-  n.by = std::ldexp(1.0f, -kStored);
+  n.by = f.gram;
   if (const int e = run_ns<In, TALL, TALL, kGram, In>(n, p.batch, work + p.splits, st)) return e;
 
   n.a = n.b = gram.m;
@@ -640,11 +704,7 @@ int run_step(const Plan& p, const Call& c, char* work, int s, hipStream_t st) {
   n.K = p.side;
   n.out = work + p.poly;
   n.add = work + p.gram, n.add_ld = gram.m.ld, n.add_matrix = gram.matrix;
-  // c (b / c A + A A); where there is no A A, or next to none, so little of it that it is rounded off and b / c is finite
-  const float square = std::fabs(c.c) > 0x1p-60f ? c.c : 0x1p-60f;
-  n.by = square * std::ldexp(1.0f, at - 2 * kStored);
-  n.linear = c.b / square * std::ldexp(1.0f, kStored);
-  n.diagonal = adds ? 0.0f : c.a * std::ldexp(1.0f, at);
+  n.by = f.poly, n.linear = f.ratio, n.diagonal = adds ? 0.0f : f.own;
   if (const int e = run_ns<In, false, false, kPoly, In>(n, p.batch, work + p.splits, st)) return e;
 
   // B X, X across; or X B, X along
@@ -653,16 +713,16 @@ int run_step(const Plan& p, const Call& c, char* work, int s, hipStream_t st) {
   n.a_matrix = TALL ? x.matrix : poly.matrix, n.b_matrix = TALL ? poly.matrix : x.matrix;
   n.M = p.rows, n.N = p.cols;
   n.add = adds ? x.m.p : nullptr, n.add_ld = x.m.ld, n.add_matrix = x.matrix, n.add_low = x.low;
-  n.linear = c.a * std::ldexp(1.0f, at);
+  n.linear = f.own;
   if (s + 1 < c.steps) {
     n.out = work + p.x[(s + 1) & 1], n.out_ld = x.m.ld, n.out_matrix = x.matrix;
     n.out_low = next_adds ? x.low : 0;
-    n.by = std::ldexp(1.0f, -at);
+    n.by = f.next;
     return run_ns<In, false, !TALL, kNext, In>(n, p.batch, work + p.splits, st);
   }
   const uint32_t w = type_bytes(c.out_type);
   n.out = c.out, n.out_ld = c.out_stride * w, n.out_matrix = c.out_matrix * w;
-  n.by = c.scale * std::ldexp(1.0f, -at - kStored);
+  n.by = c.scale * f.next;
   n.base = c.base, n.keep = c.keep;
   if constexpr (kFast)
     return run_ns<In, false, !TALL, kLast, bf16_t>(n, p.batch, work + p.splits, st);
@@ -688,8 +748,9 @@ void run_small(const Plan& p, const Call& c, hipStream_t st) {
   a.x = c.x, a.base = c.base;
   a.out = c.out, a.out_stride = c.out_stride, a.out_matrix = c.out_matrix;
   a.rows = p.rows, a.cols = p.cols, a.steps = (uint32_t)c.steps;
-  a.a = c.a, a.b = c.b, a.c = c.c, a.scale = c.scale, a.keep = c.keep, a.eps = (double)c.eps;
-  a.at_added = stored_at(c, true), a.at_plain = stored_at(c, false);
+  a.scale = c.scale, a.keep = c.keep, a.eps = (double)c.eps;
+  a.k = c.k;
+  std::copy(c.at, c.at + c.steps, a.at);
   if (p.other <= kSmallSide / 2)
     small_kernel<T, Out, K, kSmallSide / 2><<<p.batch, SmallShape<kSmallSide / 2>::kLanes, 0, st>>>(a);
   else
@@ -732,8 +793,9 @@ int ec_orthogonalize(const void* d_x, int type, uint64_t batch, uint64_t rows, u
   c.base = {(const char*)d_base, base_stride, base_matrix};
   c.out = (char*)d_out, c.out_stride = out_stride, c.out_matrix = out_matrix;
   c.out_type = out_type, c.steps = steps;
-  c.a = coefficients[0], c.b = coefficients[1], c.c = coefficients[2];
   c.eps = eps, c.scale = scale, c.keep = keep;
+  c.k = {coefficients[0], coefficients[1], coefficients[2]};
+  exponents_of(c.k, steps, fast(p, out_type), c.at);
   if (small(rows, cols)) {
     with_type(type, [&](auto t) {
       return with_type(out_type, [&](auto o) {

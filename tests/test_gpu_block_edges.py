@@ -1,8 +1,11 @@
-"""The block operators' edges on the GPU: empty batches."""
+"""The block operators' edges on the GPU: empty batches, iterates that grow."""
+import math
+
 import pytest
 import torch
 
-from test_gpu_step import types
+from test_gpu_block_ortho import steps_of
+from test_gpu_step import E, UNIT, gen, types
 
 pytestmark = pytest.mark.gpu
 
@@ -36,3 +39,54 @@ def test_the_input_gradient_of_no_rows(pkg, dev, dtype):
         assert got.dx is None and not got.dw_gate.any() and not got.dw_up.any()
         pkg.gated_ff(x.requires_grad_(), w[:300], w[300:]).sum().backward()
         assert x.grad.shape == x.shape
+
+
+def grown(s, abc, steps):
+    """Singular values from s on, step by step."""
+    a, b, c = abc
+    values = [s]
+    for _ in range(steps):
+        s = values[-1]
+        values.append(a * s + b * s ** 3 + c * s ** 5)
+    return values
+
+
+def nearly_one(rows, cols):
+    """A matrix whose largest singular value is close to its norm."""
+    g = gen("grown", rows, cols)
+    u, v = (torch.randn(k, 1, generator=g, dtype=torch.float64) for k in (rows, cols))
+    x = u @ v.T + 0.02 * torch.randn(rows, cols, generator=g, dtype=torch.float64)
+    return (x / x.norm()).float()
+
+
+GROWING = [((4.0, 0.0, 0.0), 2), ((4.0, 0.0, 0.0), 9), ((0.0, 0.0, 3.0), 3), ((2.5, 1.0, 0.5), 3), ((1.5, 1.5, 0.0), 4),
+           ((14.9, 0.0, 0.0), 2), ((1024.0, 0.0, 0.0), 3), ((0.01, 0.0, 0.0), 5), ((0.001, 0.0005, 0.0), 4), ((30.0, 20.0, 10.0), 2), ((0.0, 1024.0, 0.0), 2), ((0.0, 0.0, 1024.0), 2)]
+
+
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(1, 1), (60, 100), (100, 60), (150, 200), (200, 150), (300, 520)], ids=str)
+def test_growing_iterates(pkg, dev, shape, out):
+    """Coefficients that take singular values far from 1, to 2^20 or 2^-30 before the last step.
+
+    With a, b, c >= 0 a step p stretches a difference by at most p'(s) at the largest singular value s, and s p' <= 5 p: errors
+    relative to it grow by 5 a step at most.  A step's own, relative to p(s) and over `side` singular values: X is in it five times,
+    A twice, B once as stored, and so are the products' left out second parts, and four sums of `other` terms, whose
+    roundings by at most 2 E are independent.  X as stored has 22 bits, or 11 for a bf16 result of 64 rows and more."""
+    x = nearly_one(*shape)
+    side, other = min(shape), max(shape)
+    bits = 11 if out == torch.bfloat16 and side >= 64 else 22
+    own = 12 * 2.0 ** -bits + 4 * 2 * E * math.sqrt(other)
+    for abc, steps in GROWING:
+        want = steps_of(x.double(), steps, abc)
+        most = grown(float(torch.linalg.matrix_norm(x.double(), 2)), abc, steps)[-1]
+        got = pkg.orthogonalize(x.to(dev), steps=steps, coefficients=abc, dtype=out).double().cpu()
+        assert bool(got.isfinite().all()), (abc, steps)
+        bound = most * math.sqrt(side) * own * sum(5.0 ** k for k in range(steps)) + 1.01 * UNIT[out] * float(want.norm())
+        assert float((got - want).norm()) <= bound, (abc, steps, float((got - want).norm()) / most)
+
+
+@pytest.mark.parametrize("shape", [(1, 1), (60, 100), (150, 200)], ids=str)
+def test_iterates_past_the_range_are_not_finite(pkg, dev, shape):
+    """2^30 before the last step: past 2^20, and said by what comes out."""
+    got = pkg.orthogonalize(nearly_one(*shape).to(dev), steps=4, coefficients=(1024.0, 0.0, 0.0))
+    assert not bool(got.isfinite().all())
