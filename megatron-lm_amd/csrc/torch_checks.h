@@ -34,6 +34,9 @@ inline at::ScalarType torch_type(int64_t code) {
 }
 
 inline void check_device(const Tensor& t, const char* what, const c10::Device* device) {
+  // (the operators have no forward-mode derivatives, and a result without a tangent would pass for one whose is zero)
+  if (t._fw_grad(/*level=*/0).defined())
+    throw py::value_error(std::string(what) + " has a forward-mode tangent, which the operators do not pass on");
   if (!t.is_cuda()) throw py::value_error(std::string(what) + " must be a device (HIP) tensor");
   if (device && t.device() != *device)
     throw py::value_error(std::string(what) + " is on " + t.device().str() +

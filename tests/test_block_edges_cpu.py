@@ -3,6 +3,8 @@ never touched."""
 import ctypes
 
 import pytest
+import torch
+from torch.autograd import forward_ad
 
 P = ctypes.c_void_p(4096)
 
@@ -29,3 +31,18 @@ def test_the_input_gradient_of_no_rows(pkg, accumulate):
                                   1 << 20, None)
 
     assert call(0) == pkg._lib.EC_OK and call(4) == pkg._lib.EC_EINVAL
+
+
+def test_tangents_are_refused(pkg):
+    """Forward-mode derivatives are not had, and not dropped either: of every operand, of the step's operators too."""
+    w, v, p = torch.ones(4, 8), torch.ones(8), torch.ones(3, 4)
+    tokens = torch.zeros(3, dtype=torch.int64)
+    with forward_ad.dual_level():
+        x = forward_ad.make_dual(torch.ones(3, 8), torch.ones(3, 8))
+        for call in (lambda: pkg.gated_ff(x, w, w), lambda: pkg.gated_ff_grad(p, x, w, w),
+                     lambda: pkg.residual_norm(x, weight=v), lambda: pkg.residual_norm_grad(x, None, x, x),
+                     lambda: pkg.orthogonalize(x), lambda: pkg.embed(tokens, x), lambda: pkg.token_logprobs(x, tokens)):
+            with torch.no_grad(), pytest.raises(ValueError, match="tangent"):
+                call()
+            with pytest.raises(ValueError, match="tangent"):
+                call()

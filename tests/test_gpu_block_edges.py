@@ -1,8 +1,9 @@
-"""The block operators' edges on the GPU: empty batches, iterates that grow."""
+"""The block operators' edges on the GPU: empty batches, iterates that grow, tangents."""
 import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from test_gpu_block_ortho import steps_of
 from test_gpu_step import E, UNIT, gen, types
@@ -90,3 +91,24 @@ def test_iterates_past_the_range_are_not_finite(pkg, dev, shape):
     """2^30 before the last step: past 2^20, and said by what comes out."""
     got = pkg.orthogonalize(nearly_one(*shape).to(dev), steps=4, coefficients=(1024.0, 0.0, 0.0))
     assert not bool(got.isfinite().all())
+
+
+def test_tangents_are_refused(pkg, dev):
+    """A tangent of any operand, and what torch's own transforms make of one."""
+    one, v = torch.ones(8, 8, device=dev), torch.ones(8, device=dev)
+    tokens = torch.zeros(8, dtype=torch.int64, device=dev)
+    calls = {"x": lambda t: pkg.gated_ff(t, one, one), "w_up": lambda t: pkg.gated_ff(one, one, t),
+             "dh": lambda t: pkg.gated_ff_grad(t, one, one, one), "branch": lambda t: pkg.residual_norm(one, t, weight=v),
+             "weight": lambda t: pkg.residual_norm(one, weight=t[0].clone()), "gate": lambda t: pkg.residual_norm(one, one, gate=t),
+             "dresidual": lambda t: pkg.residual_norm_grad(t, None, one, one), "base": lambda t: pkg.orthogonalize(one, base=t),
+             "table": lambda t: pkg.embed(tokens, t), "logits": lambda t: pkg.token_logprobs(t, tokens),
+             "dout": lambda t: pkg.embed_grad(tokens, t, 8)}
+    for name, call in calls.items():
+        with forward_ad.dual_level(), pytest.raises(ValueError, match=f"{name} has a forward-mode tangent"):
+            call(forward_ad.make_dual(one, one))
+        with pytest.raises((ValueError, RuntimeError)):
+            torch.func.jvp(call, (one,), (one,))
+        call(one)
+    leaf = one.clone().requires_grad_()
+    with forward_ad.dual_level(), pytest.raises((ValueError, RuntimeError, NotImplementedError)):
+        pkg.gated_ff(forward_ad.make_dual(leaf, one), one, one)
