@@ -46,3 +46,24 @@ def test_tangents_are_refused(pkg):
                 call()
             with pytest.raises(ValueError, match="tangent"):
                 call()
+
+
+def test_calls_without_gradients_of_their_own_refuse_operands_that_need_one(pkg):
+    """With gradients enabled their results would be cut from the graph; not under no_grad, where an update belongs."""
+    x, p, w, v, r = torch.ones(3, 8), torch.ones(3, 4), torch.ones(4, 8), torch.ones(8), torch.ones(3)
+    calls = {
+        "gated_ff_grad": (lambda **k: pkg.gated_ff_grad(*k.values()), dict(dh=p, x=x, w_gate=w, w_up=w)),
+        "residual_norm_grad": (lambda dr, dn, t, b, **k: pkg.residual_norm_grad(dr, dn, t, b, **k),
+                               dict(dr=x, dn=x, t=x, b=x, rstd=r, branch_rstd=r, gate=v, branch_weight=v, weight=v)),
+        "orthogonalize": (lambda x, **k: pkg.orthogonalize(x, **k), dict(x=w, base=w, out=w))}
+    for name, (call, operands) in calls.items():
+        for which in operands:
+            one = {k: t.clone().requires_grad_() if k == which else t for k, t in operands.items()}
+            with pytest.raises(ValueError, match=f"{name} has no gradient"):
+                call(**one)
+            with torch.no_grad(), pytest.raises(ValueError, match="device"):   # host tensors, and nothing else
+                call(**one)
+        with pytest.raises(ValueError, match="device"):
+            call(**operands)
+    with pytest.raises(ValueError, match="gated_ff_grad has no gradient"):
+        pkg.gated_ff_grad(p, x, w, w, out=(w, w.clone().requires_grad_()))
