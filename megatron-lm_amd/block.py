@@ -106,6 +106,9 @@ def gated_ff_grad(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up:
         raise ValueError(f"dtype must be float32, bfloat16 or float16, not {dtype}")
     if out is not None and len(out) != 2:
         raise ValueError("out must be a pair of tensors")
+    for t in out or ():
+        if dtype is not None and getattr(t, "dtype", dtype) != dtype:
+            raise ValueError(f"out is {t.dtype}, dtype {dtype}")
     _no_graph("gated_ff_grad", dh, x, w_gate, w_up, *(out or ()))
     dtype = dtype or getattr(x, "dtype", None)
     return GatedGrads(*_call(

@@ -67,3 +67,13 @@ def test_calls_without_gradients_of_their_own_refuse_operands_that_need_one(pkg)
             call(**operands)
     with pytest.raises(ValueError, match="gated_ff_grad has no gradient"):
         pkg.gated_ff_grad(p, x, w, w, out=(w, w.clone().requires_grad_()))
+
+
+def test_a_dtype_other_than_that_of_out_is_refused(pkg):
+    x, p, w = (torch.ones(s, dtype=torch.bfloat16) for s in ((3, 8), (3, 4), (4, 8)))
+    for out in ((w, w), (w.float(), w), (w, w.float())):
+        with pytest.raises(ValueError, match="out is torch.bfloat16, dtype torch.float32"):
+            pkg.gated_ff_grad(p, x, w, w, dtype=torch.float32, out=out)
+    for dtype in (None, torch.bfloat16):   # the host tensors are what is left to refuse
+        with pytest.raises(ValueError, match="device"):
+            pkg.gated_ff_grad(p, x, w, w, dtype=dtype, out=(w, w))
