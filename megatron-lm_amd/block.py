@@ -106,14 +106,15 @@ def gated_ff_grad(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up:
         raise ValueError(f"dtype must be float32, bfloat16 or float16, not {dtype}")
     if out is not None and len(out) != 2:
         raise ValueError("out must be a pair of tensors")
-    for t in out or ():
+    pair = (None, None) if out is None else tuple(out)
+    for t in pair:
         if dtype is not None and getattr(t, "dtype", dtype) != dtype:
             raise ValueError(f"out is {t.dtype}, dtype {dtype}")
-    _no_graph("gated_ff_grad", dh, x, w_gate, w_up, *(out or ()))
+    _no_graph("gated_ff_grad", dh, x, w_gate, w_up, *pair)
     dtype = dtype or getattr(x, "dtype", None)
     return GatedGrads(*_call(
         "ec_gated_ff_grad", _lib.shards().gated_ff_grad, x, stream, dh, x, w_gate, w_up, _activation(activation),
-        bool(inputs), bool(weights), _TYPES.get(dtype, 0), *(out if out is not None else (None, None)), accumulate)[:3])
+        bool(inputs), bool(weights), _TYPES.get(dtype, 0), *pair, accumulate)[:3])
 
 
 # ------------------------------------------------- norms around a block --

@@ -77,3 +77,11 @@ def test_a_dtype_other_than_that_of_out_is_refused(pkg):
     for dtype in (None, torch.bfloat16):   # the host tensors are what is left to refuse
         with pytest.raises(ValueError, match="device"):
             pkg.gated_ff_grad(p, x, w, w, dtype=dtype, out=(w, w))
+
+
+def test_a_pair_in_one_tensor_is_a_pair(pkg):
+    x, p, w = torch.ones(3, 8), torch.ones(3, 4), torch.ones(4, 8)
+    with pytest.raises(ValueError, match="device"):
+        pkg.gated_ff_grad(p, x, w, w, out=torch.ones(2, 4, 8))
+    with pytest.raises(ValueError, match="pair"):
+        pkg.gated_ff_grad(p, x, w, w, out=torch.ones(0, 4, 8))

@@ -112,3 +112,12 @@ def test_tangents_are_refused(pkg, dev):
     leaf = one.clone().requires_grad_()
     with forward_ad.dual_level(), pytest.raises((ValueError, RuntimeError, NotImplementedError)):
         pkg.gated_ff(forward_ad.make_dual(leaf, one), one, one)
+
+
+def test_a_pair_in_one_tensor(pkg, dev):
+    """The weights' gradients into the halves of one tensor [2, inner, width], given as it is."""
+    x, w, dh = (torch.randn(*s, device=dev) for s in ((40, 24), (32, 24), (40, 16)))
+    want = pkg.gated_ff_grad(dh, x, w[:16], w[16:])
+    out = torch.empty(2, 16, 24, device=dev)
+    pkg.gated_ff_grad(dh, x, w[:16], w[16:], dtype=torch.float32, out=out)
+    assert torch.equal(out[0], want.dw_gate) and torch.equal(out[1], want.dw_up)
