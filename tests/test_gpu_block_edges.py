@@ -1,12 +1,13 @@
-"""The block operators' edges on the GPU: empty batches, iterates that grow, tangents."""
+"""The block operators' edges on the GPU: empty batches, iterates that grow, tangents, longest rows."""
 import math
 
 import pytest
 import torch
 from torch.autograd import forward_ad
 
+import test_gpu_block_norms as norms
 from test_gpu_block_ortho import steps_of
-from test_gpu_step import E, UNIT, gen, types
+from test_gpu_step import E, UNIT, check, gen, rounded, types
 
 pytestmark = pytest.mark.gpu
 
@@ -121,3 +122,27 @@ def test_a_pair_in_one_tensor(pkg, dev):
     out = torch.empty(2, 16, 24, device=dev)
     pkg.gated_ff_grad(dh, x, w[:16], w[16:], dtype=torch.float32, out=out)
     assert torch.equal(out[0], want.dw_gate) and torch.equal(out[1], want.dw_up)
+
+
+@pytest.mark.parametrize("dtype,n,width,gates", [
+    (torch.float32, 301, 9001, 1), (torch.float32, 600, 8200, 300), (torch.float32, 603, 16384, 603),
+    (torch.bfloat16, 1301, 9001, 1), (torch.bfloat16, 600, 8200, 300), (torch.float16, 603, 16384, 603),
+    (torch.float16, 1800, 8203, 600), (torch.float32, 1100, 8193, 4)], ids=str)
+def test_longest_rows(pkg, dev, dtype, n, width, gates):
+    """Rows whose sums over rows are partly in LDS, for teams of several rows: parts of a gate's rows, and whole gates, whose
+    sums are written and begun anew row by row of the gate."""
+    o = norms.operands(dtype, n, width, gates, True, True)
+    o = {k: v.to(dev) for k, v in o.items()}
+    rest = {k: o[k] for k in ("gate", "branch_weight", "weight")}
+    r = pkg.residual_norm(o["residual"], o["branch"], scale=0.4, **rest)
+    for name, (value, bound) in norms.forward(o, 0.4).items():
+        check(getattr(r, name), value, rounded(value, getattr(r, name).dtype, bound).cpu(), name)
+    g = gen("dlongest", n, width)
+    ds, dn = (torch.randn(n, width, generator=g).to(dtype).to(dev) for _ in range(2))
+    saved = dict(rstd=r.rstd, branch_rstd=r.branch_rstd, scale=0.4, **rest)
+    got = pkg.residual_norm_grad(ds, dn, r.residual, o["branch"], **saved)
+    for name, (value, bound) in norms.gradients(o, r.residual, ds, dn, r.rstd, r.branch_rstd, 0.4).items():
+        v = getattr(got, name)
+        check(v, value, rounded(value, v.dtype, bound * 1.05).cpu(), name)
+    again = pkg.residual_norm_grad(ds, dn, r.residual, o["branch"], **saved)
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
