@@ -36,12 +36,6 @@ def _differentiable(*tensors) -> bool:
     return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
 
 
-def _no_graph(name: str, *tensors) -> None:
-    """Nobody takes a result for a differentiable one that is not."""
-    if _differentiable(*tensors):
-        raise ValueError(f"{name} has no gradient: call it under torch.no_grad(), or with detached tensors")
-
-
 def _plain(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return None if t is None else t.detach()
 
@@ -110,7 +104,6 @@ def gated_ff_grad(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up:
     for t in pair:
         if dtype is not None and getattr(t, "dtype", dtype) != dtype:
             raise ValueError(f"out is {t.dtype}, dtype {dtype}")
-    _no_graph("gated_ff_grad", dh, x, w_gate, w_up, *pair)
     dtype = dtype or getattr(x, "dtype", None)
     return GatedGrads(*_call(
         "ec_gated_ff_grad", _lib.shards().gated_ff_grad, x, stream, dh, x, w_gate, w_up, _activation(activation),
@@ -202,7 +195,6 @@ def residual_norm_grad(dresidual: Optional[torch.Tensor], dnormed: Optional[torc
     """The gradients of ``residual_norm`` from those of its stream (``dresidual``) and its normed rows (``dnormed``;
     one of them may be None), with the stream ``total``, ``rstd`` and ``branch_rstd`` that it returned and the
     branch, gate and weights that it was given.  The weights' and the gate's are sums over rows in fixed places."""
-    _no_graph("residual_norm_grad", dresidual, dnormed, total, branch, rstd, branch_rstd, gate, branch_weight, weight)
     return ResidualNormGrads(*_call(
         "ec_residual_norm_grad", _lib.shards().residual_norm_grad, total, stream, dresidual, dnormed, total, branch,
         rstd, branch_rstd, gate, _finite(scale, "scale"), branch_weight, weight)[:5])
@@ -240,6 +232,5 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Sequence[flo
         raise ValueError(f"dtype must be float32, bfloat16 or float16, not {dtype}")
     if out is not None and dtype is not None and getattr(out, "dtype", dtype) != dtype:
         raise ValueError(f"out is {out.dtype}, dtype {dtype}")
-    _no_graph("orthogonalize", x, base, out)
     return _call("ec_orthogonalize", _lib.shards().orthogonalize, x, stream, x, steps, a, b, c, eps,
                  _finite(scale, "scale"), base, _finite(keep, "keep"), -1 if dtype is None else _TYPES[dtype], out)[0]

@@ -11,6 +11,16 @@ Tensor bytes_on(const c10::Device& device, uint64_t n) {
   return at::empty({(int64_t)n}, at::TensorOptions().dtype(at::kByte).device(device));
 }
 
+// Nobody takes a result for a differentiable one that is not.
+bool needs_grad(const Tensor& t) { return t.requires_grad(); }
+bool needs_grad(const std::optional<Tensor>& t) { return t && t->requires_grad(); }
+template <typename... T>
+void no_graph(const char* name, const T&... operands) {
+  if (at::GradMode::is_enabled() && (needs_grad(operands) || ...))
+    throw py::value_error(std::string(name) +
+                          " has no gradient: call it under torch.no_grad(), or with detached tensors");
+}
+
 uint32_t narrow(uint64_t v) { return (uint32_t)std::min<uint64_t>(v, 0xffffffffull); }
 
 Rows weight_rows(const Tensor& t, const char* what, const Tensor& x, const Rows& rows) {
@@ -102,6 +112,7 @@ py::tuple gated_ff_grad(const Tensor& dh, const Tensor& x, const Tensor& gate, c
                         int64_t activation, bool with_dx, bool with_dw, int64_t grad_type,
                         std::optional<Tensor> dgate_out, std::optional<Tensor> dup_out,
                         bool accumulate) {
+  no_graph("gated_ff_grad", dh, x, gate, up, dgate_out, dup_out);
   const Ff f = ff_of(x, gate, up);
   const c10::Device device = x.device();
   const c10::DeviceGuard guard(device);
@@ -171,6 +182,7 @@ bool same_place(const Tensor& a, const Tensor& b) {
 py::tuple orthogonalize(const Tensor& x, int64_t steps, double a, double b, double c, double eps,
                         double scale, std::optional<Tensor> base, double keep, int64_t out_type,
                         std::optional<Tensor> out) {
+  no_graph("orthogonalize", x, base, out);
   const int type = type_code(x, "x");
   const Matrix m = matrix_of(x, "x", nullptr);
   const c10::Device device = x.device();
@@ -294,6 +306,7 @@ py::tuple residual_norm_grad(std::optional<Tensor> dsum, std::optional<Tensor> d
                              std::optional<Tensor> rstd, std::optional<Tensor> branch_rstd,
                              std::optional<Tensor> gate, double scale,
                              std::optional<Tensor> branch_weight, std::optional<Tensor> weight) {
+  no_graph("residual_norm_grad", dsum, dnormed, sum, branch, rstd, branch_rstd, gate, branch_weight, weight);
   const int type = type_code(sum, "sum");
   const Rows rows = rows_of(sum, "sum", nullptr);
   const c10::Device device = sum.device();
