@@ -102,7 +102,7 @@ struct Exponents {
 };
 
 struct Coefficients {
-  float a, b, c;
+  float a, b, c, b_by_c;   // b / c where it is finite
 };
 
 // A step's factors between stored values.
@@ -120,8 +120,9 @@ __host__ __device__ __forceinline__ Factors factors_of(const Exponents& at, cons
   // where there is no A A, or next to none, so little of it that it is rounded off (as stored it is below 2^30) and b / c
   // is finite
   f.poly = k.c * __builtin_ldexpf(1.0f, at.poly - 2 * at.gram);
-  if (__builtin_fabsf(f.poly) < 0x1p-72f) f.poly = 0x1p-72f;
-  f.ratio = k.b * __builtin_ldexpf(1.0f, at.poly - at.gram) / f.poly;
+  const bool none = __builtin_fabsf(f.poly) < 0x1p-72f;
+  f.ratio = none ? __builtin_ldexpf(k.b, at.poly - at.gram + 72) : __builtin_ldexpf(k.b_by_c, at.gram);
+  f.poly = none ? 0x1p-72f : f.poly;
   f.own = k.a * __builtin_ldexpf(1.0f, at.poly);
   f.next = __builtin_ldexpf(1.0f, at.next - at.poly - at.x);
   return f;
@@ -794,7 +795,8 @@ int ec_orthogonalize(const void* d_x, int type, uint64_t batch, uint64_t rows, u
   c.out = (char*)d_out, c.out_stride = out_stride, c.out_matrix = out_matrix;
   c.out_type = out_type, c.steps = steps;
   c.eps = eps, c.scale = scale, c.keep = keep;
-  c.k = {coefficients[0], coefficients[1], coefficients[2]};
+  c.k = {coefficients[0], coefficients[1], coefficients[2], 0.0f};
+  if (std::isfinite(c.k.b / c.k.c)) c.k.b_by_c = c.k.b / c.k.c;
   exponents_of(c.k, steps, fast(p, out_type), c.at);
   if (small(rows, cols)) {
     with_type(type, [&](auto t) {
