@@ -382,14 +382,15 @@ int run_ns(NsArgs& p, uint32_t batch, char* parts, hipStream_t st) {
 // A matrix of at most D x D: one workgroup takes all steps, with everything in LDS, one launch instead of seventeen.  A tall
 // matrix is taken transposed.  A matrix lies there as D-row tiles along k, one behind another; B takes A's place and
 // the next X that of X, when all waves have read them.
+// (Those of ordinary calls are in the first 128 bytes, two lines, to the fifth step's exponents.)
 struct SmallArgs {
   Matrices x, base;
   char* out;
   uint64_t out_stride, out_matrix;   // elements
-  uint32_t rows, cols, steps;
+  uint16_t rows, cols;
+  uint32_t steps;
   Coefficients k;
-  float scale, keep;
-  double eps;
+  float scale, keep, eps;
   Exponents at[EC_MAX_STEPS];
 };
 
@@ -471,7 +472,7 @@ __global__ void __launch_bounds__(SmallShape<D>::kLanes) small_kernel(SmallArgs 
 #pragma unroll
       for (int e = 0; e < 8; ++e) sum = __builtin_fma((double)v[g][e], (double)v[g][e], sum);
     }
-    const double by = (double)(1 << kStored) / (__builtin_sqrt(block_sum<S::kLanes>(sum)) + p.eps);
+    const double by = (double)(1 << kStored) / (__builtin_sqrt(block_sum<S::kLanes>(sum)) + (double)p.eps);
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
       const uint32_t at = g * S::kLanes + threadIdx.x, row = at / (D / 8), col = at % (D / 8) * 8;
@@ -526,9 +527,9 @@ __global__ void __launch_bounds__(SmallShape<D>::kLanes) small_kernel(SmallArgs 
   };
   for (uint32_t s = 0; s < p.steps; ++s) {
     const bool adds = kFast && s + kPlainSteps < p.steps;
-    const Factors f = factors_of(p.at[s], p.k);
-    const float diagonal = adds ? 0.0f : f.own;
     __syncthreads();
+    const Factors f = factors_of(p.at[s], p.k);   // behind the barrier: 64 x 64 9.3 us, before it 9.5
+    const float diagonal = adds ? 0.0f : f.own;
     acc.clear();
     multiply(x, x, std::false_type());
     acc.each([&](uint32_t m, uint32_t n, f8 v) { R::put(a, nullptr, m, n, f.gram * v); });
@@ -639,10 +640,10 @@ Stored stored(char* at, uint32_t batch, uint32_t rows, uint32_t cols, bool low) 
 // The exponent that values up to `most` are stored with: at most half of what fp16 holds, as roundings may pass the bounds, and
 // so much that ordinary entries, a fraction of the largest, keep their second parts' bits.
 int stored_at(double most) {
-  int at = kStored;
-  while (std::ldexp(most, at) > 32768.0) --at;
-  while (std::ldexp(most, at) < 512.0 && at < kMostStored) ++at;
-  return at;
+  int e;
+  const bool exact = std::frexp(most, &e) == 0.5;   // most is in [2^(e - 1), 2^e)
+  const int high = 15 - e + exact, low = 10 - e;    // most 2^high is at most 2^15, most 2^low at least 2^9
+  return std::max(std::min(kStored, high), std::min(kMostStored, most > 0.0 ? low : kMostStored));
 }
 
 // The largest singular value after a step from values in [0, most]: s (a + b s^2 + c s^4) at the end, or where
@@ -748,8 +749,8 @@ void run_small(const Plan& p, const Call& c, hipStream_t st) {
   SmallArgs a = {};
   a.x = c.x, a.base = c.base;
   a.out = c.out, a.out_stride = c.out_stride, a.out_matrix = c.out_matrix;
-  a.rows = p.rows, a.cols = p.cols, a.steps = (uint32_t)c.steps;
-  a.scale = c.scale, a.keep = c.keep, a.eps = (double)c.eps;
+  a.rows = (uint16_t)p.rows, a.cols = (uint16_t)p.cols, a.steps = (uint32_t)c.steps;
+  a.scale = c.scale, a.keep = c.keep, a.eps = c.eps;
   a.k = c.k;
   std::copy(c.at, c.at + c.steps, a.at);
   if (p.other <= kSmallSide / 2)
