@@ -498,8 +498,9 @@ int ec_gated_ff(const void* d_x, uint64_t x_stride, const void* d_gate, uint64_t
  * g and u are computed again. dx is of `type`; dgate and dup are of grad_type (EC_F32 or
  * `type`), written, or added to where accumulate is 1. dx, or both others, may be null: not
  * computed. dg and du are rounded to `type` for the products (with 256 rows and fewer they keep
- * their rounding error as a second part); sums are in fp32, each result is rounded once. n 0: dgate
- * and dup are zeros, or left as they are. */
+ * their rounding error as a second part): 1.7e-3 of a bf16 gradient, also of an fp32 dgate. In fp16 a dg or du past 65504 is
+ * infinite, and what it is part of not finite. Sums are in fp32, each result is rounded once. n 0: dgate and dup are zeros, or
+ * left as they are. */
 int ec_gated_ff_grad(const void* d_dh, uint64_t dh_stride, const void* d_x, uint64_t x_stride,
                      const void* d_gate, uint64_t gate_stride, const void* d_up, uint64_t up_stride,
                      int type, uint64_t n, uint32_t width, uint32_t inner, int activation, void* d_dx,

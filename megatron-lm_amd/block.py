@@ -92,8 +92,9 @@ def gated_ff_grad(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up:
 
     The weights' gradients are of ``dtype``, x's type (the default) or float32, or of that of ``out``, a pair
     of tensors that they are written to, or with ``accumulate`` added to (a micro-batch's part of a gradient buffer).
-    The gradients of the two projections, which the products read, are rounded to x's type; with 256 rows or
-    fewer, whose roundings average out less, their rounding errors are taken along."""
+    The gradients of the two projections, which the products read, are rounded to x's type (in fp16, past 65504, to
+    infinities, and results are not finite); with 256 rows or fewer, whose roundings average out less, their rounding errors
+    are taken along."""
     if not inputs and not weights:
         raise ValueError("neither the inputs' nor the weights' gradients are asked for")
     if dtype is not None and dtype not in _TYPES:

@@ -146,3 +146,21 @@ def test_longest_rows(pkg, dev, dtype, n, width, gates):
         check(v, value, rounded(value, v.dtype, bound * 1.05).cpu(), name)
     again = pkg.residual_norm_grad(ds, dn, r.residual, o["branch"], **saved)
     assert all(torch.equal(a, b) for a, b in zip(got, again))
+
+
+@pytest.mark.parametrize("n", [5, 300])
+def test_fp16_gradients_past_the_type_are_not_finite(pkg, dev, n):
+    """dg = dh u act' past 65504 is infinite, as any fp16 gradient, and shows in every result that it is part of; the rows and
+    outputs beside it stay."""
+    g = gen("overflow", n)
+    x = torch.randn(n, 64, generator=g).half()
+    w = (torch.randn(96, 64, generator=g) / 80).half()
+    dh = torch.randn(n, 48, generator=g).half()
+    x[2] = 4.0
+    w[48 + 7], w[7] = 1.0, 0.01   # u = 256, g = 2.56 of row 2, output 7
+    dh[2, 7] = 6e4
+    got = pkg.gated_ff_grad(dh.to(dev), x.to(dev), w[:48].to(dev), w[48:].to(dev), dtype=torch.float32)
+    assert not got.dx[2].isfinite().any() and not got.dw_gate[7].isfinite().any()
+    rows, outputs = [i for i in range(n) if i != 2], [i for i in range(48) if i != 7]
+    assert bool(got.dx[rows].isfinite().all())
+    assert bool(got.dw_gate[outputs].isfinite().all()) and bool(got.dw_up[outputs].isfinite().all())
