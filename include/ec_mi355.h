@@ -522,11 +522,12 @@ uint64_t ec_orthogonalize_workspace(uint64_t batch, uint64_t rows, uint64_t cols
  * up to 1024: each singular value s of X becomes a s + b s^3 + c s^5. base null: out = scale * X; base may be out.
  * base and out are of out_type. Row strides and the distances from matrix to matrix are in elements.
  * Products are of values of 22 bits, in fp32 sums, and |x| is summed in fp64; where out is bf16 and rows and cols are 64 or
- * more, products are of 11 bits, added to a X with 22: about 1e-3 of the result. What is stored between products is
- * scaled for the largest singular values that the coefficients can give, from 1 on, 2^-30 to 2^20 before the last
- * step; larger ones may come out infinite or NaN, smaller ones as zeros. A matrix with a value that is not finite gives NaN; one of zeros gives
- * keep * base. A matrix whose |x| is far below eps keeps fewer bits. EC_ERANGE for rows or cols > 65536, batch > 65535, steps past
- * EC_MAX_STEPS or below 1, or a launch of 2^32 lanes. */
+ * more, products are of 11 bits, added to a X with 22: about 1e-3 of the result, up to 3e-3 where x has a single nonzero
+ * row (an fp32 out has 22 bits of any x). What is stored between products is scaled for the largest singular values that the
+ * coefficients can give, from 1 on, 2^-30 to 2^20 before the last step; larger ones may come out infinite or NaN, smaller
+ * ones as zeros. A matrix with a value that is not finite gives NaN; one of zeros gives keep * base. A matrix whose |x| is
+ * far below eps keeps fewer bits. EC_ERANGE for rows or cols > 65536, batch > 65535, steps past EC_MAX_STEPS or below 1, or
+ * a launch of 2^32 lanes. */
 int ec_orthogonalize(const void* d_x, int type, uint64_t batch, uint64_t rows, uint64_t cols,
                      uint64_t x_stride, uint64_t x_matrix, int steps, const float* coefficients,
                      float eps, float scale, const void* d_base, uint64_t base_stride,

@@ -218,7 +218,8 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Sequence[flo
     A weight update in place: ``orthogonalize(momentum, scale=-lr, base=weight, keep=1 - lr * decay, out=weight)``.
     The result is of ``out``'s type, or ``dtype``, or the base's, or x's; base and out are of the same.  Products
     are of values of 22 bits with fp32 sums; for a bf16 result with 64 or more rows and columns of
-    11 bits, added to a X with 22, which leaves about 1e-3 of the result.  The coefficients are of magnitude up to 1024, and may
+    11 bits, added to a X with 22, which leaves about 1e-3 of the result, up to 3e-3 where x has a single nonzero row
+    (``dtype=torch.float32`` takes 22 whatever x is).  The coefficients are of magnitude up to 1024, and may
     take singular values from 1 to 2^-30 or 2^20 before the last step (results of larger ones may be infinite or NaN, of
     smaller ones zeros).  A value that is not finite makes its matrix NaN."""
     steps = int(steps)

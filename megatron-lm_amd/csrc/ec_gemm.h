@@ -19,7 +19,7 @@
 //
 // Pairs: a value as the sum of two fp16 ones, 22 bits of significand: eight high parts, then the
 // eight low parts, in 32 bytes.  A product of two pairs takes three of the matrix cores' products
-// (the low parts' is below the fp32 accumulator's rounding), at 3/16 of the time of fp32 products.  The matrix
+// (the low parts' is below the fp32 accumulator's rounding), at three tenths of the time of fp32 products.  The matrix
 // cores truncate where they add to an accumulator, so the two small products have accumulators of their own, which
 // are added at the end: five Newton-Schulz steps on 1001 x 777 are 3.5e-6 off with one accumulator, 2.0e-6 with two, and
 // those of fp32 products 2.3e-6.

@@ -8,13 +8,14 @@
 // Small singular values grow by `a` a step, and so do the rounding errors of what is
 // stored in between: with X, A and B in 16 bits 0.2 % (fp16) or 2 % (bf16) of the result after five
 // steps.  There are two kinds of steps:
-// - exact ones: all matrices are pairs of fp16 values (22 bits, ec_gemm.h).  The result is as good as that of
-//   fp32 products (4.5e-7 off after five steps), at a third of the fp16 rate instead of a sixteenth.
+// - exact ones: all matrices are pairs of fp16 values (22 bits, ec_gemm.h).  The result is as good as that of fp32 products
+//   (five steps, off by 1.2e-6 at 128 x 128, 2.0e-6 at 1001 x 777 and 2.7e-6 at 2048 x 2048, where those are by 1.4e-6, 2.3e-6
+//   and 2.9e-6; at 16 x 256 9.5e-7 against 7.4e-7), at a third of the fp16 rate instead of a tenth.
 // - fast ones: the products are of fp16 values, but all but the last two steps take X = a X + (b A + c A A) X, and
 //   the X that a stands before has a second fp16 part.  What small singular values consist of is that first
 //   term; the products' errors are small where they are.  Five steps leave 0.7e-3 to 0.8e-3 of the result
 //   (with second parts in the last two steps too 0.8e-3 to 1.1e-3, without any 1.9e-3 to 2.5e-3), against 1.7e-3 by the
-//   rounding to bf16; an update of a single nonzero row, whose roundings do not average out, has 2e-3 to 4e-3.
+//   rounding to bf16; an update of a single nonzero row, whose roundings do not average out, has 1.5e-3 to 2.7e-3.
 // A bf16 result takes fast steps, from kFastSide rows and columns on (smaller matrices are bound by the launches, and
 // their roundings average out less); an fp16 or fp32 one exact steps.
 //
