@@ -6,7 +6,7 @@ import torch
 from torch.autograd import forward_ad
 
 import test_gpu_block_norms as norms
-from test_gpu_block_ortho import steps_of
+from test_gpu_block_ortho import steps_of, update
 from test_gpu_step import E, UNIT, check, gen, rounded, types
 
 pytestmark = pytest.mark.gpu
@@ -164,3 +164,18 @@ def test_fp16_gradients_past_the_type_are_not_finite(pkg, dev, n):
     rows, outputs = [i for i in range(n) if i != 2], [i for i in range(48) if i != 7]
     assert bool(got.dx[rows].isfinite().all())
     assert bool(got.dw_gate[outputs].isfinite().all()) and bool(got.dw_up[outputs].isfinite().all())
+
+
+@pytest.mark.parametrize("out", [torch.float32, torch.float16])
+@pytest.mark.parametrize("shape", [(128, 128), (100, 60), (60, 100), (127, 65), (64, 64), (300, 90), (129, 200)], ids=str)
+def test_small_updates_keep_22_bits(pkg, dev, shape, out):
+    """Within eight times the error of the same steps in fp32, whose values have 24 bits, by rows and columns too (against the largest
+    one's); products of 11 bits are a hundred times that.  A result's own rounding has a mean square of a third of its
+    bound's, and over a row's values not above it."""
+    x = update(torch.float32, *shape)
+    want = steps_of(x.double())
+    near = steps_of(x).double() - want
+    far = pkg.orthogonalize(x.to(dev), dtype=out).double().cpu() - want
+    assert float(far.norm()) <= 8 * float(near.norm()) + 0.6 * UNIT[out] * float(want.norm())
+    for d in (0, 1):
+        assert bool((far.norm(dim=d) <= 8 * near.norm(dim=d).max() + UNIT[out] * 1.01 * want.norm(dim=d)).all()), d
