@@ -525,8 +525,8 @@ uint64_t ec_orthogonalize_workspace(uint64_t batch, uint64_t rows, uint64_t cols
  * more, products are of 11 bits, added to a X with 22: about 1e-3 of the result, up to 3e-3 where x has a single nonzero
  * row (an fp32 out has 22 bits of any x). What is stored between products is scaled for the largest singular values that the
  * coefficients can give, from 1 on, 2^-30 to 2^20 before the last step; larger ones may come out infinite or NaN, smaller
- * ones as zeros. A matrix with a value that is not finite gives NaN; one of zeros gives keep * base. A matrix whose |x| is
- * far below eps keeps fewer bits. EC_ERANGE for rows or cols > 65536, batch > 65535, steps past EC_MAX_STEPS or below 1, or
+ * ones as zeros, and a matrix whose singular values stay far below those keeps fewer bits, as does one whose |x| is far below
+ * eps. A matrix with a value that is not finite gives NaN; one of zeros gives keep * base. EC_ERANGE for rows or cols > 65536, batch > 65535, steps past EC_MAX_STEPS or below 1, or
  * a launch of 2^32 lanes. */
 int ec_orthogonalize(const void* d_x, int type, uint64_t batch, uint64_t rows, uint64_t cols,
                      uint64_t x_stride, uint64_t x_matrix, int steps, const float* coefficients,

@@ -9,9 +9,10 @@ orthogonalised by Newton-Schulz products, scaled and added to the decayed weight
 Every function takes HIP tensors of float32, bfloat16 or float16, sums in fp32 (products on the matrix
 cores), rounds once where it stores unless it says otherwise, and enqueues on the given stream or torch's current one, through
 the C ABI of ``include/ec_mi355.h``.  The same inputs give the same bits.  With gradients enabled,
-``gated_ff`` and ``residual_norm`` are differentiable functions of all their tensors, backward only: a forward-mode tangent
-is refused, and so is a tensor that requires a gradient by the other three, but under ``torch.no_grad()``.  A backward pass is captured into a HIP graph, as with torch's own operators, while no eager pass's
-results of the same leaves are held.
+``gated_ff`` and ``residual_norm`` are differentiable functions of all their tensors, backward only: a forward-mode
+tangent is refused.  The other three have no gradient, and refuse tensors that require one but under
+``torch.no_grad()``.  A backward pass is captured into a HIP graph, as with torch's own operators, while no eager
+pass's results of the same leaves are held.
 """
 from __future__ import annotations
 

@@ -383,7 +383,7 @@ int run_ns(NsArgs& p, uint32_t batch, char* parts, hipStream_t st) {
 // A matrix of at most D x D: one workgroup takes all steps, with everything in LDS, one launch instead of seventeen.  A tall
 // matrix is taken transposed.  A matrix lies there as D-row tiles along k, one behind another; B takes A's place and
 // the next X that of X, when all waves have read them.
-// (Those of ordinary calls are in the first 128 bytes, two lines, to the fifth step's exponents.)
+// The arguments of up to five steps are in 128 bytes.
 struct SmallArgs {
   Matrices x, base;
   char* out;
